@@ -224,6 +224,67 @@ int qw_kv_update_and_attention_general(qw_kv_cache* cache, const void* q, int n_
                                        const void* mask, int mask_dtype, int64_t mask_head_stride,
                                        int64_t mask_row_stride, void* out, void* stream);
 
+/* No counterpart in the reference, which has one cache a sequence: attention of
+ * n_seq sequences that share a prefix, read once for all of them. `prefix` is a
+ * cache of n_kv_heads heads; `tails` (NULL: none) one of n_seq * n_kv_heads,
+ * head b * n_kv_heads + h being KV head h of sequence b, of the same head_dim and
+ * device, in any mode (one launch more where the modes' widths differ). For row
+ * r of sequence b, on the caches' dequantized values,
+ *   out = softmax(scale q . k) . v over all `offset` keys of the prefix and keys
+ *   starts[b] .. offset_tails - n_rows + r of the tails (starts [n_seq] int32
+ *   device, clamped to 0 .. offset_tails; NULL: 0), in fp32 but for the weights'
+ *   rounding to fp16 in P . V. A row that sees no key is 0.
+ * So sequences of different lengths end together: a shorter one starts later,
+ * and what its head holds below starts[b] takes no part. All of them are appended
+ * to by one update of n_seq * n_kv_heads heads; the update form appends k_new /
+ * v_new [n_seq][n_kv_heads][n_rows][head_dim] first.
+ *   q, out [n_seq][n_q_heads][n_rows][head_dim] fp16
+ * Keys that a later row of its own sequence sees and this one does not must be
+ * finite. Either cache may be empty, not both. QW_ERR_UNSUPPORTED on Turbo4 caches. */
+int qw_kv_shared_attention(qw_kv_cache* prefix, qw_kv_cache* tails, int n_seq, const int32_t* starts,
+                           const void* q, int n_q_heads, int n_rows, float scale, void* out,
+                           void* stream);
+int qw_kv_update_and_shared_attention(qw_kv_cache* prefix, qw_kv_cache* tails, int n_seq,
+                                      const int32_t* starts, const void* q, int n_q_heads, int n_rows,
+                                      const void* k_new, const void* v_new, float scale, void* out,
+                                      void* stream);
+
+/* No counterpart in the reference: attention over a cache (out = softmax(scale q
+ * . k) . v in the arithmetic of qw_kv_shared_attention; causal as
+ * qw_kv_attention) that counts what weight each key got,
+ *   weights_out[h][t] = decay * weights[h][t] + sum of the softmax weights of key t
+ *     over the n_rows rows and the query heads of KV head h,   t < offset,
+ * fp32 throughout. weights (fp32 [n_kv_heads][>= n_weights], row stride in
+ * elements; NULL, or decay 0: not read) counts as 0 from n_weights on, as for keys
+ * appended since; weights_out [n_kv_heads][>= offset] may be the same array, else not overlap it. The
+ * update form appends k_new / v_new first. QW_ERR_UNSUPPORTED on Turbo4 caches. */
+int qw_kv_attention_scored(qw_kv_cache* cache, const void* q, int n_q_heads, int n_rows, float scale,
+                           int causal, const float* weights, int64_t weights_stride, int n_weights,
+                           float decay, float* weights_out, int64_t weights_out_stride, void* out,
+                           void* stream);
+int qw_kv_update_and_attention_scored(qw_kv_cache* cache, const void* q, int n_q_heads, int n_rows,
+                                      const void* k_new, const void* v_new, float scale, int causal,
+                                      const float* weights, int64_t weights_stride, int n_weights,
+                                      float decay, float* weights_out, int64_t weights_out_stride,
+                                      void* out, void* stream);
+
+/* No counterpart in the reference: cuts a cache of any mode to a budget by its
+ * keys' weights (fp32 [n_kv_heads][>= offset]). Each KV head keeps n = min(offset,
+ * budget) keys of its own: t < sink, t >= offset - recent, and of the others those
+ * of the largest weight, equal ones by the lower t, -0 equal to 0, a NaN below
+ * every number. Their rows become rows 0 .. n - 1, ascending, code for code, of `into` (a
+ * cache of the same mode, heads, head_dim, Turbo4 seed and device, whose contents
+ * are replaced; NULL or `cache` itself: in place), whose offset is n. A key keeps
+ * the rotation that it was stored with: the caller counts positions on from its own.
+ *   kept [n_kv_heads][n] int32: the kept positions, ascending
+ *   weights_out (or NULL) [n_kv_heads][>= n]: their weights; not inside weights
+ *   *n_kept (host, or NULL) = n
+ * sink + recent <= budget. In place the moved rows pass through a workspace of
+ * their size. */
+int qw_kv_evict(qw_kv_cache* cache, qw_kv_cache* into, const float* weights, int64_t weights_stride,
+                int budget, int sink, int recent, int32_t* kept, float* weights_out,
+                int64_t weights_out_stride, int* n_kept, void* stream);
+
 /* KVCache::trim (cache.rs:2251): drop the last n tokens (clamped to the
  * cached length); *trimmed receives the number removed. No device work. */
 int qw_kv_trim(qw_kv_cache* cache, int n, int* trimmed);

@@ -82,6 +82,12 @@ _SIGNATURES = {
                                      _p]),
     "qw_kv_update_and_attention_general": (_i, [_p, _p, _i, _i, _p, _p, _f, _i, _i, _f, _p, _i,
                                                 _i64, _i64, _p, _p]),
+    "qw_kv_shared_attention": (_i, [_p, _p, _i, _p, _p, _i, _i, _f, _p, _p]),
+    "qw_kv_update_and_shared_attention": (_i, [_p, _p, _i, _p, _p, _i, _i, _p, _p, _f, _p, _p]),
+    "qw_kv_attention_scored": (_i, [_p, _p, _i, _i, _f, _i, _p, _i64, _i, _f, _p, _i64, _p, _p]),
+    "qw_kv_update_and_attention_scored": (_i, [_p, _p, _i, _i, _p, _p, _f, _i, _p, _i64, _i, _f, _p,
+                                               _i64, _p, _p]),
+    "qw_kv_evict": (_i, [_p, _p, _p, _i64, _i, _i, _i, _p, _p, _i64, ctypes.POINTER(_i), _p]),
     "qw_kv_trim": (_i, [_p, _i, ctypes.POINTER(_i)]),
     "qw_kv_dlsa_attention": (_i, [_p, _p, _i, _i, _p, _p, _i, _f, _p, _p]),
     "qw_kv_update_and_dlsa_attention": (_i, [_p, _p, _i, _i, _p, _p, _p, _p, _i, _f, _p, _p]),
@@ -169,6 +175,13 @@ def _hld(t, name: str):
     if not t.is_cuda:
         raise QwError(1, f"{name}: must be a device tensor")
     return t if t.is_contiguous() else t.contiguous(), H, L, D
+
+
+def _bhld(t, name: str, D: int):
+    """(B, H, L) of a batch [B, H, L, D] of fp16 rows on the device."""
+    if len(t.shape) != 4 or t.shape[3] != D or t.dtype is not _torch().float16 or not t.is_cuda:
+        raise QwError(1, f"{name}: fp16 device tensor [B, H, L, {D}] expected")
+    return tuple(t.shape[:3])
 
 
 def _rows2(qkv, what: str):
@@ -430,6 +443,114 @@ class KVCache:
     def update_and_dlsa_attention(self, q, keys, values, lists, lengths, scale: float):
         """Append the L new rows, then :meth:`dlsa_attention`."""
         return self._dlsa(q, keys, values, lists, lengths, scale)
+
+    # -- a prefix shared by a batch
+    def _shared(self, q, tails, keys, values, scale, starts):
+        torch = _torch()
+        B, hq, L = _bhld(q, "q", self.head_dim)
+        if tails is not None and tails.n_kv_heads != B * self.n_kv_heads:
+            raise QwError(1, "shared_attention: tails must have n_seq * n_kv_heads heads")
+        if starts is not None:
+            if starts.shape != (B,) or starts.dtype is not torch.int32 or not starts.is_cuda:
+                raise QwError(1, "shared_attention: starts must be a [n_seq] int32 device tensor")
+            starts = starts.contiguous()
+        qq = q.contiguous()
+        out = qq.new_empty((B, hq, L, self.head_dim))
+        ps = None if starts is None else starts.data_ptr()
+        st = _stream(self.device)
+        if keys is None:
+            _check(lib().qw_kv_shared_attention(self._h, None if tails is None else tails._h, B, ps,
+                                                qq.data_ptr(), hq, L, float(scale), out.data_ptr(), st))
+            return out
+        for name, t in (("keys", keys), ("values", values)):
+            if _bhld(t, name, self.head_dim) != (B, self.n_kv_heads, L):
+                raise QwError(1, f"shared_attention: {name} must be [n_seq, n_kv_heads, L, head_dim]")
+        k, v = keys.contiguous(), values.contiguous()
+        _check(lib().qw_kv_update_and_shared_attention(
+            self._h, tails._h, B, ps, qq.data_ptr(), hq, L, k.data_ptr(), v.data_ptr(), float(scale),
+            out.data_ptr(), st))
+        return out
+
+    def shared_attention(self, q, tails, scale: float, starts=None):
+        """Attention of a batch whose sequences share this cache as their prefix, read once
+        for all: ``q`` [B, Hq, L, D] fp16; ``tails`` a cache of B * n_kv_heads heads (head
+        b * n_kv_heads + h is sequence b's KV head h; None: the prefix alone), of which
+        sequence b sees keys ``starts[b]`` (int32 [B]; None: 0) to its row's own, causal
+        among the last L rows. Returns [B, Hq, L, D]."""
+        return self._shared(q, tails, None, None, scale, starts)
+
+    def update_and_shared_attention(self, q, tails, keys, values, scale: float, starts=None):
+        """Append the sequences' L new rows (``keys``, ``values`` [B, Hkv, L, D]) to ``tails``,
+        then :meth:`shared_attention`."""
+        if tails is None:
+            raise QwError(1, "update_and_shared_attention: tails expected")
+        return self._shared(q, tails, keys, values, scale, starts)
+
+    # -- key weights and eviction by them
+    def _weights(self, weights, what: str, n: int):
+        torch = _torch()
+        if weights.dim() != 2 or weights.shape[0] != self.n_kv_heads or weights.shape[1] < n or \
+                weights.dtype is not torch.float32 or not weights.is_cuda:
+            raise QwError(1, f"{what}: weights must be a [n_kv_heads, >= {n}] f32 device tensor")
+        return weights if weights.stride(1) == 1 and weights.stride(0) >= weights.shape[1] \
+            else weights.contiguous()
+
+    def _scored(self, q, keys, values, scale, weights, decay, causal, weights_out):
+        qq, hq, L, D = _hld(q, "q")
+        if D != self.head_dim:
+            raise QwError(1, "attention_scored: q must have the cache's head_dim")
+        T = self.offset + (0 if keys is None else L)
+        w = None if weights is None else self._weights(weights, "attention_scored", 0)
+        if weights_out is None:
+            wo = qq.new_empty((self.n_kv_heads, T), dtype=_torch().float32)
+        else:
+            wo = self._weights(weights_out, "attention_scored", T)
+            if wo is not weights_out:
+                raise QwError(1, "attention_scored: weights_out must have unit key stride")
+        out = _out_like(qq, hq, L, D)
+        st = _stream(self.device)
+        head = (self._h, qq.data_ptr(), hq, L)
+        rest = (float(scale), int(causal), None if w is None else w.data_ptr(),
+                0 if w is None else w.stride(0), 0 if w is None else min(T, w.shape[1]), float(decay),
+                wo.data_ptr(), wo.stride(0), out.data_ptr(), st)
+        if keys is None:
+            _check(lib().qw_kv_attention_scored(*head, *rest))
+        else:
+            k, *ks = _hld(keys, "keys")
+            v, *vs = _hld(values, "values")
+            if ks != vs or ks != [self.n_kv_heads, L, D]:
+                raise QwError(1, "attention_scored: new keys/values must be [n_kv_heads, L, head_dim]")
+            _check(lib().qw_kv_update_and_attention_scored(*head, k.data_ptr(), v.data_ptr(), *rest))
+        return out, wo if wo.shape[1] == T else wo[:, :T]
+
+    def attention_scored(self, q, scale: float, weights=None, decay: float = 1.0, causal: bool = False,
+                         weights_out=None):
+        """Attention over the cache, and each key's softmax weight summed over the rows and the
+        query heads of its KV head, added to ``decay`` times ``weights`` (f32 [Hkv, n]; keys
+        from n on count from 0; None: all do). Returns (out [1, Hq, L, D], weights [Hkv,
+        offset]); ``weights_out`` (f32 [Hkv, >= offset], ``weights`` itself too) receives
+        the latter."""
+        return self._scored(q, None, None, scale, weights, decay, causal, weights_out)
+
+    def update_and_attention_scored(self, q, keys, values, scale: float, weights=None, decay: float = 1.0,
+                                    causal: bool = False, weights_out=None):
+        """Append the L new rows, then :meth:`attention_scored`."""
+        return self._scored(q, keys, values, scale, weights, decay, causal, weights_out)
+
+    def evict(self, weights, budget: int, sink: int = 0, recent: int = 0, into=None):
+        """Cuts the cache to ``budget`` keys: each KV head keeps its first ``sink``, its last
+        ``recent`` and, of the others, those of the largest ``weights`` (f32 [Hkv, >= offset];
+        ties to the earlier key). The kept rows move, as they are stored, to ``into`` (a cache of the
+        same mode and geometry, whose contents they replace) or stay here. Returns (kept
+        positions [Hkv, n] int32 ascending, their weights [Hkv, n]), n = min(offset, budget)."""
+        w = self._weights(weights, "evict", self.offset)
+        n = max(min(self.offset, int(budget)), 0)
+        kept = w.new_empty((self.n_kv_heads, n), dtype=_torch().int32)
+        wo = w.new_empty((self.n_kv_heads, n))
+        _check(lib().qw_kv_evict(self._h, None if into is None else into._h, w.data_ptr(), w.stride(0),
+                                 int(budget), int(sink), int(recent), kept.data_ptr(), wo.data_ptr(), n,
+                                 None, _stream(self.device)))
+        return kept, wo
 
     # -- lifecycle
     def demote_fp16_to_affine(self, target_mode: int | str) -> bool:

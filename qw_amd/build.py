@@ -24,7 +24,8 @@ ARCH = "gfx950"
 
 SOURCES = ["kv_cache.hip", "attend_decode.hip", "attend_block.hip", "attend_rows.hip",
            "dlsa.hip", "dlsa_rows.hip", "dlsa_typed.hip", "sdpa_general.hip",
-           "dlsa_select.hip", "rope.hip", "turbo4.hip", "abi.hip"]
+           "dlsa_select.hip", "rope.hip", "turbo4.hip", "attend_shared.hip", "key_weights.hip",
+           "evict.hip", "abi.hip"]
 # The measurement library (read-floor and copy kernels), loaded by bench.py only.
 CEIL_SOURCES = ["ceiling.hip"]
 CEIL_OUT = os.path.join(HERE, "libqwceil.so")

@@ -233,6 +233,61 @@ int qw_kv_update_and_attention_general(qw_kv_cache* cache, const void* q, int n_
                                   out, (hipStream_t)stream));
 }
 
+int qw_kv_shared_attention(qw_kv_cache* prefix, qw_kv_cache* tails, int n_seq, const int32_t* starts,
+                           const void* q, int n_q_heads, int n_rows, float scale, void* out,
+                           void* stream) {
+    QW_HANDLE(prefix);
+    QW_GUARDED(qw::shared_attention(prefix->impl, tails ? &tails->impl : nullptr, n_seq, starts, q, n_q_heads,
+                                    n_rows, nullptr, nullptr, scale, out, (hipStream_t)stream));
+}
+
+int qw_kv_update_and_shared_attention(qw_kv_cache* prefix, qw_kv_cache* tails, int n_seq,
+                                      const int32_t* starts, const void* q, int n_q_heads, int n_rows,
+                                      const void* k_new, const void* v_new, float scale, void* out,
+                                      void* stream) {
+    QW_HANDLE(prefix);
+    QW_HANDLE(tails);
+    if (!k_new || !v_new) {
+        qw::set_error("shared attention: null k_new/v_new");
+        return QW_ERR_INVALID_ARGUMENT;
+    }
+    QW_GUARDED(qw::shared_attention(prefix->impl, &tails->impl, n_seq, starts, q, n_q_heads, n_rows, k_new,
+                                    v_new, scale, out, (hipStream_t)stream));
+}
+
+int qw_kv_attention_scored(qw_kv_cache* cache, const void* q, int n_q_heads, int n_rows, float scale,
+                           int causal, const float* weights, int64_t weights_stride, int n_weights,
+                           float decay, float* weights_out, int64_t weights_out_stride, void* out,
+                           void* stream) {
+    QW_HANDLE(cache);
+    QW_GUARDED(qw::attention_scored(cache->impl, q, n_q_heads, n_rows, nullptr, nullptr, scale, causal != 0,
+                                    weights, weights_stride, n_weights, decay, weights_out,
+                                    weights_out_stride, out, (hipStream_t)stream));
+}
+
+int qw_kv_update_and_attention_scored(qw_kv_cache* cache, const void* q, int n_q_heads, int n_rows,
+                                      const void* k_new, const void* v_new, float scale, int causal,
+                                      const float* weights, int64_t weights_stride, int n_weights,
+                                      float decay, float* weights_out, int64_t weights_out_stride,
+                                      void* out, void* stream) {
+    QW_HANDLE(cache);
+    if (!k_new || !v_new) {
+        qw::set_error("scored attention: null k_new/v_new");
+        return QW_ERR_INVALID_ARGUMENT;
+    }
+    QW_GUARDED(qw::attention_scored(cache->impl, q, n_q_heads, n_rows, k_new, v_new, scale, causal != 0,
+                                    weights, weights_stride, n_weights, decay, weights_out,
+                                    weights_out_stride, out, (hipStream_t)stream));
+}
+
+int qw_kv_evict(qw_kv_cache* cache, qw_kv_cache* into, const float* weights, int64_t weights_stride,
+                int budget, int sink, int recent, int32_t* kept, float* weights_out,
+                int64_t weights_out_stride, int* n_kept, void* stream) {
+    QW_HANDLE(cache);
+    QW_GUARDED(qw::evict(cache->impl, into ? &into->impl : nullptr, weights, weights_stride, budget, sink,
+                         recent, kept, weights_out, weights_out_stride, n_kept, (hipStream_t)stream));
+}
+
 int qw_kv_dlsa_attention(qw_kv_cache* cache, const void* q, int n_q_heads, int n_rows,
                          const int32_t* lists, const int32_t* lengths, int width, float scale,
                          void* out, void* stream) {

@@ -348,6 +348,18 @@ int launch_partial_merge_h(const f16* part_o, const float2* part_ml, int nc, int
                            int R, int hkv, int D, int G, int Tq, f16* out, hipStream_t stream,
                            int slot_bits);
 
+// Attention of n_seq sequences over a cache they share and their tails (attend_shared.hip):
+// tails (or null) has head b * prefix.hkv + h for KV head h of sequence b, of which keys
+// starts[b] .. are its own (starts null: all). With k_new / v_new the tails grow by
+// n_rows rows first.
+int shared_attention(KVCache& prefix, KVCache* tails, int n_seq, const int32_t* starts, const void* q, int n_q_heads,
+                     int n_rows, const void* k_new, const void* v_new, float scale, void* out, hipStream_t stream);
+// Attention that counts the keys' weights (key_weights.hip), and eviction by them (evict.hip).
+int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const void* k_new, const void* v_new,
+                     float scale, bool causal, const float* weights, int64_t weights_stride, int n_weights,
+                     float decay, float* weights_out, int64_t weights_out_stride, void* out, hipStream_t stream);
+int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_stride, int budget, int sink, int recent,
+          int32_t* kept, float* weights_out, int64_t weights_out_stride, int* n_kept, hipStream_t stream);
 
 // D-LSA K1 select (dlsa_select.hip).
 int dlsa_select(const float* scores, int64_t stride, const int32_t* members, int n_member_rows,

@@ -267,6 +267,9 @@ enum Workspace {
     kWsTurbo4,   // a Turbo4 attention's rotated rows and partials
     kWsDlsa,     // split-K partials of the D-LSA read
     kWsTyped,    // and of the typed one
+    kWsShared,   // partials of attention over a shared prefix and tails (attend_shared.hip)
+    kWsRowSums,  // the rows' softmax statistics for the key weights (key_weights.hip)
+    kWsEvict,    // the rows that an eviction in place moves (evict.hip)
     kWorkspaces
 };
 int workspace(Workspace kind, int device, hipStream_t stream, size_t need, void** out);
