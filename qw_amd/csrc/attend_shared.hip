@@ -43,16 +43,14 @@ namespace {
 constexpr int kWaves = 8;
 
 // KIND: 16, 8 (affine and Int8) or 4 bits.
-template <int KIND, int D>
-__global__ __launch_bounds__(64 * kWaves, 1) void shared_attend_kernel(SharedArgs a) {
+template <int KIND, int D, bool FAST>
+__device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds) {
     using S = BlockShape<D>;
     constexpr int KT = S::KT, NSUB = S::NSUB, NM = S::NM, NT = S::NT, NG = S::NG;
     constexpr int TPR = S::TPR, LTPR = S::LTPR, TPB = S::TPB, BUF = S::BUF, KBUF = S::KBUF, VROW = S::VROW;
     constexpr int KU = KIND / 4;               // 16-byte loads of a 32-dim K slice / 4-slot V slice
-    constexpr int NST = KIND == 4 ? 3 : 2;     // register stages: tiles of codes in flight
+    constexpr int NST = 2;                     // register stages: tiles of codes in flight
     static_assert(KT * TPR == 64 * kWaves && (KT / 8) * TPB == 64 * kWaves, "a slice of each kind a thread");
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-
     // ---- the unit: a split of a query tile of a head of one of the two caches
     const bool is_tail = (int)blockIdx.x >= a.seg[0].n_units;
     const int u_id = (int)blockIdx.x - (is_tail ? a.seg[0].n_units : 0);
@@ -148,11 +146,11 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attend_kernel(SharedArg
             for (int w = 0; w < 4; w++) kdst[w * KT] = as_h8(st.kc[w]);
         } else {
             const half2v sb = h2(st.kp), s = {sb.x, sb.x}, b = {sb.y, sb.y};
-            const PairConsts c = make_consts<false, KIND>(s, s, s, s, b, b, b, b, code_off);
+            const PairConsts c = make_consts<FAST, KIND>(s, s, s, s, b, b, b, b, code_off);
 #pragma unroll
             for (int w = 0; w < 4; w++)
-                kdst[w * KT] = KIND == 4 ? deq4<false>(st.kc[0][w], c, magic)
-                                         : deq8<false>(st.kc[KU / 2 * (w / 2)][2 * (w % 2)],
+                kdst[w * KT] = KIND == 4 ? deq4<FAST>(st.kc[0][w], c, magic)
+                                         : deq8<FAST>(st.kc[KU / 2 * (w / 2)][2 * (w % 2)],
                                                        st.kc[KU / 2 * (w / 2)][2 * (w % 2) + 1], c);
         }
         half8 y[4];
@@ -160,13 +158,13 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attend_kernel(SharedArg
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = as_h8(st.vc[e]);
         } else {
-            const PairConsts c = make_consts<false, KIND>(h2(st.vp[0][0]), h2(st.vp[0][1]), h2(st.vp[0][2]), h2(st.vp[0][3]),
+            const PairConsts c = make_consts<FAST, KIND>(h2(st.vp[0][0]), h2(st.vp[0][1]), h2(st.vp[0][2]), h2(st.vp[0][3]),
                                                           h2(st.vp[1][0]), h2(st.vp[1][1]), h2(st.vp[1][2]), h2(st.vp[1][3]),
                                                           code_off);
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                y[e] = KIND == 4 ? deq4<false>(st.vc[0][e], c, magic)
-                                 : deq8<false>(st.vc[KU / 2 * (e / 2)][2 * (e % 2)],
+                y[e] = KIND == 4 ? deq4<FAST>(st.vc[0][e], c, magic)
+                                 : deq8<FAST>(st.vc[KU / 2 * (e / 2)][2 * (e % 2)],
                                                st.vc[KU / 2 * (e / 2)][2 * (e % 2) + 1], c);
         }
         const int key0 = (t0 + i) * KT;
@@ -257,40 +255,47 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attend_kernel(SharedArg
                 acc_o[mm] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p16[u], sV[(4 * u + g) * VROW + r16 + 17 * mm],
                                                                    acc_o[mm], 0, 0, 0);
     };
-    const int per = NSUB / parts, ub0 = part * per;
-    auto compute = [&](int i) {
-        if (!live) return;
-        if (per == 1) {
-            if ((t0 + i) * KT + 32 * ub0 <= wave_lim) step(i, ub0, std::integral_constant<int, 1>{});
-        } else {
-            for (int ub = ub0; ub < ub0 + per; ub += 2)
-                if ((t0 + i) * KT + 32 * ub <= wave_lim) step(i, ub, std::integral_constant<int, 2>{});
+
+    // ---- rounds: stage x holds tile i where i mod NST == x. A loop of its own for the waves
+    // that take one sub-block of a tile and for those that take PER = 2 or 4 of them, two at a
+    // time (one loop for both spilled registers); the barriers pair up all the same.
+    auto rounds = [&](auto per_c) {
+        constexpr int PER = decltype(per_c)::value, NU = PER < 2 ? 1 : 2;
+        const int ub0 = part * PER;
+        auto compute = [&](int i) {
+#pragma unroll
+            for (int ub = 0; ub < PER; ub += NU)
+                if (live && (t0 + i) * KT + 32 * (ub0 + ub) <= wave_lim)
+                    step(i, ub0 + ub, std::integral_constant<int, NU>{});
+        };
+        Stage st[NST];
+        if (n > 0) {
+#pragma unroll
+            for (int x = 0; x < NST; x++)
+                if (x < n) load(st[x], x);
+            store(st[0], 0);
+            if (NST < n) load(st[0], NST);
+        }
+        __syncthreads();
+        for (int i = 0; i < n; i += NST) {
+#pragma unroll
+            for (int x = 0; x < NST; x++) {
+                if (i + x >= n) break;
+                if (i + x + 1 < n) {
+                    store(st[(x + 1) % NST], i + x + 1);
+                    if (i + x + 1 + NST < n) load(st[(x + 1) % NST], i + x + 1 + NST);
+                }
+                compute(i + x);
+                __syncthreads();
+            }
         }
     };
-
-    // ---- rounds: stage x holds tile i where i mod NST == x
-    Stage st[NST];
-    if (n > 0) {
-#pragma unroll
-        for (int x = 0; x < NST; x++)
-            if (x < n) load(st[x], x);
-        store(st[0], 0);
-        if (NST < n) load(st[0], NST);
-    }
-    __syncthreads();
-    for (int i = 0; i < n; i += NST) {
-#pragma unroll
-        for (int x = 0; x < NST; x++) {
-            if (i + x >= n) break;
-            constexpr int Y = NST;
-            if (i + x + 1 < n) {
-                store(st[(x + 1) % Y], i + x + 1);
-                if (i + x + 1 + NST < n) load(st[(x + 1) % Y], i + x + 1 + NST);
-            }
-            compute(i + x);
-            __syncthreads();
-        }
-    }
+    if (parts == NSUB)
+        rounds(std::integral_constant<int, 1>{});
+    else if (NSUB == 2 || parts == 2)
+        rounds(std::integral_constant<int, 2>{});
+    else
+        rounds(std::integral_constant<int, NSUB>{});
 
     // ---- the parts of a row tile joined in its part 0, through LDS
     float l = wave_sum_g(l_run);
@@ -358,6 +363,15 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_attend_kernel(SharedArg
 #undef QW_SEG
 }
 
+template <int KIND, int D>
+__global__ __launch_bounds__(64 * kWaves, 1) void shared_attend_kernel(SharedArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const bool fast = KIND != 16 && *((int)blockIdx.x >= a.seg[0].n_units ? a.seg[1].fast_flag : a.seg[0].fast_flag);
+    if constexpr (KIND != 16)
+        if (fast) return shared_body<KIND, D, true>(a, lds);
+    shared_body<KIND, D, false>(a, lds);
+}
+
 // Joins a row's partials: grid (R, hkv), D / 4 threads a partial row, 1024 / D partial rows
 // at a time, their sums joined through LDS.
 template <int D>
@@ -421,6 +435,7 @@ void fill_cache(SharedSegment& s, const KVCache& c) {
     s.cap = c.cap;
     s.T = c.offset;
     s.code_off2 = c.code_offset2();
+    s.fast_flag = c.fast_flag;
 }
 
 template <int KIND, int D>

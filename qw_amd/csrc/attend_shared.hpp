@@ -13,6 +13,7 @@ struct SharedSegment {
     const uint32_t* k_params;
     const uint32_t* v_data;
     const uint32_t* v_params;
+    const int* fast_flag;         // device: every stored scale is in the range of the short dequantization
     int cap, T;
     uint32_t code_off2;
     int heads, rows;              // the cache's heads; query rows of each
