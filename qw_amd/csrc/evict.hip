@@ -7,11 +7,11 @@
 // Each head keeps its own set. The reference's caches shrink at the end only (KVCache::trim,
 // crates/mlxcel-core/src/cache.rs:2251).
 //
-// Two launches (three in place):
-//   evict_select_kernel, a workgroup a head: a radix select finds the weight of the last kept
-//     key (11 + 11 + 10 bits of the float in an order-preserving integer form, one LDS histogram a digit),
-//     then each wave walks a run of the keys and writes the kept positions at the places that
-//     counts of the runs before it give;
+// The launches:
+//   the select: the weight of the last kept key by its digits (11 + 11 + 10 bits of the float in
+//     an order-preserving integer form, a histogram in LDS a digit), then the kept positions at the places that
+//     scans of the counts before them give; a workgroup a head (evict_select_kernel) or, for
+//     longer caches, one a chunk (evict_digit_kernel);
 //   evict_rows_kernel copies 16-byte pieces: K rows whole; V, stored in 8-key blocks with the
 //     8 keys of a dim together, key by key out of up to 8 source blocks.
 // In place the rows go through a workspace: a row's new place may be another's old one.
@@ -24,6 +24,9 @@ namespace qw {
 namespace {
 
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kBins = 2048;
+constexpr int kDigits = 3;
+__host__ __device__ constexpr int digit_shift(int d) { return d == 0 ? 21 : d == 1 ? 10 : 0; }
+__host__ __device__ constexpr int digit_bits(int d) { return d < 2 ? 11 : 10; }
 
 // Order-preserving: larger weight, larger integer; NaN 0.
 __device__ __forceinline__ uint32_t weight_rank(float w) {
@@ -39,102 +42,228 @@ struct SelectArgs {
     int32_t* kept;                 // [hkv][n]
     float* weights_out;            // [hkv][out_stride] or null
     int64_t out_stride;
+    // the form of several workgroups a head (evict_digit_kernel): per head and chunk
+    uint32_t* hist;                // [kDigits][hkv][chunks][kBins / 2]: two 16-bit counts a word
+    uint32_t* above;               // [2][hkv][chunks]: keys above the cut by their first, second digit
+    uint2* pick;                   // [kDigits][hkv]: the cut's digit, the kept keys left within it
+    int chunks;
 };
 
+// hist[bin] += 1 for every lane that is in. Keys of one weight (those that no row ever looked
+// at are 0) would queue on one counter: where the first such lane's bin is shared by many,
+// one lane adds for all of them.
+__device__ __forceinline__ void add_bin(uint32_t* hist, uint32_t bin, bool in) {
+    const uint64_t live = __ballot(in);
+    if (!live) return;
+    const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)bin, __ffsll((unsigned long long)live) - 1);
+    const uint64_t same = __ballot(in && bin == first);
+    if (__popcll(same) > 4) {
+        if ((int)__lane_id() == __ffsll((unsigned long long)same) - 1) atomicAdd(&hist[first], (uint32_t)__popcll(same));
+        in = in && bin != first;
+    }
+    if (in) atomicAdd(&hist[bin], 1u);
+}
+
+// The sum of x over the threads before this one, over the workgroup; *total: over all.
+__device__ __forceinline__ uint32_t scan_before(uint32_t x, uint32_t* s_wave, uint32_t* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t upto = x;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const uint32_t y = __shfl_up(upto, s);
+        if (lane >= s) upto += y;
+    }
+    __syncthreads();  // s_wave is free
+    if (lane == 63) s_wave[wave] = upto;
+    __syncthreads();
+    uint32_t before = upto - x, all = 0;
+#pragma unroll
+    for (int v = 0; v < kSelWaves; v++) {
+        const uint32_t y = s_wave[v];
+        before += v < wave ? y : 0u;
+        all += y;
+    }
+    *total = all;
+    return before;
+}
+
+// The bin in which the count from the top reaches left, and what is left within it: thread i
+// holds the counts of bins kBins - 1 - 2 i (hi) and the one below it (lo).
+__device__ __forceinline__ uint2 pick_bin(uint32_t hi, uint32_t lo, uint32_t left, uint32_t* s_wave, uint2* s_pick) {
+    uint32_t total;
+    const uint32_t before = scan_before(hi + lo, s_wave, &total);
+    const int top = kBins - 1 - 2 * (int)threadIdx.x;
+    if (left == 0 && threadIdx.x == 0) *s_pick = uint2{kBins - 1, 0u};  // (above every digit, or ties = 0)
+    if (before < left && left <= before + hi)
+        *s_pick = uint2{(uint32_t)top, left - before};
+    else if (before + hi < left && left <= before + hi + lo)
+        *s_pick = uint2{(uint32_t)top - 1, left - before - hi};
+    __syncthreads();
+    return *s_pick;
+}
+
+// Writes the kept keys among KPT consecutive ones a thread, from key t0: rank above the cut or
+// outside the middle, and of those equal to it the first `ties` (eq0 of them and at0 kept keys in the
+// chunks before).
+template <int KPT>
+__device__ __forceinline__ void emit(const SelectArgs& a, int h, int t0, const float (&x)[KPT], uint32_t cut,
+                                     uint32_t ties, uint32_t at0, uint32_t eq0, uint32_t* s_wave) {
+    const int lo = a.sink, hi = a.T - a.recent;
+    uint32_t n_above = 0, n_equal = 0;
+    uint32_t kind[KPT];  // 2: kept, 1: a tie, 0: gone
+#pragma unroll
+    for (int e = 0; e < KPT; e++) {
+        const int t = t0 + e;
+        const bool mid = t >= lo && t < hi;
+        const uint32_t u = weight_rank(x[e]);
+        kind[e] = t >= a.T ? 0u : !mid || u > cut ? 2u : u == cut ? 1u : 0u;
+        n_above += kind[e] == 2u;
+        n_equal += kind[e] == 1u;
+    }
+    uint32_t total;
+    uint32_t at = at0 + scan_before(n_above, s_wave, &total), eq = eq0 + scan_before(n_equal, s_wave, &total);
+#pragma unroll
+    for (int e = 0; e < KPT; e++) {
+        if (kind[e] == 2u || (kind[e] == 1u && eq < ties)) {
+            const uint32_t pos = at + min(eq, ties);
+            a.kept[(int64_t)h * a.n + pos] = t0 + e;
+            if (a.weights_out) a.weights_out[h * a.out_stride + pos] = x[e];
+        }
+        at += kind[e] == 2u;
+        eq += kind[e] == 1u;
+    }
+}
+
+// A head in one workgroup, its keys (KPT consecutive ones a thread) in registers.
+template <int KPT>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(SelectArgs a) {
     __shared__ uint32_t hist[kBins];
-    __shared__ uint32_t s_wave[kSelWaves][2];
-    __shared__ uint32_t s_pick[2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = blockIdx.x;
+    __shared__ uint32_t s_wave[kSelWaves];
+    __shared__ uint2 s_pick;
+    const int tid = threadIdx.x, h = blockIdx.x, t0 = tid * KPT;
     const float* w = a.weights + h * a.stride;
-    const int lo = a.sink, hi = a.T - a.recent;  // the middle
-    // the rank of the last kept key, digit by digit; left: kept keys among those that share
-    // the digits so far
+    const int lo = a.sink, hi = a.T - a.recent;
+    float x[KPT];
+#pragma unroll
+    for (int e = 0; e < KPT; e++) x[e] = t0 + e < a.T ? w[t0 + e] : 0.0f;
     uint32_t prefix = 0, left = (uint32_t)a.need;
-    const int shifts[3] = {21, 10, 0};
-    for (int d = 0; d < 3; d++) {
-        const int shift = shifts[d], bits = d < 2 ? 11 : 10;
-        for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+#pragma unroll
+    for (int d = 0; d < kDigits; d++) {
+        hist[2 * tid] = hist[2 * tid + 1] = 0;
         __syncthreads();
-        for (int t = lo + tid; t < hi; t += kSelThreads) {
-            const uint32_t u = weight_rank(w[t]);
-            const bool in = d == 0 || (u >> (shift + bits)) == prefix;
-            const uint32_t bin = (u >> shift) & ((1u << bits) - 1);
-            if (in) atomicAdd(&hist[bin], 1u);
+#pragma unroll
+        for (int e = 0; e < KPT; e++) {
+            const uint32_t u = weight_rank(x[e]);
+            const bool in = t0 + e >= lo && t0 + e < hi && (d == 0 || u >> (digit_shift(d) + digit_bits(d)) == prefix);
+            add_bin(hist, u >> digit_shift(d) & ((1u << digit_bits(d)) - 1), in);
         }
         __syncthreads();
-        // the bin in which the count from the top reaches left
-        if (wave == 0) {
-            uint32_t mine = 0;
-            for (int i = 0; i < kBins / 64; i++) mine += hist[kBins - 1 - (lane * (kBins / 64) + i)];
-            uint32_t upto = mine;
-            for (int s = 1; s < 64; s <<= 1) {
-                const uint32_t x = __shfl_up(upto, s);
-                if (lane >= s) upto += x;
-            }
-            const uint32_t before = upto - mine;
-            if (before < left && left <= upto) {
-                uint32_t c = before;
-                for (int i = 0; i < kBins / 64; i++) {
-                    const int b = kBins - 1 - (lane * (kBins / 64) + i);
-                    if (c + hist[b] >= left) {
-                        s_pick[0] = b;
-                        s_pick[1] = left - c;
-                        break;
-                    }
-                    c += hist[b];
-                }
-            }
-            if (left == 0 && lane == 0) s_pick[0] = (1u << bits) - 1, s_pick[1] = 0;
+        const uint2 p = pick_bin(hist[kBins - 1 - 2 * tid], hist[kBins - 2 - 2 * tid], left, s_wave, &s_pick);
+        prefix = prefix << digit_bits(d) | (p.x & ((1u << digit_bits(d)) - 1));
+        left = p.y;
+    }
+    emit<KPT>(a, h, t0, x, prefix, left, 0, 0, s_wave);
+}
+
+// The same by chunks of kChunk keys, a workgroup each (grid (chunks, hkv)), in four launches: d = 0,
+// 1, 2 count digit d of the chunk's keys that share the cut's digits before it (found from the last
+// launch's counts by every workgroup for itself), d = 3 writes the kept keys.
+constexpr int kChunkKeys = 4, kChunk = kSelThreads * kChunkKeys;
+
+__global__ __launch_bounds__(kSelThreads) void evict_digit_kernel(SelectArgs a, int d) {
+    __shared__ uint32_t hist[kBins];
+    __shared__ uint32_t s_wave[kSelWaves];
+    __shared__ uint2 s_pick;
+    const int tid = threadIdx.x, c = blockIdx.x, h = blockIdx.y, hkv = gridDim.y, t0 = c * kChunk + tid * kChunkKeys;
+    const float* w = a.weights + h * a.stride;
+    const int lo = a.sink, hi = a.T - a.recent;
+    float x[kChunkKeys];
+#pragma unroll
+    for (int e = 0; e < kChunkKeys; e++) x[e] = t0 + e < a.T ? w[t0 + e] : 0.0f;
+    const uint32_t* hist_d = nullptr;  // the last digit's counts of this head
+    uint32_t prefix = 0, left = (uint32_t)a.need;
+    if (d > 0) {
+        hist_d = a.hist + ((int64_t)(d - 1) * hkv + h) * a.chunks * (kBins / 2);
+        uint32_t n_hi = 0, n_lo = 0;
+#pragma unroll 8
+        for (int i = 0; i < a.chunks; i++) {
+            const uint32_t v = hist_d[(int64_t)i * (kBins / 2) + kBins / 2 - 1 - tid];
+            n_hi += v >> 16;
+            n_lo += v & 0xFFFFu;
         }
-        __syncthreads();
-        prefix = prefix << bits | s_pick[0];
-        left = s_pick[1];
-        __syncthreads();
-    }
-    const uint32_t cut = prefix, ties = left;  // kept: rank > cut, and the first `ties` of rank == cut
-    // need == 0: nothing above the largest integer, no ties
-    // runs of whole 64-key steps a wave
-    const int per = ((a.T + kSelWaves - 1) / kSelWaves + 63) / 64 * 64;
-    const int r0 = min(a.T, wave * per), r1 = min(a.T, r0 + per);
-    uint32_t above = 0, equal = 0;
-    for (int t = r0 + lane; t < r1; t += 64) {
-        const bool mid = t >= lo && t < hi;
-        const uint32_t u = mid ? weight_rank(w[t]) : 0;
-        above += !mid || u > cut;
-        equal += mid && u == cut;
-    }
-    for (int s = 32; s; s >>= 1) {
-        above += __shfl_xor(above, s);
-        equal += __shfl_xor(equal, s);
-    }
-    if (lane == 0) {
-        s_wave[wave][0] = above;
-        s_wave[wave][1] = equal;
-    }
-    __syncthreads();
-    uint32_t at = 0, eq = 0;  // kept keys above the cut and ties in the runs before this one
-    for (int v = 0; v < wave; v++) {
-        at += s_wave[v][0];
-        eq += s_wave[v][1];
-    }
-    int32_t* kept = a.kept + (int64_t)h * a.n;
-    for (int t = r0 + lane; t - lane < r1; t += 64) {
-        const bool in = t < r1, mid = t >= lo && t < hi;
-        const float x = in ? w[t] : 0.0f;
-        const uint32_t u = weight_rank(x);
-        const uint64_t m_above = __ballot(in && (!mid || u > cut)), m_equal = __ballot(in && mid && u == cut);
-        const uint64_t below = ((uint64_t)1 << lane) - 1;
-        const uint32_t tie = eq + __popcll(m_equal & below);  // ties before this key
-        const bool keep = (m_above >> lane & 1) || ((m_equal >> lane & 1) && tie < ties);
-        const uint32_t pos = at + __popcll(m_above & below) + min(tie, ties);
-        if (keep) {
-            kept[pos] = t;
-            if (a.weights_out) a.weights_out[h * a.out_stride + pos] = x;
+        for (int i = 0; i < d - 1; i++) {
+            const uint2 p = a.pick[i * hkv + h];
+            prefix = prefix << digit_bits(i) | (p.x & ((1u << digit_bits(i)) - 1));
+            left = p.y;
         }
-        at += __popcll(m_above);
-        eq += __popcll(m_equal);
+        const uint2 p = pick_bin(n_hi, n_lo, left, s_wave, &s_pick);
+        if (c == 0 && tid == 0) a.pick[(d - 1) * hkv + h] = p;
+        prefix = prefix << digit_bits(d - 1) | (p.x & ((1u << digit_bits(d - 1)) - 1));
+        left = p.y;
     }
+    if (d < kDigits) {
+        hist[2 * tid] = hist[2 * tid + 1] = 0;
+        __syncthreads();
+        const int shift = digit_shift(d), bits = digit_bits(d);
+        uint32_t n_above = 0;  // keys that the last digit put above the cut
+#pragma unroll
+        for (int e = 0; e < kChunkKeys; e++) {
+            const uint32_t u = weight_rank(x[e]);
+            const bool mid = t0 + e >= lo && t0 + e < hi;
+            const uint32_t head = d == 0 ? 0 : u >> (shift + bits);
+            add_bin(hist, u >> shift & ((1u << bits) - 1), mid && head == prefix);
+            // (the digits before the last are equal, the last is larger)
+            n_above += d > 0 && mid && head > prefix && (d == 1 || head >> digit_bits(1) == prefix >> digit_bits(1));
+        }
+        uint32_t total;
+        scan_before(n_above, s_wave, &total);
+        if (d > 0 && tid == 0) a.above[((d - 1) * hkv + h) * a.chunks + c] = total;
+        a.hist[(((int64_t)d * hkv + h) * a.chunks + c) * (kBins / 2) + tid] = hist[2 * tid] | hist[2 * tid + 1] << 16;
+        return;
+    }
+    // kept keys above the cut and ties in the chunks before this one; protected ones too
+    uint32_t n_above = 0, n_equal = 0;
+    const uint32_t b2 = prefix & ((1u << digit_bits(2)) - 1);
+#pragma unroll 8
+    for (int i = 0; i < c; i++) {
+        const uint32_t v = hist_d[(int64_t)i * (kBins / 2) + tid];
+        n_above += (2u * tid > b2 ? v & 0xFFFFu : 0u) + (2u * tid + 1 > b2 ? v >> 16 : 0u);
+        n_equal += (2u * tid == b2 ? v & 0xFFFFu : 0u) + (2u * tid + 1 == b2 ? v >> 16 : 0u);
+    }
+    for (int i = tid; i < c; i += kSelThreads)
+        n_above += a.above[h * a.chunks + i] + a.above[(hkv + h) * a.chunks + i];
+    uint32_t at, eq;
+    scan_before(n_above, s_wave, &at);
+    scan_before(n_equal, s_wave, &eq);
+    const int start = c * kChunk;
+    at += min(start, lo) + max(0, start - max(hi, lo));
+    emit<kChunkKeys>(a, h, t0, x, prefix, left, at, eq, s_wave);
+}
+
+// Keys up to which one workgroup a head does it.
+constexpr int kOneGroup = 16 * kSelThreads;
+
+int launch_select(SelectArgs a, int hkv, int device, hipStream_t stream) {
+    if (a.T <= kOneGroup) {
+        auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(hkv), dim3(kSelThreads), 0, stream, a); };
+        a.T <= kSelThreads ? run(evict_select_kernel<1>)
+        : a.T <= 4 * kSelThreads ? run(evict_select_kernel<4>) : run(evict_select_kernel<16>);
+        QW_HIP_CHECK(hipGetLastError());
+        return QW_OK;
+    }
+    a.chunks = (a.T + kChunk - 1) / kChunk;
+    const size_t per = (size_t)hkv * a.chunks;
+    const size_t h_bytes = kDigits * per * (kBins / 2) * 4, p_bytes = kDigits * (size_t)hkv * sizeof(uint2);
+    void* ws = nullptr;
+    if (int rc = workspace(kWsSelect, device, stream, h_bytes + p_bytes + 2 * per * 4, &ws)) return rc;
+    a.hist = (uint32_t*)ws;
+    a.pick = (uint2*)((char*)ws + h_bytes);
+    a.above = (uint32_t*)((char*)ws + h_bytes + p_bytes);
+    for (int d = 0; d <= kDigits; d++) {
+        hipLaunchKernelGGL(evict_digit_kernel, dim3(a.chunks, hkv), dim3(kSelThreads), 0, stream, a, d);
+        QW_HIP_CHECK(hipGetLastError());
+    }
+    return QW_OK;
 }
 
 struct RowsCopy {
@@ -145,71 +274,75 @@ struct RowsCopy {
     const int32_t* kept;     // [hkv][n]
     const int* flag;         // the source's fast flag, copied where flag_to is not null
     int* flag_to;
-    int hkv, n, cap, cap_to, bits, D, kp_words;  // kp_words: words of a K row's params
+    int n, cap, cap_to, D, kp_words;  // kp_words: words of a K row's params
     int row_major_v;         // Turbo4: V rows like K's, one params word a row
 };
 
-// BITS: of a code (or 16). A thread copies one 16-byte piece of one 8-row block of one plane.
+// BITS: of a code (or 16). A thread copies a 16-byte piece of a block's 8 rows of one plane:
+// grid (pieces of all blocks / 256, hkv, plane). All its loads are issued before the first is used.
 template <int BITS>
 __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
     const int pieces = a.D * BITS / 16;  // of a block, in each plane
-    const int64_t n_blk = (a.n + 7) / 8, total = a.hkv * n_blk * 2 * pieces;
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id == 0 && a.flag_to) *a.flag_to = *a.flag;
-    if (id >= total) return;
-    const int pc = (int)(id % pieces), plane = (int)(id / pieces % 2);
-    const int64_t hb = id / pieces / 2;
-    const int h = (int)(hb / n_blk), b = (int)(hb % n_blk);
+    const int id = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+    if (id == 0 && h == 0 && blockIdx.z == 0 && a.flag_to) *a.flag_to = *a.flag;
+    const int b = id / pieces, pc = id - b * pieces;  // (pieces is a power of two below 2^9, id below 2^31)
+    if (8 * b >= a.n) return;
     const int32_t* kept = a.kept + (int64_t)h * a.n + 8 * b;
     const int rows = min(8, a.n - 8 * b);
-    if (plane == 0 || a.row_major_v) {
-        const u32x4* from = plane == 0 ? a.k : a.v;
-        u32x4* to = plane == 0 ? a.k_to : a.v_to;
-        const int ppr = pieces / 8, r = pc / ppr, c = pc % ppr;
+    if (blockIdx.z == 0 || a.row_major_v) {
+        const u32x4* from = blockIdx.z == 0 ? a.k : a.v;
+        u32x4* to = blockIdx.z == 0 ? a.k_to : a.v_to;
+        const int ppr = pieces / 8, r = pc / ppr, c = pc - r * ppr;
         if (r >= rows) return;
         const int64_t src = (int64_t)h * a.cap + kept[r], dst = (int64_t)h * a.cap_to + 8 * b + r;
         to[dst * ppr + c] = from[src * ppr + c];
-        const uint32_t* pf = plane == 0 ? a.kp : a.vp;
-        uint32_t* pt = plane == 0 ? a.kp_to : a.vp_to;
+        const uint32_t* pf = blockIdx.z == 0 ? a.kp : a.vp;
+        uint32_t* pt = blockIdx.z == 0 ? a.kp_to : a.vp_to;
         const int pw = a.row_major_v ? 1 : a.kp_words;
         if (c < pw) pt[dst * pw + c] = pf[src * pw + c];
         return;
     }
     const int64_t sblk = (int64_t)h * (a.cap / 8), dblk = (int64_t)h * (a.cap_to / 8) + b;
-    // piece pc of the block: 4 dims' words of 8 nibbles, 2 dims' of 8 bytes or one dim's of 8 halves
-    u32x4 out = {0, 0, 0, 0}, x = {0, 0, 0, 0};
-    int have = -1;
+    int t[8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-        if (k >= rows) break;
-        const int t = kept[k];
-        if (t / 8 != have) {
-            have = t / 8;
-            x = a.v[(sblk + have) * pieces + pc];
-        }
-        const int f = t & 7;
-        if constexpr (BITS == 4) {
-            const int from = 4 * v4_nibble_pos(f), to = 4 * v4_nibble_pos(k);
+    for (int k = 0; k < 8; k++) t[k] = kept[min(k, rows - 1)];
+    // piece pc of the block: 4 dims' words of 8 nibbles, 2 dims' of 8 bytes or one dim's of 8
+    // halves; slots of rows past the last one take its row (as anything may stand there)
+    u32x4 out = {0, 0, 0, 0};
+    if constexpr (BITS == 16) {
+        uint32_t x[8];
 #pragma unroll
-            for (int j = 0; j < 4; j++) out[j] |= (x[j] >> from & 0xFu) << to;
-        } else if constexpr (BITS == 8) {
-            const int from = 8 * (f & 3), to = 8 * (k & 3);
+        for (int k = 0; k < 8; k++) x[k] = ((const uint16_t*)(a.v + (sblk + t[k] / 8) * pieces + pc))[t[k] & 7];
 #pragma unroll
-            for (int j = 0; j < 2; j++) out[2 * j + k / 4] |= ((f & 4 ? x[2 * j + 1] : x[2 * j]) >> from & 0xFFu) << to;
-        } else {
-            const uint32_t w = f & 4 ? (f & 2 ? x[3] : x[2]) : (f & 2 ? x[1] : x[0]);
-            out[k / 2] |= (w >> (16 * (f & 1)) & 0xFFFFu) << (16 * (k & 1));
+        for (int k = 0; k < 4; k++) out[k] = x[2 * k] | x[2 * k + 1] << 16;
+    } else {
+        u32x4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = a.v[(sblk + t[k] / 8) * pieces + pc];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int f = t[k] & 7;
+            if constexpr (BITS == 4) {
+                const int from = 4 * v4_nibble_pos(f), to = 4 * v4_nibble_pos(k);
+#pragma unroll
+                for (int j = 0; j < 4; j++) out[j] |= (x[k][j] >> from & 0xFu) << to;
+            } else {
+                const int from = 8 * (f & 3), to = 8 * (k & 3);
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    out[2 * j + k / 4] |= ((f & 4 ? x[k][2 * j + 1] : x[k][2 * j]) >> from & 0xFFu) << to;
+            }
         }
     }
     a.v_to[dblk * pieces + pc] = out;
     if (BITS != 16 && pc < a.kp_words * 8) {  // scale and bias of key pc & 7 in group pc >> 3
         const int grp = pc >> 3, k = pc & 7;
         if (k < rows) {
-            const int t = kept[k];
-            const f16* from = (const f16*)a.vp + ((sblk + t / 8) * a.kp_words + grp) * 16;
+            const int tk = kept[k];
+            const f16* from = (const f16*)a.vp + ((sblk + tk / 8) * a.kp_words + grp) * 16;
             f16* to = (f16*)a.vp_to + (dblk * a.kp_words + grp) * 16;
-            to[k] = from[t & 7];
-            to[8 + k] = from[8 + (t & 7)];
+            to[k] = from[tk & 7];
+            to[8 + k] = from[8 + (tk & 7)];
         }
     }
 }
@@ -270,11 +403,9 @@ int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_str
         if (int rc = workspace(kWsEvict, src.device, stream, at[3] + src.v_param_bytes(rows8), &p)) return rc;
         ws = (char*)p;
     }
-    const int first_need = std::max(0, n - std::min(sink, T) - std::min(recent, T - std::min(sink, T)));
-    SelectArgs s{weights, weights_stride, T, n, std::min(sink, T), std::min(recent, T - std::min(sink, T)), first_need,
-                 kept, weights_out, weights_out_stride};
-    hipLaunchKernelGGL(evict_select_kernel, dim3(src.hkv), dim3(kSelThreads), 0, stream, s);
-    QW_HIP_CHECK(hipGetLastError());
+    const int first = std::min(sink, T), last = std::min(recent, T - first);  // (first + last <= n)
+    SelectArgs s{weights, weights_stride, T, n, first, last, n - first - last, kept, weights_out, weights_out_stride};
+    if (int rc = launch_select(s, src.hkv, src.device, stream)) return rc;
     if (in_place && n == T) return QW_OK;  // every row stays where it is
     RowsCopy c{};
     c.k = (const u32x4*)src.k_data;
@@ -288,16 +419,13 @@ int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_str
     c.kept = kept;
     c.flag = src.fast_flag;
     c.flag_to = in_place ? nullptr : dst.fast_flag;
-    c.hkv = src.hkv;
     c.n = n;
     c.cap = src.cap;
     c.cap_to = staged ? rows8 : dst.cap;
-    c.bits = src.bits;
     c.D = src.D;
     c.kp_words = src.affine() ? src.D / kGroup : src.turbo4() ? 1 : 0;
     c.row_major_v = src.turbo4() ? 1 : 0;
-    const int64_t pieces = (int64_t)src.hkv * (rows8 / 8) * 2 * (src.D * src.bits / 16);
-    const dim3 grid((unsigned)((pieces + 255) / 256));
+    const dim3 grid((unsigned)(((int64_t)(rows8 / 8) * (src.D * src.bits / 16) + 255) / 256), src.hkv, 2);
     if (src.bits == 4)
         hipLaunchKernelGGL(evict_rows_kernel<4>, grid, dim3(256), 0, stream, c);
     else if (src.bits == 8)

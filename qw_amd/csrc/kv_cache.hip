@@ -817,75 +817,94 @@ int KVCache::update_and_fetch(const void* k_new, const void* v_new, int n_tokens
 // MLX-packed codes and separate fp16 scale and bias planes (cache.rs:570-626
 // exports packed tensors as they are, without requantizing).
 
-// V blocks <-> rows, plus the K param split/merge. dir = 0: export.
-// Int8 mode: codes leave and enter as signed bytes (stored + 128, i.e. XOR
-// 0x80 per byte) and one scale per row (the first group's; every group holds
-// it, with bias 0).
-__global__ __launch_bounds__(256) void snapshot_affine_kernel(
-    int dir, int bits, int int8, int D, int cap, int hkv, int n, int* __restrict__ fast_flag,
-    uint32_t* __restrict__ k_params,
-    uint32_t* __restrict__ v_codes, f16* __restrict__ v_params, f16* __restrict__ ks_out,
-    f16* __restrict__ kb_out, uint32_t* __restrict__ vc_rows, f16* __restrict__ vs_rows,
-    f16* __restrict__ vb_rows) {
+// Import of the scales and biases: a thread per (head, row, group). Int8 mode: one scale per
+// row, which every group holds with bias 0.
+__global__ __launch_bounds__(256) void import_params_kernel(
+    int bits, int int8, int D, int cap, int hkv, int n, int* __restrict__ fast_flag,
+    uint32_t* __restrict__ k_params, f16* __restrict__ v_params, const f16* __restrict__ ks,
+    const f16* __restrict__ kb, const f16* __restrict__ vs, const f16* __restrict__ vb) {
     const int NG = D / kGroup;
-    const int nw = D * bits / 32;
-    const int epw = 32 / bits;
-    const uint32_t m = (1u << bits) - 1u;
-    const int64_t total = (int64_t)hkv * n * nw;
+    const int64_t total = (int64_t)hkv * n * NG;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
          i += (int64_t)gridDim.x * blockDim.x) {
-        const int h = (int)(i / ((int64_t)n * nw));
-        const int t = (int)((i / nw) % n);
-        const int w = (int)(i % nw);
-        const int k = t & 7;
-        uint32_t* vblk = v_codes + ((int64_t)h * (cap / 8) + t / 8) * (D * bits / 4);
-        const int64_t row = (int64_t)h * n + t;
-        if (dir == 0) {
-            uint32_t word = 0;
-            for (int e = 0; e < epw; e++) {
-                const int p = v_phys_dim(w * epw + e, D, bits);
-                const uint32_t c = bits == 4 ? (vblk[p] >> (4 * v4_nibble_pos(k))) & m
-                                             : (vblk[2 * p + (k >> 2)] >> (8 * (k & 3))) & m;
-                word |= c << (e * bits);
-            }
-            vc_rows[row * nw + w] = int8 ? word ^ 0x80808080u : word;
-        }
-        if (w < NG) {
-            const int g = w;
-            const int64_t kp = ((int64_t)h * cap + t) * NG + k_param_slot(g, NG);
-            f16* vp = v_params + (((int64_t)h * (cap / 8) + t / 8) * NG + g) * 16;
-            if (int8) {
-                if (dir == 0) {
-                    if (g == 0) {
-                        ks_out[row] = __builtin_bit_cast(half2v, k_params[kp]).x;
-                        vs_rows[row] = vp[k];
-                    }
-                } else {
-                    half2v sb;
-                    sb.x = ks_out[row];
-                    sb.y = (f16)0.0f;
-                    k_params[kp] = __builtin_bit_cast(uint32_t, sb);
-                    vp[k] = vs_rows[row];
-                    vp[8 + k] = (f16)0.0f;
-                }
-            } else if (dir == 0) {
-                const half2v sb = __builtin_bit_cast(half2v, k_params[kp]);
-                ks_out[row * NG + g] = sb.x;
-                kb_out[row * NG + g] = sb.y;
-                vs_rows[row * NG + g] = vp[k];
-                vb_rows[row * NG + g] = vp[8 + k];
-            } else {
-                half2v sb;
-                sb.x = ks_out[row * NG + g];
-                sb.y = kb_out[row * NG + g];
-                k_params[kp] = __builtin_bit_cast(uint32_t, sb);
-                vp[k] = vs_rows[row * NG + g];
-                vp[8 + k] = vb_rows[row * NG + g];
-                check_fast_scale(sb.x, bits, fast_flag);
-                check_fast_scale(vp[k], bits, fast_flag);
-            }
+        const int g = (int)(i % NG);
+        const int64_t row = i / NG;
+        const int h = (int)(row / n), t = (int)(row % n), k = t & 7;
+        f16* vp = v_params + (((int64_t)h * (cap / 8) + t / 8) * NG + g) * 16;
+        half2v sb;
+        sb.x = int8 ? ks[row] : ks[i];
+        sb.y = int8 ? (f16)0.0f : kb[i];
+        k_params[((int64_t)h * cap + t) * NG + k_param_slot(g, NG)] = __builtin_bit_cast(uint32_t, sb);
+        vp[k] = int8 ? vs[row] : vs[i];
+        vp[8 + k] = int8 ? (f16)0.0f : vb[i];
+        if (!int8) {
+            check_fast_scale(sb.x, bits, fast_flag);
+            check_fast_scale(vp[k], bits, fast_flag);
         }
     }
+}
+
+// Export of the affine layouts in one launch: a thread takes 8 dims of the 8 keys of one V
+// block, as fetch_kernel does: V's words turned from 8 keys of a dim to 8 dims of a key, K's
+// copied, and one thread of a group the scales and biases. (As a copy a head and an element-wise kernel,
+// 16387 8-bit rows of 4 heads, D = 256, took 63 us.)
+template <int BITS, int D>
+__global__ __launch_bounds__(256) void export_affine_kernel(const uint32_t* __restrict__ k_codes,
+                                                            const uint32_t* __restrict__ k_params,
+                                                            const uint32_t* __restrict__ v_codes,
+                                                            const f16* __restrict__ v_params, int int8, int cap, int n,
+                                                            uint32_t* __restrict__ kc_out, f16* __restrict__ ks_out,
+                                                            f16* __restrict__ kb_out, uint32_t* __restrict__ vc_out,
+                                                            f16* __restrict__ vs_out, f16* __restrict__ vb_out) {
+    constexpr int OCT = D / 8, NG = D / kGroup, NV = BITS / 2, E = 16 / BITS, KW = BITS / 4;
+    const int h = blockIdx.y, unit = blockIdx.x * 256 + threadIdx.x, oct = unit % OCT, blk = unit / OCT;
+    if (8 * blk >= n) return;
+    const int64_t gblk = (int64_t)h * (cap / 8) + blk;
+    const uint32_t flip = int8 ? 0x80808080u : 0u;
+    u32x4 vc[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) vc[j] = ((const u32x4*)v_codes)[(gblk * D + v_phys_dim(8 * oct + E * j, D, BITS)) / E];
+    uint32_t kc[8][KW];
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+#pragma unroll
+        for (int w = 0; w < KW; w++) kc[k][w] = k_codes[(gblk * 8 + k) * (D * BITS / 32) + oct * KW + w];
+    const int rows = min(8, n - 8 * blk);
+    const int64_t row0 = (int64_t)h * n + 8 * blk;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        if (k >= rows) break;
+        uint32_t v[KW] = {};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const u32x4 w = vc[e / E];
+            if constexpr (BITS == 4)
+                v[0] |= (w[e & 3] >> (4 * v4_nibble_pos(k)) & 0xFu) << (4 * e);
+            else
+                v[e / 4] |= (w[2 * (e & 1) + k / 4] >> (8 * (k & 3)) & 0xFFu) << (8 * (e & 3));
+        }
+#pragma unroll
+        for (int w = 0; w < KW; w++) {
+            kc_out[(row0 + k) * (D * BITS / 32) + oct * KW + w] = kc[k][w] ^ flip;
+            vc_out[(row0 + k) * (D * BITS / 32) + oct * KW + w] = v[w] ^ flip;
+        }
+    }
+    // lane k of a group's 8 threads: the scales and biases of key k (Int8: one scale a row)
+    const int g = oct / 8, k = oct % 8;
+    if (k >= rows) return;
+    const half2v sb = h2(k_params[(gblk * 8 + k) * NG + k_param_slot(g, NG)]);
+    const f16* vp = v_params + (gblk * NG + g) * 16;
+    if (int8) {
+        if (g == 0) {
+            ks_out[row0 + k] = sb.x;
+            vs_out[row0 + k] = vp[k];
+        }
+        return;
+    }
+    ks_out[(row0 + k) * NG + g] = sb.x;
+    kb_out[(row0 + k) * NG + g] = sb.y;
+    vs_out[(row0 + k) * NG + g] = vp[k];
+    vb_out[(row0 + k) * NG + g] = vp[8 + k];
 }
 
 __global__ void set_flag_kernel(int* flag, int v) { *flag = v; }
@@ -959,22 +978,16 @@ int KVCache::export_tensors(void* k_codes, void* k_scales, void* k_biases, void*
         // Same as a full fetch in fp16 mode.
         return dequantize(0, n, k_codes, v_codes, stream);
     }
-    const size_t kr = (size_t)D * bits / 8;
-    for (int h = 0; h < hkv; h++)
-        QW_HIP_CHECK(hipMemcpyAsync((char*)k_codes + h * (size_t)n * kr,
-                                    (const char*)k_data + h * (size_t)cap * kr, n * kr,
-                                    hipMemcpyDeviceToDevice, stream));
-    const int64_t work = (int64_t)hkv * n * (D * bits / 32);
-    const unsigned nb = (unsigned)std::min<int64_t>((work + 255) / 256, 4096);
-    if (int8()) {
-        hipLaunchKernelGGL(flip_code_sign_kernel, dim3(nb), dim3(256), 0, stream,
-                           (uint32_t*)k_codes, hkv, n, D / 4, n);
-        QW_HIP_CHECK(hipGetLastError());
-    }
-    hipLaunchKernelGGL(snapshot_affine_kernel, dim3(nb), dim3(256), 0, stream, 0, bits,
-                       int8() ? 1 : 0, D, cap, hkv, n, fast_flag, k_params, (uint32_t*)v_data,
-                       (f16*)v_params, (f16*)k_scales, (f16*)k_biases, (uint32_t*)v_codes,
-                       (f16*)v_scales, (f16*)v_biases);
+    const dim3 grid((unsigned)(((int64_t)(n + 7) / 8 * (D / 8) + 255) / 256), hkv);
+    auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, (const uint32_t*)k_data, k_params,
+                           (const uint32_t*)v_data, (const f16*)v_params, int8() ? 1 : 0, cap, n, (uint32_t*)k_codes,
+                           (f16*)k_scales, (f16*)k_biases, (uint32_t*)v_codes, (f16*)v_scales, (f16*)v_biases);
+    };
+    if (D == 256)
+        bits == 4 ? launch(export_affine_kernel<4, 256>) : launch(export_affine_kernel<8, 256>);
+    else
+        bits == 4 ? launch(export_affine_kernel<4, 128>) : launch(export_affine_kernel<8, 128>);
     QW_HIP_CHECK(hipGetLastError());
     return QW_OK;
 }
@@ -1009,10 +1022,9 @@ int KVCache::import_tensors(int n_tokens, const void* k_codes, const void* k_sca
                            (uint32_t*)k_data, hkv, n, D / 4, cap);
         QW_HIP_CHECK(hipGetLastError());
     }
-    hipLaunchKernelGGL(snapshot_affine_kernel, dim3(nb), dim3(256), 0, stream, 1, bits,
-                       int8() ? 1 : 0, D, cap, hkv, n, fast_flag, k_params, (uint32_t*)v_data,
-                       (f16*)v_params, (f16*)k_scales, (f16*)k_biases, (uint32_t*)v_codes,
-                       (f16*)v_scales, (f16*)v_biases);
+    hipLaunchKernelGGL(import_params_kernel, dim3(nb), dim3(256), 0, stream, bits, int8() ? 1 : 0, D, cap,
+                       hkv, n, fast_flag, k_params, (f16*)v_params, (const f16*)k_scales,
+                       (const f16*)k_biases, (const f16*)v_scales, (const f16*)v_biases);
     QW_HIP_CHECK(hipGetLastError());
     const int64_t vwork = (int64_t)hkv * ((n + 7) / 8) * D;
     hipLaunchKernelGGL(import_v_codes_kernel,

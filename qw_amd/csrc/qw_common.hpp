@@ -269,6 +269,7 @@ enum Workspace {
     kWsTyped,    // and of the typed one
     kWsShared,   // partials of attention over a shared prefix and tails (attend_shared.hip)
     kWsRowSums,  // the rows' softmax statistics for the key weights (key_weights.hip)
+    kWsSelect,   // an eviction's digit counts (evict.hip)
     kWsEvict,    // the rows that an eviction in place moves (evict.hip)
     kWorkspaces
 };
