@@ -274,34 +274,55 @@ struct RowsCopy {
     const int32_t* kept;     // [hkv][n]
     const int* flag;         // the source's fast flag, copied where flag_to is not null
     int* flag_to;
-    int n, cap, cap_to, D, kp_words;  // kp_words: words of a K row's params
+    int n, cap, cap_to, groups_v, kp_words;  // kp_words: words of a K row's params
     int row_major_v;         // Turbo4: V rows like K's, one params word a row
 };
 
-// BITS: of a code (or 16). A thread copies a 16-byte piece of a block's 8 rows of one plane:
-// grid (pieces of all blocks / 256, hkv, plane). All its loads are issued before the first is used.
-template <int BITS>
+// BITS: of a code (or 16). Grid (groups, hkv), the first `groups_v` groups V's: a thread takes a
+// 16-byte piece of V of a block's 8 rows, or of K (and of a row-major V) the same piece of each of
+// the 8 rows. All its loads are issued before the first is used.
+template <int BITS, int D>
 __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
-    const int pieces = a.D * BITS / 16;  // of a block, in each plane
-    const int id = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
-    if (id == 0 && h == 0 && blockIdx.z == 0 && a.flag_to) *a.flag_to = *a.flag;
-    const int b = id / pieces, pc = id - b * pieces;  // (pieces is a power of two below 2^9, id below 2^31)
+    constexpr int pieces = D * BITS / 16;  // of a block of V
+    const int h = blockIdx.y, group = (int)blockIdx.x;
+    const bool rows_of_v = a.row_major_v && group < a.groups_v;
+    if (group >= a.groups_v || rows_of_v) {
+        constexpr int ppr = pieces / 8;
+        const int id = (group - (rows_of_v ? 0 : a.groups_v)) * 256 + threadIdx.x;
+        const int b = id / ppr, c = id - b * ppr;
+        if (id == 0 && h == 0 && !rows_of_v && a.flag_to) *a.flag_to = *a.flag;
+        if (8 * b >= a.n) return;
+        const u32x4* from = rows_of_v ? a.v : a.k;
+        u32x4* to = rows_of_v ? a.v_to : a.k_to;
+        const uint32_t* pf = rows_of_v ? a.vp : a.kp;
+        uint32_t* pt = rows_of_v ? a.vp_to : a.kp_to;
+        const int32_t* kept = a.kept + (int64_t)h * a.n + 8 * b;
+        const int rows = min(8, a.n - 8 * b), pw = a.row_major_v ? 1 : a.kp_words;
+        const int64_t dst = (int64_t)h * a.cap_to + 8 * b;
+        int64_t src[8];
+        u32x4 x[8];
+        uint32_t p[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) src[k] = (int64_t)h * a.cap + kept[min(k, rows - 1)];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            x[k] = from[src[k] * ppr + c];
+            p[k] = c < pw ? pf[src[k] * pw + c] : 0u;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (k >= rows) break;
+            to[(dst + k) * ppr + c] = x[k];
+            if (c < pw) pt[(dst + k) * pw + c] = p[k];
+        }
+        return;
+    }
+    const int id = group * 256 + threadIdx.x, pc = id % pieces;
+    int b = id / pieces;
+    if constexpr (pieces >= 64) b = __builtin_amdgcn_readfirstlane(b);  // a wave's pieces are one block's: its positions go through scalar loads
     if (8 * b >= a.n) return;
     const int32_t* kept = a.kept + (int64_t)h * a.n + 8 * b;
     const int rows = min(8, a.n - 8 * b);
-    if (blockIdx.z == 0 || a.row_major_v) {
-        const u32x4* from = blockIdx.z == 0 ? a.k : a.v;
-        u32x4* to = blockIdx.z == 0 ? a.k_to : a.v_to;
-        const int ppr = pieces / 8, r = pc / ppr, c = pc - r * ppr;
-        if (r >= rows) return;
-        const int64_t src = (int64_t)h * a.cap + kept[r], dst = (int64_t)h * a.cap_to + 8 * b + r;
-        to[dst * ppr + c] = from[src * ppr + c];
-        const uint32_t* pf = blockIdx.z == 0 ? a.kp : a.vp;
-        uint32_t* pt = blockIdx.z == 0 ? a.kp_to : a.vp_to;
-        const int pw = a.row_major_v ? 1 : a.kp_words;
-        if (c < pw) pt[dst * pw + c] = pf[src * pw + c];
-        return;
-    }
     const int64_t sblk = (int64_t)h * (a.cap / 8), dblk = (int64_t)h * (a.cap_to / 8) + b;
     int t[8];
 #pragma unroll
@@ -422,16 +443,16 @@ int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_str
     c.n = n;
     c.cap = src.cap;
     c.cap_to = staged ? rows8 : dst.cap;
-    c.D = src.D;
     c.kp_words = src.affine() ? src.D / kGroup : src.turbo4() ? 1 : 0;
     c.row_major_v = src.turbo4() ? 1 : 0;
-    const dim3 grid((unsigned)(((int64_t)(rows8 / 8) * (src.D * src.bits / 16) + 255) / 256), src.hkv, 2);
-    if (src.bits == 4)
-        hipLaunchKernelGGL(evict_rows_kernel<4>, grid, dim3(256), 0, stream, c);
-    else if (src.bits == 8)
-        hipLaunchKernelGGL(evict_rows_kernel<8>, grid, dim3(256), 0, stream, c);
+    const int64_t of_v = (int64_t)(rows8 / 8) * (src.D * src.bits / 16), of_k = of_v / 8;  // threads of a head
+    c.groups_v = (int)((src.turbo4() ? of_k + 255 : of_v + 255) / 256);
+    const dim3 grid((unsigned)(c.groups_v + (of_k + 255) / 256), src.hkv);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, c); };
+    if (src.D == 256)
+        src.bits == 4 ? launch(evict_rows_kernel<4, 256>) : src.bits == 8 ? launch(evict_rows_kernel<8, 256>) : launch(evict_rows_kernel<16, 256>);
     else
-        hipLaunchKernelGGL(evict_rows_kernel<16>, grid, dim3(256), 0, stream, c);
+        src.bits == 4 ? launch(evict_rows_kernel<4, 128>) : src.bits == 8 ? launch(evict_rows_kernel<8, 128>) : launch(evict_rows_kernel<16, 128>);
     QW_HIP_CHECK(hipGetLastError());
     if (staged) {
         void* const to[4] = {src.k_data, src.v_data, src.k_params, src.v_params};
