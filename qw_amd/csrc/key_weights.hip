@@ -8,10 +8,14 @@
 // crates/mlxcel-core/src/cache.rs:922) or are trimmed at the end (:2251).
 //
 // p needs the row's whole sum, so K is seen twice: the attention launch leaves each row's
-// maximum and sum, and key_weights_kernel forms the scores again. A wave owns 32 keys: it
+// maximum and sum, and key_weights_kernel forms the scores again. A wave owns 64 keys: it
 // dequantizes their K rows once, into registers as the A operand of S^T = K . Q^T, and runs
-// over the row tiles; a lane keeps its 8 keys' sums over its rows in fp32 and 16 lanes add
-// theirs up at the end. Every key belongs to one wave: no atomics, the same bits each time.
+// over the rows, 32 a step, whose q the workgroup's 8 waves share through LDS (LDS-DMA, the next
+// step's while this one computes). A lane keeps its 16 keys' sums over its rows in fp32 and 16
+// lanes add theirs up at the end. Where the keys alone leave CUs idle the rows are split too, each
+// split's sums to a workspace, added up in order: no atomics, the same bits each time.
+// Bound by the MFMAs and the exponentials beside them (a product-and-sum, an exponential and a
+// product-and-sum a weight).
 #include <algorithm>
 #include <cmath>
 
@@ -27,10 +31,19 @@ struct WeightArgs {
     const float2* row_ml;    // [hkv][R]: the row's maximum (log2 units) and 1 / its sum
     const float* weights;    // [hkv][ws_in] or null
     float* weights_out;      // [hkv][ws_out]
+    float* part;             // [row_splits][hkv][T] where the rows are split
     int64_t ws_in, ws_out;
     int n_weights;           // keys that weights covers
     float decay;
+    int row_splits, rows_per_split;  // (rows_per_split a multiple of kStepRows)
 };
+
+constexpr int kWaveKeys = 64, kWgWaves = 8, kWgKeys = kWaveKeys * kWgWaves, kStepRows = 32;
+
+__device__ __forceinline__ void store_weight(const WeightArgs& w, int h, int key, float x) {
+    if (w.weights && key < w.n_weights) x += w.decay * w.weights[h * w.ws_in + key];
+    w.weights_out[h * w.ws_out + key] = x;
+}
 
 // A row's maximum and 1 / sum over its partials (apart: one logarithm of the sum would round
 // at the maximum's size): grid (R / 4, hkv), a wave a row.
@@ -52,88 +65,177 @@ __global__ __launch_bounds__(256) void row_sums_kernel(SharedArgs a, float2* __r
 }
 
 template <int KIND, int D>
-__global__ __launch_bounds__(256) void key_weights_kernel(WeightArgs w) {
+__global__ __launch_bounds__(64 * kWgWaves) void key_weights_kernel(WeightArgs w) {
     constexpr int NM = D / 32, NG = D / kGroup, DG = D / 4;  // DG: dims of a lane group
+    constexpr int TILE = D * 2 * 16;                         // bytes of 16 rows of q
+    constexpr int KP = DG * KIND / 128;                      // 16-byte pieces of them in a K row
+    __shared__ __attribute__((aligned(16))) char lds[2][2 * TILE];  // [buffer][row tile][D / 8 chunks][16 rows]
     const SharedSegment& c = w.s.seg[1];
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4, h = blockIdx.y;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int key0 = (blockIdx.x * 4 + wave) * 32, T = c.T;
-    if (key0 >= T) return;
+    const int T = c.T, G = w.s.G, Tq = w.s.Tq, R = w.s.R;
+    const int key0 = blockIdx.x * kWgKeys + wave * kWaveKeys;
+    const bool live = key0 < T;
     const uint32_t magic = vconst(kMagic);
-    // A operand: lane (g, r16) holds dims DG g .. + DG - 1 of key 8 (r16 >> 2) + 4 tt + (r16 & 3),
-    // so that a lane of S^T gets keys 8 g + e of row r16
-    half8 ka[2][NM];
+    // A operands: lane (g, r16) holds dims DG g .. + DG - 1 of key 32 u + 8 (r16 >> 2) + 4 tt +
+    // (r16 & 3), so that a lane of S^T gets keys 32 u + 8 g + e of row r16
+    half8 ka[2][2][NM];
 #pragma unroll
-    for (int tt = 0; tt < 2; tt++) {
-        const int64_t row = (int64_t)h * c.cap + key0 + 8 * (r16 >> 2) + 4 * tt + (r16 & 3);
-        const u32x4* src = (const u32x4*)(c.k_data + row * (D * KIND / 32) + g * (DG * KIND / 32));
-        u32x4 x[DG * KIND / 128];
+    for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int u = 0; u < DG * KIND / 128; u++) x[u] = src[u];
-        if constexpr (KIND == 16) {
+        for (int tt = 0; tt < 2; tt++) {
+            const int key = min(key0 + 32 * u + 8 * (r16 >> 2) + 4 * tt + (r16 & 3), c.cap - 1);
+            const int64_t row = (int64_t)h * c.cap + key;
+            const u32x4* src = (const u32x4*)(c.k_data + row * (D * KIND / 32) + g * (DG * KIND / 32));
+            u32x4 x[KP];
 #pragma unroll
-            for (int m = 0; m < NM; m++) ka[tt][m] = as_h8(x[m]);
-        } else {
-            const half2v sb = h2(c.k_params[row * NG + k_param_slot(g * DG / kGroup, NG)]);
-            const half2v s = {sb.x, sb.x}, b = {sb.y, sb.y};
-            const PairConsts pc = make_consts<false, KIND>(s, s, s, s, b, b, b, b, c.code_off2);
+            for (int i = 0; i < KP; i++) x[i] = src[i];
+            if constexpr (KIND == 16) {
 #pragma unroll
-            for (int m = 0; m < NM; m++)
-                ka[tt][m] = KIND == 4 ? deq4<false>(x[m / 4][m % 4], pc, magic)
-                                      : deq8<false>(x[m * KIND / 16 % (DG * KIND / 128)][2 * m % 4],
-                                                    x[m * KIND / 16 % (DG * KIND / 128)][2 * m % 4 + 1], pc);
+                for (int m = 0; m < NM; m++) ka[u][tt][m] = as_h8(x[m]);
+            } else {
+                const half2v sb = h2(c.k_params[row * NG + k_param_slot(g * DG / kGroup, NG)]);
+                const half2v s = {sb.x, sb.x}, b = {sb.y, sb.y};
+                const PairConsts pc = make_consts<false, KIND>(s, s, s, s, b, b, b, b, c.code_off2);
+#pragma unroll
+                for (int m = 0; m < NM; m++) {
+                    if constexpr (KIND == 4) {  // dims come as pairs (0,4), (1,5), (2,6), (3,7)
+                        const u32x4 y = __builtin_bit_cast(u32x4, deq4<false>(x[m / 4][m % 4], pc, magic));
+                        ka[u][tt][m] = as_h8(u32x4{__builtin_amdgcn_perm(y.y, y.x, 0x05040100u),
+                                                   __builtin_amdgcn_perm(y.w, y.z, 0x05040100u),
+                                                   __builtin_amdgcn_perm(y.y, y.x, 0x07060302u),
+                                                   __builtin_amdgcn_perm(y.w, y.z, 0x07060302u)});
+                    } else {
+                        ka[u][tt][m] = deq8<false>(x[m / 2][2 * m % 4], x[m / 2][2 * m % 4 + 1], pc);
+                    }
+                }
+            }
         }
-    }
-    const int G = w.s.G, Tq = w.s.Tq, R = w.s.R;
     auto limit = [&](int row) { return c.causal_rows ? T - c.causal_rows + row / G : T - 1; };
-    // the first row tile with a row that sees key0
-    const int first = c.causal_rows ? max(0, key0 - (T - c.causal_rows)) * G / 16 * 16 : 0;
-    float sum[8] = {};
-    for (int row0 = first; row0 < R; row0 += 16) {
-        const int row = row0 + r16, rr = min(row, R - 1);
-        const f16* qrow = w.s.q + ((int64_t)(h * G + rr % G) * Tq + rr / G) * D + DG * g;
-        const float2 ml = w.row_ml[(int64_t)h * R + rr];
-        half8 qb[NM];
+    // rows: the split's, from the first step that holds a row which sees the workgroup's first key
+    const int wg_key0 = blockIdx.x * kWgKeys;
+    const int first = c.causal_rows ? max(0, wg_key0 - (T - c.causal_rows)) * G : 0;
+    const int row_end = min(R, ((int)blockIdx.z + 1) * w.rows_per_split);
+    const int row_begin = max((int)blockIdx.z * w.rows_per_split, first / kStepRows * kStepRows);
+    // q of 32 rows into a buffer: wave i copies chunks 4 j .. + 3 of both row tiles for j = i, i + 8, ..
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)&lds[0][0];
+    auto dma = [&](int row0, int buf) {
 #pragma unroll
-        for (int m = 0; m < NM; m++) {
-            u32x4 x = *(const u32x4*)(qrow + 8 * m);
-            if constexpr (KIND == 4)  // dims in the order of deq4
-                x = u32x4{__builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
-                          __builtin_amdgcn_perm(x.w, x.y, 0x05040100u), __builtin_amdgcn_perm(x.w, x.y, 0x07060302u)};
-            qb[m] = as_h8(x);
+        for (int i = 0; i < 2 * (D / 32) / kWgWaves; i++) {
+            const int j = wave + kWgWaves * i, rt = j / (D / 32), c4 = j % (D / 32);
+            const int row = min(row0 + 16 * rt + r16, R - 1), r = row / G;
+            const f16* src = w.s.q + ((int64_t)(h * G + row - r * G) * Tq + r) * D + 8 * (4 * c4 + g);
+            uint32_t saved;
+            asm volatile(
+                "s_mov_b32 %0, m0\n\t"
+                "s_mov_b32 m0, %2\n\t"
+                "s_nop 0\n\t"
+                "global_load_lds_dwordx4 %1, off\n\t"
+                "s_nop 0\n\t"
+                "s_mov_b32 m0, %0"
+                : "=&s"(saved)
+                : "v"(src), "s"(__builtin_amdgcn_readfirstlane(lds0 + buf * 2 * TILE + rt * TILE + c4 * 1024))
+                : "memory");
         }
-        float4v acc[2] = {float4v{0.f, 0.f, 0.f, 0.f}, float4v{0.f, 0.f, 0.f, 0.f}};
+    };
+    auto stats = [&](int row) {  // (a row past the last: weights of 2^-inf times 0)
+        const float2 ml = w.row_ml[(int64_t)h * R + min(row, R - 1)];
+        return row < R ? ml : float2{INFINITY, 0.0f};
+    };
+    float sum[2][8] = {};
+    float2 ml[2], ml_next[2] = {};
+    if (row_begin < row_end) {
+        dma(row_begin, 0);
 #pragma unroll
-        for (int m = 0; m < NM; m++) {
-            acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[0][m], qb[m], acc[0], 0, 0, 0);
-            acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[1][m], qb[m], acc[1], 0, 0, 0);
+        for (int rt = 0; rt < 2; rt++) ml_next[rt] = stats(row_begin + 16 * rt + r16);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int row0 = row_begin; row0 < row_end; row0 += kStepRows) {
+        const int buf = (row0 - row_begin) / kStepRows & 1;
+#pragma unroll
+        for (int rt = 0; rt < 2; rt++) ml[rt] = ml_next[rt];
+        if (row0 + kStepRows < row_end) {
+            dma(row0 + kStepRows, buf ^ 1);
+#pragma unroll
+            for (int rt = 0; rt < 2; rt++) ml_next[rt] = stats(row0 + kStepRows + 16 * rt + r16);
         }
-        const int lim = limit(rr);
+        if (live) {
+#pragma unroll
+            for (int rt = 0; rt < 2; rt++) {
+                const half8* q8 = (const half8*)(lds[buf] + rt * TILE) + (DG / 8) * 16 * g + r16;
+                float4v acc[2][2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) acc[u][0] = acc[u][1] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int m = 0; m < NM; m++) {
+                    const half8 qb = q8[16 * m];
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int tt = 0; tt < 2; tt++)
+                            acc[u][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[u][tt][m], qb, acc[u][tt], 0, 0, 0);
+                }
+                auto weight = [&](int u, int e) {
+                    return __builtin_amdgcn_exp2f(__builtin_fmaf(acc[u][e >> 2][e & 3], w.s.scale2, -ml[rt].x));
+                };
+                // the tile's first row's limit decides whether any key of the wave is hidden in it
+                if (limit(row0 + 16 * rt) < key0 + kWaveKeys - 1) {
+                    const int lim = limit(row0 + 16 * rt + r16);
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            if (key0 + 32 * u + 8 * g + e <= lim) sum[u][e] = __builtin_fmaf(weight(u, e), ml[rt].y, sum[u][e]);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) sum[u][e] = __builtin_fmaf(weight(u, e), ml[rt].y, sum[u][e]);
+                }
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+    if (!live) return;
+#pragma unroll
+    for (int u = 0; u < 2; u++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const float p = __builtin_amdgcn_exp2f(acc[e >> 2][e & 3] * w.s.scale2 - ml.x) * ml.y;
-            if (key0 + 8 * g + e <= lim && row < R) sum[e] += p;
+            float x = sum[u][e];
+            x += lane_xor<1>(x, lane);
+            x += lane_xor<2>(x, lane);
+            x += lane_xor<4>(x, lane);
+            x += lane_xor<8>(x, lane);
+            const int key = key0 + 32 * u + 8 * g + e;
+            if (r16 != e + 8 * u || key >= T) continue;
+            if (w.row_splits > 1)
+                w.part[((int64_t)blockIdx.z * w.s.hkv + h) * T + key] = x;
+            else
+                store_weight(w, h, key, x);
         }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        float x = sum[e];
-        x += lane_xor<1>(x, lane);
-        x += lane_xor<2>(x, lane);
-        x += lane_xor<4>(x, lane);
-        x += lane_xor<8>(x, lane);
-        const int key = key0 + 8 * g + e;
-        if (r16 == e && key < T) {
-            if (w.weights && key < w.n_weights) x += w.decay * w.weights[h * w.ws_in + key];
-            w.weights_out[h * w.ws_out + key] = x;
-        }
-    }
+}
+
+// The row splits' sums, in order.
+__global__ __launch_bounds__(256) void add_weights_kernel(WeightArgs w) {
+    const int T = w.s.seg[1].T, key = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+    if (key >= T) return;
+    float x = 0.0f;
+    for (int i = 0; i < w.row_splits; i++) x += w.part[((int64_t)i * w.s.hkv + h) * T + key];
+    store_weight(w, h, key, x);
 }
 
 template <int KIND, int D>
 int launch_weights(const WeightArgs& w, hipStream_t stream) {
-    hipLaunchKernelGGL((key_weights_kernel<KIND, D>), dim3((w.s.seg[1].T + 127) / 128, w.s.hkv), dim3(256), 0, stream, w);
+    const int T = w.s.seg[1].T;
+    hipLaunchKernelGGL((key_weights_kernel<KIND, D>), dim3((T + kWgKeys - 1) / kWgKeys, w.s.hkv, w.row_splits),
+                       dim3(64 * kWgWaves), 0, stream, w);
     QW_HIP_CHECK(hipGetLastError());
+    if (w.row_splits > 1) {
+        hipLaunchKernelGGL(add_weights_kernel, dim3((T + 255) / 256, w.s.hkv), dim3(256), 0, stream, w);
+        QW_HIP_CHECK(hipGetLastError());
+    }
     return QW_OK;
 }
 
@@ -170,8 +272,16 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
     WeightArgs w;
     if (int rc = plan_shared(nullptr, &c, q, 1, n_rows, n_q_heads / c.hkv, c.hkv, nullptr, scale, causal, out, stream, &w.s))
         return rc;
+    // row splits: about one workgroup a CU, of at least four steps each
+    const int groups = (c.offset + kWgKeys - 1) / kWgKeys * c.hkv, steps = (w.s.R + kStepRows - 1) / kStepRows;
+    w.row_splits = std::max(1, std::min({256 / groups, steps / 4, 64}));
+    w.rows_per_split = (steps + w.row_splits - 1) / w.row_splits * kStepRows;
+    w.row_splits = (w.s.R + w.rows_per_split - 1) / w.rows_per_split;
+    const size_t ml_bytes = (size_t)c.hkv * w.s.R * sizeof(float2);
+    const size_t part_bytes = w.row_splits > 1 ? (size_t)w.row_splits * c.hkv * c.offset * sizeof(float) : 0;
     void* row_ml = nullptr;
-    if (int rc = workspace(kWsRowSums, c.device, stream, (size_t)c.hkv * w.s.R * sizeof(float2), &row_ml)) return rc;
+    if (int rc = workspace(kWsRowSums, c.device, stream, ml_bytes + part_bytes, &row_ml)) return rc;
+    w.part = (float*)((char*)row_ml + ml_bytes);
     if (int rc = launch_shared(nullptr, &c, w.s, stream)) return rc;
     if (int rc = launch_shared_merge(c.D, w.s, stream)) return rc;
     w.row_ml = (const float2*)row_ml;
