@@ -40,7 +40,7 @@ namespace qw {
 
 namespace {
 
-constexpr int kWaves = 8;
+constexpr int kWaves = 8, kFewRows = 16;
 
 // KIND: 16, 8 (affine and Int8) or 4 bits.
 template <int KIND, int D, bool FAST>
@@ -360,58 +360,240 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds) {
                 *(float4v*)(o + c) = float4v{acc_o[c][e], acc_o[c + 1][e], acc_o[c + 2][e], acc_o[c + 3][e]};
         }
     }
-#undef QW_SEG
 }
+
+// Units of at most 16 rows: nothing to share through LDS, so each wave reads 32-key chunks of its
+// own (chunk c of the unit's keys to wave c mod 8) straight into MFMA operands - K rows as A, a lane
+// (g, r16) taking dims D/4 g .. of its key, V's 8-key blocks as B - and requests the next chunk's K
+// once this one's scores are formed, its V once this one's P . V is. Bound by HBM latency and
+// bandwidth; the waves' sums join through LDS.
+template <int KIND, int D, bool FAST>
+__device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
+    constexpr int NM = D / 32, NT = D / 16, NG = D / kGroup, DG = D / 4, DPL = D / 16;
+    constexpr int KP = DG * KIND / 128, VP = DPL * KIND / 16, E = 16 / KIND;  // 16-byte pieces a lane; dims a piece of V
+    const bool is_tail = (int)blockIdx.x >= a.seg[0].n_units;
+    const int u_id = (int)blockIdx.x - (is_tail ? a.seg[0].n_units : 0);
+    const int n_split = QW_SEG(n_split), heads = QW_SEG(heads), T = QW_SEG(T), cap = QW_SEG(cap);
+    const int sp = u_id % n_split, hc = u_id / n_split;
+    const int h = hc % a.hkv, rows = QW_SEG(rows), row_base = hc / a.hkv * rows;
+    (void)heads;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const uint32_t magic = vconst(kMagic);
+    const int causal_rows = QW_SEG(causal_rows);
+    int lo = 0;
+    if (is_tail && a.starts) lo = min(max(a.starts[hc / a.hkv], 0), T);
+    const bool row_ok = r16 < rows;
+    const int rr = row_ok ? r16 : 0, lim = !row_ok ? -1 : causal_rows ? T - causal_rows + rr / a.G : T - 1;
+    const int first_lim = causal_rows ? T - causal_rows : T - 1;
+    constexpr int KT = BlockShape<D>::KT;
+    const int keys = QW_SEG(tiles_per_split) * KT, k_begin = lo / 32 * 32 + sp * keys, k_end = min(T, k_begin + keys);
+    half8 qb[NM];
+    {
+        const int seq = (row_base + rr) / (a.Tq * a.G), x = (row_base + rr) % (a.Tq * a.G);
+        const f16* qrow = a.q + (((int64_t)seq * a.hkv * a.G + h * a.G + x % a.G) * a.Tq + x / a.G) * D + DG * g;
+#pragma unroll
+        for (int m = 0; m < NM; m++) {
+            u32x4 w = *(const u32x4*)(qrow + 8 * m);
+            if (!row_ok) w = u32x4{0, 0, 0, 0};
+            if constexpr (KIND == 4)  // dims in deq4's order
+                w = u32x4{__builtin_amdgcn_perm(w.z, w.x, 0x05040100u), __builtin_amdgcn_perm(w.z, w.x, 0x07060302u),
+                          __builtin_amdgcn_perm(w.w, w.y, 0x05040100u), __builtin_amdgcn_perm(w.w, w.y, 0x07060302u)};
+            qb[m] = as_h8(w);
+        }
+    }
+    const uint32_t code_off = QW_SEG(code_off2);
+    const int64_t krow0 = (int64_t)hc * cap + 8 * (r16 >> 2) + (r16 & 3), vblk0 = (int64_t)hc * (cap / 8) + g;
+    const u32x4* const ksrc = (const u32x4*)(QW_SEG(k_data) + krow0 * (D * KIND / 32) + g * (DG * KIND / 32));
+    const uint32_t* const kpsrc = KIND == 16 ? nullptr : QW_SEG(k_params) + krow0 * NG + k_param_slot(g * DG / kGroup, NG);
+    const u32x4* const vsrc = (const u32x4*)(QW_SEG(v_data) + vblk0 * (D * KIND / 4)) + r16;
+    const u32x4* const vpsrc =
+        KIND == 16 ? nullptr : (const u32x4*)(QW_SEG(v_params) + (vblk0 * NG + r16 * DPL / kGroup) * 8);
+    u32x4 kc[2][KP], vc[VP], vp[2];
+    uint32_t kp[2];
+    auto load_k = [&](int key) {
+#pragma unroll
+        for (int tt = 0; tt < 2; tt++) {
+#pragma unroll
+            for (int i = 0; i < KP; i++) kc[tt][i] = ksrc[(int64_t)(key + 4 * tt) * (D * KIND / 128) + i];
+            if constexpr (KIND != 16) kp[tt] = kpsrc[(int64_t)(key + 4 * tt) * NG];
+        }
+    };
+    auto load_v = [&](int key) {
+        // piece j holds slots 16 E j + E n ..: dims DPL n + E j .. of column n
+#pragma unroll
+        for (int j = 0; j < VP; j++) vc[j] = vsrc[(int64_t)(key / 8) * (D * KIND / 16) + 16 * j];
+        if constexpr (KIND != 16) {
+            vp[0] = vpsrc[(int64_t)(key / 8) * (NG * 2)];
+            vp[1] = vpsrc[(int64_t)(key / 8) * (NG * 2) + 1];
+        }
+    };
+    float m_run = -INFINITY, l_run = 0.0f;
+    float4v acc_o[NT];
+#pragma unroll
+    for (int mm = 0; mm < NT; mm++) acc_o[mm] = float4v{0.f, 0.f, 0.f, 0.f};
+    int key = k_begin + 32 * wave;
+    if (key < k_end) {
+        load_k(key);
+        load_v(key);
+    }
+    for (; key < k_end; key += 32 * kWaves) {
+        const bool more = key + 32 * kWaves < k_end;
+        float4v acc[2] = {float4v{0.f, 0.f, 0.f, 0.f}, float4v{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int tt = 0; tt < 2; tt++) {
+            PairConsts pc;
+            if constexpr (KIND != 16) {
+                const half2v sb = h2(kp[tt]), s = {sb.x, sb.x}, b = {sb.y, sb.y};
+                pc = make_consts<FAST, KIND>(s, s, s, s, b, b, b, b, code_off);
+            }
+#pragma unroll
+            for (int m = 0; m < NM; m++) {
+                half8 ka;
+                if constexpr (KIND == 16)
+                    ka = as_h8(kc[tt][m]);
+                else if constexpr (KIND == 8)
+                    ka = deq8<FAST>(kc[tt][m / 2][2 * m % 4], kc[tt][m / 2][2 * m % 4 + 1], pc);
+                else
+                    ka = deq4<FAST>(kc[tt][m / 4][m % 4], pc, magic);
+                acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qb[m], acc[tt], 0, 0, 0);
+            }
+        }
+        if (more) load_k(key + 32 * kWaves);
+        float s[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) s[e] = acc[e >> 2][e & 3] * a.scale2;
+        if (a.scores && row_ok) {
+            float4v* to = (float4v*)(a.scores + ((int64_t)h * a.R + row_base + r16) * a.score_stride + key + 8 * g);
+            to[0] = float4v{s[0], s[1], s[2], s[3]};
+            to[1] = float4v{s[4], s[5], s[6], s[7]};
+        }
+        const bool edge = key < lo || key + 31 > first_lim;
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (key + 8 * g + e > lim || key + 8 * g + e < lo) s[e] = -INFINITY;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) mx = fmaxf(mx, s[e]);
+        if (__any(mx > m_run)) {
+            const float m_new = fmaxf(m_run, wave_max_g(mx));
+            const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+            l_run *= alpha;
+            float f[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) f[e] = __shfl(alpha, 4 * g + e);
+#pragma unroll
+            for (int mm = 0; mm < NT; mm++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc_o[mm][e] *= f[e];
+            m_run = m_new;
+        }
+        const float mref = m_run == -INFINITY ? 0.0f : m_run;
+        half8 p16;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float p = __builtin_amdgcn_exp2f(s[e] - mref);
+            l_run += p;
+            p16[e] = (f16)p;
+        }
+        PairConsts pc;
+        if constexpr (KIND != 16)
+            pc = make_consts<FAST, KIND>(h2(vp[0][0]), h2(vp[0][1]), h2(vp[0][2]), h2(vp[0][3]), h2(vp[1][0]), h2(vp[1][1]),
+                                         h2(vp[1][2]), h2(vp[1][3]), code_off);
+        const u32x4 keep = keep_keys(T - (key + 8 * g)) & ~keep_keys(lo - (key + 8 * g));
+#pragma unroll
+        for (int j = 0; j < VP; j++) {
+            half8 y[E];
+#pragma unroll
+            for (int i = 0; i < E; i++)
+                y[i] = KIND == 16  ? as_h8(vc[j])
+                       : KIND == 8 ? deq8<FAST>(vc[j][2 * i % 4], vc[j][(2 * i + 1) % 4], pc)
+                                   : deq4<FAST>(vc[j][i % 4], pc, magic);
+            if (edge) {  // hidden keys have weight 0, but 0 x inf is NaN
+#pragma unroll
+                for (int i = 0; i < E; i++) y[i] = as_h8(__builtin_bit_cast(u32x4, y[i]) & keep);
+            }
+#pragma unroll
+            for (int i = 0; i < E; i++)
+                acc_o[E * j + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p16, y[i], acc_o[E * j + i], 0, 0, 0);
+        }
+        if (more) load_v(key + 32 * kWaves);
+    }
+    // the waves' sums against one maximum: m of all waves, then O and l rescaled, parked, added up
+    float* const s_m = (float*)lds;                    // [8 waves][16 rows]
+    float* const s_l = s_m + 16 * kWaves;              // [8][16]
+    float* const s_o = s_l + 16 * kWaves;              // [8][rows][D]
+    static_assert((16 * kWaves * 2 + kWaves * 16 * D) * 4 <= 2 * BlockShape<D>::BUF, "the waves' sums fit the tile buffers");
+    if (g == 0) s_m[16 * wave + r16] = m_run;
+    __syncthreads();
+    float M = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < kWaves; v++) M = fmaxf(M, s_m[16 * v + r16]);
+    const float f = __builtin_amdgcn_exp2f(m_run - (M == -INFINITY ? 0.0f : M));
+    const float l = wave_sum_g(l_run) * f;
+    if (g == 0) s_l[16 * wave + r16] = l;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float fe = __shfl(f, 4 * g + e);
+        if (4 * g + e >= rows) continue;
+        float* o = s_o + (wave * rows + 4 * g + e) * D + NT * r16;
+#pragma unroll
+        for (int c = 0; c < NT; c += 4)
+            *(float4v*)(o + c) = float4v{acc_o[c][e] * fe, acc_o[c + 1][e] * fe, acc_o[c + 2][e] * fe, acc_o[c + 3][e] * fe};
+    }
+    __syncthreads();
+    const int64_t pbase = ((int64_t)(QW_SEG(slot0) + sp) * a.hkv + h) * a.R + row_base;
+    for (int i = tid; i < rows * (D / 4); i += 64 * kWaves) {
+        const int row = i / (D / 4), c = i % (D / 4);
+        float4v o = {0.f, 0.f, 0.f, 0.f};
+        float lr = 0.0f, mr = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < kWaves; v++) {
+            const float4v x = *(const float4v*)(s_o + (v * rows + row) * D + 4 * c);
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] += x[j];
+            lr += s_l[16 * v + row];
+            mr = fmaxf(mr, s_m[16 * v + row]);
+        }
+        if (c == 0) a.part_ml[pbase + row] = float2{mr, lr};
+        if (a.n_slots == 1) {
+            const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+            const int seq = (row_base + row) / (a.Tq * a.G), x = (row_base + row) % (a.Tq * a.G);
+            half4v y;
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = (f16)(o[j] * inv);
+            *(half4v*)(a.out + (((int64_t)seq * a.hkv * a.G + h * a.G + x % a.G) * a.Tq + x / a.G) * D + 4 * c) = y;
+        } else {
+            *(float4v*)(a.part_o + (pbase + row) * D + 4 * c) = o;
+        }
+    }
+}
+
+template <int KIND, int D, bool FAST>
+__device__ __forceinline__ void unit_body(const SharedArgs& a, char* lds) {
+    if (((int)blockIdx.x >= a.seg[0].n_units ? a.seg[1].rows : a.seg[0].rows) <= kFewRows)
+        few_body<KIND, D, FAST>(a, lds);
+    else
+        shared_body<KIND, D, FAST>(a, lds);
+}
+#undef QW_SEG
 
 template <int KIND, int D>
 __global__ __launch_bounds__(64 * kWaves, 1) void shared_attend_kernel(SharedArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const bool fast = KIND != 16 && *((int)blockIdx.x >= a.seg[0].n_units ? a.seg[1].fast_flag : a.seg[0].fast_flag);
     if constexpr (KIND != 16)
-        if (fast) return shared_body<KIND, D, true>(a, lds);
-    shared_body<KIND, D, false>(a, lds);
+        if (fast) return unit_body<KIND, D, true>(a, lds);
+    unit_body<KIND, D, false>(a, lds);
 }
 
-// Joins a row's partials: grid (R, hkv), D / 4 threads a partial row, 1024 / D partial rows
-// at a time, their sums joined through LDS.
 template <int D>
 __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
-    constexpr int LPR = D / 4, NS = 256 / LPR;  // threads a partial row, partial rows at a time
-    __shared__ float4v sO[256];
-    __shared__ float sL[NS];
-    const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, c = tid % LPR, s0 = tid / LPR;
-    const int64_t stride = (int64_t)a.hkv * a.R, at = (int64_t)h * a.R + row;
-    float M = -INFINITY;
-    for (int s = tid & 63; s < a.n_slots; s += 64) M = fmaxf(M, a.part_ml[s * stride + at].x);
-    M = wave_reduce(M, OpMax{});
-    const float mr = M == -INFINITY ? 0.0f : M;
-    float4v o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.0f;
-    for (int s = s0; s < a.n_slots; s += NS) {
-        const float2 ml = a.part_ml[s * stride + at];
-        const float4v x = *(const float4v*)(a.part_o + (s * stride + at) * D + 4 * c);
-        const float f = __builtin_amdgcn_exp2f(ml.x - mr);
-        l += f * ml.y;
-#pragma unroll
-        for (int j = 0; j < 4; j++) o[j] += f * x[j];
-    }
-    sO[tid] = o;
-    if (c == 0) sL[s0] = l;
-    __syncthreads();
-    if (s0 > 0) return;
-#pragma unroll
-    for (int s = 1; s < NS; s++) {
-        const float4v x = sO[s * LPR + c];
-#pragma unroll
-        for (int j = 0; j < 4; j++) o[j] += x[j];
-        l += sL[s];
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int seq = row / (a.Tq * a.G), rr = row % (a.Tq * a.G);
-    half4v y;
-#pragma unroll
-    for (int j = 0; j < 4; j++) y[j] = (f16)(o[j] * inv);
-    *(half4v*)(a.out + (((int64_t)seq * a.hkv * a.G + h * a.G + rr % a.G) * a.Tq + rr / a.G) * D + 4 * c) = y;
+    __shared__ SharedMerge<D> sm;
+    merge_row<D>(a, blockIdx.x, blockIdx.y, sm);
 }
 
 // What a launch of a prefix and tail units costs on 256 CUs, in key tiles: prefix units of a

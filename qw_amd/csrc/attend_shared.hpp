@@ -32,6 +32,8 @@ struct SharedArgs {
     const int32_t* starts;  // [n_seq] or null: a sequence's first tail key
     int Tq, G, hkv, R;      // R = n_seq * Tq * G: row (b * Tq + r) * G + head in group
     int n_slots;
+    float* scores;          // null, or [hkv][R][score_stride]: the scores (log2 units) of one cache's few rows
+    int64_t score_stride;   // a multiple of 32
     float scale2;           // scale * log2 e
     SharedSegment seg[2];   // the prefix, the tails
 };
@@ -43,5 +45,60 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int 
                 const int32_t* starts, float scale, bool causal, void* out, hipStream_t stream, SharedArgs* a);
 int launch_shared(const KVCache* prefix, const KVCache* tails, const SharedArgs& a, hipStream_t stream);
 int launch_shared_merge(int D, const SharedArgs& a, hipStream_t stream);
+
+// A row's partials joined by a workgroup of 256: D / 4 threads a partial row, 1024 / D partial rows
+// at a time and four such in flight, their sums over LDS.
+template <int D>
+struct SharedMerge {
+    float4v o[256];
+    float l[1024 / D];
+};
+template <int D>
+__device__ __forceinline__ void merge_row(const SharedArgs& a, int row, int h, SharedMerge<D>& sm) {
+    constexpr int LPR = D / 4, NS = 256 / LPR, AHEAD = 4;
+    const int tid = threadIdx.x, c = tid % LPR, s0 = tid / LPR;
+    const int64_t stride = (int64_t)a.hkv * a.R, at = (int64_t)h * a.R + row;
+    float M = -INFINITY;
+    for (int s = tid & 63; s < a.n_slots; s += 64) M = fmaxf(M, a.part_ml[s * stride + at].x);
+    M = wave_reduce(M, OpMax{});
+    const float mr = M == -INFINITY ? 0.0f : M;
+    float4v o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.0f;
+    for (int s = s0; s < a.n_slots; s += NS * AHEAD) {
+        float2 ml[AHEAD];
+        float4v x[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const int64_t p = min(s + NS * i, a.n_slots - 1) * stride + at;
+            ml[i] = a.part_ml[p];
+            x[i] = *(const float4v*)(a.part_o + p * D + 4 * c);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            if (s + NS * i >= a.n_slots) break;
+            const float f = __builtin_amdgcn_exp2f(ml[i].x - mr);
+            l += f * ml[i].y;
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] += f * x[i][j];
+        }
+    }
+    sm.o[tid] = o;
+    if (c == 0) sm.l[s0] = l;
+    __syncthreads();
+    if (s0 > 0) return;
+#pragma unroll
+    for (int s = 1; s < NS; s++) {
+        const float4v x = sm.o[s * LPR + c];
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] += x[j];
+        l += sm.l[s];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int seq = row / (a.Tq * a.G), rr = row % (a.Tq * a.G);
+    half4v y;
+#pragma unroll
+    for (int j = 0; j < 4; j++) y[j] = (f16)(o[j] * inv);
+    *(half4v*)(a.out + (((int64_t)seq * a.hkv * a.G + h * a.G + rr % a.G) * a.Tq + rr / a.G) * D + 4 * c) = y;
+}
 
 }  // namespace qw

@@ -7,8 +7,10 @@
 // The reference's runtime has no such call; its caches only grow (KVCache::update,
 // crates/mlxcel-core/src/cache.rs:922) or are trimmed at the end (:2251).
 //
-// p needs the row's whole sum, so K is seen twice: the attention launch leaves each row's
-// maximum and sum, and key_weights_kernel forms the scores again. A wave owns 64 keys: it
+// p needs the row's whole sum. Up to 16 rows a KV head the attention launch keeps its scores
+// (4 bytes a row and key, where K again would be 144 to 512 a key) and finish_few_kernel turns them
+// into weights beside the merge. For more rows K is seen twice: the attention launch leaves each
+// row's maximum and sum, and key_weights_kernel forms the scores again. A wave owns 64 keys: it
 // dequantizes their K rows once, into registers as the A operand of S^T = K . Q^T, and runs
 // over the rows, 32 a step, whose q the workgroup's 8 waves share through LDS (LDS-DMA, the next
 // step's while this one computes). A lane keeps its 16 keys' sums over its rows in fp32 and 16
@@ -226,6 +228,60 @@ __global__ __launch_bounds__(256) void add_weights_kernel(WeightArgs w) {
     store_weight(w, h, key, x);
 }
 
+// Few rows (the attention launch kept their scores): the rows merged by the first R workgroups of
+// a head and the keys' weights formed by the others, 1024 keys each, from the scores and the rows'
+// statistics, which every one of them joins for itself.
+template <int D>
+__global__ __launch_bounds__(256) void finish_few_kernel(WeightArgs w, int n_merge) {
+    __shared__ SharedMerge<D> sm;
+    __shared__ float2 s_ml[16];
+    const int h = blockIdx.y, tid = threadIdx.x, R = w.s.R, T = w.s.seg[1].T;
+    if ((int)blockIdx.x < n_merge) {
+        merge_row<D>(w.s, blockIdx.x, h, sm);
+        return;
+    }
+    {
+        const int row = min(tid / 16, R - 1), i16 = tid % 16;  // 16 lanes a row
+        const int64_t stride = (int64_t)w.s.hkv * R, at = (int64_t)h * R + row;
+        float M = -INFINITY, l = 0.0f;
+        for (int s = i16; s < w.s.n_slots; s += 16) M = fmaxf(M, w.s.part_ml[s * stride + at].x);
+        const int lane = tid & 63;
+        M = fmaxf(M, lane_xor<1>(M, lane));
+        M = fmaxf(M, lane_xor<2>(M, lane));
+        M = fmaxf(M, lane_xor<4>(M, lane));
+        M = fmaxf(M, lane_xor<8>(M, lane));
+        const float mr = M == -INFINITY ? 0.0f : M;
+        for (int s = i16; s < w.s.n_slots; s += 16) {
+            const float2 ml = w.s.part_ml[s * stride + at];
+            l += __builtin_amdgcn_exp2f(ml.x - mr) * ml.y;
+        }
+        l += lane_xor<1>(l, lane);
+        l += lane_xor<2>(l, lane);
+        l += lane_xor<4>(l, lane);
+        l += lane_xor<8>(l, lane);
+        if (i16 == 0) s_ml[tid / 16] = float2{mr, l == 0.0f ? 0.0f : 1.0f / l};
+    }
+    __syncthreads();
+    const int key = ((int)blockIdx.x - n_merge) * 1024 + 4 * tid;
+    if (key >= T) return;
+    const int causal = w.s.seg[1].causal_rows, first_lim = causal ? T - causal : T - 1;
+    float sum[4] = {};
+    const float* sc = w.s.scores + (int64_t)h * R * w.s.score_stride + key;
+    for (int row = 0; row < R; row++) {
+        const float4v s = *(const float4v*)(sc + row * w.s.score_stride);
+        const float2 ml = s_ml[row];
+        const int lim = causal ? first_lim + row / w.s.G : first_lim;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float p = __builtin_amdgcn_exp2f(s[e] - ml.x) * ml.y;
+            sum[e] += key + e <= lim ? p : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (key + e < T) store_weight(w, h, key + e, sum[e]);
+}
+
 template <int KIND, int D>
 int launch_weights(const WeightArgs& w, hipStream_t stream) {
     const int T = w.s.seg[1].T;
@@ -272,6 +328,28 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
     WeightArgs w;
     if (int rc = plan_shared(nullptr, &c, q, 1, n_rows, n_q_heads / c.hkv, c.hkv, nullptr, scale, causal, out, stream, &w.s))
         return rc;
+    w.weights = decay > 0.0f ? weights : nullptr;
+    w.weights_out = weights_out;
+    w.ws_in = weights_stride;
+    w.ws_out = weights_out_stride;
+    w.n_weights = n_weights;
+    w.decay = decay;
+    if (w.s.R <= 16) {
+        w.s.score_stride = ((int64_t)c.offset + 31) / 32 * 32;
+        void* scores = nullptr;
+        if (int rc = workspace(kWsRowSums, c.device, stream, (size_t)c.hkv * w.s.R * w.s.score_stride * sizeof(float), &scores))
+            return rc;
+        w.s.scores = (float*)scores;
+        if (int rc = launch_shared(nullptr, &c, w.s, stream)) return rc;
+        const int n_merge = w.s.n_slots > 1 ? w.s.R : 0;
+        const dim3 grid(n_merge + (c.offset + 1023) / 1024, c.hkv);
+        if (c.D == 256)
+            hipLaunchKernelGGL(finish_few_kernel<256>, grid, dim3(256), 0, stream, w, n_merge);
+        else
+            hipLaunchKernelGGL(finish_few_kernel<128>, grid, dim3(256), 0, stream, w, n_merge);
+        QW_HIP_CHECK(hipGetLastError());
+        return QW_OK;
+    }
     // row splits: about one workgroup a CU, of at least four steps each
     const int groups = (c.offset + kWgKeys - 1) / kWgKeys * c.hkv, steps = (w.s.R + kStepRows - 1) / kStepRows;
     w.row_splits = std::max(1, std::min({256 / groups, steps / 4, 64}));
@@ -285,12 +363,6 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
     if (int rc = launch_shared(nullptr, &c, w.s, stream)) return rc;
     if (int rc = launch_shared_merge(c.D, w.s, stream)) return rc;
     w.row_ml = (const float2*)row_ml;
-    w.weights = decay > 0.0f ? weights : nullptr;
-    w.weights_out = weights_out;
-    w.ws_in = weights_stride;
-    w.ws_out = weights_out_stride;
-    w.n_weights = n_weights;
-    w.decay = decay;
     hipLaunchKernelGGL(row_sums_kernel, dim3((w.s.R + 3) / 4, c.hkv), dim3(256), 0, stream, w.s, (float2*)row_ml);
     QW_HIP_CHECK(hipGetLastError());
     if (c.D == 256)
