@@ -30,6 +30,7 @@
 // quarters of each tile's keys and join them through LDS.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "attend_shared.hpp"
 #include "block_tile.hpp"
@@ -40,324 +41,404 @@ namespace qw {
 
 namespace {
 
-constexpr int kWaves = 8, kFewRows = 16;
+constexpr int kWaves = 8, kFillWaves = 4;
+constexpr int kFewRows = 16;  // of a unit of the kernel for few rows
+// 16-row tiles a computing wave of the other: what 168 registers hold (three waves a SIMD).
+__host__ __device__ constexpr int many_tiles(int D) { return D == 256 ? 1 : 2; }
 
-// KIND: 16, 8 (affine and Int8) or 4 bits.
-template <int KIND, int D, bool FAST>
-__device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds) {
-    using S = BlockShape<D>;
-    constexpr int KT = S::KT, NSUB = S::NSUB, NM = S::NM, NT = S::NT, NG = S::NG;
-    constexpr int TPR = S::TPR, LTPR = S::LTPR, TPB = S::TPB, BUF = S::BUF, KBUF = S::KBUF, VROW = S::VROW;
-    constexpr int KU = KIND / 4;               // 16-byte loads of a 32-dim K slice / 4-slot V slice
-    constexpr int NST = 2;                     // register stages: tiles of codes in flight
-    static_assert(KT * TPR == 64 * kWaves && (KT / 8) * TPB == 64 * kWaves, "a slice of each kind a thread");
-    // ---- the unit: a split of a query tile of a head of one of the two caches
-    const bool is_tail = (int)blockIdx.x >= a.seg[0].n_units;
-    const int u_id = (int)blockIdx.x - (is_tail ? a.seg[0].n_units : 0);
-#define QW_SEG(f) (is_tail ? a.seg[1].f : a.seg[0].f)
-    const int n_split = QW_SEG(n_split), heads = QW_SEG(heads), T = QW_SEG(T), cap = QW_SEG(cap);
-    const int sp = u_id % n_split, hc = u_id / n_split % heads, qt = u_id / n_split / heads;
-    const int h = hc % a.hkv, seg_rows = QW_SEG(rows), unit_rows = QW_SEG(unit_rows);
-    const int row_base = hc / a.hkv * seg_rows;  // the head's rows of its KV head's R
-    const int row0 = row_base + qt * unit_rows;
-    const int row_end = row_base + min(seg_rows, (qt + 1) * unit_rows);
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r16 = lane & 15, g = lane >> 4;
-    const uint32_t magic = vconst(kMagic);
-
-    // visible keys: [lo, hi) of the unit's rows together
-    const int causal_rows = QW_SEG(causal_rows);  // 0: every key to T - 1
-    int lo = 0;
-    if (is_tail && a.starts) lo = min(max(a.starts[hc / a.hkv], 0), T);
-    auto limit = [&](int row) {  // a row's last visible key
-        return causal_rows ? T - causal_rows + (row - row_base) / a.G : T - 1;
-    };
-    const int hi = limit(row_end - 1) + 1;
-    const int tps = QW_SEG(tiles_per_split);
-    const int t0 = lo / KT + sp * tps, t1 = min((hi + KT - 1) / KT, t0 + tps);
-    const int n = max(t1 - t0, 0);
-
-    // ---- waves: row tile and part of each tile's keys
-    const int n_rt = (row_end - row0 + 15) / 16;
-    const int lrt = n_rt <= 1 ? 0 : n_rt <= 2 ? 1 : n_rt <= 4 ? 2 : 3;  // log2 of the row tiles, padded
-    const int parts = min(kWaves >> lrt, NSUB);
-    const int part = wave >> lrt, wrow0 = row0 + 16 * (wave & ((1 << lrt) - 1));
-    const bool live = part < parts && wrow0 < row_end;
-    const int rho = wrow0 + r16;
-    const bool row_ok = live && rho < row_end;
-    const int lim = row_ok ? limit(rho) : -1;
-    const int wave_first_lim = limit(min(wrow0, row_end - 1)), wave_lim = limit(min(wrow0 + 15, row_end - 1));
-
-    half8 qb[NM];
-    {
-        const int row = row_ok ? rho : row0, seq = row / (a.Tq * a.G), rr = row % (a.Tq * a.G);
-        const f16* qrow = a.q + (((int64_t)seq * a.hkv * a.G + h * a.G + rr % a.G) * a.Tq + rr / a.G) * D;
-#pragma unroll
-        for (int m = 0; m < NM; m++) {
-            u32x4 w = *(const u32x4*)(qrow + 32 * m + 8 * g);
-            if (!row_ok) w = u32x4{0, 0, 0, 0};
-            if constexpr (KIND == 4)  // K rows sit in LDS as dim pairs (0,4),(1,5),(2,6),(3,7)
-                w = u32x4{__builtin_amdgcn_perm(w.z, w.x, 0x05040100u), __builtin_amdgcn_perm(w.z, w.x, 0x07060302u),
-                          __builtin_amdgcn_perm(w.w, w.y, 0x05040100u), __builtin_amdgcn_perm(w.w, w.y, 0x07060302u)};
-            qb[m] = as_h8(w);
-        }
+// A unit: a split of a query tile of a head of one of the two caches.
+struct Unit {
+    int sp, hc, h, row_base;      // split; the cache's head, the KV head; the head's first row of the KV head's R
+    int row0, row_end;            // the unit's rows
+    int lo, hi;                   // keys that any of them sees
+    int k_begin, k_end;           // the split's keys
+    int T, cap, causal_rows;
+    int64_t slot_base;            // partial rows: slot_base + row
+    uint32_t code_off;
+    const uint32_t *k_data, *k_params, *v_data, *v_params;
+    __device__ int limit(int row, int G) const {  // a row's last visible key
+        return causal_rows ? T - causal_rows + (row - row_base) / G : T - 1;
     }
+};
+template <int D>
+__device__ __forceinline__ Unit this_unit(const SharedArgs& a) {
+    const bool tail = (int)blockIdx.x >= a.seg[0].n_units;
+    const int id = (int)blockIdx.x - (tail ? a.seg[0].n_units : 0);
+#define QW_SEG(f) (tail ? a.seg[1].f : a.seg[0].f)
+    Unit u;
+    const int n_split = QW_SEG(n_split), heads = QW_SEG(heads), rows = QW_SEG(rows), unit_rows = QW_SEG(unit_rows);
+    const int qt = id / n_split / heads;
+    u.sp = id % n_split;
+    u.hc = id / n_split % heads;
+    u.h = u.hc % a.hkv;
+    u.row_base = u.hc / a.hkv * rows;
+    u.row0 = u.row_base + qt * unit_rows;
+    u.row_end = u.row_base + min(rows, (qt + 1) * unit_rows);
+    u.T = QW_SEG(T);
+    u.cap = QW_SEG(cap);
+    u.causal_rows = QW_SEG(causal_rows);
+    u.lo = tail && a.starts ? min(max(a.starts[u.hc / a.hkv], 0), u.T) : 0;
+    u.hi = u.limit(u.row_end - 1, a.G) + 1;
+    const int tile = shared_tile(D), keys = QW_SEG(tiles_per_split) * tile;
+    u.k_begin = u.lo / tile * tile + u.sp * keys;
+    u.k_end = min(u.hi, u.k_begin + keys);
+    u.slot_base = ((int64_t)(QW_SEG(slot0) + u.sp) * a.hkv + u.h) * a.R;
+    u.code_off = QW_SEG(code_off2);
+    u.k_data = QW_SEG(k_data);
+    u.k_params = QW_SEG(k_params);
+    u.v_data = QW_SEG(v_data);
+    u.v_params = QW_SEG(v_params);
+#undef QW_SEG
+    return u;
+}
+// Row `row` of KV head h: its place in q and out, in rows of D.
+__device__ __forceinline__ int64_t q_row(const SharedArgs& a, int h, int row) {
+    const int seq = row / (a.Tq * a.G), x = row % (a.Tq * a.G);
+    return ((int64_t)seq * a.hkv * a.G + h * a.G + x % a.G) * a.Tq + x / a.G;
+}
+// 16 bytes of q as the kernels take them: negated where the scale is negative, and for 4-bit
+// codes in the order in which deq4 leaves a word's dims, (0,4), (1,5), (2,6), (3,7).
+template <int KIND>
+__device__ __forceinline__ u32x4 q_piece(u32x4 w, uint32_t flip) {
+    w ^= u32x4{flip, flip, flip, flip};
+    if constexpr (KIND == 4)
+        w = u32x4{__builtin_amdgcn_perm(w.z, w.x, 0x05040100u), __builtin_amdgcn_perm(w.z, w.x, 0x07060302u),
+                  __builtin_amdgcn_perm(w.w, w.y, 0x05040100u), __builtin_amdgcn_perm(w.w, w.y, 0x07060302u)};
+    return w;
+}
 
-    // ---- tile loads: key kk's 32-dim slice q32, V block vb's 4 physical slots from 4 vj
-    struct Stage {
-        u32x4 kc[KU], vc[KU], vp[2];
-        uint32_t kp;
-    };
-    const int q32 = (tid >> 4) & (TPR - 1), kk = (tid & 15) | ((tid >> (4 + LTPR)) << 4);
-    const int vb = tid / TPB, vj = tid % TPB;
-    // slots 4 vj .. + 3 are dims vd + step e (KIND 8: two dims of two lane groups)
+// Schedules a run of N LDS reads that each feed MF MFMAs with four reads kept ahead of them (left to
+// itself the compiler waits for each).
+template <int GROUP, int N, int MF>
+__device__ __forceinline__ void keep_reads_ahead() {
+    constexpr int AH = 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, AH, GROUP);
+#pragma unroll
+    for (int i = 0; i < N - AH; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, MF, GROUP);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, GROUP);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, MF * AH, GROUP);
+}
+
+// Units of many rows, 12 waves. Waves 8 to 11, one a SIMD, dequantize: tile i + 1 (its codes in
+// registers since two tiles ago) into the free one of two LDS buffers (block_tile.hpp's layout, V's
+// slots in the fp16 order whatever the codes'), then request tile i + 3's codes. Waves 0 to 7, two a
+// SIMD, compute tile i, RT row tiles of 16 each:
+//   S^T = K . Q^T (a lane then holds 8 consecutive keys of a row, the A operand of P . V), scores in
+//   fp32, P in fp16 against a reference that moves when a score passes it by kLazy = 8 powers of two
+//   (fp16 keeps 11 bits of p up to 2^8 as well; the accumulators are rescaled in few tiles),
+//   O += P . V in fp32.
+// Where the rows leave waves free these take parts of each tile's keys, joined at the end through LDS.
+// One barrier a tile. (With 8 waves that dequantize and compute in turn, all of them were in the same
+// phase: LDS idle while they dequantize, the VALU while they read.)
+template <int KIND, int D, bool FAST>
+__device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
+    using S = BlockShape<D>;
+    constexpr int KT = S::KT, NSUB = S::NSUB, NM = S::NM, NT = S::NT, NG = S::NG, VROW = S::VROW;
+    constexpr int TPR = S::TPR, LTPR = S::LTPR, TPB = S::TPB, BUF = S::BUF, KBUF = S::KBUF;
+    constexpr int PER = KT * TPR / (64 * kFillWaves);  // slices of each kind a dequantizing thread
+    constexpr int RT = many_tiles(D);
+    constexpr int KU = KIND / 4;               // 16-byte loads of a 32-dim K slice / 4-slot V slice
     constexpr int DPL = D / 16;
-    const int vn = KIND == 16 ? 0 : KIND == 8 ? (2 * vj) % 16 : vj % 16;
-    const int vr = KIND == 8 ? 2 * (vj / 8) : 4 * (vj / 16);
-    const int64_t krow = (int64_t)hc * cap + kk, vblk = (int64_t)hc * (cap / 8) + vb;
-    const u32x4* const ksrc = (const u32x4*)(QW_SEG(k_data) + krow * (D * KIND / 32)) + KU * q32;
-    const u32x4* const vsrc = (const u32x4*)(QW_SEG(v_data) + vblk * (D * KIND / 4)) + KU * vj;
-    const uint32_t* const kpsrc = KIND == 16 ? nullptr : QW_SEG(k_params) + krow * NG + k_param_slot(q32 >> 1, NG);
-    const u32x4* const vpsrc =
-        KIND == 16 ? nullptr : (const u32x4*)(QW_SEG(v_params) + (vblk * NG + vn * DPL / kGroup) * 8);
-    auto load = [&](Stage& st, int i) {
-        const int64_t rows = (int64_t)(t0 + i) * KT, blks = rows / 8;
-#pragma unroll
-        for (int u = 0; u < KU; u++) st.kc[u] = ksrc[rows * (D * KIND / 128) + u];
-#pragma unroll
-        for (int u = 0; u < KU; u++) st.vc[u] = vsrc[blks * (D * KIND / 16) + u];
-        if constexpr (KIND != 16) {
-            st.kp = kpsrc[rows * NG];
-            st.vp[0] = vpsrc[blks * (NG * 2)];
-            st.vp[1] = vpsrc[blks * (NG * 2) + 1];
-        }
-    };
-    const uint32_t code_off = QW_SEG(code_off2);
-    // Tile i dequantized into buffer i & 1: f16(f16(code * scale) + bias), as the fetch gives
-    // it; V in the fp16 slot order whatever the codes'. Keys outside [lo, hi) go in as
-    // zeros of V: they have weight 0, but 0 x inf is NaN.
-    auto store = [&](const Stage& st, int i) {
-        half8* const sK = (half8*)(lds + BUF * (i & 1));
-        half8* const sV = (half8*)(lds + BUF * (i & 1) + KBUF) + vb * VROW;
-        half8* const kdst = sK + kaddr<KT>(kk, 4 * q32);
-        if constexpr (KIND == 16) {
-#pragma unroll
-            for (int w = 0; w < 4; w++) kdst[w * KT] = as_h8(st.kc[w]);
-        } else {
-            const half2v sb = h2(st.kp), s = {sb.x, sb.x}, b = {sb.y, sb.y};
-            const PairConsts c = make_consts<FAST, KIND>(s, s, s, s, b, b, b, b, code_off);
-#pragma unroll
-            for (int w = 0; w < 4; w++)
-                kdst[w * KT] = KIND == 4 ? deq4<FAST>(st.kc[0][w], c, magic)
-                                         : deq8<FAST>(st.kc[KU / 2 * (w / 2)][2 * (w % 2)],
-                                                       st.kc[KU / 2 * (w / 2)][2 * (w % 2) + 1], c);
-        }
-        half8 y[4];
-        if constexpr (KIND == 16) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = as_h8(st.vc[e]);
-        } else {
-            const PairConsts c = make_consts<FAST, KIND>(h2(st.vp[0][0]), h2(st.vp[0][1]), h2(st.vp[0][2]), h2(st.vp[0][3]),
-                                                          h2(st.vp[1][0]), h2(st.vp[1][1]), h2(st.vp[1][2]), h2(st.vp[1][3]),
-                                                          code_off);
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                y[e] = KIND == 4 ? deq4<FAST>(st.vc[0][e], c, magic)
-                                 : deq8<FAST>(st.vc[KU / 2 * (e / 2)][2 * (e % 2)],
-                                               st.vc[KU / 2 * (e / 2)][2 * (e % 2) + 1], c);
-        }
-        const int key0 = (t0 + i) * KT;
-        if (key0 < lo || key0 + KT > hi) {
-            const u32x4 keep = keep_keys(hi - (key0 + 8 * vb)) & ~keep_keys(lo - (key0 + 8 * vb));
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = as_h8(__builtin_bit_cast(u32x4, y[e]) & keep);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int at = KIND == 16  ? 4 * vj + e + (vj >> 2)
-                           : KIND == 8 ? 17 * (vr + e % 2) + vn + e / 2
-                                       : 17 * (vr + e) + vn;
-            sV[at] = y[e];
-        }
-    };
+    constexpr float kLazy = 8.0f;
+    static_assert(PER * 64 * kFillWaves == KT * TPR && (KT / 8) * TPB == KT * TPR, "whole slices a thread");
+    static_assert(2 * BUF <= kSharedLds, "LDS");
+    const Unit u = this_unit<D>(a);
+    const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = max(0, (u.k_end - u.k_begin + KT - 1) / KT);  // tiles
+    const int n_rt = (u.row_end - u.row0 + 16 * RT - 1) / (16 * RT);  // a computing wave each
+    const int lrt = n_rt <= 1 ? 0 : n_rt <= 2 ? 1 : n_rt <= 4 ? 2 : 3;
+    const int parts = min(kWaves >> lrt, NSUB);
+    constexpr int REG = RT * (64 * NT * 16 + 64 * 8);  // a parked part
+    static_assert((kWaves - kWaves / (NSUB < 8 ? NSUB : 8)) * REG <= kSharedLds, "the parked parts fit");
 
-    float m_run = -INFINITY, l_run = 0.0f;  // log2 units; l: this lane's share
-    float4v acc_o[NT];
-#pragma unroll
-    for (int mm = 0; mm < NT; mm++) acc_o[mm] = float4v{0.f, 0.f, 0.f, 0.f};
-
-    // NU sub-blocks of 32 keys, from sub-block ub of tile i
-    auto step = [&](int i, int ub, auto nu_c) {
-        constexpr int NU = decltype(nu_c)::value;
-        const half8* const sK = (const half8*)(lds + BUF * (i & 1)) + 32 * ub;
-        const half8* const sV = (const half8*)(lds + BUF * (i & 1) + KBUF) + 4 * ub * VROW;
-        const int kt0 = (t0 + i) * KT + 32 * ub;
-        const int key0 = 8 * (r16 >> 2) + (r16 & 3), b4 = (key0 >> 4) & 1;
-        const half8* const k0 = sK + g * KT + key0 + 4 * b4;
-        const half8* const k1 = sK + g * KT + key0 + 4 * (b4 ^ 1);
-        float4v acc[NU][2];
-#pragma unroll
-        for (int u = 0; u < NU; u++) acc[u][0] = acc[u][1] = float4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int m = 0; m < NM; m++)
-#pragma unroll
-            for (int u = 0; u < NU; u++) {
-                acc[u][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0[4 * m * KT + 32 * u], qb[m], acc[u][0], 0, 0, 0);
-                acc[u][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1[4 * m * KT + 32 * u], qb[m], acc[u][1], 0, 0, 0);
-            }
-        float s[NU][8];
-#pragma unroll
-        for (int u = 0; u < NU; u++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) s[u][e] = acc[u][e >> 2][e & 3] * a.scale2;
-        if (kt0 + 32 * NU - 1 > wave_first_lim || kt0 < lo) {
-#pragma unroll
-            for (int u = 0; u < NU; u++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int key = kt0 + 32 * u + 8 * g + e;
-                    if (key > lim || key < lo) s[u][e] = -INFINITY;
-                }
-        }
-        float mx = s[0][0];
-#pragma unroll
-        for (int u = 0; u < NU; u++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) mx = fmaxf(mx, s[u][e]);
-        if (__any(mx > m_run)) {
-            const float m_new = fmaxf(m_run, wave_max_g(mx));
-            const float alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m_new);
-            l_run *= alpha;
-            float f[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) f[e] = __shfl(alpha, 4 * g + e);
-#pragma unroll
-            for (int mm = 0; mm < NT; mm++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc_o[mm][e] *= f[e];
-            m_run = m_new;
-        }
-        const float mref = m_run == -INFINITY ? 0.0f : m_run;
-        half8 p16[NU];
-#pragma unroll
-        for (int u = 0; u < NU; u++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float p = __builtin_amdgcn_exp2f(s[u][e] - mref);
-                l_run += p;
-                p16[u][e] = (f16)p;
-            }
-#pragma unroll
-        for (int u = 0; u < NU; u++)
-#pragma unroll
-            for (int mm = 0; mm < NT; mm++)
-                acc_o[mm] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p16[u], sV[(4 * u + g) * VROW + r16 + 17 * mm],
-                                                                   acc_o[mm], 0, 0, 0);
-    };
-
-    // ---- rounds: stage x holds tile i where i mod NST == x. A loop of its own for the waves
-    // that take one sub-block of a tile and for those that take PER = 2 or 4 of them, two at a
-    // time (one loop for both spilled registers); the barriers pair up all the same.
-    auto rounds = [&](auto per_c) {
-        constexpr int PER = decltype(per_c)::value, NU = PER < 2 ? 1 : 2;
-        const int ub0 = part * PER;
-        auto compute = [&](int i) {
-#pragma unroll
-            for (int ub = 0; ub < PER; ub += NU)
-                if (live && (t0 + i) * KT + 32 * (ub0 + ub) <= wave_lim)
-                    step(i, ub0 + ub, std::integral_constant<int, NU>{});
+    if (wave >= kWaves) {
+        // ---- dequantizing waves
+        struct Stage {
+            u32x4 kc[PER][KU], vc[PER][KU], vp[PER][2];
+            uint32_t kp[PER];
         };
-        Stage st[NST];
-        if (n > 0) {
+        const uint32_t magic = vconst(kMagic);
+        const char* const k_head = (const char*)u.k_data + ((int64_t)u.hc * u.cap + u.k_begin) * (D * KIND / 8);
+        const char* const kp_head = (const char*)u.k_params + ((int64_t)u.hc * u.cap + u.k_begin) * (NG * 4);
+        const char* const v_head = (const char*)u.v_data + (((int64_t)u.hc * u.cap + u.k_begin) / 8) * (D * KIND);
+        const char* const vp_head = (const char*)u.v_params + (((int64_t)u.hc * u.cap + u.k_begin) / 8) * (NG * 32);
+        // slice j: key kk's 32 dims from 32 q32, V block vb's 4 slots from 4 vj
+        int q32[PER], kk[PER], vb[PER], vj[PER];
 #pragma unroll
-            for (int x = 0; x < NST; x++)
-                if (x < n) load(st[x], x);
-            store(st[0], 0);
-            if (NST < n) load(st[0], NST);
+        for (int j = 0; j < PER; j++) {
+            const int t = tid - 64 * kWaves + 64 * kFillWaves * j;
+            q32[j] = (t >> 4) & (TPR - 1);
+            kk[j] = (t & 15) | ((t >> (4 + LTPR)) << 4);
+            vb[j] = t / TPB;
+            vj[j] = t % TPB;
+        }
+        auto v_n = [&](int j) { return KIND == 16 ? 0 : KIND == 8 ? (2 * vj[j]) % 16 : vj[j] % 16; };  // lane group of slot 4 vj
+        auto load = [&](Stage& st, int i) {
+            const int64_t key = (int64_t)i * KT;
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                const u32x4* k = (const u32x4*)(k_head + key * (D * KIND / 8) + (kk[j] * (D * KIND / 8) + 16 * KU * q32[j]));
+                const u32x4* v = (const u32x4*)(v_head + key / 8 * (D * KIND) + (vb[j] * (D * KIND) + 16 * KU * vj[j]));
+#pragma unroll
+                for (int x = 0; x < KU; x++) st.kc[j][x] = k[x];
+#pragma unroll
+                for (int x = 0; x < KU; x++) st.vc[j][x] = v[x];
+                if constexpr (KIND != 16) {
+                    st.kp[j] = *(const uint32_t*)(kp_head + key * (NG * 4) + (kk[j] * (NG * 4) + 4 * k_param_slot(q32[j] >> 1, NG)));
+                    const u32x4* p = (const u32x4*)(vp_head + key / 8 * (NG * 32) + (vb[j] * (NG * 32) + v_n(j) * DPL / kGroup * 32));
+                    st.vp[j][0] = p[0];
+                    st.vp[j][1] = p[1];
+                }
+            }
+        };
+        // f16(f16(code * scale) + bias), as the fetch gives it
+        auto store = [&](const Stage& st, int i) {
+            half8* const sK = (half8*)(lds + BUF * (i & 1));
+            half8* const sV = (half8*)(lds + BUF * (i & 1) + KBUF);
+            const int key0 = u.k_begin + i * KT;
+            const bool edge = key0 < u.lo || key0 + KT > u.hi;
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                half8* const kdst = sK + kaddr<KT>(kk[j], 4 * q32[j]);
+                half8 y[4];
+                if constexpr (KIND == 16) {
+#pragma unroll
+                    for (int w = 0; w < 4; w++) kdst[w * KT] = as_h8(st.kc[j][w]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[e] = as_h8(st.vc[j][e]);
+                } else {
+                    const half2v sb = h2(st.kp[j]), s = {sb.x, sb.x}, b = {sb.y, sb.y};
+                    const PairConsts kc = make_consts<FAST, KIND>(s, s, s, s, b, b, b, b, u.code_off);
+                    const u32x4 vs = st.vp[j][0], vo = st.vp[j][1];
+                    const PairConsts vc = make_consts<FAST, KIND>(h2(vs[0]), h2(vs[1]), h2(vs[2]), h2(vs[3]), h2(vo[0]), h2(vo[1]),
+                                                                  h2(vo[2]), h2(vo[3]), u.code_off);
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        if constexpr (KIND == 4) {
+                            kdst[w * KT] = deq4<FAST>(st.kc[j][0][w], kc, magic);
+                            y[w] = deq4<FAST>(st.vc[j][0][w], vc, magic);
+                        } else {
+                            kdst[w * KT] = deq8<FAST>(st.kc[j][KU / 2 * (w / 2)][2 * (w % 2)], st.kc[j][KU / 2 * (w / 2)][2 * (w % 2) + 1], kc);
+                            y[w] = deq8<FAST>(st.vc[j][KU / 2 * (w / 2)][2 * (w % 2)], st.vc[j][KU / 2 * (w / 2)][2 * (w % 2) + 1], vc);
+                        }
+                    }
+                }
+                if (edge) {  // keys that no row sees have weight 0, but 0 x inf is NaN
+                    asm volatile("");
+                    const int key = key0 + 8 * vb[j];
+                    const u32x4 keep = keep_keys(u.hi - key) & ~keep_keys(u.lo - key);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[e] = as_h8(__builtin_bit_cast(u32x4, y[e]) & keep);
+                }
+                const int vr = KIND == 8 ? 2 * (vj[j] / 8) : 4 * (vj[j] / 16);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int at = KIND == 16  ? 4 * vj[j] + e + (vj[j] >> 2)
+                                   : KIND == 8 ? 17 * (vr + e % 2) + v_n(j) + e / 2
+                                               : 17 * (vr + e) + v_n(j);
+                    sV[vb[j] * VROW + at] = y[e];
+                }
+            }
+        };
+        Stage s0, s1;  // tiles 1, 3, .. and 2, 4, ..
+        if (n > 0) {
+            load(s0, 0);
+            if (n > 2) load(s1, 2);
+            store(s0, 0);
+            if (n > 1) load(s0, 1);
         }
         __syncthreads();
-        for (int i = 0; i < n; i += NST) {
+        for (int i = 0; i < n; i += 2) {
+            if (i + 1 < n) {
+                store(s0, i + 1);
+                if (i + 3 < n) load(s0, i + 3);
+            }
+            __syncthreads();
+            if (i + 1 >= n) break;
+            if (i + 2 < n) {
+                store(s1, i + 2);
+                if (i + 4 < n) load(s1, i + 4);
+            }
+            __syncthreads();
+        }
+        if (parts > 1) __syncthreads();
+        return;
+    }
+
+    // ---- computing waves: RT row tiles, and a part of each tile's keys
+    const int part = wave >> lrt, wrow0 = u.row0 + 16 * RT * (wave & ((1 << lrt) - 1));
+    const bool live = part < parts && wrow0 < u.row_end;
+    const int wave_first_lim = u.limit(min(wrow0, u.row_end - 1), a.G), wave_lim = u.limit(min(wrow0 + 16 * RT - 1, u.row_end - 1), a.G);
+    int lim[RT];
+    half8 qb[RT][NM];
 #pragma unroll
-            for (int x = 0; x < NST; x++) {
-                if (i + x >= n) break;
-                if (i + x + 1 < n) {
-                    store(st[(x + 1) % NST], i + x + 1);
-                    if (i + x + 1 + NST < n) load(st[(x + 1) % NST], i + x + 1 + NST);
-                }
-                compute(i + x);
-                __syncthreads();
+    for (int rt = 0; rt < RT; rt++) {
+        const int row = wrow0 + 16 * rt + r16;
+        const bool ok = live && row < u.row_end;
+        lim[rt] = ok ? u.limit(row, a.G) : -1;
+        const f16* q = a.q + q_row(a, u.h, ok ? row : u.row0) * D + 8 * g;
+#pragma unroll
+        for (int m = 0; m < NM; m++) {
+            const u32x4 w = *(const u32x4*)(q + 32 * m);
+            qb[rt][m] = as_h8(q_piece<KIND>(ok ? w : u32x4{0, 0, 0, 0}, a.q_flip));
+        }
+    }
+    float m_ref[RT], l_run[RT];  // log2 units; l: this lane's share
+    float4v acc_o[RT][NT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        m_ref[rt] = -INFINITY;
+        l_run[rt] = 0.0f;
+#pragma unroll
+        for (int mm = 0; mm < NT; mm++) acc_o[rt][mm] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+    // 32 keys: sub-block ub of tile i
+    auto step = [&](int i, int ub) {
+        const half8* const sK = (const half8*)(lds + BUF * (i & 1)) + 32 * ub;
+        const half8* const sV = (const half8*)(lds + BUF * (i & 1) + KBUF) + (4 * ub + g) * VROW + r16;
+        const int key0 = u.k_begin + i * KT + 32 * ub;
+        const int kr = 8 * (r16 >> 2) + (r16 & 3), b4 = (kr >> 4) & 1;
+        const half8* const k0 = sK + g * KT + kr + 4 * b4;
+        const half8* const k1 = sK + g * KT + kr + 4 * (b4 ^ 1);
+        float4v s[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) s[rt][0] = s[rt][1] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int m = 0; m < NM; m++) {
+            const half8 x0 = k0[4 * m * KT], x1 = k1[4 * m * KT];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                s[rt][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, qb[rt][m], s[rt][0], 0, 0, 0);
+                s[rt][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, qb[rt][m], s[rt][1], 0, 0, 0);
             }
         }
+        keep_reads_ahead<0, 2 * NM, RT>();
+        if (key0 + 31 > wave_first_lim || key0 < u.lo) {
+            asm volatile("");  // a branch, not selects in every step
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int key = key0 + 8 * g + e;
+                    if (key > lim[rt] || key < u.lo) s[rt][e >> 2][e & 3] = -INFINITY;
+                }
+        }
+        half8 p16[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            float mx = s[rt][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; e++) mx = fmaxf(mx, s[rt][e >> 2][e & 3]);
+            mx *= a.scale2;
+            if (__any(mx > m_ref[rt] + kLazy)) {
+                const float m_new = fmaxf(m_ref[rt], wave_max_g(mx));
+                const float alpha = m_ref[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_ref[rt] - m_new);
+                l_run[rt] *= alpha;
+                float f[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) f[e] = __shfl(alpha, 4 * g + e);
+#pragma unroll
+                for (int mm = 0; mm < NT; mm++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc_o[rt][mm][e] *= f[e];
+                m_ref[rt] = m_new;
+            }
+            const float ref = m_ref[rt] == -INFINITY ? 0.0f : -m_ref[rt];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][e >> 2][e & 3], a.scale2, ref));
+                l_run[rt] += p;
+                p16[rt][e] = (f16)p;
+            }
+        }
+#pragma unroll
+        for (int mm = 0; mm < NT; mm++) {
+            const half8 x = sV[17 * mm];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+                acc_o[rt][mm] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p16[rt], x, acc_o[rt][mm], 0, 0, 0);
+        }
+        keep_reads_ahead<1, NT, RT>();
     };
-    if (parts == NSUB)
-        rounds(std::integral_constant<int, 1>{});
-    else if (NSUB == 2 || parts == 2)
-        rounds(std::integral_constant<int, 2>{});
-    else
-        rounds(std::integral_constant<int, NSUB>{});
-
-    // ---- the parts of a row tile joined in its part 0, through LDS
-    float l = wave_sum_g(l_run);
+    const int per = NSUB / parts, ub0 = part * per;
+    __syncthreads();
+    for (int i = 0; i < n; i++) {
+        if (live)
+            for (int ub = ub0; ub < ub0 + per; ub++)
+                if (u.k_begin + i * KT + 32 * ub <= wave_lim) step(i, ub);
+        __syncthreads();
+    }
+    // ---- the parts of a wave's rows joined in its part 0, through LDS
+    float l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) l[rt] = wave_sum_g(l_run[rt]);
     if (parts > 1) {
-        constexpr int REG = 64 * NT * 16 + 64 * 8;
-        static_assert(6 * REG <= 2 * BUF && 4 * REG <= 2 * BUF, "the parked parts fit the tile buffers");
         if (live && part > 0) {
             char* reg = lds + (wave - (1 << lrt)) * REG;
 #pragma unroll
-            for (int mm = 0; mm < NT; mm++) ((float4v*)reg)[mm * 64 + lane] = acc_o[mm];
-            ((float2*)(reg + 64 * NT * 16))[lane] = float2{m_run, l};
+            for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+                for (int mm = 0; mm < NT; mm++) ((float4v*)reg)[(rt * NT + mm) * 64 + lane] = acc_o[rt][mm];
+                ((float2*)(reg + RT * NT * 64 * 16))[rt * 64 + lane] = float2{m_ref[rt], l[rt]};
+            }
         }
         __syncthreads();
         if (live && part == 0) {
             for (int p = 1; p < parts; p++) {
                 const char* reg = lds + (((p - 1) << lrt) + wave) * REG;
-                const float2 ml = ((const float2*)(reg + 64 * NT * 16))[lane];
-                const float M = fmaxf(m_run, ml.x), mr = M == -INFINITY ? 0.0f : M;
-                const float fa = __builtin_amdgcn_exp2f(m_run - mr), fb = __builtin_amdgcn_exp2f(ml.x - mr);
-                l = l * fa + ml.y * fb;
-                m_run = M;
-                float xa[4], xb[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    xa[e] = __shfl(fa, 4 * g + e);
-                    xb[e] = __shfl(fb, 4 * g + e);
-                }
+                for (int rt = 0; rt < RT; rt++) {
+                    const float2 ml = ((const float2*)(reg + RT * NT * 64 * 16))[rt * 64 + lane];
+                    const float M = fmaxf(m_ref[rt], ml.x), mr = M == -INFINITY ? 0.0f : M;
+                    const float fa = __builtin_amdgcn_exp2f(m_ref[rt] - mr), fb = __builtin_amdgcn_exp2f(ml.x - mr);
+                    l[rt] = l[rt] * fa + ml.y * fb;
+                    m_ref[rt] = M;
+                    float xa[4], xb[4];
 #pragma unroll
-                for (int mm = 0; mm < NT; mm++) {
-                    const float4v o = ((const float4v*)reg)[mm * 64 + lane];
+                    for (int e = 0; e < 4; e++) {
+                        xa[e] = __shfl(fa, 4 * g + e);
+                        xb[e] = __shfl(fb, 4 * g + e);
+                    }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc_o[mm][e] = acc_o[mm][e] * xa[e] + o[e] * xb[e];
+                    for (int mm = 0; mm < NT; mm++) {
+                        const float4v o = ((const float4v*)reg)[(rt * NT + mm) * 64 + lane];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc_o[rt][mm][e] = acc_o[rt][mm][e] * xa[e] + o[e] * xb[e];
+                    }
                 }
             }
         }
     }
     if (!live || part > 0) return;
-
-    // ---- rows out: lane (g, r16) holds dims NT r16 .. + NT - 1 of rows 4g + e
-    const int64_t pbase = ((int64_t)(QW_SEG(slot0) + sp) * a.hkv + h) * a.R;
-    if (g == 0 && row_ok) a.part_ml[pbase + rho] = float2{m_run, l};
+    // ---- rows out: lane (g, r16) holds dims NT r16 .. + NT - 1 of rows 16 rt + 4 g + e
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const int row = wrow0 + 4 * g + e;
-        const float le = __shfl(l, 4 * g + e);
-        if (row >= row_end) continue;
-        if (a.n_slots == 1) {
-            const float inv = le == 0.0f ? 0.0f : 1.0f / le;
-            const int seq = row / (a.Tq * a.G), rr = row % (a.Tq * a.G);
-            f16* o = a.out + (((int64_t)seq * a.hkv * a.G + h * a.G + rr % a.G) * a.Tq + rr / a.G) * D + NT * r16;
+    for (int rt = 0; rt < RT; rt++) {
+        if (g == 0 && wrow0 + 16 * rt + r16 < u.row_end)
+            a.part_ml[u.slot_base + wrow0 + 16 * rt + r16] = float2{m_ref[rt], l[rt]};
 #pragma unroll
-            for (int c = 0; c < NT; c += 8) {
-                half8 y;
+        for (int e = 0; e < 4; e++) {
+            const int row = wrow0 + 16 * rt + 4 * g + e;
+            const float le = __shfl(l[rt], 4 * g + e);
+            if (row >= u.row_end) continue;
+            if (a.n_slots == 1) {
+                const float inv = le == 0.0f ? 0.0f : 1.0f / le;
+                f16* o = a.out + q_row(a, u.h, row) * D + NT * r16;
 #pragma unroll
-                for (int j = 0; j < 8; j++) y[j] = (f16)(acc_o[c + j][e] * inv);
-                *(half8*)(o + c) = y;
+                for (int c = 0; c < NT; c += 8) {
+                    half8 y;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) y[j] = (f16)(acc_o[rt][c + j][e] * inv);
+                    *(half8*)(o + c) = y;
+                }
+            } else {
+                float* o = a.part_o + (u.slot_base + row) * D + NT * r16;
+#pragma unroll
+                for (int c = 0; c < NT; c += 4)
+                    *(float4v*)(o + c) = float4v{acc_o[rt][c][e], acc_o[rt][c + 1][e], acc_o[rt][c + 2][e], acc_o[rt][c + 3][e]};
             }
-        } else {
-            float* o = a.part_o + (pbase + row) * D + NT * r16;
-#pragma unroll
-            for (int c = 0; c < NT; c += 4)
-                *(float4v*)(o + c) = float4v{acc_o[c][e], acc_o[c + 1][e], acc_o[c + 2][e], acc_o[c + 3][e]};
         }
     }
 }
@@ -371,54 +452,39 @@ template <int KIND, int D, bool FAST>
 __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
     constexpr int NM = D / 32, NT = D / 16, NG = D / kGroup, DG = D / 4, DPL = D / 16;
     constexpr int KP = DG * KIND / 128, VP = DPL * KIND / 16, E = 16 / KIND;  // 16-byte pieces a lane; dims a piece of V
-    const bool is_tail = (int)blockIdx.x >= a.seg[0].n_units;
-    const int u_id = (int)blockIdx.x - (is_tail ? a.seg[0].n_units : 0);
-    const int n_split = QW_SEG(n_split), heads = QW_SEG(heads), T = QW_SEG(T), cap = QW_SEG(cap);
-    const int sp = u_id % n_split, hc = u_id / n_split;
-    const int h = hc % a.hkv, rows = QW_SEG(rows), row_base = hc / a.hkv * rows;
-    (void)heads;
+    const Unit u = this_unit<D>(a);
+    const int rows = u.row_end - u.row0, cap = u.cap, lo = u.lo, hc = u.hc, h = u.h, row_base = u.row0;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     const uint32_t magic = vconst(kMagic);
-    const int causal_rows = QW_SEG(causal_rows);
-    int lo = 0;
-    if (is_tail && a.starts) lo = min(max(a.starts[hc / a.hkv], 0), T);
     const bool row_ok = r16 < rows;
-    const int rr = row_ok ? r16 : 0, lim = !row_ok ? -1 : causal_rows ? T - causal_rows + rr / a.G : T - 1;
-    const int first_lim = causal_rows ? T - causal_rows : T - 1;
-    constexpr int KT = BlockShape<D>::KT;
-    const int keys = QW_SEG(tiles_per_split) * KT, k_begin = lo / 32 * 32 + sp * keys, k_end = min(T, k_begin + keys);
+    const int rr = row_ok ? r16 : 0, lim = row_ok ? u.limit(row_base + rr, a.G) : -1, first_lim = u.limit(row_base, a.G);
+    const int k_begin = max(u.k_begin, lo / 32 * 32), k_end = u.k_end;
     half8 qb[NM];
-    {
-        const int seq = (row_base + rr) / (a.Tq * a.G), x = (row_base + rr) % (a.Tq * a.G);
-        const f16* qrow = a.q + (((int64_t)seq * a.hkv * a.G + h * a.G + x % a.G) * a.Tq + x / a.G) * D + DG * g;
 #pragma unroll
-        for (int m = 0; m < NM; m++) {
-            u32x4 w = *(const u32x4*)(qrow + 8 * m);
-            if (!row_ok) w = u32x4{0, 0, 0, 0};
-            if constexpr (KIND == 4)  // dims in deq4's order
-                w = u32x4{__builtin_amdgcn_perm(w.z, w.x, 0x05040100u), __builtin_amdgcn_perm(w.z, w.x, 0x07060302u),
-                          __builtin_amdgcn_perm(w.w, w.y, 0x05040100u), __builtin_amdgcn_perm(w.w, w.y, 0x07060302u)};
-            qb[m] = as_h8(w);
-        }
+    for (int m = 0; m < NM; m++) {
+        const u32x4 w = *(const u32x4*)(a.q + q_row(a, h, row_base + rr) * D + 8 * k_chunk<KIND>(m, g));
+        qb[m] = as_h8(q_piece<KIND>(row_ok ? w : u32x4{0, 0, 0, 0}, a.q_flip));
     }
-    const uint32_t code_off = QW_SEG(code_off2);
+    const uint32_t code_off = u.code_off;
     const int64_t krow0 = (int64_t)hc * cap + 8 * (r16 >> 2) + (r16 & 3), vblk0 = (int64_t)hc * (cap / 8) + g;
-    const u32x4* const ksrc = (const u32x4*)(QW_SEG(k_data) + krow0 * (D * KIND / 32) + g * (DG * KIND / 32));
-    const uint32_t* const kpsrc = KIND == 16 ? nullptr : QW_SEG(k_params) + krow0 * NG + k_param_slot(g * DG / kGroup, NG);
-    const u32x4* const vsrc = (const u32x4*)(QW_SEG(v_data) + vblk0 * (D * KIND / 4)) + r16;
+    const u32x4* const ksrc = (const u32x4*)(u.k_data + krow0 * (D * KIND / 32)) + g;
+    const uint32_t* const kpsrc = KIND == 16 ? nullptr : u.k_params + krow0 * NG;
+    const u32x4* const vsrc = (const u32x4*)(u.v_data + vblk0 * (D * KIND / 4)) + r16;
     const u32x4* const vpsrc =
-        KIND == 16 ? nullptr : (const u32x4*)(QW_SEG(v_params) + (vblk0 * NG + r16 * DPL / kGroup) * 8);
+        KIND == 16 ? nullptr : (const u32x4*)(u.v_params + (vblk0 * NG + r16 * DPL / kGroup) * 8);
     u32x4 kc[2][KP], vc[VP], vp[2];
-    uint32_t kp[2];
+    uint32_t kp[2][KP];
     auto load_k = [&](int key) {
 #pragma unroll
-        for (int tt = 0; tt < 2; tt++) {
+        for (int tt = 0; tt < 2; tt++)
 #pragma unroll
-            for (int i = 0; i < KP; i++) kc[tt][i] = ksrc[(int64_t)(key + 4 * tt) * (D * KIND / 128) + i];
-            if constexpr (KIND != 16) kp[tt] = kpsrc[(int64_t)(key + 4 * tt) * NG];
-        }
+            for (int i = 0; i < KP; i++) {
+                kc[tt][i] = ksrc[(int64_t)(key + 4 * tt) * (D * KIND / 128) + 4 * i];
+                if constexpr (KIND != 16)
+                    kp[tt][i] = kpsrc[(int64_t)(key + 4 * tt) * NG + k_param_slot(k_piece_group<KIND>(i, g), NG)];
+            }
     };
     auto load_v = [&](int key) {
         // piece j holds slots 16 E j + E n ..: dims DPL n + E j .. of column n
@@ -444,12 +510,13 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
 #pragma unroll
         for (int tt = 0; tt < 2; tt++) {
             PairConsts pc;
-            if constexpr (KIND != 16) {
-                const half2v sb = h2(kp[tt]), s = {sb.x, sb.x}, b = {sb.y, sb.y};
-                pc = make_consts<FAST, KIND>(s, s, s, s, b, b, b, b, code_off);
-            }
 #pragma unroll
             for (int m = 0; m < NM; m++) {
+                if constexpr (KIND != 16)
+                    if (m % E == 0) {
+                        const half2v sb = h2(kp[tt][m / E]), s = {sb.x, sb.x}, b = {sb.y, sb.y};
+                        pc = make_consts<FAST, KIND>(s, s, s, s, b, b, b, b, code_off);
+                    }
                 half8 ka;
                 if constexpr (KIND == 16)
                     ka = as_h8(kc[tt][m]);
@@ -471,6 +538,7 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
         }
         const bool edge = key < lo || key + 31 > first_lim;
         if (edge) {
+            asm volatile("");  // a branch, not selects in every step
 #pragma unroll
             for (int e = 0; e < 8; e++)
                 if (key + 8 * g + e > lim || key + 8 * g + e < lo) s[e] = -INFINITY;
@@ -503,7 +571,6 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
         if constexpr (KIND != 16)
             pc = make_consts<FAST, KIND>(h2(vp[0][0]), h2(vp[0][1]), h2(vp[0][2]), h2(vp[0][3]), h2(vp[1][0]), h2(vp[1][1]),
                                          h2(vp[1][2]), h2(vp[1][3]), code_off);
-        const u32x4 keep = keep_keys(T - (key + 8 * g)) & ~keep_keys(lo - (key + 8 * g));
 #pragma unroll
         for (int j = 0; j < VP; j++) {
             half8 y[E];
@@ -513,6 +580,8 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
                        : KIND == 8 ? deq8<FAST>(vc[j][2 * i % 4], vc[j][(2 * i + 1) % 4], pc)
                                    : deq4<FAST>(vc[j][i % 4], pc, magic);
             if (edge) {  // hidden keys have weight 0, but 0 x inf is NaN
+                asm volatile("");
+                const u32x4 keep = keep_keys(u.hi - (key + 8 * g)) & ~keep_keys(lo - (key + 8 * g));
 #pragma unroll
                 for (int i = 0; i < E; i++) y[i] = as_h8(__builtin_bit_cast(u32x4, y[i]) & keep);
             }
@@ -526,7 +595,7 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
     float* const s_m = (float*)lds;                    // [8 waves][16 rows]
     float* const s_l = s_m + 16 * kWaves;              // [8][16]
     float* const s_o = s_l + 16 * kWaves;              // [8][rows][D]
-    static_assert((16 * kWaves * 2 + kWaves * 16 * D) * 4 <= 2 * BlockShape<D>::BUF, "the waves' sums fit the tile buffers");
+    static_assert((16 * kWaves * 2 + kWaves * 16 * D) * 4 <= kSharedLds, "the waves' sums fit the tile buffers");
     if (g == 0) s_m[16 * wave + r16] = m_run;
     __syncthreads();
     float M = -INFINITY;
@@ -545,7 +614,7 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
             *(float4v*)(o + c) = float4v{acc_o[c][e] * fe, acc_o[c + 1][e] * fe, acc_o[c + 2][e] * fe, acc_o[c + 3][e] * fe};
     }
     __syncthreads();
-    const int64_t pbase = ((int64_t)(QW_SEG(slot0) + sp) * a.hkv + h) * a.R + row_base;
+    const int64_t pbase = u.slot_base + row_base;
     for (int i = tid; i < rows * (D / 4); i += 64 * kWaves) {
         const int row = i / (D / 4), c = i % (D / 4);
         float4v o = {0.f, 0.f, 0.f, 0.f};
@@ -561,33 +630,32 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
         if (c == 0) a.part_ml[pbase + row] = float2{mr, lr};
         if (a.n_slots == 1) {
             const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
-            const int seq = (row_base + row) / (a.Tq * a.G), x = (row_base + row) % (a.Tq * a.G);
             half4v y;
 #pragma unroll
             for (int j = 0; j < 4; j++) y[j] = (f16)(o[j] * inv);
-            *(half4v*)(a.out + (((int64_t)seq * a.hkv * a.G + h * a.G + x % a.G) * a.Tq + x / a.G) * D + 4 * c) = y;
+            *(half4v*)(a.out + q_row(a, h, row_base + row) * D + 4 * c) = y;
         } else {
             *(float4v*)(a.part_o + (pbase + row) * D + 4 * c) = o;
         }
     }
 }
 
-template <int KIND, int D, bool FAST>
-__device__ __forceinline__ void unit_body(const SharedArgs& a, char* lds) {
-    if (((int)blockIdx.x >= a.seg[0].n_units ? a.seg[1].rows : a.seg[0].rows) <= kFewRows)
-        few_body<KIND, D, FAST>(a, lds);
-    else
-        shared_body<KIND, D, FAST>(a, lds);
+__device__ __forceinline__ bool unit_fast(const SharedArgs& a) {
+    return *((int)blockIdx.x >= a.seg[0].n_units ? a.seg[1].fast_flag : a.seg[0].fast_flag) != 0;
 }
-#undef QW_SEG
-
 template <int KIND, int D>
-__global__ __launch_bounds__(64 * kWaves, 1) void shared_attend_kernel(SharedArgs a) {
+__global__ __launch_bounds__(64 * (kWaves + kFillWaves), 1) void shared_many_kernel(SharedArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const bool fast = KIND != 16 && *((int)blockIdx.x >= a.seg[0].n_units ? a.seg[1].fast_flag : a.seg[0].fast_flag);
     if constexpr (KIND != 16)
-        if (fast) return unit_body<KIND, D, true>(a, lds);
-    unit_body<KIND, D, false>(a, lds);
+        if (unit_fast(a)) return many_body<KIND, D, true>(a, lds);
+    many_body<KIND, D, false>(a, lds);
+}
+template <int KIND, int D>
+__global__ __launch_bounds__(64 * kWaves, 1) void shared_few_kernel(SharedArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    if constexpr (KIND != 16)
+        if (unit_fast(a)) return few_body<KIND, D, true>(a, lds);
+    few_body<KIND, D, false>(a, lds);
 }
 
 template <int D>
@@ -622,10 +690,14 @@ void fill_cache(SharedSegment& s, const KVCache& c) {
 
 template <int KIND, int D>
 int launch_units(const SharedArgs& a, hipStream_t stream) {
-    const size_t shmem = (size_t)2 * BlockShape<D>::BUF;
-    if (int rc = ensure_dynamic_lds((const void*)shared_attend_kernel<KIND, D>, shmem)) return rc;
-    hipLaunchKernelGGL((shared_attend_kernel<KIND, D>), dim3(a.seg[0].n_units + a.seg[1].n_units),
-                       dim3(64 * kWaves), shmem, stream, a);
+    const dim3 grid(a.seg[0].n_units + a.seg[1].n_units);
+    const bool few = std::max(a.seg[0].n_units ? a.seg[0].unit_rows : 0, a.seg[1].n_units ? a.seg[1].unit_rows : 0) <= kFewRows;
+    const void* const kernel = few ? (const void*)shared_few_kernel<KIND, D> : (const void*)shared_many_kernel<KIND, D>;
+    if (int rc = ensure_dynamic_lds(kernel, kSharedLds)) return rc;
+    if (few)
+        hipLaunchKernelGGL((shared_few_kernel<KIND, D>), grid, dim3(64 * kWaves), kSharedLds, stream, a);
+    else
+        hipLaunchKernelGGL((shared_many_kernel<KIND, D>), grid, dim3(64 * (kWaves + kFillWaves)), kSharedLds, stream, a);
     QW_HIP_CHECK(hipGetLastError());
     return QW_OK;
 }
@@ -648,7 +720,7 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int 
     SharedArgs& a = *pa;
     a = SharedArgs{};
     const KVCache* c[2] = {prefix && prefix->offset > 0 ? prefix : nullptr, tails && tails->offset > 0 ? tails : nullptr};
-    const int D = (prefix ? prefix : tails)->D, KT = 16384 / D;
+    const int D = (prefix ? prefix : tails)->D, KT = shared_tile(D);
     a.q = (const f16*)q;
     a.out = (f16*)out;
     a.starts = starts;
@@ -656,7 +728,9 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int 
     a.G = G;
     a.hkv = hkv;
     a.R = n_seq * n_rows * G;
-    a.scale2 = scale * kLog2e;
+    // (a scale of 0 stands as a tiny one, which leaves every score 0 and a hidden key's -inf itself)
+    a.scale2 = std::max(std::fabs(scale) * kLog2e, 1e-37f);
+    a.q_flip = scale < 0.0f ? 0x80008000u : 0u;
     int tiles[2] = {0, 0}, n_qt[2] = {0, 0};
     for (int i = 0; i < 2; i++) {
         SharedSegment& s = a.seg[i];
@@ -665,9 +739,10 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int 
         fill_cache(s, *c[i]);
         s.heads = c[i]->hkv;
         s.rows = i == 0 ? a.R : n_rows * G;
-        const int rt = (s.rows + 15) / 16;
+        // query tiles of equal size, in row tiles (few rows: one)
+        const int wave_rows = 16 * many_tiles(D), rt = (s.rows + wave_rows - 1) / wave_rows;
         n_qt[i] = (rt + kWaves - 1) / kWaves;
-        s.unit_rows = 16 * ((rt + n_qt[i] - 1) / n_qt[i]);
+        s.unit_rows = s.rows <= kFewRows ? s.rows : wave_rows * ((rt + n_qt[i] - 1) / n_qt[i]);
         s.causal_rows = i == 1 && causal ? n_rows : 0;
         tiles[i] = (s.T + KT - 1) / KT;
     }

@@ -34,11 +34,29 @@ struct SharedArgs {
     int n_slots;
     float* scores;          // null, or [hkv][R][score_stride]: the scores (log2 units) of one cache's few rows
     int64_t score_stride;   // a multiple of 32
-    float scale2;           // scale * log2 e
+    float scale2;           // |scale| * log2 e
+    uint32_t q_flip;        // the sign bits of two halves where scale is negative: q is taken negated
     SharedSegment seg[2];   // the prefix, the tails
 };
 
+// Dims of a K row that a lane group g (lane >> 4) holds as a QK operand: 16-byte pieces 4 i + g of
+// the row's codes, so that one load of a wave takes 64 whole bytes of each of 16 rows (pieces of one
+// group side by side took each line four to eight times over from a cache that holds none of them
+// that long). Step m then multiplies dims 8 k_chunk(m, g) .. + 7, E = 16 / KIND steps a piece, and
+// piece i's scale is of group k_piece_group(i, g).
+template <int KIND>
+__host__ __device__ constexpr int k_chunk(int m, int g) {
+    constexpr int E = 16 / KIND;
+    return E * (4 * (m / E) + g) + m % E;
+}
+template <int KIND>
+__host__ __device__ constexpr int k_piece_group(int i, int g) {
+    return KIND == 16 ? 0 : KIND == 8 ? i : 2 * i + g / 2;
+}
+
 constexpr int kSharedMaxSlots = 512;
+__host__ __device__ constexpr int shared_tile(int D) { return 16384 / D; }  // keys of a split's tile
+constexpr int kSharedLds = 146 * 1024;  // a workgroup's
 
 // Fills the arguments and takes the workspace (either cache may be null); the launches.
 int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int n_seq, int n_rows, int G, int hkv,

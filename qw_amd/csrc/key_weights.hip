@@ -68,9 +68,9 @@ __global__ __launch_bounds__(256) void row_sums_kernel(SharedArgs a, float2* __r
 
 template <int KIND, int D>
 __global__ __launch_bounds__(64 * kWgWaves) void key_weights_kernel(WeightArgs w) {
-    constexpr int NM = D / 32, NG = D / kGroup, DG = D / 4;  // DG: dims of a lane group
+    constexpr int NM = D / 32, NG = D / kGroup, E = 16 / KIND;
     constexpr int TILE = D * 2 * 16;                         // bytes of 16 rows of q
-    constexpr int KP = DG * KIND / 128;                      // 16-byte pieces of them in a K row
+    constexpr int KP = D * KIND / 512;                       // 16-byte pieces of a K row a lane group
     __shared__ __attribute__((aligned(16))) char lds[2][2 * TILE];  // [buffer][row tile][D / 8 chunks][16 rows]
     const SharedSegment& c = w.s.seg[1];
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4, h = blockIdx.y;
@@ -79,8 +79,8 @@ __global__ __launch_bounds__(64 * kWgWaves) void key_weights_kernel(WeightArgs w
     const int key0 = blockIdx.x * kWgKeys + wave * kWaveKeys;
     const bool live = key0 < T;
     const uint32_t magic = vconst(kMagic);
-    // A operands: lane (g, r16) holds dims DG g .. + DG - 1 of key 32 u + 8 (r16 >> 2) + 4 tt +
-    // (r16 & 3), so that a lane of S^T gets keys 32 u + 8 g + e of row r16
+    // A operands: lane (g, r16) holds its pieces (k_chunk) of key 32 u + 8 (r16 >> 2) + 4 tt + (r16 &
+    // 3), so that a lane of S^T gets keys 32 u + 8 g + e of row r16
     half8 ka[2][2][NM];
 #pragma unroll
     for (int u = 0; u < 2; u++)
@@ -88,19 +88,21 @@ __global__ __launch_bounds__(64 * kWgWaves) void key_weights_kernel(WeightArgs w
         for (int tt = 0; tt < 2; tt++) {
             const int key = min(key0 + 32 * u + 8 * (r16 >> 2) + 4 * tt + (r16 & 3), c.cap - 1);
             const int64_t row = (int64_t)h * c.cap + key;
-            const u32x4* src = (const u32x4*)(c.k_data + row * (D * KIND / 32) + g * (DG * KIND / 32));
+            const u32x4* src = (const u32x4*)(c.k_data + row * (D * KIND / 32)) + g;
             u32x4 x[KP];
 #pragma unroll
-            for (int i = 0; i < KP; i++) x[i] = src[i];
+            for (int i = 0; i < KP; i++) x[i] = src[4 * i];
             if constexpr (KIND == 16) {
 #pragma unroll
                 for (int m = 0; m < NM; m++) ka[u][tt][m] = as_h8(x[m]);
             } else {
-                const half2v sb = h2(c.k_params[row * NG + k_param_slot(g * DG / kGroup, NG)]);
-                const half2v s = {sb.x, sb.x}, b = {sb.y, sb.y};
-                const PairConsts pc = make_consts<false, KIND>(s, s, s, s, b, b, b, b, c.code_off2);
+                uint32_t kp[KP];
+#pragma unroll
+                for (int i = 0; i < KP; i++) kp[i] = c.k_params[row * NG + k_param_slot(k_piece_group<KIND>(i, g), NG)];
 #pragma unroll
                 for (int m = 0; m < NM; m++) {
+                    const half2v sb = h2(kp[m / E]), s = {sb.x, sb.x}, b = {sb.y, sb.y};
+                    const PairConsts pc = make_consts<false, KIND>(s, s, s, s, b, b, b, b, c.code_off2);
                     if constexpr (KIND == 4) {  // dims come as pairs (0,4), (1,5), (2,6), (3,7)
                         const u32x4 y = __builtin_bit_cast(u32x4, deq4<false>(x[m / 4][m % 4], pc, magic));
                         ka[u][tt][m] = as_h8(u32x4{__builtin_amdgcn_perm(y.y, y.x, 0x05040100u),
@@ -165,13 +167,13 @@ __global__ __launch_bounds__(64 * kWgWaves) void key_weights_kernel(WeightArgs w
         if (live) {
 #pragma unroll
             for (int rt = 0; rt < 2; rt++) {
-                const half8* q8 = (const half8*)(lds[buf] + rt * TILE) + (DG / 8) * 16 * g + r16;
+                const half8* q8 = (const half8*)(lds[buf] + rt * TILE) + E * 16 * g + r16;
                 float4v acc[2][2];
 #pragma unroll
                 for (int u = 0; u < 2; u++) acc[u][0] = acc[u][1] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int m = 0; m < NM; m++) {
-                    const half8 qb = q8[16 * m];
+                    const half8 qb = q8[16 * k_chunk<KIND>(m, 0)];
 #pragma unroll
                     for (int u = 0; u < 2; u++)
 #pragma unroll
