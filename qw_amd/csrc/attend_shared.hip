@@ -30,6 +30,7 @@
 // quarters of each tile's keys and join them through LDS.
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <type_traits>
 
 #include "attend_shared.hpp"
@@ -664,8 +665,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
     merge_row<D>(a, blockIdx.x, blockIdx.y, sm);
 }
 
-// What a launch of a prefix and tail units costs on 256 CUs, in key tiles: prefix units of a
-// tiles first, tail units of b as CUs come free.
+// What a launch of n_pre units of a us and, behind them, n_tail units of b us takes on 256 CUs.
 double makespan(int64_t n_pre, double a, int64_t n_tail, double b) {
     const int64_t full = n_pre / 256, rest = n_pre % 256;
     const double base = full * a;
@@ -682,6 +682,7 @@ void fill_cache(SharedSegment& s, const KVCache& c) {
     s.k_params = c.k_params;
     s.v_data = (const uint32_t*)c.v_data;
     s.v_params = c.v_params;
+    s.bits = c.bits;
     s.cap = c.cap;
     s.T = c.offset;
     s.code_off2 = c.code_offset2();
@@ -746,33 +747,63 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int 
         s.causal_rows = i == 1 && causal ? n_rows : 0;
         tiles[i] = (s.T + KT - 1) / KT;
     }
-    // Tiles a split: the count with the shortest launch (a unit's prologue and partials cost
-    // about two tiles, a partial row read again by the merge a share of one).
-    const int most = std::max(tiles[0], tiles[1]);
-    const int64_t u0 = (int64_t)n_qt[0] * a.seg[0].heads, u1 = (int64_t)n_qt[1] * a.seg[1].heads;
-    int best = most;
-    double best_cost = 1e30;
-    for (int tps = 1; tps <= most; tps += std::max(1, tps / 16)) {
-        const int s0 = (tiles[0] + tps - 1) / tps, s1 = (tiles[1] + tps - 1) / tps;
-        if (s0 + s1 > kSharedMaxSlots) continue;
-        const double cost = makespan(u0 * s0, std::min(tps, tiles[0]) + 2.0, u1 * s1, std::min(tps, tiles[1]) + 2.0) +
-                            (s0 + s1) * (double)a.R * hkv * D * 2e-7;
-        if (cost < best_cost) {
-            best_cost = cost;
-            best = tps;
-        }
-    }
+    // Tiles a split, for each launch: the count with the shortest estimate. A unit's us: a start and an
+    // end that grow with its rows, and a time a tile (measured: 30 and 126 rows of 8-bit keys at D = 256
+    // 23.6 and 38.4 us in 8 tiles, 126 rows 103 us in 32; few rows 14.5 us in 9); a partial row costs its
+    // write and its read by the merge.
     a.n_slots = 0;
-    for (int i = 0; i < 2; i++) {
-        SharedSegment& s = a.seg[i];
-        if (!c[i]) continue;
-        s.tiles_per_split = best;
-        s.n_split = (tiles[i] + best - 1) / best;
-        s.slot0 = a.n_slots;
-        a.n_slots += s.n_split;
-        const int64_t units = (int64_t)n_qt[i] * s.heads * s.n_split;
-        QW_REQUIRE(units < (int64_t)1 << 30, QW_ERR_UNSUPPORTED, "shared attention: too many rows for one call");
-        s.n_units = (int)units;
+    auto plan = [&](std::initializer_list<int> in) -> int {
+        bool few = true;
+        int most = 0;
+        for (int i : in)
+            if (c[i]) {
+                few = few && a.seg[i].unit_rows <= kFewRows;
+                most = std::max(most, tiles[i]);
+            }
+        auto unit_us = [&](int i, int n) {
+            const SharedSegment& s = a.seg[i];
+            if (few) return 5.0 + 0.65 * n;
+            const double fill = (double)s.unit_rows / (16 * many_tiles(D) * kWaves);
+            return 6.0 + 4.0 * fill + n * (1.0 + 1.5 * fill + (s.bits == 16 ? 0.6 : 0.0));
+        };
+        int best = most;
+        double best_cost = 1e30;
+        for (int tps = 1; tps <= most; tps += std::max(1, tps / 16)) {
+            double us[2] = {0.0, 1.0};
+            int64_t units[2] = {0, 0};
+            int slots = 0;
+            for (int i : in) {
+                if (!c[i]) continue;
+                const int n = (tiles[i] + tps - 1) / tps;
+                us[i] = unit_us(i, std::min(tps, tiles[i]));
+                units[i] = (int64_t)n_qt[i] * a.seg[i].heads * n;
+                slots += n;
+            }
+            if (slots > kSharedMaxSlots) continue;
+            const double cost = makespan(units[0], us[0], units[1], us[1]) + 1.8e-6 * slots * a.R * hkv * D;
+            if (cost < best_cost) {
+                best_cost = cost;
+                best = tps;
+            }
+        }
+        for (int i : in) {
+            SharedSegment& s = a.seg[i];
+            if (!c[i]) continue;
+            s.tiles_per_split = best;
+            s.n_split = (tiles[i] + best - 1) / best;
+            s.slot0 = a.n_slots;
+            a.n_slots += s.n_split;
+            const int64_t units = (int64_t)n_qt[i] * s.heads * s.n_split;
+            QW_REQUIRE(units < (int64_t)1 << 30, QW_ERR_UNSUPPORTED, "shared attention: too many rows for one call");
+            s.n_units = (int)units;
+        }
+        return QW_OK;
+    };
+    if (c[0] && c[1] && c[0]->bits != c[1]->bits) {
+        if (int rc = plan({0})) return rc;
+        if (int rc = plan({1})) return rc;
+    } else if (int rc = plan({0, 1})) {
+        return rc;
     }
     const size_t rows = (size_t)a.n_slots * hkv * a.R;
     const size_t o_bytes = a.n_slots > 1 ? rows * D * sizeof(float) : 0;

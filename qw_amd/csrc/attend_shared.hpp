@@ -14,7 +14,7 @@ struct SharedSegment {
     const uint32_t* v_data;
     const uint32_t* v_params;
     const int* fast_flag;         // device: every stored scale is in the range of the short dequantization
-    int cap, T;
+    int bits, cap, T;
     uint32_t code_off2;
     int heads, rows;              // the cache's heads; query rows of each
     int unit_rows;                // rows of a unit (the head's rows in equal query tiles)
