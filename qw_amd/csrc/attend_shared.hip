@@ -661,8 +661,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_few_kernel(SharedArgs a
 
 template <int D>
 __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
-    __shared__ SharedMerge<D> sm;
-    merge_row<D>(a, blockIdx.x, blockIdx.y, sm);
+    __shared__ SharedMerge sm;
+    merge_group<D>(a, blockIdx.x, blockIdx.y, sm);
 }
 
 // What a launch of n_pre units of a us and, behind them, n_tail units of b us takes on 256 CUs.
@@ -830,10 +830,11 @@ int launch_shared(const KVCache* prefix, const KVCache* tails, const SharedArgs&
 
 int launch_shared_merge(int D, const SharedArgs& a, hipStream_t stream) {
     if (a.n_slots == 1) return QW_OK;
+    const dim3 grid(merge_groups(D, a.R, a.hkv, a.n_slots), a.hkv);
     if (D == 256)
-        hipLaunchKernelGGL(shared_merge_kernel<256>, dim3(a.R, a.hkv), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(shared_merge_kernel<256>, grid, dim3(256), 0, stream, a);
     else
-        hipLaunchKernelGGL(shared_merge_kernel<128>, dim3(a.R, a.hkv), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(shared_merge_kernel<128>, grid, dim3(256), 0, stream, a);
     QW_HIP_CHECK(hipGetLastError());
     return QW_OK;
 }

@@ -32,6 +32,7 @@ struct SharedArgs {
     const int32_t* starts;  // [n_seq] or null: a sequence's first tail key
     int Tq, G, hkv, R;      // R = n_seq * Tq * G: row (b * Tq + r) * G + head in group
     int n_slots;
+    float2* row_ml;         // null, or [hkv][R]: the merge leaves a row's maximum (log2 units) and 1 / its sum
     float* scores;          // null, or [hkv][R][score_stride]: the scores (log2 units) of one cache's few rows
     int64_t score_stride;   // a multiple of 32
     float scale2;           // |scale| * log2 e
@@ -64,59 +65,89 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int 
 int launch_shared(const KVCache* prefix, const KVCache* tails, const SharedArgs& a, hipStream_t stream);
 int launch_shared_merge(int D, const SharedArgs& a, hipStream_t stream);
 
-// A row's partials joined by a workgroup of 256: D / 4 threads a partial row, 1024 / D partial rows
-// at a time and four such in flight, their sums over LDS.
-template <int D>
+// Rows' partials joined by workgroups of 256, each partial row by TC threads and SG of them at a
+// time, four such in flight, their sums over LDS. A workgroup a row (TC = D / 4), but: few rows of
+// many slots are cut into 64 dims a workgroup (24 rows of 57 slots 7.0 -> 4.9 us beside the key
+// weights, 960 of 45 7.8 -> 10.1), and of many rows of few slots a workgroup takes 1024 / D
+// (36864 rows of 3 slots 34.7 -> 30.4 us, 64 of 3 3.2 -> 4.3).
+enum MergeForm { kMergeRow, kMergeCut, kMergeRows };
+__host__ __device__ inline MergeForm merge_form(int64_t rows, int n_slots) {
+    return n_slots > 16 && rows <= 512 ? kMergeCut : n_slots <= 8 && rows >= 4096 ? kMergeRows : kMergeRow;
+}
+__host__ __device__ inline int merge_groups(int D, int R, int hkv, int n_slots) {
+    const MergeForm f = merge_form((int64_t)R * hkv, n_slots);
+    return f == kMergeCut ? R * (D / 64) : f == kMergeRow ? R : (R + 1024 / D - 1) / (1024 / D);
+}
 struct SharedMerge {
     float4v o[256];
-    float l[1024 / D];
+    float l[16];
 };
-template <int D>
-__device__ __forceinline__ void merge_row(const SharedArgs& a, int row, int h, SharedMerge<D>& sm) {
-    constexpr int LPR = D / 4, NS = 256 / LPR, AHEAD = 4;
-    const int tid = threadIdx.x, c = tid % LPR, s0 = tid / LPR;
+template <int D, int SG, int TC>
+__device__ __forceinline__ void merge_rows(const SharedArgs& a, int group, int h, SharedMerge& sm) {
+    constexpr int AHEAD = 4, CUTS = SG == 1 ? 1 : D / 4 / TC;  // workgroups a row
+    const int tid = threadIdx.x, sg = SG == 1 ? 0 : tid / TC;
+    const int row = SG == 1 ? group * (256 / TC) + tid / TC : group / CUTS;
+    const int c = group % CUTS * TC + tid % TC;
+    if (row >= a.R) return;  // (SG == 1: no barrier follows)
     const int64_t stride = (int64_t)a.hkv * a.R, at = (int64_t)h * a.R + row;
     float M = -INFINITY;
-    for (int s = tid & 63; s < a.n_slots; s += 64) M = fmaxf(M, a.part_ml[s * stride + at].x);
-    M = wave_reduce(M, OpMax{});
+    if constexpr (SG == 1) {
+        for (int s = 0; s < a.n_slots; s++) M = fmaxf(M, a.part_ml[s * stride + at].x);
+    } else {
+        for (int s = tid & 63; s < a.n_slots; s += 64) M = fmaxf(M, a.part_ml[s * stride + at].x);
+        M = wave_reduce(M, OpMax{});
+    }
     const float mr = M == -INFINITY ? 0.0f : M;
     float4v o = {0.f, 0.f, 0.f, 0.f};
     float l = 0.0f;
-    for (int s = s0; s < a.n_slots; s += NS * AHEAD) {
+    for (int s = sg; s < a.n_slots; s += SG * AHEAD) {
         float2 ml[AHEAD];
         float4v x[AHEAD];
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
-            const int64_t p = min(s + NS * i, a.n_slots - 1) * stride + at;
+            const int64_t p = min(s + SG * i, a.n_slots - 1) * stride + at;
             ml[i] = a.part_ml[p];
             x[i] = *(const float4v*)(a.part_o + p * D + 4 * c);
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
-            if (s + NS * i >= a.n_slots) break;
+            if (s + SG * i >= a.n_slots) break;
             const float f = __builtin_amdgcn_exp2f(ml[i].x - mr);
             l += f * ml[i].y;
 #pragma unroll
             for (int j = 0; j < 4; j++) o[j] += f * x[i][j];
         }
     }
-    sm.o[tid] = o;
-    if (c == 0) sm.l[s0] = l;
-    __syncthreads();
-    if (s0 > 0) return;
+    if constexpr (SG > 1) {
+        sm.o[tid] = o;
+        if (tid % TC == 0) sm.l[sg] = l;
+        __syncthreads();
+        if (sg > 0) return;
 #pragma unroll
-    for (int s = 1; s < NS; s++) {
-        const float4v x = sm.o[s * LPR + c];
+        for (int s = 1; s < SG; s++) {
+            const float4v x = sm.o[s * TC + tid];
 #pragma unroll
-        for (int j = 0; j < 4; j++) o[j] += x[j];
-        l += sm.l[s];
+            for (int j = 0; j < 4; j++) o[j] += x[j];
+            l += sm.l[s];
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (a.row_ml && c == 0) a.row_ml[at] = float2{mr, inv};
     const int seq = row / (a.Tq * a.G), rr = row % (a.Tq * a.G);
     half4v y;
 #pragma unroll
     for (int j = 0; j < 4; j++) y[j] = (f16)(o[j] * inv);
     *(half4v*)(a.out + (((int64_t)seq * a.hkv * a.G + h * a.G + rr % a.G) * a.Tq + rr / a.G) * D + 4 * c) = y;
+}
+template <int D>
+__device__ __forceinline__ void merge_group(const SharedArgs& a, int group, int h, SharedMerge& sm) {
+    const MergeForm f = merge_form((int64_t)a.R * a.hkv, a.n_slots);
+    if (f == kMergeCut)
+        merge_rows<D, 16, 16>(a, group, h, sm);
+    else if (f == kMergeRow)
+        merge_rows<D, 1024 / D, D / 4>(a, group, h, sm);
+    else
+        merge_rows<D, 1, D / 4>(a, group, h, sm);
 }
 
 }  // namespace qw

@@ -30,7 +30,6 @@ namespace {
 
 struct WeightArgs {
     SharedArgs s;            // seg[1]: the cache
-    const float2* row_ml;    // [hkv][R]: the row's maximum (log2 units) and 1 / its sum
     const float* weights;    // [hkv][ws_in] or null
     float* weights_out;      // [hkv][ws_out]
     float* part;             // [row_splits][hkv][T] where the rows are split
@@ -47,23 +46,14 @@ __device__ __forceinline__ void store_weight(const WeightArgs& w, int h, int key
     w.weights_out[h * w.ws_out + key] = x;
 }
 
-// A row's maximum and 1 / sum over its partials (apart: one logarithm of the sum would round
-// at the maximum's size): grid (R / 4, hkv), a wave a row.
-__global__ __launch_bounds__(256) void row_sums_kernel(SharedArgs a, float2* __restrict__ row_ml) {
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y, lane = threadIdx.x & 63;
+// A row's maximum and 1 / sum (apart: one logarithm of the sum would round at the maximum's size)
+// where one slot holds it and no merge runs: a thread a row, grid (R / 256, hkv).
+__global__ __launch_bounds__(256) void row_sums_kernel(SharedArgs a) {
+    const int row = blockIdx.x * 256 + threadIdx.x;
     if (row >= a.R) return;
-    const int64_t stride = (int64_t)a.hkv * a.R, at = (int64_t)h * a.R + row;
-    float M = -INFINITY;
-    for (int s = lane; s < a.n_slots; s += 64) M = fmaxf(M, a.part_ml[s * stride + at].x);
-    M = wave_reduce(M, OpMax{});
-    const float mr = M == -INFINITY ? 0.0f : M;
-    float l = 0.0f;
-    for (int s = lane; s < a.n_slots; s += 64) {
-        const float2 ml = a.part_ml[s * stride + at];
-        l += __builtin_amdgcn_exp2f(ml.x - mr) * ml.y;
-    }
-    l = wave_reduce(l, OpSum{});
-    if (lane == 0) row_ml[at] = float2{mr, l == 0.0f ? 0.0f : 1.0f / l};
+    const int64_t at = (int64_t)blockIdx.y * a.R + row;
+    const float2 ml = a.part_ml[at];
+    a.row_ml[at] = float2{ml.x == -INFINITY ? 0.0f : ml.x, ml.y == 0.0f ? 0.0f : 1.0f / ml.y};
 }
 
 template <int KIND, int D>
@@ -143,7 +133,7 @@ __global__ __launch_bounds__(64 * kWgWaves) void key_weights_kernel(WeightArgs w
         }
     };
     auto stats = [&](int row) {  // (a row past the last: weights of 2^-inf times 0)
-        const float2 ml = w.row_ml[(int64_t)h * R + min(row, R - 1)];
+        const float2 ml = w.s.row_ml[(int64_t)h * R + min(row, R - 1)];
         return row < R ? ml : float2{INFINITY, 0.0f};
     };
     float sum[2][8] = {};
@@ -230,16 +220,16 @@ __global__ __launch_bounds__(256) void add_weights_kernel(WeightArgs w) {
     store_weight(w, h, key, x);
 }
 
-// Few rows (the attention launch kept their scores): the rows merged by the first R workgroups of
+// Few rows (the attention launch kept their scores): the rows merged by the first workgroups of
 // a head and the keys' weights formed by the others, 1024 keys each, from the scores and the rows'
 // statistics, which every one of them joins for itself.
 template <int D>
 __global__ __launch_bounds__(256) void finish_few_kernel(WeightArgs w, int n_merge) {
-    __shared__ SharedMerge<D> sm;
+    __shared__ SharedMerge sm;
     __shared__ float2 s_ml[16];
     const int h = blockIdx.y, tid = threadIdx.x, R = w.s.R, T = w.s.seg[1].T;
     if ((int)blockIdx.x < n_merge) {
-        merge_row<D>(w.s, blockIdx.x, h, sm);
+        merge_group<D>(w.s, blockIdx.x, h, sm);
         return;
     }
     {
@@ -343,7 +333,7 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
             return rc;
         w.s.scores = (float*)scores;
         if (int rc = launch_shared(nullptr, &c, w.s, stream)) return rc;
-        const int n_merge = w.s.n_slots > 1 ? w.s.R : 0;
+        const int n_merge = w.s.n_slots > 1 ? merge_groups(c.D, w.s.R, c.hkv, w.s.n_slots) : 0;
         const dim3 grid(n_merge + (c.offset + 1023) / 1024, c.hkv);
         if (c.D == 256)
             hipLaunchKernelGGL(finish_few_kernel<256>, grid, dim3(256), 0, stream, w, n_merge);
@@ -362,11 +352,13 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
     void* row_ml = nullptr;
     if (int rc = workspace(kWsRowSums, c.device, stream, ml_bytes + part_bytes, &row_ml)) return rc;
     w.part = (float*)((char*)row_ml + ml_bytes);
+    w.s.row_ml = (float2*)row_ml;
     if (int rc = launch_shared(nullptr, &c, w.s, stream)) return rc;
     if (int rc = launch_shared_merge(c.D, w.s, stream)) return rc;
-    w.row_ml = (const float2*)row_ml;
-    hipLaunchKernelGGL(row_sums_kernel, dim3((w.s.R + 3) / 4, c.hkv), dim3(256), 0, stream, w.s, (float2*)row_ml);
-    QW_HIP_CHECK(hipGetLastError());
+    if (w.s.n_slots == 1) {
+        hipLaunchKernelGGL(row_sums_kernel, dim3((w.s.R + 255) / 256, c.hkv), dim3(256), 0, stream, w.s);
+        QW_HIP_CHECK(hipGetLastError());
+    }
     if (c.D == 256)
         return c.bits == 4   ? launch_weights<4, 256>(w, stream)
                : c.bits == 8 ? launch_weights<8, 256>(w, stream)
