@@ -43,6 +43,11 @@ namespace qw {
 namespace {
 
 constexpr int kWaves = 8, kFillWaves = 4;
+// Query tiles from which the key tiles of one quantized cache are laid out once. 256-row tiles of 8 heads,
+// D = 128, and 128-row ones of 4, D = 256, over 4k and 32k 4- and 8-bit keys: dequantized in each / laid
+// out, 2 tiles 33 / 34 and 62 / 93 us, 6 tiles 41 / 43 and 143 / 162, 10 tiles 52 / 54 and 216 / 228 (8-bit 233 /
+// 232); 72 tiles over 9.7k Int8 keys 513 / 421.
+constexpr int kImageQueryTiles = 16;
 constexpr int kFewRows = 16;  // of a unit of the kernel for few rows
 // 16-row tiles a computing wave of the other: what 168 registers hold (three waves a SIMD).
 __host__ __device__ constexpr int many_tiles(int D) { return D == 256 ? 1 : 2; }
@@ -122,9 +127,122 @@ __device__ __forceinline__ void keep_reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x008, MF * AH, GROUP);
 }
 
+// A dequantizing group of 256 threads: a key tile's codes through registers into an LDS tile of
+// block_tile.hpp's layout, V's slots in the fp16 order whatever the codes'. The values are
+// f16(f16(code * scale) + bias), as the fetch gives them. NATURAL: K's dims in order also from 4-bit
+// codes (else pairs (0,4), (1,5), (2,6), (3,7) of each eight).
+template <int KIND, int D, bool FAST, bool NATURAL>
+struct TileFiller {
+    using S = BlockShape<D>;
+    static constexpr int KT = S::KT, TPR = S::TPR, TPB = S::TPB, NG = S::NG, DPL = D / 16;
+    static constexpr int PER = KT * TPR / (64 * kFillWaves);  // slices of each kind a thread
+    static constexpr int KU = KIND / 4;                       // 16-byte loads of a 32-dim K slice / 4-slot V slice
+    static_assert(PER * 64 * kFillWaves == KT * TPR && (KT / 8) * TPB == KT * TPR, "whole slices a thread");
+    struct Stage {
+        u32x4 kc[PER][KU], vc[PER][KU], vp[PER][2];
+        uint32_t kp[PER];
+    };
+    const char *k_head, *kp_head, *v_head, *vp_head;
+    // slice j: key kk's 32 dims from 32 q32, V block vb's 4 slots from 4 vj
+    int q32[PER], kk[PER], vb[PER], vj[PER];
+    uint32_t code_off, magic;
+    // key0: the first key of tile 0 of head hc; t: the thread's place in the group
+    __device__ TileFiller(const SharedSegment& c, int hc, int key0, int t) {
+        const int64_t row = (int64_t)hc * c.cap + key0;
+        k_head = (const char*)c.k_data + row * (D * KIND / 8);
+        kp_head = (const char*)c.k_params + row * (NG * 4);
+        v_head = (const char*)c.v_data + row / 8 * (D * KIND);
+        vp_head = (const char*)c.v_params + row / 8 * (NG * 32);
+        code_off = c.code_off2;
+        magic = vconst(kMagic);
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int x = t + 64 * kFillWaves * j;
+            q32[j] = (x >> 4) & (TPR - 1);
+            kk[j] = (x & 15) | ((x >> (4 + S::LTPR)) << 4);
+            vb[j] = x / TPB;
+            vj[j] = x % TPB;
+        }
+    }
+    __device__ __forceinline__ int v_n(int j) const {  // lane group of slot 4 vj
+        return KIND == 16 ? 0 : KIND == 8 ? (2 * vj[j]) % 16 : vj[j] % 16;
+    }
+    __device__ __forceinline__ void load(Stage& st, int i) const {
+        const int64_t key = (int64_t)i * KT;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const u32x4* k = (const u32x4*)(k_head + key * (D * KIND / 8) + (kk[j] * (D * KIND / 8) + 16 * KU * q32[j]));
+            const u32x4* v = (const u32x4*)(v_head + key / 8 * (D * KIND) + (vb[j] * (D * KIND) + 16 * KU * vj[j]));
+#pragma unroll
+            for (int x = 0; x < KU; x++) st.kc[j][x] = k[x];
+#pragma unroll
+            for (int x = 0; x < KU; x++) st.vc[j][x] = v[x];
+            if constexpr (KIND != 16) {
+                st.kp[j] = *(const uint32_t*)(kp_head + key * (NG * 4) + (kk[j] * (NG * 4) + 4 * k_param_slot(q32[j] >> 1, NG)));
+                const u32x4* p = (const u32x4*)(vp_head + key / 8 * (NG * 32) + (vb[j] * (NG * 32) + v_n(j) * DPL / kGroup * 32));
+                st.vp[j][0] = p[0];
+                st.vp[j][1] = p[1];
+            }
+        }
+    }
+    // The tile whose first key is key0; keys outside [lo, hi), which no row sees, go in as zeros of V:
+    // they have weight 0, but 0 x inf is NaN.
+    __device__ __forceinline__ void store(const Stage& st, char* buf, int key0, int lo, int hi) const {
+        const bool edge = key0 < lo || key0 + KT > hi;
+        half8* const sK = (half8*)buf;
+        half8* const sV = (half8*)(buf + S::KBUF);
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            half8* const kdst = sK + kaddr<KT>(kk[j], 4 * q32[j]);
+            half8 y[4];
+            if constexpr (KIND == 16) {
+#pragma unroll
+                for (int w = 0; w < 4; w++) kdst[w * KT] = as_h8(st.kc[j][w]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = as_h8(st.vc[j][e]);
+            } else {
+                const half2v sb = h2(st.kp[j]), s = {sb.x, sb.x}, b = {sb.y, sb.y};
+                const PairConsts kc = make_consts<FAST, KIND>(s, s, s, s, b, b, b, b, code_off);
+                const u32x4 vs = st.vp[j][0], vo = st.vp[j][1];
+                const PairConsts vc = make_consts<FAST, KIND>(h2(vs[0]), h2(vs[1]), h2(vs[2]), h2(vs[3]), h2(vo[0]), h2(vo[1]),
+                                                              h2(vo[2]), h2(vo[3]), code_off);
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    if constexpr (KIND == 4) {
+                        u32x4 x = __builtin_bit_cast(u32x4, deq4<FAST>(st.kc[j][0][w], kc, magic));
+                        if constexpr (NATURAL)
+                            x = u32x4{__builtin_amdgcn_perm(x.y, x.x, 0x05040100u), __builtin_amdgcn_perm(x.w, x.z, 0x05040100u),
+                                      __builtin_amdgcn_perm(x.y, x.x, 0x07060302u), __builtin_amdgcn_perm(x.w, x.z, 0x07060302u)};
+                        kdst[w * KT] = as_h8(x);
+                        y[w] = deq4<FAST>(st.vc[j][0][w], vc, magic);
+                    } else {
+                        kdst[w * KT] = deq8<FAST>(st.kc[j][KU / 2 * (w / 2)][2 * (w % 2)], st.kc[j][KU / 2 * (w / 2)][2 * (w % 2) + 1], kc);
+                        y[w] = deq8<FAST>(st.vc[j][KU / 2 * (w / 2)][2 * (w % 2)], st.vc[j][KU / 2 * (w / 2)][2 * (w % 2) + 1], vc);
+                    }
+                }
+            }
+            if (edge) {
+                asm volatile("");
+                const int key = key0 + 8 * vb[j];
+                const u32x4 keep = keep_keys(hi - key) & ~keep_keys(lo - key);
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = as_h8(__builtin_bit_cast(u32x4, y[e]) & keep);
+            }
+            const int vr = KIND == 8 ? 2 * (vj[j] / 8) : 4 * (vj[j] / 16);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int at = KIND == 16  ? 4 * vj[j] + e + (vj[j] >> 2)
+                               : KIND == 8 ? 17 * (vr + e % 2) + v_n(j) + e / 2
+                                           : 17 * (vr + e) + v_n(j);
+                sV[vb[j] * S::VROW + at] = y[e];
+            }
+        }
+    }
+};
+
 // Units of many rows, 12 waves. Waves 8 to 11, one a SIMD, dequantize: tile i + 1 (its codes in
-// registers since two tiles ago) into the free one of two LDS buffers (block_tile.hpp's layout, V's
-// slots in the fp16 order whatever the codes'), then request tile i + 3's codes. Waves 0 to 7, two a
+// registers since two tiles ago) into the free one of two LDS buffers, then request tile i + 3's codes;
+// IMAGE: they copy tile i + 1 from images of the tiles that a launch before made once. Waves 0 to 7, two a
 // SIMD, compute tile i, RT row tiles of 16 each:
 //   S^T = K . Q^T (a lane then holds 8 consecutive keys of a row, the A operand of P . V), scores in
 //   fp32, P in fp16 against a reference that moves when a score passes it by kLazy = 8 powers of two
@@ -133,17 +251,12 @@ __device__ __forceinline__ void keep_reads_ahead() {
 // Where the rows leave waves free these take parts of each tile's keys, joined at the end through LDS.
 // One barrier a tile. (With 8 waves that dequantize and compute in turn, all of them were in the same
 // phase: LDS idle while they dequantize, the VALU while they read.)
-template <int KIND, int D, bool FAST>
+template <int KIND, int D, bool FAST, bool IMAGE>
 __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
     using S = BlockShape<D>;
-    constexpr int KT = S::KT, NSUB = S::NSUB, NM = S::NM, NT = S::NT, NG = S::NG, VROW = S::VROW;
-    constexpr int TPR = S::TPR, LTPR = S::LTPR, TPB = S::TPB, BUF = S::BUF, KBUF = S::KBUF;
-    constexpr int PER = KT * TPR / (64 * kFillWaves);  // slices of each kind a dequantizing thread
+    constexpr int KT = S::KT, NSUB = S::NSUB, NM = S::NM, NT = S::NT, VROW = S::VROW, BUF = S::BUF, KBUF = S::KBUF;
     constexpr int RT = many_tiles(D);
-    constexpr int KU = KIND / 4;               // 16-byte loads of a 32-dim K slice / 4-slot V slice
-    constexpr int DPL = D / 16;
     constexpr float kLazy = 8.0f;
-    static_assert(PER * 64 * kFillWaves == KT * TPR && (KT / 8) * TPB == KT * TPR, "whole slices a thread");
     static_assert(2 * BUF <= kSharedLds, "LDS");
     const Unit u = this_unit<D>(a);
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
@@ -156,114 +269,64 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
     static_assert((kWaves - kWaves / (NSUB < 8 ? NSUB : 8)) * REG <= kSharedLds, "the parked parts fit");
 
     if (wave >= kWaves) {
-        // ---- dequantizing waves
-        struct Stage {
-            u32x4 kc[PER][KU], vc[PER][KU], vp[PER][2];
-            uint32_t kp[PER];
-        };
-        const uint32_t magic = vconst(kMagic);
-        const char* const k_head = (const char*)u.k_data + ((int64_t)u.hc * u.cap + u.k_begin) * (D * KIND / 8);
-        const char* const kp_head = (const char*)u.k_params + ((int64_t)u.hc * u.cap + u.k_begin) * (NG * 4);
-        const char* const v_head = (const char*)u.v_data + (((int64_t)u.hc * u.cap + u.k_begin) / 8) * (D * KIND);
-        const char* const vp_head = (const char*)u.v_params + (((int64_t)u.hc * u.cap + u.k_begin) / 8) * (NG * 32);
-        // slice j: key kk's 32 dims from 32 q32, V block vb's 4 slots from 4 vj
-        int q32[PER], kk[PER], vb[PER], vj[PER];
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int t = tid - 64 * kWaves + 64 * kFillWaves * j;
-            q32[j] = (t >> 4) & (TPR - 1);
-            kk[j] = (t & 15) | ((t >> (4 + LTPR)) << 4);
-            vb[j] = t / TPB;
-            vj[j] = t % TPB;
-        }
-        auto v_n = [&](int j) { return KIND == 16 ? 0 : KIND == 8 ? (2 * vj[j]) % 16 : vj[j] % 16; };  // lane group of slot 4 vj
-        auto load = [&](Stage& st, int i) {
-            const int64_t key = (int64_t)i * KT;
-#pragma unroll
-            for (int j = 0; j < PER; j++) {
-                const u32x4* k = (const u32x4*)(k_head + key * (D * KIND / 8) + (kk[j] * (D * KIND / 8) + 16 * KU * q32[j]));
-                const u32x4* v = (const u32x4*)(v_head + key / 8 * (D * KIND) + (vb[j] * (D * KIND) + 16 * KU * vj[j]));
-#pragma unroll
-                for (int x = 0; x < KU; x++) st.kc[j][x] = k[x];
-#pragma unroll
-                for (int x = 0; x < KU; x++) st.vc[j][x] = v[x];
-                if constexpr (KIND != 16) {
-                    st.kp[j] = *(const uint32_t*)(kp_head + key * (NG * 4) + (kk[j] * (NG * 4) + 4 * k_param_slot(q32[j] >> 1, NG)));
-                    const u32x4* p = (const u32x4*)(vp_head + key / 8 * (NG * 32) + (vb[j] * (NG * 32) + v_n(j) * DPL / kGroup * 32));
-                    st.vp[j][0] = p[0];
-                    st.vp[j][1] = p[1];
+        // ---- filling waves
+        const SharedSegment& seg = (int)blockIdx.x >= a.seg[0].n_units ? a.seg[1] : a.seg[0];
+        if constexpr (IMAGE) {
+            // tile i's image into its buffer by LDS-DMA, 1 KB a wave instruction; M0, which gives its place
+            // in LDS, is saved and restored so that the compiler's view of it holds
+            const char* const img = seg.images + ((int64_t)u.hc * seg.n_tiles + u.k_begin / KT) * BUF + 16 * lane;
+            const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds;
+            static_assert(BUF % 1024 == 0, "whole DMA instructions");
+            auto copy = [&](int i) {
+                for (int c = wave - kWaves; c < BUF / 1024; c += kFillWaves) {
+                    uint32_t saved;
+                    asm volatile(
+                        "s_mov_b32 %0, m0\n\t"
+                        "s_mov_b32 m0, %2\n\t"
+                        "s_nop 0\n\t"
+                        "global_load_lds_dwordx4 %1, off\n\t"
+                        "s_nop 0\n\t"
+                        "s_mov_b32 m0, %0"
+                        : "=&s"(saved)
+                        : "v"(img + (int64_t)i * BUF + 1024 * c),
+                          "s"(__builtin_amdgcn_readfirstlane(lds0 + BUF * (i & 1) + 1024 * c))
+                        : "memory");
                 }
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            };
+            if (n > 0) copy(0);
+            __syncthreads();
+            for (int i = 0; i < n; i++) {
+                if (i + 1 < n) copy(i + 1);
+                __syncthreads();
             }
-        };
-        // f16(f16(code * scale) + bias), as the fetch gives it
-        auto store = [&](const Stage& st, int i) {
-            half8* const sK = (half8*)(lds + BUF * (i & 1));
-            half8* const sV = (half8*)(lds + BUF * (i & 1) + KBUF);
-            const int key0 = u.k_begin + i * KT;
-            const bool edge = key0 < u.lo || key0 + KT > u.hi;
-#pragma unroll
-            for (int j = 0; j < PER; j++) {
-                half8* const kdst = sK + kaddr<KT>(kk[j], 4 * q32[j]);
-                half8 y[4];
-                if constexpr (KIND == 16) {
-#pragma unroll
-                    for (int w = 0; w < 4; w++) kdst[w * KT] = as_h8(st.kc[j][w]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) y[e] = as_h8(st.vc[j][e]);
-                } else {
-                    const half2v sb = h2(st.kp[j]), s = {sb.x, sb.x}, b = {sb.y, sb.y};
-                    const PairConsts kc = make_consts<FAST, KIND>(s, s, s, s, b, b, b, b, u.code_off);
-                    const u32x4 vs = st.vp[j][0], vo = st.vp[j][1];
-                    const PairConsts vc = make_consts<FAST, KIND>(h2(vs[0]), h2(vs[1]), h2(vs[2]), h2(vs[3]), h2(vo[0]), h2(vo[1]),
-                                                                  h2(vo[2]), h2(vo[3]), u.code_off);
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        if constexpr (KIND == 4) {
-                            kdst[w * KT] = deq4<FAST>(st.kc[j][0][w], kc, magic);
-                            y[w] = deq4<FAST>(st.vc[j][0][w], vc, magic);
-                        } else {
-                            kdst[w * KT] = deq8<FAST>(st.kc[j][KU / 2 * (w / 2)][2 * (w % 2)], st.kc[j][KU / 2 * (w / 2)][2 * (w % 2) + 1], kc);
-                            y[w] = deq8<FAST>(st.vc[j][KU / 2 * (w / 2)][2 * (w % 2)], st.vc[j][KU / 2 * (w / 2)][2 * (w % 2) + 1], vc);
-                        }
-                    }
-                }
-                if (edge) {  // keys that no row sees have weight 0, but 0 x inf is NaN
-                    asm volatile("");
-                    const int key = key0 + 8 * vb[j];
-                    const u32x4 keep = keep_keys(u.hi - key) & ~keep_keys(u.lo - key);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) y[e] = as_h8(__builtin_bit_cast(u32x4, y[e]) & keep);
-                }
-                const int vr = KIND == 8 ? 2 * (vj[j] / 8) : 4 * (vj[j] / 16);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int at = KIND == 16  ? 4 * vj[j] + e + (vj[j] >> 2)
-                                   : KIND == 8 ? 17 * (vr + e % 2) + v_n(j) + e / 2
-                                               : 17 * (vr + e) + v_n(j);
-                    sV[vb[j] * VROW + at] = y[e];
-                }
-            }
-        };
-        Stage s0, s1;  // tiles 1, 3, .. and 2, 4, ..
-        if (n > 0) {
-            load(s0, 0);
-            if (n > 2) load(s1, 2);
-            store(s0, 0);
-            if (n > 1) load(s0, 1);
-        }
-        __syncthreads();
-        for (int i = 0; i < n; i += 2) {
-            if (i + 1 < n) {
-                store(s0, i + 1);
-                if (i + 3 < n) load(s0, i + 3);
+        } else {
+            using Filler = TileFiller<KIND, D, FAST, false>;
+            const Filler f(seg, u.hc, u.k_begin, tid - 64 * kWaves);
+            auto put = [&](const typename Filler::Stage& st, int i) {
+                f.store(st, lds + BUF * (i & 1), u.k_begin + i * KT, u.lo, u.hi);
+            };
+            typename Filler::Stage s0, s1;  // tiles 1, 3, .. and 2, 4, ..
+            if (n > 0) {
+                f.load(s0, 0);
+                if (n > 2) f.load(s1, 2);
+                put(s0, 0);
+                if (n > 1) f.load(s0, 1);
             }
             __syncthreads();
-            if (i + 1 >= n) break;
-            if (i + 2 < n) {
-                store(s1, i + 2);
-                if (i + 4 < n) load(s1, i + 4);
+            for (int i = 0; i < n; i += 2) {
+                if (i + 1 < n) {
+                    put(s0, i + 1);
+                    if (i + 3 < n) f.load(s0, i + 3);
+                }
+                __syncthreads();
+                if (i + 1 >= n) break;
+                if (i + 2 < n) {
+                    put(s1, i + 2);
+                    if (i + 4 < n) f.load(s1, i + 4);
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
         if (parts > 1) __syncthreads();
         return;
@@ -648,8 +711,34 @@ template <int KIND, int D>
 __global__ __launch_bounds__(64 * (kWaves + kFillWaves), 1) void shared_many_kernel(SharedArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     if constexpr (KIND != 16)
-        if (unit_fast(a)) return many_body<KIND, D, true>(a, lds);
-    many_body<KIND, D, false>(a, lds);
+        if (unit_fast(a)) return many_body<KIND, D, true, false>(a, lds);
+    many_body<KIND, D, false, false>(a, lds);
+}
+template <int D>
+__global__ __launch_bounds__(64 * (kWaves + kFillWaves), 1) void shared_image_many_kernel(SharedArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    many_body<16, D, false, true>(a, lds);
+}
+// The key tiles of a cache as the kernel above copies them: grid (tiles, heads).
+template <int KIND, int D>
+__global__ __launch_bounds__(64 * kFillWaves) void shared_image_kernel(SharedSegment c, char* images) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    using S = BlockShape<D>;
+    const int tid = threadIdx.x, t = blockIdx.x, hc = blockIdx.y;
+    auto fill = [&](auto fast_c) {
+        using Filler = TileFiller<KIND, D, decltype(fast_c)::value, true>;
+        const Filler f(c, hc, t * S::KT, tid);
+        typename Filler::Stage st;
+        f.load(st, 0);
+        f.store(st, lds, t * S::KT, 0, c.T);
+    };
+    if (KIND != 16 && *c.fast_flag)
+        fill(std::true_type{});
+    else
+        fill(std::false_type{});
+    __syncthreads();
+    char* const to = images + ((int64_t)hc * c.n_tiles + t) * S::BUF;
+    for (int i = 16 * tid; i < S::BUF; i += 16 * 64 * kFillWaves) *(u32x4*)(to + i) = *(const u32x4*)(lds + i);
 }
 template <int KIND, int D>
 __global__ __launch_bounds__(64 * kWaves, 1) void shared_few_kernel(SharedArgs a) {
@@ -690,7 +779,21 @@ void fill_cache(SharedSegment& s, const KVCache& c) {
 }
 
 template <int KIND, int D>
+int launch_images(const SharedArgs& a, hipStream_t stream) {
+    const SharedSegment& c = a.seg[1];
+    if (int rc = ensure_dynamic_lds((const void*)shared_image_kernel<KIND, D>, BlockShape<D>::BUF)) return rc;
+    hipLaunchKernelGGL((shared_image_kernel<KIND, D>), dim3(c.n_tiles, c.heads), dim3(64 * kFillWaves),
+                       BlockShape<D>::BUF, stream, c, (char*)c.images);
+    QW_HIP_CHECK(hipGetLastError());
+    if (int rc = ensure_dynamic_lds((const void*)shared_image_many_kernel<D>, kSharedLds)) return rc;
+    hipLaunchKernelGGL((shared_image_many_kernel<D>), dim3(c.n_units), dim3(64 * (kWaves + kFillWaves)), kSharedLds,
+                       stream, a);
+    QW_HIP_CHECK(hipGetLastError());
+    return QW_OK;
+}
+template <int KIND, int D>
 int launch_units(const SharedArgs& a, hipStream_t stream) {
+    if (a.seg[1].images) return launch_images<KIND, D>(a, stream);
     const dim3 grid(a.seg[0].n_units + a.seg[1].n_units);
     const bool few = std::max(a.seg[0].n_units ? a.seg[0].unit_rows : 0, a.seg[1].n_units ? a.seg[1].unit_rows : 0) <= kFewRows;
     const void* const kernel = few ? (const void*)shared_few_kernel<KIND, D> : (const void*)shared_many_kernel<KIND, D>;
@@ -747,6 +850,10 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int 
         s.causal_rows = i == 1 && causal ? n_rows : 0;
         tiles[i] = (s.T + KT - 1) / KT;
     }
+    // One quantized cache under many query tiles: its key tiles are dequantized once, into images
+    // (1.03 times its fp16 K and V), not once a query tile.
+    const bool images = c[1] && !c[0] && !starts && c[1]->bits != 16 && n_qt[1] >= kImageQueryTiles &&
+                        (int64_t)hkv * c[1]->offset * D <= (int64_t)1 << 29;
     // Tiles a split, for each launch: the count with the shortest estimate. A unit's us: a start and an
     // end that grow with its rows, and a time a tile (measured: 30 and 126 rows of 8-bit keys at D = 256
     // 23.6 and 38.4 us in 8 tiles, 126 rows 103 us in 32; few rows 14.5 us in 9); a partial row costs its
@@ -764,7 +871,7 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int 
             const SharedSegment& s = a.seg[i];
             if (few) return 5.0 + 0.65 * n;
             const double fill = (double)s.unit_rows / (16 * many_tiles(D) * kWaves);
-            return 6.0 + 4.0 * fill + n * (1.0 + 1.5 * fill + (s.bits == 16 ? 0.6 : 0.0));
+            return 6.0 + 4.0 * fill + n * (images ? 1.9 : 1.0 + 1.5 * fill + (s.bits == 16 ? 0.6 : 0.0));
         };
         int best = most;
         double best_cost = 1e30;
@@ -806,12 +913,15 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int 
         return rc;
     }
     const size_t rows = (size_t)a.n_slots * hkv * a.R;
-    const size_t o_bytes = a.n_slots > 1 ? rows * D * sizeof(float) : 0;
+    const size_t o_bytes = a.n_slots > 1 ? rows * D * sizeof(float) : 0, ml_bytes = (rows * sizeof(float2) + 15) / 16 * 16;
+    const size_t img_bytes = images ? (size_t)a.seg[1].heads * tiles[1] * (D == 256 ? BlockShape<256>::BUF : BlockShape<128>::BUF) : 0;
     void* ws = nullptr;
-    if (int rc = workspace(kWsShared, (prefix ? prefix : tails)->device, stream, o_bytes + rows * sizeof(float2), &ws))
+    if (int rc = workspace(kWsShared, (prefix ? prefix : tails)->device, stream, o_bytes + ml_bytes + img_bytes, &ws))
         return rc;
     a.part_o = (float*)ws;
     a.part_ml = (float2*)((char*)ws + o_bytes);
+    if (images) a.seg[1].images = (const char*)ws + o_bytes + ml_bytes;
+    a.seg[1].n_tiles = tiles[1];
     return QW_OK;
 }
 

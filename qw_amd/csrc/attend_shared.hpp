@@ -21,6 +21,8 @@ struct SharedSegment {
     int n_split, tiles_per_split;
     int n_units;                  // heads * query tiles * n_split; 0: no such keys
     int slot0;                    // its first split's partial slot
+    const char* images;           // null, or its key tiles dequantized (the tails alone): [heads][n_tiles]
+    int n_tiles;
     int causal_rows;              // > 0: of that many last rows, row r sees keys to T - causal_rows + r
 };
 

@@ -185,7 +185,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_digit_kernel(SelectArgs a, 
     if (d > 0) {
         hist_d = a.hist + ((int64_t)(d - 1) * hkv + h) * a.chunks * (kBins / 2);
         uint32_t n_hi = 0, n_lo = 0;
-#pragma unroll 8
+#pragma unroll 16
         for (int i = 0; i < a.chunks; i++) {
             const uint32_t v = hist_d[(int64_t)i * (kBins / 2) + kBins / 2 - 1 - tid];
             n_hi += v >> 16;
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_digit_kernel(SelectArgs a, 
     // kept keys above the cut and ties in the chunks before this one; protected ones too
     uint32_t n_above = 0, n_equal = 0;
     const uint32_t b2 = prefix & ((1u << digit_bits(2)) - 1);
-#pragma unroll 8
+#pragma unroll 16
     for (int i = 0; i < c; i++) {
         const uint32_t v = hist_d[(int64_t)i * (kBins / 2) + tid];
         n_above += (2u * tid > b2 ? v & 0xFFFFu : 0u) + (2u * tid + 1 > b2 ? v >> 16 : 0u);
@@ -368,14 +368,22 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
     }
 }
 
-// In place: the staged rows (cap_to rows a head) back to the cache's planes; 16-byte pieces.
-__global__ __launch_bounds__(256) void evict_back_kernel(const u32x4* __restrict__ from, u32x4* __restrict__ to,
-                                                         int64_t per_head, int64_t from_stride, int64_t to_stride,
-                                                         int64_t total) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t h = i / per_head, r = i % per_head;
-        to[h * to_stride + r] = from[h * from_stride + r];
-    }
+// In place: the staged rows back to the cache's planes, in 16-byte pieces: grid (groups, hkv, plane).
+struct BackCopy {
+    const u32x4* from[4];
+    u32x4* to[4];
+    int64_t per_head[4], stride[4];  // pieces of a head's staged rows; of its rows in the cache
+};
+__global__ __launch_bounds__(256) void evict_back_kernel(BackCopy a) {
+    const u32x4* from = a.from[0];
+    u32x4* to = a.to[0];
+    int64_t per = a.per_head[0], stride = a.stride[0];
+#pragma unroll
+    for (int p = 1; p < 4; p++)
+        if ((int)blockIdx.z == p) from = a.from[p], to = a.to[p], per = a.per_head[p], stride = a.stride[p];
+    const int h = blockIdx.y;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < per; i += (int64_t)gridDim.x * 256)
+        to[h * stride + i] = from[h * per + i];
 }
 
 }  // namespace
@@ -460,14 +468,16 @@ int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_str
                                src.v_param_bytes(rows8)};
         const size_t full[4] = {src.k_data_bytes(src.cap), src.v_data_bytes(src.cap), src.k_param_bytes(src.cap),
                                 src.v_param_bytes(src.cap)};
+        BackCopy b;
         for (int i = 0; i < 4; i++) {
-            if (!per[i]) continue;
-            const int64_t ph = per[i] / src.hkv / 16, total = ph * src.hkv;
-            hipLaunchKernelGGL(evict_back_kernel, dim3((unsigned)std::min<int64_t>((total + 255) / 256, 2048)),
-                               dim3(256), 0, stream, (const u32x4*)(ws + at[i]), (u32x4*)to[i], ph, ph,
-                               (int64_t)(full[i] / src.hkv / 16), total);
-            QW_HIP_CHECK(hipGetLastError());
+            b.from[i] = (const u32x4*)(ws + at[i]);
+            b.to[i] = (u32x4*)to[i];
+            b.per_head[i] = per[i] / src.hkv / 16;
+            b.stride[i] = full[i] / src.hkv / 16;
         }
+        const int64_t groups = std::min<int64_t>((b.per_head[0] + 255) / 256, 1024);
+        hipLaunchKernelGGL(evict_back_kernel, dim3((unsigned)groups, src.hkv, src.bits == 16 ? 2 : 4), dim3(256), 0, stream, b);
+        QW_HIP_CHECK(hipGetLastError());
     }
     dst.offset = n;
     return QW_OK;

@@ -54,6 +54,9 @@ CASES = [
     ("fp16", 8, 8, 128, 130, 130, True),        # a prompt's first rows: row r sees r + 1 keys
     ("int8", 24, 4, 256, 24, 300, False),
     ("affine4", 4, 4, 128, 1, 4097, False),
+    ("affine4", 16, 1, 256, 140, 333, True),    # 2240 rows: key tiles laid out once
+    ("affine8", 32, 2, 256, 130, 130, True),
+    ("int8", 16, 1, 128, 257, 500, False),      # 4112 rows
 ]
 
 
