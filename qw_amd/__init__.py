@@ -177,10 +177,10 @@ def _hld(t, name: str):
     return t if t.is_contiguous() else t.contiguous(), H, L, D
 
 
-def _bhld(t, name: str, D: int):
-    """(B, H, L) of a batch [B, H, L, D] of fp16 rows on the device."""
-    if len(t.shape) != 4 or t.shape[3] != D or t.dtype is not _torch().float16 or not t.is_cuda:
-        raise QwError(1, f"{name}: fp16 device tensor [B, H, L, {D}] expected")
+def _bhld(t, name: str, D: int, device):
+    """(B, H, L) of a batch [B, H, L, D] of fp16 rows on the cache's device."""
+    if len(t.shape) != 4 or t.shape[3] != D or t.dtype is not _torch().float16 or t.device != device:
+        raise QwError(1, f"{name}: fp16 tensor [B, H, L, {D}] on {device} expected")
     return tuple(t.shape[:3])
 
 
@@ -447,11 +447,11 @@ class KVCache:
     # -- a prefix shared by a batch
     def _shared(self, q, tails, keys, values, scale, starts):
         torch = _torch()
-        B, hq, L = _bhld(q, "q", self.head_dim)
-        if tails is not None and tails.n_kv_heads != B * self.n_kv_heads:
-            raise QwError(1, "shared_attention: tails must have n_seq * n_kv_heads heads")
+        B, hq, L = _bhld(q, "q", self.head_dim, self.device)
+        if tails is not None and (not tails._h or tails.n_kv_heads != B * self.n_kv_heads):
+            raise QwError(1, "shared_attention: tails must be open, with n_seq * n_kv_heads heads")
         if starts is not None:
-            if starts.shape != (B,) or starts.dtype is not torch.int32 or not starts.is_cuda:
+            if starts.shape != (B,) or starts.dtype is not torch.int32 or starts.device != self.device:
                 raise QwError(1, "shared_attention: starts must be a [n_seq] int32 device tensor")
             starts = starts.contiguous()
         qq = q.contiguous()
@@ -463,7 +463,7 @@ class KVCache:
                                                 qq.data_ptr(), hq, L, float(scale), out.data_ptr(), st))
             return out
         for name, t in (("keys", keys), ("values", values)):
-            if _bhld(t, name, self.head_dim) != (B, self.n_kv_heads, L):
+            if _bhld(t, name, self.head_dim, self.device) != (B, self.n_kv_heads, L):
                 raise QwError(1, f"shared_attention: {name} must be [n_seq, n_kv_heads, L, head_dim]")
         k, v = keys.contiguous(), values.contiguous()
         _check(lib().qw_kv_update_and_shared_attention(
@@ -490,15 +490,15 @@ class KVCache:
     def _weights(self, weights, what: str, n: int):
         torch = _torch()
         if weights.dim() != 2 or weights.shape[0] != self.n_kv_heads or weights.shape[1] < n or \
-                weights.dtype is not torch.float32 or not weights.is_cuda:
-            raise QwError(1, f"{what}: weights must be a [n_kv_heads, >= {n}] f32 device tensor")
+                weights.dtype is not torch.float32 or weights.device != self.device:
+            raise QwError(1, f"{what}: weights must be [n_kv_heads, >= {n}] f32 on {self.device}")
         return weights if weights.stride(1) == 1 and weights.stride(0) >= weights.shape[1] \
             else weights.contiguous()
 
     def _scored(self, q, keys, values, scale, weights, decay, causal, weights_out):
         qq, hq, L, D = _hld(q, "q")
-        if D != self.head_dim:
-            raise QwError(1, "attention_scored: q must have the cache's head_dim")
+        if D != self.head_dim or qq.device != self.device:
+            raise QwError(1, "attention_scored: q must have the cache's head_dim and device")
         T = self.offset + (0 if keys is None else L)
         w = None if weights is None else self._weights(weights, "attention_scored", 0)
         if weights_out is None:
@@ -518,7 +518,7 @@ class KVCache:
         else:
             k, *ks = _hld(keys, "keys")
             v, *vs = _hld(values, "values")
-            if ks != vs or ks != [self.n_kv_heads, L, D]:
+            if ks != vs or ks != [self.n_kv_heads, L, D] or k.device != self.device or v.device != self.device:
                 raise QwError(1, "attention_scored: new keys/values must be [n_kv_heads, L, head_dim]")
             _check(lib().qw_kv_update_and_attention_scored(*head, k.data_ptr(), v.data_ptr(), *rest))
         return out, wo if wo.shape[1] == T else wo[:, :T]
@@ -544,11 +544,14 @@ class KVCache:
         same mode and geometry, whose contents they replace) or stay here. Returns (kept
         positions [Hkv, n] int32 ascending, their weights [Hkv, n]), n = min(offset, budget)."""
         w = self._weights(weights, "evict", self.offset)
-        n = max(min(self.offset, int(budget)), 0)
+        if into is not None and not into._h:
+            raise QwError(1, "evict: into is closed")
+        budget, sink, recent = (min(int(x), 2 ** 31 - 1) for x in (budget, sink, recent))
+        n = max(min(self.offset, budget), 0)
         kept = w.new_empty((self.n_kv_heads, n), dtype=_torch().int32)
         wo = w.new_empty((self.n_kv_heads, n))
         _check(lib().qw_kv_evict(self._h, None if into is None else into._h, w.data_ptr(), w.stride(0),
-                                 int(budget), int(sink), int(recent), kept.data_ptr(), wo.data_ptr(), n,
+                                 budget, sink, recent, kept.data_ptr(), wo.data_ptr(), n,
                                  None, _stream(self.device)))
         return kept, wo
 

@@ -819,11 +819,23 @@ int launch_units(int bits, int D, const SharedArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int n_seq, int n_rows, int G, int hkv,
-                const int32_t* starts, float scale, bool causal, void* out, hipStream_t stream, SharedArgs* pa) {
+int make_room(KVCache& c, int n_rows, hipStream_t stream) {
+    const int64_t need = (int64_t)c.offset + n_rows;
+    if (need <= c.cap) return QW_OK;
+    QW_REQUIRE(need <= INT32_MAX - 256, QW_ERR_INVALID_ARGUMENT, "append: too many rows");
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    QW_HIP_CHECK(hipStreamIsCapturing(stream, &cs));
+    QW_REQUIRE(cs == hipStreamCaptureStatusNone, QW_ERR_STATE,
+               "append: the cache has to grow and the stream is being captured; reserve it before");
+    // (geometric, as KVCache::update grows it)
+    return c.reserve((int)std::min<int64_t>(std::max(need, (int64_t)c.cap + c.cap / 2), INT32_MAX - 256), stream);
+}
+
+int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, const void* q, int n_seq, int n_rows, int G,
+                int hkv, const int32_t* starts, float scale, bool causal, void* out, hipStream_t stream, SharedArgs* pa) {
     SharedArgs& a = *pa;
     a = SharedArgs{};
-    const KVCache* c[2] = {prefix && prefix->offset > 0 ? prefix : nullptr, tails && tails->offset > 0 ? tails : nullptr};
+    const KVCache* c[2] = {prefix && prefix->offset > 0 ? prefix : nullptr, tails && tail_rows > 0 ? tails : nullptr};
     const int D = (prefix ? prefix : tails)->D, KT = shared_tile(D);
     a.q = (const f16*)q;
     a.out = (f16*)out;
@@ -841,6 +853,7 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int 
         s.n_split = s.heads = 1;
         if (!c[i]) continue;
         fill_cache(s, *c[i]);
+        if (i == 1) s.T = tail_rows;
         s.heads = c[i]->hkv;
         s.rows = i == 0 ? a.R : n_rows * G;
         // query tiles of equal size, in row tiles (few rows: one)
@@ -853,7 +866,7 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int 
     // One quantized cache under many query tiles: its key tiles are dequantized once, into images
     // (1.03 times its fp16 K and V), not once a query tile.
     const bool images = c[1] && !c[0] && !starts && c[1]->bits != 16 && n_qt[1] >= kImageQueryTiles &&
-                        (int64_t)hkv * c[1]->offset * D <= (int64_t)1 << 29;
+                        (int64_t)hkv * tail_rows * D <= (int64_t)1 << 29;
     // Tiles a split, for each launch: the count with the shortest estimate. A unit's us: a start and an
     // end that grow with its rows, and a time a tile (measured: 30 and 126 rows of 8-bit keys at D = 256
     // 23.6 and 38.4 us in 8 tiles, 126 rows 103 us in 32; few rows 14.5 us in 9); a partial row costs its
@@ -950,7 +963,7 @@ int launch_shared_merge(int D, const SharedArgs& a, hipStream_t stream) {
 }
 
 static int check_shared(const KVCache& p, const KVCache* t, int n_seq, const void* q, int n_q_heads, int n_rows,
-                        float scale, const void* out, int tail_rows) {
+                        float scale, const void* out, int64_t tail_rows) {
     QW_REQUIRE(q && out, QW_ERR_INVALID_ARGUMENT, "shared attention: null q/out");
     QW_REQUIRE(n_seq > 0 && n_rows > 0 && n_q_heads > 0 && n_q_heads % p.hkv == 0, QW_ERR_INVALID_ARGUMENT,
                "shared attention: n_seq, n_rows > 0 and n_q_heads a positive multiple of n_kv_heads");
@@ -974,16 +987,19 @@ int shared_attention(KVCache& prefix, KVCache* tails, int n_seq, const int32_t* 
     const bool append = k_new || v_new;
     QW_REQUIRE(!append || (tails && k_new && v_new), QW_ERR_INVALID_ARGUMENT,
                "shared attention: an append needs tails, k_new and v_new");
-    const int tail_rows = tails ? tails->offset + (append ? n_rows : 0) : 0;
+    const int64_t tail_rows = tails ? (int64_t)tails->offset + (append ? n_rows : 0) : 0;
     if (int rc = check_shared(prefix, tails, n_seq, q, n_q_heads, n_rows, scale, out, tail_rows)) return rc;
     DeviceGuard dg(prefix.device);
     QW_REQUIRE(dg.ok, QW_ERR_HIP, "shared attention: hipSetDevice failed");
+    // (what can fail for want of memory comes before the append)
     if (append)
-        if (int rc = tails->update(k_new, v_new, n_rows, stream)) return rc;
+        if (int rc = make_room(*tails, n_rows, stream)) return rc;
     SharedArgs a;
-    if (int rc = plan_shared(&prefix, tails, q, n_seq, n_rows, n_q_heads / prefix.hkv, prefix.hkv, starts, scale, true,
+    if (int rc = plan_shared(&prefix, tails, (int)tail_rows, q, n_seq, n_rows, n_q_heads / prefix.hkv, prefix.hkv, starts, scale, true,
                              out, stream, &a))
         return rc;
+    if (append)
+        if (int rc = tails->update(k_new, v_new, n_rows, stream)) return rc;
     if (int rc = launch_shared(&prefix, tails, a, stream)) return rc;
     return launch_shared_merge(prefix.D, a, stream);
 }

@@ -61,9 +61,13 @@ constexpr int kSharedMaxSlots = 512;
 __host__ __device__ constexpr int shared_tile(int D) { return 16384 / D; }  // keys of a split's tile
 constexpr int kSharedLds = 146 * 1024;  // a workgroup's
 
-// Fills the arguments and takes the workspace (either cache may be null); the launches.
-int plan_shared(const KVCache* prefix, const KVCache* tails, const void* q, int n_seq, int n_rows, int G, int hkv,
-                const int32_t* starts, float scale, bool causal, void* out, hipStream_t stream, SharedArgs* a);
+// Makes room for n_rows more rows, so that the append that follows moves no buffer; refused while
+// the stream is captured where that needs memory.
+int make_room(KVCache& c, int n_rows, hipStream_t stream);
+// Fills the arguments, the tails (or the one cache) taken as tail_rows long, and takes the workspace
+// (either cache may be null); the launches.
+int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, const void* q, int n_seq, int n_rows, int G,
+                int hkv, const int32_t* starts, float scale, bool causal, void* out, hipStream_t stream, SharedArgs* a);
 int launch_shared(const KVCache* prefix, const KVCache* tails, const SharedArgs& a, hipStream_t stream);
 int launch_shared_merge(int D, const SharedArgs& a, hipStream_t stream);
 

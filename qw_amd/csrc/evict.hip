@@ -49,19 +49,21 @@ struct SelectArgs {
     int chunks;
 };
 
-// hist[bin] += 1 for every lane that is in. Keys of one weight (those that no row ever looked
-// at are 0) would queue on one counter: where the first such lane's bin is shared by many,
-// one lane adds for all of them.
-__device__ __forceinline__ void add_bin(uint32_t* hist, uint32_t bin, bool in) {
-    const uint64_t live = __ballot(in);
-    if (!live) return;
-    const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)bin, __ffsll((unsigned long long)live) - 1);
-    const uint64_t same = __ballot(in && bin == first);
-    if (__popcll(same) > 4) {
-        if ((int)__lane_id() == __ffsll((unsigned long long)same) - 1) atomicAdd(&hist[first], (uint32_t)__popcll(same));
-        in = in && bin != first;
+// Counts digit d of the KPT keys a thread holds as ranks into hist: those of the middle (bit e of mid)
+// that share the cut's digits before it. Weights of 0, which keys that no row ever looked at have
+// in common, would queue on one counter: a wave counts its own and adds them at once.
+template <int KPT>
+__device__ __forceinline__ void count_digit(uint32_t* hist, const uint32_t (&u)[KPT], uint32_t mid, int d, uint32_t prefix) {
+    const int shift = digit_shift(d), bits = digit_bits(d);
+    constexpr uint32_t kZero = 0x80000000u;  // the rank of 0
+    uint32_t zeros = 0;
+#pragma unroll
+    for (int e = 0; e < KPT; e++) {
+        const bool in = (mid >> e & 1) && (d == 0 || u[e] >> (shift + bits) == prefix);
+        zeros += __popcll(__ballot(in && u[e] == kZero));
+        if (in && u[e] != kZero) atomicAdd(&hist[u[e] >> shift & ((1u << bits) - 1)], 1u);
     }
-    if (in) atomicAdd(&hist[bin], 1u);
+    if (zeros && (threadIdx.x & 63) == 0) atomicAdd(&hist[kZero >> shift & ((1u << bits) - 1)], zeros);
 }
 
 // The sum of x over the threads before this one, over the workgroup; *total: over all.
@@ -104,34 +106,47 @@ __device__ __forceinline__ uint2 pick_bin(uint32_t hi, uint32_t lo, uint32_t lef
 
 // Writes the kept keys among KPT consecutive ones a thread, from key t0: rank above the cut or
 // outside the middle, and of those equal to it the first `ties` (eq0 of them and at0 kept keys in the
-// chunks before).
+// chunks before). (A workgroup holds fewer than 2^16 keys: both counts in one scan.)
 template <int KPT>
-__device__ __forceinline__ void emit(const SelectArgs& a, int h, int t0, const float (&x)[KPT], uint32_t cut,
-                                     uint32_t ties, uint32_t at0, uint32_t eq0, uint32_t* s_wave) {
-    const int lo = a.sink, hi = a.T - a.recent;
-    uint32_t n_above = 0, n_equal = 0;
-    uint32_t kind[KPT];  // 2: kept, 1: a tie, 0: gone
+__device__ __forceinline__ void emit(const SelectArgs& a, int h, int t0, const float (&x)[KPT], const uint32_t (&u)[KPT],
+                                     uint32_t mid, uint32_t cut, uint32_t ties, uint32_t at0, uint32_t eq0,
+                                     uint32_t* s_wave) {
+    uint32_t above = 0, equal = 0;  // bit e: key t0 + e
 #pragma unroll
     for (int e = 0; e < KPT; e++) {
-        const int t = t0 + e;
-        const bool mid = t >= lo && t < hi;
-        const uint32_t u = weight_rank(x[e]);
-        kind[e] = t >= a.T ? 0u : !mid || u > cut ? 2u : u == cut ? 1u : 0u;
-        n_above += kind[e] == 2u;
-        n_equal += kind[e] == 1u;
+        const bool m = mid >> e & 1;
+        above |= (uint32_t)(t0 + e < a.T && (!m || u[e] > cut)) << e;
+        equal |= (uint32_t)(m && u[e] == cut) << e;
     }
     uint32_t total;
-    uint32_t at = at0 + scan_before(n_above, s_wave, &total), eq = eq0 + scan_before(n_equal, s_wave, &total);
+    const uint32_t before = scan_before((uint32_t)__popc(above) << 16 | (uint32_t)__popc(equal), s_wave, &total);
+    uint32_t at = at0 + (before >> 16), eq = eq0 + (before & 0xFFFFu);
 #pragma unroll
     for (int e = 0; e < KPT; e++) {
-        if (kind[e] == 2u || (kind[e] == 1u && eq < ties)) {
+        const bool ab = above >> e & 1, eqe = equal >> e & 1;
+        if (ab || (eqe && eq < ties)) {
             const uint32_t pos = at + min(eq, ties);
             a.kept[(int64_t)h * a.n + pos] = t0 + e;
             if (a.weights_out) a.weights_out[h * a.out_stride + pos] = x[e];
         }
-        at += kind[e] == 2u;
-        eq += kind[e] == 1u;
+        at += ab;
+        eq += eqe;
     }
+}
+
+// The keys of a thread: weights, ranks, and which of them lie in the middle.
+template <int KPT>
+__device__ __forceinline__ uint32_t load_keys(const SelectArgs& a, int h, int t0, float (&x)[KPT], uint32_t (&u)[KPT]) {
+    const float* w = a.weights + h * a.stride;
+    uint32_t mid = 0;
+#pragma unroll
+    for (int e = 0; e < KPT; e++) x[e] = t0 + e < a.T ? w[t0 + e] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < KPT; e++) {
+        u[e] = weight_rank(x[e]);
+        mid |= (uint32_t)(t0 + e >= a.sink && t0 + e < a.T - a.recent) << e;
+    }
+    return mid;
 }
 
 // A head in one workgroup, its keys (KPT consecutive ones a thread) in registers.
@@ -141,28 +156,21 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(SelectArgs a)
     __shared__ uint32_t s_wave[kSelWaves];
     __shared__ uint2 s_pick;
     const int tid = threadIdx.x, h = blockIdx.x, t0 = tid * KPT;
-    const float* w = a.weights + h * a.stride;
-    const int lo = a.sink, hi = a.T - a.recent;
     float x[KPT];
-#pragma unroll
-    for (int e = 0; e < KPT; e++) x[e] = t0 + e < a.T ? w[t0 + e] : 0.0f;
+    uint32_t u[KPT];
+    const uint32_t mid = load_keys<KPT>(a, h, t0, x, u);
     uint32_t prefix = 0, left = (uint32_t)a.need;
 #pragma unroll
     for (int d = 0; d < kDigits; d++) {
         hist[2 * tid] = hist[2 * tid + 1] = 0;
         __syncthreads();
-#pragma unroll
-        for (int e = 0; e < KPT; e++) {
-            const uint32_t u = weight_rank(x[e]);
-            const bool in = t0 + e >= lo && t0 + e < hi && (d == 0 || u >> (digit_shift(d) + digit_bits(d)) == prefix);
-            add_bin(hist, u >> digit_shift(d) & ((1u << digit_bits(d)) - 1), in);
-        }
+        count_digit<KPT>(hist, u, mid, d, prefix);
         __syncthreads();
         const uint2 p = pick_bin(hist[kBins - 1 - 2 * tid], hist[kBins - 2 - 2 * tid], left, s_wave, &s_pick);
         prefix = prefix << digit_bits(d) | (p.x & ((1u << digit_bits(d)) - 1));
         left = p.y;
     }
-    emit<KPT>(a, h, t0, x, prefix, left, 0, 0, s_wave);
+    emit<KPT>(a, h, t0, x, u, mid, prefix, left, 0, 0, s_wave);
 }
 
 // The same by chunks of kChunk keys, a workgroup each (grid (chunks, hkv)), in four launches: d = 0,
@@ -174,12 +182,14 @@ __global__ __launch_bounds__(kSelThreads) void evict_digit_kernel(SelectArgs a, 
     __shared__ uint32_t hist[kBins];
     __shared__ uint32_t s_wave[kSelWaves];
     __shared__ uint2 s_pick;
-    const int tid = threadIdx.x, c = blockIdx.x, h = blockIdx.y, hkv = gridDim.y, t0 = c * kChunk + tid * kChunkKeys;
-    const float* w = a.weights + h * a.stride;
-    const int lo = a.sink, hi = a.T - a.recent;
+    __shared__ uint32_t s_sum[2];
+    const int tid = threadIdx.x, lane = tid & 63, c = blockIdx.x, h = blockIdx.y, hkv = gridDim.y;
+    const int t0 = c * kChunk + tid * kChunkKeys;
     float x[kChunkKeys];
-#pragma unroll
-    for (int e = 0; e < kChunkKeys; e++) x[e] = t0 + e < a.T ? w[t0 + e] : 0.0f;
+    uint32_t u[kChunkKeys];
+    const uint32_t mid = load_keys<kChunkKeys>(a, h, t0, x, u);
+    hist[2 * tid] = hist[2 * tid + 1] = 0;
+    if (tid < 2) s_sum[tid] = 0;
     const uint32_t* hist_d = nullptr;  // the last digit's counts of this head
     uint32_t prefix = 0, left = (uint32_t)a.need;
     if (d > 0) {
@@ -200,24 +210,23 @@ __global__ __launch_bounds__(kSelThreads) void evict_digit_kernel(SelectArgs a, 
         if (c == 0 && tid == 0) a.pick[(d - 1) * hkv + h] = p;
         prefix = prefix << digit_bits(d - 1) | (p.x & ((1u << digit_bits(d - 1)) - 1));
         left = p.y;
+    } else {
+        __syncthreads();
     }
     if (d < kDigits) {
-        hist[2 * tid] = hist[2 * tid + 1] = 0;
-        __syncthreads();
-        const int shift = digit_shift(d), bits = digit_bits(d);
-        uint32_t n_above = 0;  // keys that the last digit put above the cut
+        count_digit<kChunkKeys>(hist, u, mid, d, prefix);
+        if (d > 0) {  // keys that the last digit put above the cut: the digits before it equal, it larger
+            const int shift = digit_shift(d - 1), bits = digit_bits(d - 1);
+            uint32_t n_above = 0;
 #pragma unroll
-        for (int e = 0; e < kChunkKeys; e++) {
-            const uint32_t u = weight_rank(x[e]);
-            const bool mid = t0 + e >= lo && t0 + e < hi;
-            const uint32_t head = d == 0 ? 0 : u >> (shift + bits);
-            add_bin(hist, u >> shift & ((1u << bits) - 1), mid && head == prefix);
-            // (the digits before the last are equal, the last is larger)
-            n_above += d > 0 && mid && head > prefix && (d == 1 || head >> digit_bits(1) == prefix >> digit_bits(1));
+            for (int e = 0; e < kChunkKeys; e++) {
+                const uint32_t head = u[e] >> shift;
+                n_above += __popcll(__ballot((mid >> e & 1) && head > prefix && (d == 1 || head >> bits == prefix >> bits)));
+            }
+            if (lane == 0 && n_above) atomicAdd(&s_sum[0], n_above);
         }
-        uint32_t total;
-        scan_before(n_above, s_wave, &total);
-        if (d > 0 && tid == 0) a.above[((d - 1) * hkv + h) * a.chunks + c] = total;
+        __syncthreads();
+        if (d > 0 && tid == 0) a.above[((d - 1) * hkv + h) * a.chunks + c] = s_sum[0];
         a.hist[(((int64_t)d * hkv + h) * a.chunks + c) * (kBins / 2) + tid] = hist[2 * tid] | hist[2 * tid + 1] << 16;
         return;
     }
@@ -232,12 +241,12 @@ __global__ __launch_bounds__(kSelThreads) void evict_digit_kernel(SelectArgs a, 
     }
     for (int i = tid; i < c; i += kSelThreads)
         n_above += a.above[h * a.chunks + i] + a.above[(hkv + h) * a.chunks + i];
-    uint32_t at, eq;
-    scan_before(n_above, s_wave, &at);
-    scan_before(n_equal, s_wave, &eq);
-    const int start = c * kChunk;
-    at += min(start, lo) + max(0, start - max(hi, lo));
-    emit<kChunkKeys>(a, h, t0, x, prefix, left, at, eq, s_wave);
+    if (n_above) atomicAdd(&s_sum[0], n_above);
+    if (n_equal) atomicAdd(&s_sum[1], n_equal);
+    __syncthreads();
+    const int start = c * kChunk, lo = a.sink, hi = a.T - a.recent;
+    const uint32_t at = s_sum[0] + min(start, lo) + max(0, start - hi);
+    emit<kChunkKeys>(a, h, t0, x, u, mid, prefix, left, at, s_sum[1], s_wave);
 }
 
 // Keys up to which one workgroup a head does it.

@@ -211,6 +211,10 @@ __global__ __launch_bounds__(64 * kWgWaves) void key_weights_kernel(WeightArgs w
         }
 }
 
+__global__ __launch_bounds__(256) void copy_halves_kernel(const f16* __restrict__ from, f16* __restrict__ to, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = from[i];
+}
+
 // The row splits' sums, in order.
 __global__ __launch_bounds__(256) void add_weights_kernel(WeightArgs w) {
     const int T = w.s.seg[1].T, key = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
@@ -315,26 +319,31 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
     }
     DeviceGuard dg(c.device);
     QW_REQUIRE(dg.ok, QW_ERR_HIP, "scored attention: hipSetDevice failed");
+    // (what can fail for want of memory comes before the append)
     if (append)
-        if (int rc = c.update(k_new, v_new, n_rows, stream)) return rc;
+        if (int rc = make_room(c, n_rows, stream)) return rc;
     WeightArgs w;
-    if (int rc = plan_shared(nullptr, &c, q, 1, n_rows, n_q_heads / c.hkv, c.hkv, nullptr, scale, causal, out, stream, &w.s))
+    if (int rc = plan_shared(nullptr, &c, (int)T, q, 1, n_rows, n_q_heads / c.hkv, c.hkv, nullptr, scale, causal, out, stream,
+                             &w.s))
         return rc;
+    const int R = w.s.R;
     w.weights = decay > 0.0f ? weights : nullptr;
     w.weights_out = weights_out;
     w.ws_in = weights_stride;
     w.ws_out = weights_out_stride;
     w.n_weights = n_weights;
     w.decay = decay;
-    if (w.s.R <= 16) {
-        w.s.score_stride = ((int64_t)c.offset + 31) / 32 * 32;
+    if (R <= 16) {
+        w.s.score_stride = (T + 31) / 32 * 32;
         void* scores = nullptr;
-        if (int rc = workspace(kWsRowSums, c.device, stream, (size_t)c.hkv * w.s.R * w.s.score_stride * sizeof(float), &scores))
+        if (int rc = workspace(kWsRowSums, c.device, stream, (size_t)c.hkv * R * w.s.score_stride * sizeof(float), &scores))
             return rc;
         w.s.scores = (float*)scores;
+        if (append)
+            if (int rc = c.update(k_new, v_new, n_rows, stream)) return rc;
         if (int rc = launch_shared(nullptr, &c, w.s, stream)) return rc;
-        const int n_merge = w.s.n_slots > 1 ? merge_groups(c.D, w.s.R, c.hkv, w.s.n_slots) : 0;
-        const dim3 grid(n_merge + (c.offset + 1023) / 1024, c.hkv);
+        const int n_merge = w.s.n_slots > 1 ? merge_groups(c.D, R, c.hkv, w.s.n_slots) : 0;
+        const dim3 grid((unsigned)(n_merge + (T + 1023) / 1024), c.hkv);
         if (c.D == 256)
             hipLaunchKernelGGL(finish_few_kernel<256>, grid, dim3(256), 0, stream, w, n_merge);
         else
@@ -343,21 +352,33 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
         return QW_OK;
     }
     // row splits: about one workgroup a CU, of at least four steps each
-    const int groups = (c.offset + kWgKeys - 1) / kWgKeys * c.hkv, steps = (w.s.R + kStepRows - 1) / kStepRows;
-    w.row_splits = std::max(1, std::min({256 / groups, steps / 4, 64}));
-    w.rows_per_split = (steps + w.row_splits - 1) / w.row_splits * kStepRows;
-    w.row_splits = (w.s.R + w.rows_per_split - 1) / w.rows_per_split;
-    const size_t ml_bytes = (size_t)c.hkv * w.s.R * sizeof(float2);
-    const size_t part_bytes = w.row_splits > 1 ? (size_t)w.row_splits * c.hkv * c.offset * sizeof(float) : 0;
-    void* row_ml = nullptr;
-    if (int rc = workspace(kWsRowSums, c.device, stream, ml_bytes + part_bytes, &row_ml)) return rc;
-    w.part = (float*)((char*)row_ml + ml_bytes);
-    w.s.row_ml = (float2*)row_ml;
+    const int64_t groups = (T + kWgKeys - 1) / kWgKeys * c.hkv, steps = (R + kStepRows - 1) / kStepRows;
+    w.row_splits = (int)std::max<int64_t>(1, std::min<int64_t>({256 / groups, steps / 4, 64}));
+    w.rows_per_split = (int)((steps + w.row_splits - 1) / w.row_splits * kStepRows);
+    w.row_splits = (R + w.rows_per_split - 1) / w.rows_per_split;
+    const size_t ml_bytes = ((size_t)c.hkv * R * sizeof(float2) + 15) / 16 * 16;
+    const size_t part_bytes = w.row_splits > 1 ? ((size_t)w.row_splits * c.hkv * T * sizeof(float) + 15) / 16 * 16 : 0;
+    // the weights' kernel copies q into LDS by pieces of 16 bytes: a q off their alignment is copied first
+    const size_t q_bytes = (uintptr_t)q % 16 ? (size_t)n_q_heads * n_rows * c.D * sizeof(f16) : 0;
+    void* ws = nullptr;
+    if (int rc = workspace(kWsRowSums, c.device, stream, ml_bytes + part_bytes + q_bytes, &ws)) return rc;
+    w.s.row_ml = (float2*)ws;
+    w.part = (float*)((char*)ws + ml_bytes);
+    if (append)
+        if (int rc = c.update(k_new, v_new, n_rows, stream)) return rc;
     if (int rc = launch_shared(nullptr, &c, w.s, stream)) return rc;
     if (int rc = launch_shared_merge(c.D, w.s, stream)) return rc;
     if (w.s.n_slots == 1) {
-        hipLaunchKernelGGL(row_sums_kernel, dim3((w.s.R + 255) / 256, c.hkv), dim3(256), 0, stream, w.s);
+        hipLaunchKernelGGL(row_sums_kernel, dim3((R + 255) / 256, c.hkv), dim3(256), 0, stream, w.s);
         QW_HIP_CHECK(hipGetLastError());
+    }
+    if (q_bytes) {
+        f16* const to = (f16*)((char*)ws + ml_bytes + part_bytes);
+        const int64_t n = q_bytes / sizeof(f16);
+        hipLaunchKernelGGL(copy_halves_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096)), dim3(256), 0, stream,
+                           (const f16*)q, to, n);
+        QW_HIP_CHECK(hipGetLastError());
+        w.s.q = to;
     }
     if (c.D == 256)
         return c.bits == 4   ? launch_weights<4, 256>(w, stream)

@@ -159,6 +159,10 @@ def test_evict_refusals():
     refused(1, cache.evict, w, 10, into=qw_amd.KVCache("affine8", 4, 128))
     refused(1, cache.evict, w, 10, into=qw_amd.KVCache("affine8", 2, 256))
     refused(1, filled("turbo4", 2, 128, 20, r).evict, w, 10, into=qw_amd.KVCache("turbo4", 2, 128, turbo_seed=5))
+    closed = qw_amd.KVCache("affine8", 2, 128)
+    closed.close()
+    refused(1, cache.evict, w, 10, into=closed)
+    refused(1, cache.evict, w, 2 ** 40, sink=2 ** 31, recent=1)
     assert cache.offset == 20
     empty = qw_amd.KVCache("affine8", 2, 128)
     kept, wo = empty.evict(w, 10)

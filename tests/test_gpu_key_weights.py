@@ -144,6 +144,39 @@ def test_scored_graph_and_streams():
         assert torch.equal(out, out2) and torch.equal(acc, w)
 
 
+def test_scored_views_off_alignment():
+    """q off any vector alignment, one row and many."""
+    r = rng(13)
+    cache = filled("affine8", 2, 128, 700, r)
+    for L in (1, 40):
+        q = queries(r, 1, 8, L, 128)
+        odd = torch.empty(q.numel() + 1, dtype=q.dtype, device="cuda")[1:].view(q.shape)
+        odd.copy_(q)
+        out, w = cache.attention_scored(q, 0.09, causal=True)
+        out2, w2 = cache.attention_scored(odd, 0.09, causal=True)
+        assert torch.equal(out, out2) and torch.equal(w, w2)
+
+
+def test_refused_in_a_capture_before_the_append():
+    """A call that needs memory in a captured stream appends nothing."""
+    import qw_amd
+
+    r = rng(14)
+    cache = filled("fp16", 2, 128, 250, r)
+    prefix = filled("fp16", 1, 128, 30, r)
+    q, kv = queries(r, 1, 8, 1, 128), dev(r.standard_normal((1, 2, 1, 128)).astype(np.float16))
+    qb, kvb = queries(r, 2, 4, 9, 128), dev(r.standard_normal((2, 1, 9, 128)).astype(np.float16))
+    torch.cuda.synchronize()
+    for call in (lambda: cache.update_and_attention_scored(q, kv, kv, 0.1),
+                 lambda: prefix.update_and_shared_attention(qb, cache, kvb, kvb, 0.1)):
+        with pytest.raises(qw_amd.QwError) as e:
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=torch.cuda.Stream()):
+                call()
+        assert e.value.status == 5 and cache.offset == 250
+    out, w = cache.update_and_attention_scored(q, kv, kv, 0.1, causal=True)
+    check_scored(out, w, q, cache, 0.1, True)
+
+
 def test_scored_refusals():
     import qw_amd
 

@@ -248,4 +248,7 @@ def test_shared_refusals():
     refused(1, one.shared_attention, q[:1, :1], one, 0.1)                 # the prefix as its own tail
     refused(1, prefix.shared_attention, queries(r, 3, 8, 1, 256), filled("fp16", 6, 256, 3, r), 0.1)
     refused(2, prefix.shared_attention, q, filled("turbo4", 6, 128, 3, r), 0.1)
+    closed = filled("fp16", 6, 128, 3, r)
+    closed.close()
+    refused(1, call, q, closed, 0.1)
     assert tails.offset == 3 and prefix.offset == 20
