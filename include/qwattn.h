@@ -240,7 +240,10 @@ int qw_kv_update_and_attention_general(qw_kv_cache* cache, const void* q, int n_
  * v_new [n_seq][n_kv_heads][n_rows][head_dim] first.
  *   q, out [n_seq][n_q_heads][n_rows][head_dim] fp16
  * Keys that a later row of its own sequence sees and this one does not must be
- * finite. Either cache may be empty, not both. QW_ERR_UNSUPPORTED on Turbo4 caches. */
+ * finite. Either cache may be empty, not both. Turbo4 caches go
+ * together, with one seed: q rotated into the K basis (rounded to fp16), the values
+ * f16(centroid * rescale), the output (rounded to fp16) rotated back out of the V
+ * basis. */
 int qw_kv_shared_attention(qw_kv_cache* prefix, qw_kv_cache* tails, int n_seq, const int32_t* starts,
                            const void* q, int n_q_heads, int n_rows, float scale, void* out,
                            void* stream);
@@ -254,10 +257,11 @@ int qw_kv_update_and_shared_attention(qw_kv_cache* prefix, qw_kv_cache* tails, i
  * qw_kv_attention) that counts what weight each key got,
  *   weights_out[h][t] = decay * weights[h][t] + sum of the softmax weights of key t
  *     over the n_rows rows and the query heads of KV head h,   t < offset,
- * fp32 throughout. weights (fp32 [n_kv_heads][>= n_weights], row stride in
+ * fp32 throughout (Turbo4 caches as there). weights (fp32 [n_kv_heads][>= n_weights], row stride in
  * elements; NULL, or decay 0: not read) counts as 0 from n_weights on, as for keys
- * appended since; weights_out [n_kv_heads][>= offset] may be the same array, else not overlap it. The
- * update form appends k_new / v_new first. QW_ERR_UNSUPPORTED on Turbo4 caches. */
+ * appended since; weights_out [n_kv_heads][>= offset] may be the same array, else not overlap it. Keys
+ * that a later row sees and this one does not must be finite. The update form
+ * appends k_new / v_new first. */
 int qw_kv_attention_scored(qw_kv_cache* cache, const void* q, int n_q_heads, int n_rows, float scale,
                            int causal, const float* weights, int64_t weights_stride, int n_weights,
                            float decay, float* weights_out, int64_t weights_out_stride, void* out,

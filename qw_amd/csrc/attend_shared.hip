@@ -37,6 +37,7 @@
 #include "block_tile.hpp"
 #include "dequant.hpp"
 #include "kv_cache.hpp"
+#include "turbo4_device.hpp"
 
 namespace qw {
 
@@ -130,8 +131,9 @@ __device__ __forceinline__ void keep_reads_ahead() {
 // A dequantizing group of 256 threads: a key tile's codes through registers into an LDS tile of
 // block_tile.hpp's layout, V's slots in the fp16 order whatever the codes'. The values are
 // f16(f16(code * scale) + bias), as the fetch gives them. NATURAL: K's dims in order also from 4-bit
-// codes (else pairs (0,4), (1,5), (2,6), (3,7) of each eight).
-template <int KIND, int D, bool FAST, bool NATURAL>
+// codes (else pairs (0,4), (1,5), (2,6), (3,7) of each eight). T4: a Turbo4 cache's 4-bit indices, K
+// and V row-major, a word a row beside them; cp: the pair of centroids of every byte of them, in LDS.
+template <int KIND, int D, bool FAST, bool NATURAL, bool T4 = false>
 struct TileFiller {
     using S = BlockShape<D>;
     static constexpr int KT = S::KT, TPR = S::TPR, TPB = S::TPB, NG = S::NG, DPL = D / 16;
@@ -141,6 +143,7 @@ struct TileFiller {
     struct Stage {
         u32x4 kc[PER][KU], vc[PER][KU], vp[PER][2];
         uint32_t kp[PER];
+        uint32_t vt[T4 ? PER : 1][8];  // 4 dims of the 8 rows
     };
     const char *k_head, *kp_head, *v_head, *vp_head;
     // slice j: key kk's 32 dims from 32 q32, V block vb's 4 slots from 4 vj
@@ -150,9 +153,9 @@ struct TileFiller {
     __device__ TileFiller(const SharedSegment& c, int hc, int key0, int t) {
         const int64_t row = (int64_t)hc * c.cap + key0;
         k_head = (const char*)c.k_data + row * (D * KIND / 8);
-        kp_head = (const char*)c.k_params + row * (NG * 4);
+        kp_head = (const char*)c.k_params + row * (T4 ? 4 : NG * 4);
         v_head = (const char*)c.v_data + row / 8 * (D * KIND);
-        vp_head = (const char*)c.v_params + row / 8 * (NG * 32);
+        vp_head = (const char*)c.v_params + row / 8 * (T4 ? 32 : NG * 32);
         code_off = c.code_off2;
         magic = vconst(kMagic);
 #pragma unroll
@@ -175,6 +178,16 @@ struct TileFiller {
             const u32x4* v = (const u32x4*)(v_head + key / 8 * (D * KIND) + (vb[j] * (D * KIND) + 16 * KU * vj[j]));
 #pragma unroll
             for (int x = 0; x < KU; x++) st.kc[j][x] = k[x];
+            if constexpr (T4) {
+                st.kp[j] = *(const uint32_t*)(kp_head + key * 4 + 4 * kk[j]);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    st.vt[j][i] = *(const uint16_t*)(v_head + key * (D / 2) + ((8 * vb[j] + i) * (D / 2) + 2 * vj[j]));
+                const u32x4* p = (const u32x4*)(vp_head + key * 4 + 32 * vb[j]);
+                st.vp[j][0] = p[0];
+                st.vp[j][1] = p[1];
+                continue;
+            }
 #pragma unroll
             for (int x = 0; x < KU; x++) st.vc[j][x] = v[x];
             if constexpr (KIND != 16) {
@@ -187,7 +200,7 @@ struct TileFiller {
     }
     // The tile whose first key is key0; keys outside [lo, hi), which no row sees, go in as zeros of V:
     // they have weight 0, but 0 x inf is NaN.
-    __device__ __forceinline__ void store(const Stage& st, char* buf, int key0, int lo, int hi) const {
+    __device__ __forceinline__ void store(const Stage& st, char* buf, int key0, int lo, int hi, const float2* cp = nullptr) const {
         const bool edge = key0 < lo || key0 + KT > hi;
         half8* const sK = (half8*)buf;
         half8* const sV = (half8*)(buf + S::KBUF);
@@ -200,6 +213,28 @@ struct TileFiller {
                 for (int w = 0; w < 4; w++) kdst[w * KT] = as_h8(st.kc[j][w]);
 #pragma unroll
                 for (int e = 0; e < 4; e++) y[e] = as_h8(st.vc[j][e]);
+            } else if constexpr (T4) {
+                const float kr = (float)h2(st.kp[j]).x;
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    half8 x;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float2 c = cp[st.kc[j][0][w] >> (8 * i) & 0xFFu];
+                        x[2 * i] = t4_f16_product(c.x, kr);
+                        x[2 * i + 1] = t4_f16_product(c.y, kr);
+                    }
+                    kdst[w * KT] = x;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float vr = (float)h2(st.vp[j][i / 4][i % 4]).y;
+                    const float2 c0 = cp[st.vt[j][i] & 0xFFu], c1 = cp[st.vt[j][i] >> 8];
+                    y[0][i] = t4_f16_product(c0.x, vr);
+                    y[1][i] = t4_f16_product(c0.y, vr);
+                    y[2][i] = t4_f16_product(c1.x, vr);
+                    y[3][i] = t4_f16_product(c1.y, vr);
+                }
             } else {
                 const half2v sb = h2(st.kp[j]), s = {sb.x, sb.x}, b = {sb.y, sb.y};
                 const PairConsts kc = make_consts<FAST, KIND>(s, s, s, s, b, b, b, b, code_off);
@@ -231,7 +266,8 @@ struct TileFiller {
             const int vr = KIND == 8 ? 2 * (vj[j] / 8) : 4 * (vj[j] / 16);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const int at = KIND == 16  ? 4 * vj[j] + e + (vj[j] >> 2)
+                const int at = T4           ? 17 * ((4 * vj[j] + e) % DPL) + (4 * vj[j] + e) / DPL
+                               : KIND == 16 ? 4 * vj[j] + e + (vj[j] >> 2)
                                : KIND == 8 ? 17 * (vr + e % 2) + v_n(j) + e / 2
                                            : 17 * (vr + e) + v_n(j);
                 sV[vb[j] * S::VROW + at] = y[e];
@@ -251,7 +287,7 @@ struct TileFiller {
 // Where the rows leave waves free these take parts of each tile's keys, joined at the end through LDS.
 // One barrier a tile. (With 8 waves that dequantize and compute in turn, all of them were in the same
 // phase: LDS idle while they dequantize, the VALU while they read.)
-template <int KIND, int D, bool FAST, bool IMAGE>
+template <int KIND, int D, bool FAST, bool IMAGE, bool T4 = false>
 __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
     using S = BlockShape<D>;
     constexpr int KT = S::KT, NSUB = S::NSUB, NM = S::NM, NT = S::NT, VROW = S::VROW, BUF = S::BUF, KBUF = S::KBUF;
@@ -268,6 +304,13 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
     constexpr int REG = RT * (64 * NT * 16 + 64 * 8);  // a parked part
     static_assert((kWaves - kWaves / (NSUB < 8 ? NSUB : 8)) * REG <= kSharedLds, "the parked parts fit");
 
+    float2* const cp = (float2*)(lds + 2 * BUF);  // T4: a byte's two centroids
+    if constexpr (T4) {
+        static_assert(2 * BUF + 256 * sizeof(float2) <= kSharedLds, "the centroid pairs behind the tiles");
+        const float* const cb = (int)blockIdx.x >= a.seg[0].n_units ? a.seg[1].t4_cb : a.seg[0].t4_cb;
+        for (int i = tid; i < 256; i += 64 * (kWaves + kFillWaves)) cp[i] = float2{cb[i & 15], cb[i >> 4]};
+        __syncthreads();
+    }
     if (wave >= kWaves) {
         // ---- filling waves
         const SharedSegment& seg = (int)blockIdx.x >= a.seg[0].n_units ? a.seg[1] : a.seg[0];
@@ -301,10 +344,10 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
                 __syncthreads();
             }
         } else {
-            using Filler = TileFiller<KIND, D, FAST, false>;
+            using Filler = TileFiller<KIND, D, FAST, false, T4>;
             const Filler f(seg, u.hc, u.k_begin, tid - 64 * kWaves);
             auto put = [&](const typename Filler::Stage& st, int i) {
-                f.store(st, lds + BUF * (i & 1), u.k_begin + i * KT, u.lo, u.hi);
+                f.store(st, lds + BUF * (i & 1), u.k_begin + i * KT, u.lo, u.hi, cp);
             };
             typename Filler::Stage s0, s1;  // tiles 1, 3, .. and 2, 4, ..
             if (n > 0) {
@@ -347,7 +390,7 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
 #pragma unroll
         for (int m = 0; m < NM; m++) {
             const u32x4 w = *(const u32x4*)(q + 32 * m);
-            qb[rt][m] = as_h8(q_piece<KIND>(ok ? w : u32x4{0, 0, 0, 0}, a.q_flip));
+            qb[rt][m] = as_h8(q_piece<T4 ? 16 : KIND>(ok ? w : u32x4{0, 0, 0, 0}, a.q_flip));
         }
     }
     float m_ref[RT], l_run[RT];  // log2 units; l: this lane's share
@@ -715,6 +758,11 @@ __global__ __launch_bounds__(64 * (kWaves + kFillWaves), 1) void shared_many_ker
     many_body<KIND, D, false, false>(a, lds);
 }
 template <int D>
+__global__ __launch_bounds__(64 * (kWaves + kFillWaves), 1) void shared_t4_many_kernel(SharedArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    many_body<4, D, false, false, true>(a, lds);
+}
+template <int D>
 __global__ __launch_bounds__(64 * (kWaves + kFillWaves), 1) void shared_image_many_kernel(SharedArgs a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     many_body<16, D, false, true>(a, lds);
@@ -732,7 +780,7 @@ __global__ __launch_bounds__(64 * kFillWaves) void shared_image_kernel(SharedSeg
         f.load(st, 0);
         f.store(st, lds, t * S::KT, 0, c.T);
     };
-    if (KIND != 16 && *c.fast_flag)
+    if (*c.fast_flag)
         fill(std::true_type{});
     else
         fill(std::false_type{});
@@ -776,6 +824,7 @@ void fill_cache(SharedSegment& s, const KVCache& c) {
     s.T = c.offset;
     s.code_off2 = c.code_offset2();
     s.fast_flag = c.fast_flag;
+    s.t4_cb = c.turbo4() ? c.t4_tables + 4 * c.D : nullptr;
 }
 
 template <int KIND, int D>
@@ -793,7 +842,8 @@ int launch_images(const SharedArgs& a, hipStream_t stream) {
 }
 template <int KIND, int D>
 int launch_units(const SharedArgs& a, hipStream_t stream) {
-    if (a.seg[1].images) return launch_images<KIND, D>(a, stream);
+    if constexpr (KIND != 16)
+        if (a.seg[1].images) return launch_images<KIND, D>(a, stream);
     const dim3 grid(a.seg[0].n_units + a.seg[1].n_units);
     const bool few = std::max(a.seg[0].n_units ? a.seg[0].unit_rows : 0, a.seg[1].n_units ? a.seg[1].unit_rows : 0) <= kFewRows;
     const void* const kernel = few ? (const void*)shared_few_kernel<KIND, D> : (const void*)shared_many_kernel<KIND, D>;
@@ -806,8 +856,17 @@ int launch_units(const SharedArgs& a, hipStream_t stream) {
     return QW_OK;
 }
 
+template <int D>
+int launch_t4_units(const SharedArgs& a, hipStream_t stream) {
+    if (int rc = ensure_dynamic_lds((const void*)shared_t4_many_kernel<D>, kSharedLds)) return rc;
+    hipLaunchKernelGGL(shared_t4_many_kernel<D>, dim3(a.seg[0].n_units + a.seg[1].n_units),
+                       dim3(64 * (kWaves + kFillWaves)), kSharedLds, stream, a);
+    QW_HIP_CHECK(hipGetLastError());
+    return QW_OK;
+}
 int launch_units(int bits, int D, const SharedArgs& a, hipStream_t stream) {
     if (a.seg[0].n_units + a.seg[1].n_units == 0) return QW_OK;
+    if (a.seg[0].t4_cb || a.seg[1].t4_cb) return D == 256 ? launch_t4_units<256>(a, stream) : launch_t4_units<128>(a, stream);
     if (D == 256)
         return bits == 4   ? launch_units<4, 256>(a, stream)
                : bits == 8 ? launch_units<8, 256>(a, stream)
@@ -865,7 +924,7 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, cons
     }
     // One quantized cache under many query tiles: its key tiles are dequantized once, into images
     // (1.03 times its fp16 K and V), not once a query tile.
-    const bool images = c[1] && !c[0] && !starts && c[1]->bits != 16 && n_qt[1] >= kImageQueryTiles &&
+    const bool images = c[1] && !c[0] && !starts && c[1]->affine() && n_qt[1] >= kImageQueryTiles &&
                         (int64_t)hkv * tail_rows * D <= (int64_t)1 << 29;
     // Tiles a split, for each launch: the count with the shortest estimate. A unit's us: a start and an
     // end that grow with its rows, and a time a tile (measured: 30 and 126 rows of 8-bit keys at D = 256
@@ -877,7 +936,7 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, cons
         int most = 0;
         for (int i : in)
             if (c[i]) {
-                few = few && a.seg[i].unit_rows <= kFewRows;
+                few = few && a.seg[i].unit_rows <= kFewRows && !c[i]->turbo4();
                 most = std::max(most, tiles[i]);
             }
         auto unit_us = [&](int i, int n) {
@@ -962,6 +1021,18 @@ int launch_shared_merge(int D, const SharedArgs& a, hipStream_t stream) {
     return QW_OK;
 }
 
+int shared_turbo4_room(const KVCache& c, int64_t q_rows, hipStream_t stream, SharedArgs* a) {
+    QW_REQUIRE(q_rows <= INT32_MAX, QW_ERR_INVALID_ARGUMENT, "attention over a Turbo4 cache: too many rows");
+    void* ws = nullptr;
+    if (int rc = workspace(kWsTurbo4, c.device, stream, 2 * (size_t)q_rows * c.D * sizeof(f16), &ws)) return rc;
+    a->q = (const f16*)ws;
+    a->out = (f16*)ws + q_rows * c.D;
+    return QW_OK;
+}
+int shared_turbo4_rotate_q(const KVCache& c, const void* q, int64_t q_rows, const SharedArgs& a, hipStream_t stream) {
+    return launch_turbo4_rotate(c, (const f16*)q, (int)q_rows, false, (f16*)a.q, stream);
+}
+
 static int check_shared(const KVCache& p, const KVCache* t, int n_seq, const void* q, int n_q_heads, int n_rows,
                         float scale, const void* out, int64_t tail_rows) {
     QW_REQUIRE(q && out, QW_ERR_INVALID_ARGUMENT, "shared attention: null q/out");
@@ -970,11 +1041,12 @@ static int check_shared(const KVCache& p, const KVCache* t, int n_seq, const voi
     QW_REQUIRE((int64_t)n_seq * n_rows * (n_q_heads / p.hkv) <= INT32_MAX / 2, QW_ERR_INVALID_ARGUMENT,
                "shared attention: too many rows");
     QW_REQUIRE(std::isfinite(scale), QW_ERR_INVALID_ARGUMENT, "shared attention: scale must be finite");
-    QW_REQUIRE(!p.turbo4() && !(t && t->turbo4()), QW_ERR_UNSUPPORTED, "shared attention: not over Turbo4 caches");
     if (t) {
         QW_REQUIRE(t != &p, QW_ERR_INVALID_ARGUMENT, "shared attention: the prefix and the tails are one cache");
         QW_REQUIRE((int64_t)n_seq * p.hkv == t->hkv && t->D == p.D && t->device == p.device, QW_ERR_INVALID_ARGUMENT,
                    "shared attention: the tails need n_seq * n_kv_heads heads of the prefix's head_dim, on its device");
+        QW_REQUIRE(t->turbo4() == p.turbo4() && (!p.turbo4() || t->turbo_seed == p.turbo_seed), QW_ERR_UNSUPPORTED,
+                   "shared attention: Turbo4 caches go with Turbo4 caches of their seed");
         QW_REQUIRE(tail_rows == 0 || tail_rows >= n_rows, QW_ERR_INVALID_ARGUMENT,
                    "shared attention: fewer tail rows than query rows");
     }
@@ -998,10 +1070,16 @@ int shared_attention(KVCache& prefix, KVCache* tails, int n_seq, const int32_t* 
     if (int rc = plan_shared(&prefix, tails, (int)tail_rows, q, n_seq, n_rows, n_q_heads / prefix.hkv, prefix.hkv, starts, scale, true,
                              out, stream, &a))
         return rc;
+    const int64_t q_rows = (int64_t)n_seq * n_q_heads * n_rows;
+    if (prefix.turbo4())
+        if (int rc = shared_turbo4_room(prefix, q_rows, stream, &a)) return rc;
     if (append)
         if (int rc = tails->update(k_new, v_new, n_rows, stream)) return rc;
+    if (prefix.turbo4())
+        if (int rc = shared_turbo4_rotate_q(prefix, q, q_rows, a, stream)) return rc;
     if (int rc = launch_shared(&prefix, tails, a, stream)) return rc;
-    return launch_shared_merge(prefix.D, a, stream);
+    if (int rc = launch_shared_merge(prefix.D, a, stream)) return rc;
+    return prefix.turbo4() ? launch_turbo4_rotate(prefix, a.out, (int)q_rows, true, (f16*)out, stream) : QW_OK;
 }
 
 }  // namespace qw

@@ -7,6 +7,9 @@
 
 namespace qw {
 
+// A Turbo4 cache: q rotated into the K basis by a launch before, keys and values as the expansion holds
+// them (f16(centroid * rescale)), the output rotated back out of the V basis by a launch behind.
+
 // One cache's part of the keys.
 struct SharedSegment {
     const uint32_t* k_data;
@@ -21,6 +24,7 @@ struct SharedSegment {
     int n_split, tiles_per_split;
     int n_units;                  // heads * query tiles * n_split; 0: no such keys
     int slot0;                    // its first split's partial slot
+    const float* t4_cb;           // Turbo4 caches: the 16 centroids on the device, else null
     const char* images;           // null, or its key tiles dequantized (the tails alone): [heads][n_tiles]
     int n_tiles;
     int causal_rows;              // > 0: of that many last rows, row r sees keys to T - causal_rows + r
@@ -70,6 +74,10 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, cons
                 int hkv, const int32_t* starts, float scale, bool causal, void* out, hipStream_t stream, SharedArgs* a);
 int launch_shared(const KVCache* prefix, const KVCache* tails, const SharedArgs& a, hipStream_t stream);
 int launch_shared_merge(int D, const SharedArgs& a, hipStream_t stream);
+// Over Turbo4 caches (c: one of them): a.q becomes the rotated q and a.out the rotated output's place, in
+// the stream's workspace; rotate_out writes the rows to out.
+int shared_turbo4_room(const KVCache& c, int64_t q_rows, hipStream_t stream, SharedArgs* a);
+int shared_turbo4_rotate_q(const KVCache& c, const void* q, int64_t q_rows, const SharedArgs& a, hipStream_t stream);
 
 // Rows' partials joined by workgroups of 256, each partial row by TC threads and SG of them at a
 // time, four such in flight, their sums over LDS. A workgroup a row (TC = D / 4), but: few rows of

@@ -23,6 +23,7 @@
 
 #include "attend_shared.hpp"
 #include "dequant.hpp"
+#include "turbo4_device.hpp"
 
 namespace qw {
 
@@ -36,6 +37,7 @@ struct WeightArgs {
     int64_t ws_in, ws_out;
     int n_weights;           // keys that weights covers
     float decay;
+    float scale2;            // scale * log2 e, with its sign (the attention launch takes q negated instead)
     int row_splits, rows_per_split;  // (rows_per_split a multiple of kStepRows)
 };
 
@@ -56,7 +58,7 @@ __global__ __launch_bounds__(256) void row_sums_kernel(SharedArgs a) {
     a.row_ml[at] = float2{ml.x == -INFINITY ? 0.0f : ml.x, ml.y == 0.0f ? 0.0f : 1.0f / ml.y};
 }
 
-template <int KIND, int D>
+template <int KIND, int D, bool T4>
 __global__ __launch_bounds__(64 * kWgWaves) void key_weights_kernel(WeightArgs w) {
     constexpr int NM = D / 32, NG = D / kGroup, E = 16 / KIND;
     constexpr int TILE = D * 2 * 16;                         // bytes of 16 rows of q
@@ -69,6 +71,11 @@ __global__ __launch_bounds__(64 * kWgWaves) void key_weights_kernel(WeightArgs w
     const int key0 = blockIdx.x * kWgKeys + wave * kWaveKeys;
     const bool live = key0 < T;
     const uint32_t magic = vconst(kMagic);
+    __shared__ float2 cp[T4 ? 256 : 1];  // Turbo4: the centroids of a byte of indices
+    if constexpr (T4) {
+        if (tid < 256) cp[tid] = float2{c.t4_cb[tid & 15], c.t4_cb[tid >> 4]};
+        __syncthreads();
+    }
     // A operands: lane (g, r16) holds its pieces (k_chunk) of key 32 u + 8 (r16 >> 2) + 4 tt + (r16 &
     // 3), so that a lane of S^T gets keys 32 u + 8 g + e of row r16
     half8 ka[2][2][NM];
@@ -85,6 +92,16 @@ __global__ __launch_bounds__(64 * kWgWaves) void key_weights_kernel(WeightArgs w
             if constexpr (KIND == 16) {
 #pragma unroll
                 for (int m = 0; m < NM; m++) ka[u][tt][m] = as_h8(x[m]);
+            } else if constexpr (T4) {
+                const float kr = (float)h2(c.k_params[row]).x;
+#pragma unroll
+                for (int m = 0; m < NM; m++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float2 y = cp[x[m / 4][m % 4] >> (8 * i) & 0xFFu];
+                        ka[u][tt][m][2 * i] = t4_f16_product(y.x, kr);
+                        ka[u][tt][m][2 * i + 1] = t4_f16_product(y.y, kr);
+                    }
             } else {
                 uint32_t kp[KP];
 #pragma unroll
@@ -171,7 +188,7 @@ __global__ __launch_bounds__(64 * kWgWaves) void key_weights_kernel(WeightArgs w
                             acc[u][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[u][tt][m], qb, acc[u][tt], 0, 0, 0);
                 }
                 auto weight = [&](int u, int e) {
-                    return __builtin_amdgcn_exp2f(__builtin_fmaf(acc[u][e >> 2][e & 3], w.s.scale2, -ml[rt].x));
+                    return __builtin_amdgcn_exp2f(__builtin_fmaf(acc[u][e >> 2][e & 3], w.scale2, -ml[rt].x));
                 };
                 // the tile's first row's limit decides whether any key of the wave is hidden in it
                 if (limit(row0 + 16 * rt) < key0 + kWaveKeys - 1) {
@@ -278,10 +295,10 @@ __global__ __launch_bounds__(256) void finish_few_kernel(WeightArgs w, int n_mer
         if (key + e < T) store_weight(w, h, key + e, sum[e]);
 }
 
-template <int KIND, int D>
+template <int KIND, int D, bool T4 = false>
 int launch_weights(const WeightArgs& w, hipStream_t stream) {
     const int T = w.s.seg[1].T;
-    hipLaunchKernelGGL((key_weights_kernel<KIND, D>), dim3((T + kWgKeys - 1) / kWgKeys, w.s.hkv, w.row_splits),
+    hipLaunchKernelGGL((key_weights_kernel<KIND, D, T4>), dim3((T + kWgKeys - 1) / kWgKeys, w.s.hkv, w.row_splits),
                        dim3(64 * kWgWaves), 0, stream, w);
     QW_HIP_CHECK(hipGetLastError());
     if (w.row_splits > 1) {
@@ -305,7 +322,6 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
                "scored attention: too many rows");
     QW_REQUIRE(std::isfinite(scale) && std::isfinite(decay) && decay >= 0.0f, QW_ERR_INVALID_ARGUMENT,
                "scored attention: scale must be finite, decay finite and >= 0");
-    QW_REQUIRE(!c.turbo4(), QW_ERR_UNSUPPORTED, "scored attention: not over Turbo4 caches");
     const int64_t T = (int64_t)c.offset + (append ? n_rows : 0);
     QW_REQUIRE(T > 0 && (!causal || T >= n_rows), QW_ERR_INVALID_ARGUMENT,
                "scored attention: empty cache, or fewer cached keys than causal query rows");
@@ -327,13 +343,18 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
                              &w.s))
         return rc;
     const int R = w.s.R;
+    const int64_t q_rows = (int64_t)n_q_heads * n_rows;
+    const bool t4 = c.turbo4();
+    if (t4)
+        if (int rc = shared_turbo4_room(c, q_rows, stream, &w.s)) return rc;
     w.weights = decay > 0.0f ? weights : nullptr;
     w.weights_out = weights_out;
     w.ws_in = weights_stride;
     w.ws_out = weights_out_stride;
     w.n_weights = n_weights;
     w.decay = decay;
-    if (R <= 16) {
+    w.scale2 = w.s.q_flip ? -w.s.scale2 : w.s.scale2;
+    if (R <= 16 && !t4) {
         w.s.score_stride = (T + 31) / 32 * 32;
         void* scores = nullptr;
         if (int rc = workspace(kWsRowSums, c.device, stream, (size_t)c.hkv * R * w.s.score_stride * sizeof(float), &scores))
@@ -359,15 +380,19 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
     const size_t ml_bytes = ((size_t)c.hkv * R * sizeof(float2) + 15) / 16 * 16;
     const size_t part_bytes = w.row_splits > 1 ? ((size_t)w.row_splits * c.hkv * T * sizeof(float) + 15) / 16 * 16 : 0;
     // the weights' kernel copies q into LDS by pieces of 16 bytes: a q off their alignment is copied first
-    const size_t q_bytes = (uintptr_t)q % 16 ? (size_t)n_q_heads * n_rows * c.D * sizeof(f16) : 0;
+    const size_t q_bytes = (uintptr_t)w.s.q % 16 ? (size_t)n_q_heads * n_rows * c.D * sizeof(f16) : 0;
     void* ws = nullptr;
     if (int rc = workspace(kWsRowSums, c.device, stream, ml_bytes + part_bytes + q_bytes, &ws)) return rc;
     w.s.row_ml = (float2*)ws;
     w.part = (float*)((char*)ws + ml_bytes);
     if (append)
         if (int rc = c.update(k_new, v_new, n_rows, stream)) return rc;
+    if (t4)
+        if (int rc = shared_turbo4_rotate_q(c, q, q_rows, w.s, stream)) return rc;
     if (int rc = launch_shared(nullptr, &c, w.s, stream)) return rc;
     if (int rc = launch_shared_merge(c.D, w.s, stream)) return rc;
+    if (t4)
+        if (int rc = launch_turbo4_rotate(c, w.s.out, (int)q_rows, true, (f16*)out, stream)) return rc;
     if (w.s.n_slots == 1) {
         hipLaunchKernelGGL(row_sums_kernel, dim3((R + 255) / 256, c.hkv), dim3(256), 0, stream, w.s);
         QW_HIP_CHECK(hipGetLastError());
@@ -380,6 +405,7 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
         QW_HIP_CHECK(hipGetLastError());
         w.s.q = to;
     }
+    if (t4) return c.D == 256 ? launch_weights<4, 256, true>(w, stream) : launch_weights<4, 128, true>(w, stream);
     if (c.D == 256)
         return c.bits == 4   ? launch_weights<4, 256>(w, stream)
                : c.bits == 8 ? launch_weights<8, 256>(w, stream)

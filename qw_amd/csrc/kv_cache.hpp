@@ -175,6 +175,10 @@ struct DeviceGuard {
 int turbo4_attention(KVCache& c, const void* q, int n_q_heads, int n_rows, float scale,
                      bool causal, void* out, hipStream_t stream);
 
+// Rows of a Turbo4 cache's head_dim into its K basis (q), or back out of its V basis (an
+// attention's output in the rotated basis); fp16 to fp16.
+int launch_turbo4_rotate(const KVCache& c, const f16* in, int rows, bool back, f16* out, hipStream_t stream);
+
 // Kernel launchers (attend_decode.hip, attend_block.hip).
 int launch_attention(KVCache& c, const void* q, int n_q_heads, int n_rows, float scale,
                      bool causal, void* out, hipStream_t stream);

@@ -1041,4 +1041,17 @@ static int turbo4_expansion_route(KVCache& c, const void* q, int n_q_heads, int 
     return QW_OK;
 }
 
+int launch_turbo4_rotate(const KVCache& c, const f16* in, int rows, bool back, f16* out, hipStream_t stream) {
+    const int D = c.D;
+    const float* const s_in = c.t4_tables + (back ? 1 : 2) * D;   // the V basis's s2, the K basis's s1
+    const float* const s_out = c.t4_tables + (back ? 0 : 3) * D;  // s1, s2
+    const dim3 grid((unsigned)((rows + 3) / 4));
+    if (D == 256)
+        hipLaunchKernelGGL(turbo4_rotate_kernel<256>, grid, dim3(256), 0, stream, in, out, rows, s_in, s_out);
+    else
+        hipLaunchKernelGGL(turbo4_rotate_kernel<128>, grid, dim3(256), 0, stream, in, out, rows, s_in, s_out);
+    QW_HIP_CHECK(hipGetLastError());
+    return QW_OK;
+}
+
 }  // namespace qw

@@ -7,8 +7,9 @@ n weights are added in fp32 in any order, n e at most; decay * weights adds a pr
 import numpy as np
 import pytest
 
+import oracle
 from conftest import rng
-from test_gpu_shared import E, attend, dev, filled, queries, rows_of
+from test_gpu_shared import E, attend, dev, filled, queries, rows_of, turbo4_close, turbo4_rows
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -79,6 +80,37 @@ def test_scored_matches_64_bits(mode, hq, hkv, D, L, T, causal):
     out, w = cache.attention_scored(q, D ** -0.5, weights=store, causal=causal, weights_out=store)
     assert w.data_ptr() == store.data_ptr() and torch.equal(store[:, T:], before[:, T:])
     check_scored(out, w, q, cache, D ** -0.5, causal, before[:, :T], 1.0)
+
+
+@pytest.mark.parametrize("L", [1, 9, 40])
+def test_scored_negative_and_zero_scale(L):
+    r = rng(L)
+    cache = filled("affine4", 2, 128, 200, r)
+    q = queries(r, 1, 8, L, 128)
+    for scale in (-0.08, 0.0):
+        out, w = cache.attention_scored(q, scale, causal=True)
+        check_scored(out, w, q, cache, scale, True)
+
+
+@pytest.mark.parametrize("hq,hkv,D,L,T", [(24, 4, 256, 1, 700), (8, 2, 128, 3, 129), (24, 4, 128, 30, 300), (12, 1, 256, 20, 64)])
+def test_scored_turbo4(hq, hkv, D, L, T):
+    r = rng(T + L)
+    cache = filled("turbo4", hkv, D, T, r)
+    q = queries(r, 1, hq, L, D)
+    before = torch.rand((hkv, T), device="cuda")
+    out, w = cache.attention_scored(q, D ** -0.5, weights=before, decay=0.5, causal=True)
+    k, v, tab = turbo4_rows(cache)
+    q = oracle.turbo4_rotate(q.double().cpu().numpy()[0], tab["k_s1"], tab["k_s2"]).astype(np.float16).astype(np.float64)
+    ref, wr = np.zeros(out.shape[1:]), 0.5 * before.double().cpu().numpy()
+    for j in range(hq):
+        h = j // (hq // hkv)
+        for i in range(L):
+            n = T - L + i + 1
+            ref[j, i], _, p, _ = attend(q[j, i], k[h, :n], v[h, :n], D ** -0.5)
+            wr[h, :n] += p
+    turbo4_close(out.double().cpu().numpy()[0], oracle.turbo4_rotate(ref, tab["v_s2"], tab["v_s1"]))
+    # a rotated q that rounds the other way moves a score by a step of fp16: 2^-10 of sum |q k| scale at most
+    assert np.allclose(w.double().cpu().numpy(), wr, rtol=2e-2, atol=1e-6)
 
 
 def test_scored_decay_zero_reads_nothing():
@@ -204,7 +236,6 @@ def test_scored_refusals():
     buf = torch.zeros((2, 44), device="cuda")
     refused(1, call, q, 0.1, weights=buf[:, :20], weights_out=buf[:, 5:25])  # shifted overlap
     refused(1, filled("fp16", 2, 128, 0, r).attention_scored, q, 0.1)
-    refused(2, filled("turbo4", 2, 128, 5, r).attention_scored, q, 0.1)
     kv = dev(np.zeros((1, 2, 1, 128), np.float16))
     refused(1, cache.update_and_attention_scored, q, kv, kv[:, :1], 0.1)
     assert cache.offset == 20

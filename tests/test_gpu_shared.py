@@ -9,6 +9,7 @@ scales a weight by 1 + g and the row's sum alike. With A = sum p |v|:
 import numpy as np
 import pytest
 
+import oracle
 from conftest import rng
 
 pytestmark = pytest.mark.gpu
@@ -195,6 +196,44 @@ def test_shared_streams_views_and_graph():
         assert torch.equal(out, prefix.shared_attention(q, tails, 0.1, starts=st))
 
 
+def turbo4_rows(cache):
+    """A Turbo4 cache's rows in their rotated bases, [H, T, D] in 64 bits, and its tables."""
+    tab = oracle.turbo4_tables(cache.head_dim, cache.turbo_seed)
+    snap = {n: x.cpu().numpy() for n, x in cache.snapshot_tensors().items()}
+    k = oracle.turbo4_expand_rotated(snap["k_packed"], snap["k_rescale"][..., 0], tab)
+    v = oracle.turbo4_expand_rotated(snap["v_packed"], snap["v_rescale"][..., 0], tab)
+    return k.astype(np.float64), v.astype(np.float64), tab
+
+
+def turbo4_close(out, ref):
+    """The bar of the other Turbo4 attention tests: 2e-3 absolute, 1e-3 relative L2 (q and the rotated
+    output are rounded to fp16 between the rotations)."""
+    err = np.abs(out - ref)
+    assert err.max() <= 2e-3 and np.linalg.norm(out - ref) <= 1e-3 * np.linalg.norm(ref), (err.max(), np.linalg.norm(out - ref) / np.linalg.norm(ref))
+
+
+@pytest.mark.parametrize("hq,hkv,D,B,L,P,T", [(24, 4, 256, 3, 1, 700, 37), (8, 2, 128, 4, 2, 127, 129), (24, 4, 128, 6, 5, 1030, 60),
+                                              (12, 1, 256, 1, 1, 64, 1), (16, 2, 256, 5, 4, 300, 70)])
+def test_shared_turbo4(hq, hkv, D, B, L, P, T):
+    r = rng(P + T)
+    prefix, tails = filled("turbo4", hkv, D, P, r), filled("turbo4", B * hkv, D, T, r)
+    q = queries(r, B, hq, L, D)
+    starts = r.integers(0, T - L + 1, B).astype(np.int32)
+    out = prefix.shared_attention(q, tails, D ** -0.5, starts=dev(starts)).double().cpu().numpy()
+    pk, pv, tab = turbo4_rows(prefix)
+    tk, tv, _ = turbo4_rows(tails)
+    q = oracle.turbo4_rotate(q.double().cpu().numpy(), tab["k_s1"], tab["k_s2"]).astype(np.float16).astype(np.float64)
+    ref = np.zeros_like(out)
+    for b in range(B):
+        for j in range(hq):
+            h = j // (hq // hkv)
+            for i in range(L):
+                t = (b * hkv + h, slice(starts[b], T - L + i + 1))
+                k, v = np.concatenate([pk[h], tk[t]]), np.concatenate([pv[h], tv[t]])
+                ref[b, j, i] = attend(q[b, j, i], k, v, D ** -0.5)[0]
+    turbo4_close(out, oracle.turbo4_rotate(ref, tab["v_s2"], tab["v_s1"]))
+
+
 def test_shared_long_offsets():
     """Rows behind element 2^31 of a plane."""
     import qw_amd
@@ -248,6 +287,9 @@ def test_shared_refusals():
     refused(1, one.shared_attention, q[:1, :1], one, 0.1)                 # the prefix as its own tail
     refused(1, prefix.shared_attention, queries(r, 3, 8, 1, 256), filled("fp16", 6, 256, 3, r), 0.1)
     refused(2, prefix.shared_attention, q, filled("turbo4", 6, 128, 3, r), 0.1)
+    refused(2, filled("turbo4", 2, 128, 20, r).shared_attention, q, filled("affine4", 6, 128, 3, r), 0.1)
+    other = qw_amd.KVCache("turbo4", 6, 128, turbo_seed=7)
+    refused(2, filled("turbo4", 2, 128, 20, r).shared_attention, q, other, 0.1)
     closed = filled("fp16", 6, 128, 3, r)
     closed.close()
     refused(1, call, q, closed, 0.1)
