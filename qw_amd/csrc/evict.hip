@@ -134,13 +134,16 @@ __device__ __forceinline__ void emit(const SelectArgs& a, int h, int t0, const f
     }
 }
 
-// The keys of a thread: weights, ranks, and which of them lie in the middle.
+// The weights of a thread's keys; their ranks, and which of them lie in the middle.
 template <int KPT>
-__device__ __forceinline__ uint32_t load_keys(const SelectArgs& a, int h, int t0, float (&x)[KPT], uint32_t (&u)[KPT]) {
+__device__ __forceinline__ void load_keys(const SelectArgs& a, int h, int t0, float (&x)[KPT]) {
     const float* w = a.weights + h * a.stride;
-    uint32_t mid = 0;
 #pragma unroll
     for (int e = 0; e < KPT; e++) x[e] = t0 + e < a.T ? w[t0 + e] : 0.0f;
+}
+template <int KPT>
+__device__ __forceinline__ uint32_t rank_keys(const SelectArgs& a, int t0, const float (&x)[KPT], uint32_t (&u)[KPT]) {
+    uint32_t mid = 0;
 #pragma unroll
     for (int e = 0; e < KPT; e++) {
         u[e] = weight_rank(x[e]);
@@ -158,7 +161,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(SelectArgs a)
     const int tid = threadIdx.x, h = blockIdx.x, t0 = tid * KPT;
     float x[KPT];
     uint32_t u[KPT];
-    const uint32_t mid = load_keys<KPT>(a, h, t0, x, u);
+    load_keys<KPT>(a, h, t0, x);
+    const uint32_t mid = rank_keys<KPT>(a, t0, x, u);
     uint32_t prefix = 0, left = (uint32_t)a.need;
 #pragma unroll
     for (int d = 0; d < kDigits; d++) {
@@ -178,6 +182,18 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(SelectArgs a)
 // launch's counts by every workgroup for itself), d = 3 writes the kept keys.
 constexpr int kChunkKeys = 4, kChunk = kSelThreads * kChunkKeys;
 
+// f of a thread's word of the first n chunks' counts, 16 loads in flight.
+template <class F>
+__device__ __forceinline__ void for_chunks(const uint32_t* word, int n, F f) {
+    for (int i = 0; i < n; i += 16) {
+        uint32_t v[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) v[j] = word[(int64_t)min(i + j, n - 1) * (kBins / 2)];
+#pragma unroll
+        for (int j = 0; j < 16; j++) f(i + j < n ? v[j] : 0u);
+    }
+}
+
 __global__ __launch_bounds__(kSelThreads) void evict_digit_kernel(SelectArgs a, int d) {
     __shared__ uint32_t hist[kBins];
     __shared__ uint32_t s_wave[kSelWaves];
@@ -185,27 +201,24 @@ __global__ __launch_bounds__(kSelThreads) void evict_digit_kernel(SelectArgs a, 
     __shared__ uint32_t s_sum[2];
     const int tid = threadIdx.x, lane = tid & 63, c = blockIdx.x, h = blockIdx.y, hkv = gridDim.y;
     const int t0 = c * kChunk + tid * kChunkKeys;
+    // (all loads first: the weights, the last digits picked, the last digit's counts)
     float x[kChunkKeys];
     uint32_t u[kChunkKeys];
-    const uint32_t mid = load_keys<kChunkKeys>(a, h, t0, x, u);
+    load_keys<kChunkKeys>(a, h, t0, x);
     hist[2 * tid] = hist[2 * tid + 1] = 0;
     if (tid < 2) s_sum[tid] = 0;
     const uint32_t* hist_d = nullptr;  // the last digit's counts of this head
     uint32_t prefix = 0, left = (uint32_t)a.need;
     if (d > 0) {
         hist_d = a.hist + ((int64_t)(d - 1) * hkv + h) * a.chunks * (kBins / 2);
+        const uint2 p0 = a.pick[h], p1 = a.pick[hkv + h];  // (read where written: d > 1, d > 2)
         uint32_t n_hi = 0, n_lo = 0;
-#pragma unroll 16
-        for (int i = 0; i < a.chunks; i++) {
-            const uint32_t v = hist_d[(int64_t)i * (kBins / 2) + kBins / 2 - 1 - tid];
+        for_chunks(hist_d + kBins / 2 - 1 - tid, a.chunks, [&](uint32_t v) {
             n_hi += v >> 16;
             n_lo += v & 0xFFFFu;
-        }
-        for (int i = 0; i < d - 1; i++) {
-            const uint2 p = a.pick[i * hkv + h];
-            prefix = prefix << digit_bits(i) | (p.x & ((1u << digit_bits(i)) - 1));
-            left = p.y;
-        }
+        });
+        if (d > 1) prefix = p0.x, left = p0.y;
+        if (d > 2) prefix = prefix << digit_bits(1) | p1.x, left = p1.y;
         const uint2 p = pick_bin(n_hi, n_lo, left, s_wave, &s_pick);
         if (c == 0 && tid == 0) a.pick[(d - 1) * hkv + h] = p;
         prefix = prefix << digit_bits(d - 1) | (p.x & ((1u << digit_bits(d - 1)) - 1));
@@ -213,6 +226,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_digit_kernel(SelectArgs a, 
     } else {
         __syncthreads();
     }
+    const uint32_t mid = rank_keys<kChunkKeys>(a, t0, x, u);
     if (d < kDigits) {
         count_digit<kChunkKeys>(hist, u, mid, d, prefix);
         if (d > 0) {  // keys that the last digit put above the cut: the digits before it equal, it larger
@@ -233,12 +247,10 @@ __global__ __launch_bounds__(kSelThreads) void evict_digit_kernel(SelectArgs a, 
     // kept keys above the cut and ties in the chunks before this one; protected ones too
     uint32_t n_above = 0, n_equal = 0;
     const uint32_t b2 = prefix & ((1u << digit_bits(2)) - 1);
-#pragma unroll 16
-    for (int i = 0; i < c; i++) {
-        const uint32_t v = hist_d[(int64_t)i * (kBins / 2) + tid];
+    for_chunks(hist_d + tid, c, [&](uint32_t v) {
         n_above += (2u * tid > b2 ? v & 0xFFFFu : 0u) + (2u * tid + 1 > b2 ? v >> 16 : 0u);
         n_equal += (2u * tid == b2 ? v & 0xFFFFu : 0u) + (2u * tid + 1 == b2 ? v >> 16 : 0u);
-    }
+    });
     for (int i = tid; i < c; i += kSelThreads)
         n_above += a.above[h * a.chunks + i] + a.above[(hkv + h) * a.chunks + i];
     if (n_above) atomicAdd(&s_sum[0], n_above);
