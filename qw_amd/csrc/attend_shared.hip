@@ -299,8 +299,16 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = max(0, (u.k_end - u.k_begin + KT - 1) / KT);  // tiles
     const int n_rt = (u.row_end - u.row0 + 16 * RT - 1) / (16 * RT);  // a computing wave each
+    // Wave w computes row tile rt_i, its part of each tile's keys; a part above 0 parks its sums in region
+    // w - park0 and part 0 joins them, dist waves apart. Five or six row tiles would leave two SIMDs
+    // (w mod 4) twice the work of the others: waves 4 to 7 then take halves of the last two.
+    const bool halves = RT == 1 && NSUB == 2 && (n_rt == 5 || n_rt == 6);
     const int lrt = n_rt <= 1 ? 0 : n_rt <= 2 ? 1 : n_rt <= 4 ? 2 : 3;
-    const int parts = min(kWaves >> lrt, NSUB);
+    const int parts = halves ? (wave < 4 ? 1 : 2) : min(kWaves >> lrt, NSUB);
+    const int dist = halves ? 2 : 1 << lrt, park0 = halves ? 6 : dist;
+    const int rt_i = !halves ? wave & (dist - 1) : wave < 4 ? wave : 4 + (wave & 1);
+    const int part = !halves ? wave >> lrt : wave < 4 ? 0 : wave >> 1 & 1;
+    const bool joined = halves || parts > 1;  // (the same in all waves)
     constexpr int REG = RT * (64 * NT * 16 + 64 * 8);  // a parked part
     static_assert((kWaves - kWaves / (NSUB < 8 ? NSUB : 8)) * REG <= kSharedLds, "the parked parts fit");
 
@@ -371,12 +379,12 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
                 __syncthreads();
             }
         }
-        if (parts > 1) __syncthreads();
+        if (joined) __syncthreads();
         return;
     }
 
     // ---- computing waves: RT row tiles, and a part of each tile's keys
-    const int part = wave >> lrt, wrow0 = u.row0 + 16 * RT * (wave & ((1 << lrt) - 1));
+    const int wrow0 = u.row0 + 16 * RT * rt_i;
     const bool live = part < parts && wrow0 < u.row_end;
     const int wave_first_lim = u.limit(min(wrow0, u.row_end - 1), a.G), wave_lim = u.limit(min(wrow0 + 16 * RT - 1, u.row_end - 1), a.G);
     int lim[RT];
@@ -482,9 +490,9 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
     float l[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) l[rt] = wave_sum_g(l_run[rt]);
-    if (parts > 1) {
+    if (joined) {
         if (live && part > 0) {
-            char* reg = lds + (wave - (1 << lrt)) * REG;
+            char* reg = lds + (wave - park0) * REG;
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
 #pragma unroll
@@ -495,7 +503,7 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
         __syncthreads();
         if (live && part == 0) {
             for (int p = 1; p < parts; p++) {
-                const char* reg = lds + (((p - 1) << lrt) + wave) * REG;
+                const char* reg = lds + (wave + p * dist - park0) * REG;
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
                     const float2 ml = ((const float2*)(reg + RT * NT * 64 * 16))[rt * 64 + lane];
