@@ -309,8 +309,8 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
     const bool rows_of_v = a.row_major_v && group < a.groups_v;
     if (group >= a.groups_v || rows_of_v) {
         constexpr int ppr = pieces / 8;
-        const int id = (group - (rows_of_v ? 0 : a.groups_v)) * 256 + threadIdx.x;
-        const int b = id / ppr, c = id - b * ppr;
+        const uint32_t id = (uint32_t)(group - (rows_of_v ? 0 : a.groups_v)) * 256u + threadIdx.x;
+        const int b = (int)(id / ppr), c = (int)(id % ppr);
         if (id == 0 && h == 0 && !rows_of_v && a.flag_to) *a.flag_to = *a.flag;
         if (8 * b >= a.n) return;
         const u32x4* from = rows_of_v ? a.v : a.k;
@@ -338,8 +338,9 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
         }
         return;
     }
-    const int id = group * 256 + threadIdx.x, pc = id % pieces;
-    int b = id / pieces;
+    const uint32_t id = (uint32_t)group * 256u + threadIdx.x;  // (past 2^31 from 67M fp16 rows of D = 256 on)
+    const int pc = (int)(id % pieces);
+    int b = (int)(id / pieces);
     if constexpr (pieces >= 64) b = __builtin_amdgcn_readfirstlane(b);  // a wave's pieces are one block's: its positions go through scalar loads
     if (8 * b >= a.n) return;
     const int32_t* kept = a.kept + (int64_t)h * a.n + 8 * b;
@@ -432,6 +433,9 @@ int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_str
         dst.offset = 0;
         return QW_OK;
     }
+    const int rows8 = (n + 7) / 8 * 8;
+    const int64_t of_v = (int64_t)(rows8 / 8) * (src.D * src.bits / 16), of_k = of_v / 8;  // threads of a head
+    QW_REQUIRE(of_v + of_k + 512 <= UINT32_MAX, QW_ERR_UNSUPPORTED, "evict: too many rows for one call");
     DeviceGuard dg(src.device);
     QW_REQUIRE(dg.ok, QW_ERR_HIP, "evict: hipSetDevice failed");
     if (dst.cap < n) {
@@ -442,7 +446,6 @@ int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_str
         if (int rc = dst.reserve(n, stream)) return rc;
     }
     // in place the rows that move are staged: planes of n rows a head, in whole 8-row blocks
-    const int rows8 = (n + 7) / 8 * 8;
     char* ws = nullptr;
     size_t at[4] = {0, src.k_data_bytes(rows8), 0, 0};
     at[2] = at[1] + src.v_data_bytes(rows8);
@@ -474,7 +477,6 @@ int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_str
     c.cap_to = staged ? rows8 : dst.cap;
     c.kp_words = src.affine() ? src.D / kGroup : src.turbo4() ? 1 : 0;
     c.row_major_v = src.turbo4() ? 1 : 0;
-    const int64_t of_v = (int64_t)(rows8 / 8) * (src.D * src.bits / 16), of_k = of_v / 8;  // threads of a head
     c.groups_v = (int)((src.turbo4() ? of_k + 255 : of_v + 255) / 256);
     const dim3 grid((unsigned)(c.groups_v + (of_k + 255) / 256), src.hkv);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, c); };
