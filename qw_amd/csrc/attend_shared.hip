@@ -910,6 +910,8 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, cons
     a.Tq = n_rows;
     a.G = G;
     a.hkv = hkv;
+    // (a merge of a workgroup of 256 a row stays below 2^32 threads)
+    QW_REQUIRE((int64_t)n_seq * n_rows * G < 1 << 24, QW_ERR_UNSUPPORTED, "attention: 2^24 or more rows a KV head in one call");
     a.R = n_seq * n_rows * G;
     // (a scale of 0 stands as a tiny one, which leaves every score 0 and a hidden key's -inf itself)
     a.scale2 = std::max(std::fabs(scale) * kLog2e, 1e-37f);
@@ -981,7 +983,9 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, cons
             s.slot0 = a.n_slots;
             a.n_slots += s.n_split;
             const int64_t units = (int64_t)n_qt[i] * s.heads * s.n_split;
-            QW_REQUIRE(units < (int64_t)1 << 30, QW_ERR_UNSUPPORTED, "shared attention: too many rows for one call");
+            // (both caches' units in one launch of fewer than 2^32 threads)
+            QW_REQUIRE(units <= UINT32_MAX / (64 * (kWaves + kFillWaves)) / 2, QW_ERR_UNSUPPORTED,
+                       "shared attention: too many rows for one call");
             s.n_units = (int)units;
         }
         return QW_OK;

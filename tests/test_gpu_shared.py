@@ -294,3 +294,18 @@ def test_shared_refusals():
     closed.close()
     refused(1, call, q, closed, 0.1)
     assert tails.offset == 3 and prefix.offset == 20
+
+
+@pytest.mark.parametrize("n_rows", [1 << 24, 1 << 26])
+def test_too_many_rows_refused(n_rows):
+    """More rows than a launch's threads cover: refused on the host, by the declared sizes alone."""
+    import qw_amd
+
+    prefix = filled("fp16", 1, 128, 20, rng(3))
+    x, w = torch.zeros(128, dtype=torch.float16, device="cuda"), torch.zeros((1, 20), device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    lib, q = qw_amd.lib(), x.data_ptr()
+    assert lib.qw_kv_shared_attention(prefix._h, None, 1, None, q, 1, n_rows, 0.1, q, st) == 2
+    assert lib.qw_kv_attention_scored(prefix._h, q, 1, n_rows, 0.1, 0, None, 0, 0, 0.0, w.data_ptr(), 20, q, st) in (1, 2)
+    torch.cuda.synchronize()
+    assert prefix.offset == 20 and not w.any()
