@@ -563,7 +563,7 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
 // (g, r16) taking dims D/4 g .. of its key, V's 8-key blocks as B - and requests the next chunk's K
 // once this one's scores are formed, its V once this one's P . V is. Bound by HBM latency and
 // bandwidth; the waves' sums join through LDS.
-template <int KIND, int D, bool FAST>
+template <int KIND, int D, bool FAST, bool T4 = false>
 __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
     constexpr int NM = D / 32, NT = D / 16, NG = D / kGroup, DG = D / 4, DPL = D / 16;
     constexpr int KP = DG * KIND / 128, VP = DPL * KIND / 16, E = 16 / KIND;  // 16-byte pieces a lane; dims a piece of V
@@ -573,6 +573,14 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     const uint32_t magic = vconst(kMagic);
+    constexpr int kSums = (16 * kWaves * 2 + kWaves * 16 * D) * 4;  // the waves' sums, joined at the end
+    float2* const cp = (float2*)(lds + kSums);  // T4: a byte's two centroids
+    static_assert(kSums + 256 * sizeof(float2) <= kSharedLds, "the waves' sums and the centroid pairs fit");
+    if constexpr (T4) {
+        const float* const cb = (int)blockIdx.x >= a.seg[0].n_units ? a.seg[1].t4_cb : a.seg[0].t4_cb;
+        if (tid < 256) cp[tid] = float2{cb[tid & 15], cb[tid >> 4]};
+        __syncthreads();
+    }
     const bool row_ok = r16 < rows;
     const int rr = row_ok ? r16 : 0, lim = row_ok ? u.limit(row_base + rr, a.G) : -1, first_lim = u.limit(row_base, a.G);
     const int k_begin = max(u.k_begin, lo / 32 * 32), k_end = u.k_end;
@@ -580,15 +588,18 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
 #pragma unroll
     for (int m = 0; m < NM; m++) {
         const u32x4 w = *(const u32x4*)(a.q + q_row(a, h, row_base + rr) * D + 8 * k_chunk<KIND>(m, g));
-        qb[m] = as_h8(q_piece<KIND>(row_ok ? w : u32x4{0, 0, 0, 0}, a.q_flip));
+        qb[m] = as_h8(q_piece<T4 ? 16 : KIND>(row_ok ? w : u32x4{0, 0, 0, 0}, a.q_flip));
     }
     const uint32_t code_off = u.code_off;
     const int64_t krow0 = (int64_t)hc * cap + 8 * (r16 >> 2) + (r16 & 3), vblk0 = (int64_t)hc * (cap / 8) + g;
     const u32x4* const ksrc = (const u32x4*)(u.k_data + krow0 * (D * KIND / 32)) + g;
-    const uint32_t* const kpsrc = KIND == 16 ? nullptr : u.k_params + krow0 * NG;
+    const uint32_t* const kpsrc = KIND == 16 ? nullptr : u.k_params + krow0 * (T4 ? 1 : NG);
     const u32x4* const vsrc = (const u32x4*)(u.v_data + vblk0 * (D * KIND / 4)) + r16;
     const u32x4* const vpsrc =
-        KIND == 16 ? nullptr : (const u32x4*)(u.v_params + (vblk0 * NG + r16 * DPL / kGroup) * 8);
+        KIND == 16 ? nullptr : (const u32x4*)(u.v_params + (T4 ? vblk0 : vblk0 * NG + r16 * DPL / kGroup) * 8);
+    // T4: V row-major, dims DPL n .. of the block's 8 rows
+    const uint32_t* const vtsrc = T4 ? u.v_data + vblk0 * D + r16 * (DPL / 8) : nullptr;
+    uint32_t vt[T4 ? 8 : 1][DPL / 8];
     u32x4 kc[2][KP], vc[VP], vp[2];
     uint32_t kp[2][KP];
     auto load_k = [&](int key) {
@@ -597,11 +608,22 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
 #pragma unroll
             for (int i = 0; i < KP; i++) {
                 kc[tt][i] = ksrc[(int64_t)(key + 4 * tt) * (D * KIND / 128) + 4 * i];
-                if constexpr (KIND != 16)
+                if constexpr (T4)
+                    kp[tt][i] = kpsrc[key + 4 * tt];
+                else if constexpr (KIND != 16)
                     kp[tt][i] = kpsrc[(int64_t)(key + 4 * tt) * NG + k_param_slot(k_piece_group<KIND>(i, g), NG)];
             }
     };
     auto load_v = [&](int key) {
+        if constexpr (T4) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int w = 0; w < DPL / 8; w++) vt[i][w] = vtsrc[(int64_t)(key + i) * (D / 8) + w];
+            vp[0] = vpsrc[(int64_t)(key / 8) * 2];
+            vp[1] = vpsrc[(int64_t)(key / 8) * 2 + 1];
+            return;
+        }
         // piece j holds slots 16 E j + E n ..: dims DPL n + E j .. of column n
 #pragma unroll
         for (int j = 0; j < VP; j++) vc[j] = vsrc[(int64_t)(key / 8) * (D * KIND / 16) + 16 * j];
@@ -627,15 +649,23 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
             PairConsts pc;
 #pragma unroll
             for (int m = 0; m < NM; m++) {
-                if constexpr (KIND != 16)
+                if constexpr (KIND != 16 && !T4)
                     if (m % E == 0) {
                         const half2v sb = h2(kp[tt][m / E]), s = {sb.x, sb.x}, b = {sb.y, sb.y};
                         pc = make_consts<FAST, KIND>(s, s, s, s, b, b, b, b, code_off);
                     }
                 half8 ka;
-                if constexpr (KIND == 16)
+                if constexpr (KIND == 16) {
                     ka = as_h8(kc[tt][m]);
-                else if constexpr (KIND == 8)
+                } else if constexpr (T4) {
+                    const float kr = (float)h2(kp[tt][0]).x;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float2 c = cp[kc[tt][m / 4][m % 4] >> (8 * i) & 0xFFu];
+                        ka[2 * i] = t4_f16_product(c.x, kr);
+                        ka[2 * i + 1] = t4_f16_product(c.y, kr);
+                    }
+                } else if constexpr (KIND == 8)
                     ka = deq8<FAST>(kc[tt][m / 2][2 * m % 4], kc[tt][m / 2][2 * m % 4 + 1], pc);
                 else
                     ka = deq4<FAST>(kc[tt][m / 4][m % 4], pc, magic);
@@ -682,6 +712,27 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
             l_run += p;
             p16[e] = (f16)p;
         }
+        if constexpr (T4) {
+            u32x4 keep = {~0u, ~0u, ~0u, ~0u};
+            if (edge) keep = keep_keys(u.hi - (key + 8 * g)) & ~keep_keys(lo - (key + 8 * g));
+#pragma unroll
+            for (int j = 0; j < NT / 2; j++) {  // two dims
+                half8 y0, y1;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float vr = (float)h2(vp[i / 4][i % 4]).y;
+                    const float2 c = cp[vt[i][j / 4] >> (8 * (j % 4)) & 0xFFu];
+                    y0[i] = t4_f16_product(c.x, vr);
+                    y1[i] = t4_f16_product(c.y, vr);
+                }
+                y0 = as_h8(__builtin_bit_cast(u32x4, y0) & keep);  // hidden keys: 0 x inf is NaN
+                y1 = as_h8(__builtin_bit_cast(u32x4, y1) & keep);
+                acc_o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p16, y0, acc_o[2 * j], 0, 0, 0);
+                acc_o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p16, y1, acc_o[2 * j + 1], 0, 0, 0);
+            }
+            if (more) load_v(key + 32 * kWaves);
+            continue;
+        }
         PairConsts pc;
         if constexpr (KIND != 16)
             pc = make_consts<FAST, KIND>(h2(vp[0][0]), h2(vp[0][1]), h2(vp[0][2]), h2(vp[0][3]), h2(vp[1][0]), h2(vp[1][1]),
@@ -710,7 +761,6 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
     float* const s_m = (float*)lds;                    // [8 waves][16 rows]
     float* const s_l = s_m + 16 * kWaves;              // [8][16]
     float* const s_o = s_l + 16 * kWaves;              // [8][rows][D]
-    static_assert((16 * kWaves * 2 + kWaves * 16 * D) * 4 <= kSharedLds, "the waves' sums fit the tile buffers");
     if (g == 0) s_m[16 * wave + r16] = m_run;
     __syncthreads();
     float M = -INFINITY;
@@ -803,6 +853,11 @@ __global__ __launch_bounds__(64 * kWaves, 1) void shared_few_kernel(SharedArgs a
         if (unit_fast(a)) return few_body<KIND, D, true>(a, lds);
     few_body<KIND, D, false>(a, lds);
 }
+template <int D>
+__global__ __launch_bounds__(64 * kWaves, 1) void shared_t4_few_kernel(SharedArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    few_body<4, D, false, true>(a, lds);
+}
 
 template <int D>
 __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a) {
@@ -848,12 +903,15 @@ int launch_images(const SharedArgs& a, hipStream_t stream) {
     QW_HIP_CHECK(hipGetLastError());
     return QW_OK;
 }
+bool few_rows(const SharedArgs& a) {
+    return std::max(a.seg[0].n_units ? a.seg[0].unit_rows : 0, a.seg[1].n_units ? a.seg[1].unit_rows : 0) <= kFewRows;
+}
 template <int KIND, int D>
 int launch_units(const SharedArgs& a, hipStream_t stream) {
     if constexpr (KIND != 16)
         if (a.seg[1].images) return launch_images<KIND, D>(a, stream);
     const dim3 grid(a.seg[0].n_units + a.seg[1].n_units);
-    const bool few = std::max(a.seg[0].n_units ? a.seg[0].unit_rows : 0, a.seg[1].n_units ? a.seg[1].unit_rows : 0) <= kFewRows;
+    const bool few = few_rows(a);
     const void* const kernel = few ? (const void*)shared_few_kernel<KIND, D> : (const void*)shared_many_kernel<KIND, D>;
     if (int rc = ensure_dynamic_lds(kernel, kSharedLds)) return rc;
     if (few)
@@ -866,9 +924,14 @@ int launch_units(const SharedArgs& a, hipStream_t stream) {
 
 template <int D>
 int launch_t4_units(const SharedArgs& a, hipStream_t stream) {
-    if (int rc = ensure_dynamic_lds((const void*)shared_t4_many_kernel<D>, kSharedLds)) return rc;
-    hipLaunchKernelGGL(shared_t4_many_kernel<D>, dim3(a.seg[0].n_units + a.seg[1].n_units),
-                       dim3(64 * (kWaves + kFillWaves)), kSharedLds, stream, a);
+    const dim3 grid(a.seg[0].n_units + a.seg[1].n_units);
+    const bool few = few_rows(a);
+    const void* const kernel = few ? (const void*)shared_t4_few_kernel<D> : (const void*)shared_t4_many_kernel<D>;
+    if (int rc = ensure_dynamic_lds(kernel, kSharedLds)) return rc;
+    if (few)
+        hipLaunchKernelGGL(shared_t4_few_kernel<D>, grid, dim3(64 * kWaves), kSharedLds, stream, a);
+    else
+        hipLaunchKernelGGL(shared_t4_many_kernel<D>, grid, dim3(64 * (kWaves + kFillWaves)), kSharedLds, stream, a);
     QW_HIP_CHECK(hipGetLastError());
     return QW_OK;
 }
@@ -946,7 +1009,7 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, cons
         int most = 0;
         for (int i : in)
             if (c[i]) {
-                few = few && a.seg[i].unit_rows <= kFewRows && !c[i]->turbo4();
+                few = few && a.seg[i].unit_rows <= kFewRows;
                 most = std::max(most, tiles[i]);
             }
         auto unit_us = [&](int i, int n) {

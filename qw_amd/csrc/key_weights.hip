@@ -354,7 +354,7 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
     w.n_weights = n_weights;
     w.decay = decay;
     w.scale2 = w.s.q_flip ? -w.s.scale2 : w.s.scale2;
-    if (R <= 16 && !t4) {
+    if (R <= 16) {
         w.s.score_stride = (T + 31) / 32 * 32;
         void* scores = nullptr;
         if (int rc = workspace(kWsRowSums, c.device, stream, (size_t)c.hkv * R * w.s.score_stride * sizeof(float), &scores))
@@ -362,6 +362,8 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
         w.s.scores = (float*)scores;
         if (append)
             if (int rc = c.update(k_new, v_new, n_rows, stream)) return rc;
+        if (t4)
+            if (int rc = shared_turbo4_rotate_q(c, q, q_rows, w.s, stream)) return rc;
         if (int rc = launch_shared(nullptr, &c, w.s, stream)) return rc;
         const int n_merge = w.s.n_slots > 1 ? merge_groups(c.D, R, c.hkv, w.s.n_slots) : 0;
         const dim3 grid((unsigned)(n_merge + (T + 1023) / 1024), c.hkv);
@@ -370,7 +372,7 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
         else
             hipLaunchKernelGGL(finish_few_kernel<128>, grid, dim3(256), 0, stream, w, n_merge);
         QW_HIP_CHECK(hipGetLastError());
-        return QW_OK;
+        return t4 ? launch_turbo4_rotate(c, w.s.out, (int)q_rows, true, (f16*)out, stream) : QW_OK;
     }
     // row splits: about one workgroup a CU, of at least four steps each
     const int64_t groups = (T + kWgKeys - 1) / kWgKeys * c.hkv, steps = (R + kStepRows - 1) / kStepRows;

@@ -239,3 +239,24 @@ def test_scored_refusals():
     kv = dev(np.zeros((1, 2, 1, 128), np.float16))
     refused(1, cache.update_and_attention_scored, q, kv, kv[:, :1], 0.1)
     assert cache.offset == 20
+
+
+@pytest.mark.parametrize("hq,hkv,D,L,T", [(24, 4, 256, 1, 5000), (8, 2, 128, 1, 1), (32, 2, 256, 1, 33), (8, 2, 128, 4, 1500)])
+def test_scored_turbo4_few_rows(hq, hkv, D, L, T):
+    """Up to 16 rows a KV head: several key splits, a single key, a chunk's first key, causal limits inside one."""
+    test_scored_turbo4(hq, hkv, D, L, T)
+
+
+def test_scored_turbo4_steps_of_decoding():
+    """Tokens appended by the call itself; the same bits as an append before it."""
+    r = rng(9)
+    cache, want = filled("turbo4", 2, 128, 30, r), filled("turbo4", 2, 128, 0, r)
+    want.restore_snapshot(cache.snapshot_tensors())
+    w = w2 = None
+    for _ in range(4):
+        q = queries(r, 1, 8, 1, 128)
+        k, v = (dev(r.standard_normal((1, 2, 1, 128)).astype(np.float16)) for _ in range(2))
+        out, w = cache.update_and_attention_scored(q, k, v, 0.09, weights=w, decay=0.5, causal=True)
+        want.update(k, v)
+        out2, w2 = want.attention_scored(q, 0.09, weights=w2, decay=0.5, causal=True)
+        assert w.shape == (2, cache.offset) and torch.equal(out, out2) and torch.equal(w, w2)

@@ -309,3 +309,9 @@ def test_too_many_rows_refused(n_rows):
     assert lib.qw_kv_attention_scored(prefix._h, q, 1, n_rows, 0.1, 0, None, 0, 0, 0.0, w.data_ptr(), 20, q, st) in (1, 2)
     torch.cuda.synchronize()
     assert prefix.offset == 20 and not w.any()
+
+
+@pytest.mark.parametrize("hq,hkv,D,B,L,P,T", [(8, 2, 128, 2, 1, 700, 300), (12, 2, 256, 1, 2, 2500, 130), (16, 1, 128, 1, 1, 1, 33)])
+def test_shared_turbo4_few_rows(hq, hkv, D, B, L, P, T):
+    """At most 16 rows of a head in both caches."""
+    test_shared_turbo4(hq, hkv, D, B, L, P, T)
