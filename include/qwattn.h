@@ -284,7 +284,8 @@ int qw_kv_update_and_attention_scored(qw_kv_cache* cache, const void* q, int n_q
  *   weights_out (or NULL) [n_kv_heads][>= n]: their weights; not inside weights
  *   *n_kept (host, or NULL) = n
  * sink + recent <= budget. In place the moved rows pass through a workspace of
- * their size. */
+ * their size. A captured call repeats its move, with the lengths of the capture, at each replay,
+ * over whatever the cache then holds; the handle's offset changes once, at the capture. */
 int qw_kv_evict(qw_kv_cache* cache, qw_kv_cache* into, const float* weights, int64_t weights_stride,
                 int budget, int sink, int recent, int32_t* kept, float* weights_out,
                 int64_t weights_out_stride, int* n_kept, void* stream);

@@ -16,6 +16,8 @@ and the tests use the reference's names:
   ``causal_attention(q, k, v, scale, softcap, window)`` (``lib.rs:3185``);
   ``KVCache.update_and_attention(..., mask)`` and
   :meth:`KVCache.attention_general` take the same options over a cache.
+* :meth:`KVCache.shared_attention`, :meth:`KVCache.attention_scored` (with their
+  update forms) and :meth:`KVCache.evict` have no counterpart in the reference.
 
 Torch is used only to hold device memory and to name the current stream.
 Tensors follow the reference's layouts: ``[1, H, L, D]`` (the batch of 1 may

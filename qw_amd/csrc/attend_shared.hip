@@ -13,21 +13,22 @@
 // s_t, l = sum e^(s_t - m), O = sum e^(s_t - m) v_t, and two sets join as
 // (max(m, m'), l e^(m-M) + l' e^(m'-M), O e^(m-M) + O' e^(m'-M)). So the
 // prefix, whose keys all rows of a KV head see (n_seq Tq G of them), and the
-// tails, each seen by Tq G rows, are units of one launch, both cut into key
-// splits, and a second launch joins the partials.
+// tails, each seen by Tq G rows, are units of one launch (of one each where the
+// caches' widths differ), both cut into key splits, and a merge launch joins the
+// partials. The splits are those of the least estimated time on 256 CUs
+// (plan_shared).
 //
-// A unit (a workgroup of 8 waves): up to 128 rows of one head over a run of key
-// tiles (KT = 16384 / D keys, the LDS layout of block_tile.hpp). In round i the
-// workgroup dequantizes tile i + 1 (its codes in registers) into the free one of
-// two LDS buffers, requests the codes of a later tile and computes tile i:
-//   S^T = K . Q^T (v_mfma_f32_16x16x32_f16; a lane then holds 8 consecutive keys
-//   of one row, the A operand of P . V), scores scaled and kept in fp32, online
-//   softmax against the running maximum (the largest weight is exactly 1), P
-//   rounded to fp16 for O += P . V, O in fp32.
-// Rounded to fewer than 32 bits: P, to fp16 (2^-12 relative rms a weight, and
-// averaged over the keys; the output's own rounding is the larger), and the
-// output. Workgroups of fewer than 8 row tiles give the free waves halves or
-// quarters of each tile's keys and join them through LDS.
+// Two kernels, by the rows of a unit: many_body up to 128 (D = 256) or 256 rows
+// over key tiles in LDS, dequantized beside the MFMAs by waves of their own;
+// few_body up to 16, which have nothing to share and read keys straight into MFMA
+// operands. Many query tiles over one quantized cache read images of its tiles,
+// dequantized once (kImageQueryTiles).
+// Rounded to fewer than 32 bits: P, to fp16 (a weight by at most 2^-11 of itself, below
+// 2^-14 by 2^-25, averaged over the keys; the output's own rounding is the larger), the
+// output, and over Turbo4 caches the rotated q and output.
+//
+// Whole calls against their floors (the keys once at 4.98 TB/s, the products at 1.15 PFLOP/s): 16
+// sequences over 32k 4-bit keys 39.9 us of 11.3, 64 over 64k fp16 keys 109 of 61.
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
@@ -286,7 +287,14 @@ struct TileFiller {
 //   O += P . V in fp32.
 // Where the rows leave waves free these take parts of each tile's keys, joined at the end through LDS.
 // One barrier a tile. (With 8 waves that dequantize and compute in turn, all of them were in the same
-// phase: LDS idle while they dequantize, the VALU while they read.)
+// phase: LDS idle while they dequantize, the VALU while they read: 126 rows over 32k 8-bit keys, D =
+// 256, 42 against 38.4 us.)
+// Bound by filling and computing at once, which share the VALU and LDS: 96 rows over 131k 4-bit keys, D =
+// 256, take 89 us with their merge; the filling waves alone 66, the computing ones alone 75; 8-bit 96, 77 and
+// 76; fp16 139, 136 and 78 (filling reads the keys' 537 MB at 4.1 TB/s). Short calls are bound by a
+// unit's start and end: over 32k 4-bit keys 34 us without the merge, 20 of them with neither.
+// Turbo4: a byte's two centroids come from a table in LDS, four reads a word where the affine modes have a
+// few VALU instructions: 16 sequences over 32k keys 63 us with the rotations, 47 over 4-bit codes.
 template <int KIND, int D, bool FAST, bool IMAGE, bool T4 = false>
 __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
     using S = BlockShape<D>;
@@ -561,8 +569,11 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
 // Units of at most 16 rows: nothing to share through LDS, so each wave reads 32-key chunks of its
 // own (chunk c of the unit's keys to wave c mod 8) straight into MFMA operands - K rows as A, a lane
 // (g, r16) taking dims D/4 g .. of its key, V's 8-key blocks as B - and requests the next chunk's K
-// once this one's scores are formed, its V once this one's P . V is. Bound by HBM latency and
-// bandwidth; the waves' sums join through LDS.
+// once this one's scores are formed, its V once this one's P . V is; the waves' sums join through
+// LDS. Bound by HBM latency and the dequantization between the loads: 6 rows over 32k 4-bit keys, D = 256,
+// 38 MB in 14.7 us, 2.6 TB/s (a second chunk in flight does not fit the registers: 19.2 us with its
+// spills). Turbo4: K and V through the table of centroid pairs in LDS; the call with weights takes 24.3 us where
+// the kernel for many rows and a second sight of K took 53.5, and 17.8 over 4-bit codes.
 template <int KIND, int D, bool FAST, bool T4 = false>
 __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
     constexpr int NM = D / 32, NT = D / 16, NG = D / kGroup, DG = D / 4, DPL = D / 16;
