@@ -28,7 +28,7 @@
 // output, and over Turbo4 caches the rotated q and output.
 //
 // Whole calls against their floors (the keys once at 4.98 TB/s, the products at 1.15 PFLOP/s): 16
-// sequences over 32k 4-bit keys 39.9 us of 11.3, 64 over 64k fp16 keys 109 of 61.
+// sequences over 32k 4-bit keys 34.1 us of 11.3, 64 over 64k fp16 keys 108 of 61.
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
@@ -291,10 +291,11 @@ struct TileFiller {
 // 256, 42 against 38.4 us.)
 // Bound by filling and computing at once, which share the VALU and LDS: 96 rows over 131k 4-bit keys, D =
 // 256, take 89 us with their merge; the filling waves alone 66, the computing ones alone 75; 8-bit 96, 77 and
-// 76; fp16 139, 136 and 78 (filling reads the keys' 537 MB at 4.1 TB/s). Short calls are bound by a
-// unit's start and end: over 32k 4-bit keys 34 us without the merge, 20 of them with neither.
+// 76; fp16 139, 136 and 78 (filling reads the keys' 537 MB at 4.1 TB/s); all nine with the partials' stores
+// some 6 us longer than part_dim's order has them. 16 sequences over 32k 4-bit keys take 31 us, 6 of them
+// without any tile or partial, and the merge 5.
 // Turbo4: a byte's two centroids come from a table in LDS, four reads a word where the affine modes have a
-// few VALU instructions: 16 sequences over 32k keys 63 us with the rotations, 47 over 4-bit codes.
+// few VALU instructions: 16 sequences over 32k keys 58 us with the rotations, 41 over 4-bit codes.
 template <int KIND, int D, bool FAST, bool IMAGE, bool T4 = false>
 __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
     using S = BlockShape<D>;
@@ -557,10 +558,10 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
                     *(half8*)(o + c) = y;
                 }
             } else {
-                float* o = a.part_o + (u.slot_base + row) * D + NT * r16;
+                float* o = a.part_o + (u.slot_base + row) * D + 4 * r16;  // (part_dim's order)
 #pragma unroll
                 for (int c = 0; c < NT; c += 4)
-                    *(float4v*)(o + c) = float4v{acc_o[rt][c][e], acc_o[rt][c + 1][e], acc_o[rt][c + 2][e], acc_o[rt][c + 3][e]};
+                    *(float4v*)(o + 16 * c) = float4v{acc_o[rt][c][e], acc_o[rt][c + 1][e], acc_o[rt][c + 2][e], acc_o[rt][c + 3][e]};
             }
         }
     }
@@ -571,9 +572,9 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
 // (g, r16) taking dims D/4 g .. of its key, V's 8-key blocks as B - and requests the next chunk's K
 // once this one's scores are formed, its V once this one's P . V is; the waves' sums join through
 // LDS. Bound by HBM latency and the dequantization between the loads: 6 rows over 32k 4-bit keys, D = 256,
-// 38 MB in 14.7 us, 2.6 TB/s (a second chunk in flight does not fit the registers: 19.2 us with its
-// spills). Turbo4: K and V through the table of centroid pairs in LDS; the call with weights takes 24.3 us where
-// the kernel for many rows and a second sight of K took 53.5, and 17.8 over 4-bit codes.
+// 38 MB in 14.4 us, 2.6 TB/s (a second chunk in flight does not fit the registers: 19.2 us with its
+// spills). Turbo4: K and V through the table of centroid pairs in LDS; the call with weights takes 23.6 us where
+// the kernel for many rows and a second sight of K took 53.5, and 17.2 over 4-bit codes.
 template <int KIND, int D, bool FAST, bool T4 = false>
 __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
     constexpr int NM = D / 32, NT = D / 16, NG = D / kGroup, DG = D / 4, DPL = D / 16;
@@ -784,10 +785,10 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
     for (int e = 0; e < 4; e++) {
         const float fe = __shfl(f, 4 * g + e);
         if (4 * g + e >= rows) continue;
-        float* o = s_o + (wave * rows + 4 * g + e) * D + NT * r16;
+        float* o = s_o + (wave * rows + 4 * g + e) * D + 4 * r16;  // (part_dim's order)
 #pragma unroll
         for (int c = 0; c < NT; c += 4)
-            *(float4v*)(o + c) = float4v{acc_o[c][e] * fe, acc_o[c + 1][e] * fe, acc_o[c + 2][e] * fe, acc_o[c + 3][e] * fe};
+            *(float4v*)(o + 16 * c) = float4v{acc_o[c][e] * fe, acc_o[c + 1][e] * fe, acc_o[c + 2][e] * fe, acc_o[c + 3][e] * fe};
     }
     __syncthreads();
     const int64_t pbase = u.slot_base + row_base;
@@ -809,7 +810,7 @@ __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
             half4v y;
 #pragma unroll
             for (int j = 0; j < 4; j++) y[j] = (f16)(o[j] * inv);
-            *(half4v*)(a.out + q_row(a, h, row_base + row) * D + 4 * c) = y;
+            *(half4v*)(a.out + q_row(a, h, row_base + row) * D + part_dim<D>(c)) = y;
         } else {
             *(float4v*)(a.part_o + (pbase + row) * D + 4 * c) = o;
         }

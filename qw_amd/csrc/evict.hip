@@ -17,7 +17,7 @@
 // In place the rows go through a workspace: a row's new place may be another's old one.
 // The select is bound by the latency of its dependent steps (32k keys of 4 heads 25 us in four launches), the
 // copy by bandwidth: 48k of 64k fp16 rows, D = 256, 297 MB read (every line of V holds a kept
-// key) and 197 written in 90 us, 5.5 TB/s; 16k of 131k 8-bit rows 151 MB in 31.6 us, 4.8 TB/s.
+// key) and 197 written in 90 us, 5.5 TB/s; 16k of 131k 8-bit rows 151 MB in 32 us, 4.7 TB/s.
 #include <algorithm>
 
 #include "kv_cache.hpp"

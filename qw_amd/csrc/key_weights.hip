@@ -9,7 +9,7 @@
 //
 // p needs the row's whole sum. Up to 16 rows a KV head the attention launch keeps its scores
 // (4 bytes a row and key, where K again would be 144 to 512 a key) and finish_few_kernel turns them
-// into weights beside the merge (one row over 32k 4-bit keys: 14.7 + 4.9 us, of which the
+// into weights beside the merge (one row over 32k 4-bit keys: 14.4 + 4.9 us, of which the
 // keys themselves at 4.98 TB/s are 7.8). For more rows K is seen twice: the attention launch leaves each
 // row's maximum and sum, and key_weights_kernel forms the scores again. A wave owns 64 keys: it
 // dequantizes their K rows once, into registers as the A operand of S^T = K . Q^T, and runs
