@@ -306,7 +306,9 @@ struct RowsCopy {
 
 // BITS: of a code (or 16). Grid (groups, hkv), the first `groups_v` groups V's: a thread takes a
 // 16-byte piece of V of a block's 8 rows, or of K (and of a row-major V) the same piece of each of
-// the 8 rows. All its loads are issued before the first is used.
+// the 8 rows. All its loads are issued before the first is used. Rows of the last block past row n - 1
+// become zeros (V's codes of them the last row's, under a scale and a bias of 0): what stands behind a
+// cache's offset has weight 0 in its attention, and has to be finite.
 template <int BITS, int D>
 __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
     constexpr int pieces = D * BITS / 16;  // of a block of V
@@ -337,9 +339,8 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
         }
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            if (k >= rows) break;
-            to[(dst + k) * ppr + c] = x[k];
-            if (c < pw) pt[(dst + k) * pw + c] = p[k];
+            to[(dst + k) * ppr + c] = k < rows ? x[k] : u32x4{0, 0, 0, 0};
+            if (c < pw) pt[(dst + k) * pw + c] = k < rows ? p[k] : 0u;
         }
         return;
     }
@@ -355,12 +356,15 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
 #pragma unroll
     for (int k = 0; k < 8; k++) t[k] = kept[min(k, rows - 1)];
     // piece pc of the block: 4 dims' words of 8 nibbles, 2 dims' of 8 bytes or one dim's of 8
-    // halves; slots of rows past the last one take its row (as anything may stand there)
+    // halves
     u32x4 out = {0, 0, 0, 0};
     if constexpr (BITS == 16) {
         uint32_t x[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = ((const uint16_t*)(a.v + (sblk + t[k] / 8) * pieces + pc))[t[k] & 7];
+        for (int k = 0; k < 8; k++) {
+            x[k] = ((const uint16_t*)(a.v + (sblk + t[k] / 8) * pieces + pc))[t[k] & 7];
+            x[k] = k < rows ? x[k] : 0u;
+        }
 #pragma unroll
         for (int k = 0; k < 4; k++) out[k] = x[2 * k] | x[2 * k + 1] << 16;
     } else {
@@ -385,13 +389,12 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
     a.v_to[dblk * pieces + pc] = out;
     if (BITS != 16 && pc < a.kp_words * 8) {  // scale and bias of key pc & 7 in group pc >> 3
         const int grp = pc >> 3, k = pc & 7;
-        if (k < rows) {
-            const int tk = kept[k];
-            const f16* from = (const f16*)a.vp + ((sblk + tk / 8) * a.kp_words + grp) * 16;
-            f16* to = (f16*)a.vp_to + (dblk * a.kp_words + grp) * 16;
-            to[k] = from[tk & 7];
-            to[8 + k] = from[8 + (tk & 7)];
-        }
+        const int tk = kept[min(k, rows - 1)];
+        const f16* from = (const f16*)a.vp + ((sblk + tk / 8) * a.kp_words + grp) * 16;
+        f16* to = (f16*)a.vp_to + (dblk * a.kp_words + grp) * 16;
+        const f16 scale = from[tk & 7], bias = from[8 + (tk & 7)];
+        to[k] = k < rows ? scale : (f16)0.0f;
+        to[8 + k] = k < rows ? bias : (f16)0.0f;
     }
 }
 
