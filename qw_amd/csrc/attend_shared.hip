@@ -986,7 +986,10 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, cons
     a.G = G;
     a.hkv = hkv;
     // (a merge of a workgroup of 256 a row stays below 2^32 threads)
-    QW_REQUIRE((int64_t)n_seq * n_rows * G < 1 << 24, QW_ERR_UNSUPPORTED, "attention: 2^24 or more rows a KV head in one call");
+    // (n_seq * n_rows is below 2^62; times G it could pass 2^63)
+    const int64_t seq_rows = (int64_t)n_seq * n_rows;
+    QW_REQUIRE(seq_rows < 1 << 24 && seq_rows * G < 1 << 24, QW_ERR_UNSUPPORTED,
+               "attention: 2^24 or more rows a KV head in one call");
     a.R = n_seq * n_rows * G;
     // (a scale of 0 stands as a tiny one, which leaves every score 0 and a hidden key's -inf itself)
     a.scale2 = std::max(std::fabs(scale) * kLog2e, 1e-37f);
@@ -1125,7 +1128,8 @@ static int check_shared(const KVCache& p, const KVCache* t, int n_seq, const voi
     QW_REQUIRE(q && out, QW_ERR_INVALID_ARGUMENT, "shared attention: null q/out");
     QW_REQUIRE(n_seq > 0 && n_rows > 0 && n_q_heads > 0 && n_q_heads % p.hkv == 0, QW_ERR_INVALID_ARGUMENT,
                "shared attention: n_seq, n_rows > 0 and n_q_heads a positive multiple of n_kv_heads");
-    QW_REQUIRE((int64_t)n_seq * n_rows * (n_q_heads / p.hkv) <= INT32_MAX / 2, QW_ERR_INVALID_ARGUMENT,
+    const int64_t seq_rows = (int64_t)n_seq * n_rows;
+    QW_REQUIRE(seq_rows <= INT32_MAX / 2 && seq_rows * (n_q_heads / p.hkv) <= INT32_MAX / 2, QW_ERR_INVALID_ARGUMENT,
                "shared attention: too many rows");
     QW_REQUIRE(std::isfinite(scale), QW_ERR_INVALID_ARGUMENT, "shared attention: scale must be finite");
     if (t) {
