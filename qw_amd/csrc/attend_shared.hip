@@ -991,6 +991,9 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, cons
     QW_REQUIRE(seq_rows < 1 << 24 && seq_rows * G < 1 << 24, QW_ERR_UNSUPPORTED,
                "attention: 2^24 or more rows a KV head in one call");
     a.R = n_seq * n_rows * G;
+    // (over Turbo4 caches q and the output pass through launches of a wave a row)
+    QW_REQUIRE(!(prefix ? prefix : tails)->turbo4() || (int64_t)a.R * hkv <= UINT32_MAX / 64 - 3, QW_ERR_UNSUPPORTED,
+               "attention over a Turbo4 cache: about 2^26 or more query rows in one call");
     // (a scale of 0 stands as a tiny one, which leaves every score 0 and a hidden key's -inf itself)
     a.scale2 = std::max(std::fabs(scale) * kLog2e, 1e-37f);
     a.q_flip = scale < 0.0f ? 0x80008000u : 0u;
@@ -1112,7 +1115,6 @@ int launch_shared_merge(int D, const SharedArgs& a, hipStream_t stream) {
 }
 
 int shared_turbo4_room(const KVCache& c, int64_t q_rows, hipStream_t stream, SharedArgs* a) {
-    QW_REQUIRE(q_rows <= INT32_MAX, QW_ERR_INVALID_ARGUMENT, "attention over a Turbo4 cache: too many rows");
     void* ws = nullptr;
     if (int rc = workspace(kWsTurbo4, c.device, stream, 2 * (size_t)q_rows * c.D * sizeof(f16), &ws)) return rc;
     a->q = (const f16*)ws;

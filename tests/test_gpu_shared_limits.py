@@ -29,3 +29,18 @@ def test_row_counts_whose_product_wraps(n_seq, n_rows, group):
     assert call(prefix._h, None, n_seq, None, x.data_ptr(), group, n_rows, 0.1, x.data_ptr(), stream()) in (1, 2)
     torch.cuda.synchronize()
     assert prefix.offset == 20 and not x.any()
+
+
+def test_too_many_turbo4_rows_refused():
+    """2^26 query rows over a Turbo4 cache, fewer than 2^24 a KV head: the rotations' launches have a wave a row, and
+    2^32 threads are one too many. Refused on the host, by the declared sizes, before workspaces and the append."""
+    import qw_amd
+
+    cache, tails = filled("turbo4", 8, 128, 20, rng(3)), filled("turbo4", 8, 128, 5, rng(4))
+    x, w = torch.zeros(128, dtype=torch.float16, device="cuda"), torch.zeros((8, 20), device="cuda")
+    lib, q, n = qw_amd.lib(), x.data_ptr(), 1 << 23
+    free = torch.cuda.mem_get_info()[0]
+    assert lib.qw_kv_shared_attention(cache._h, None, 1, None, q, 8, n, 0.1, q, stream()) == 2
+    assert lib.qw_kv_attention_scored(cache._h, q, 8, n, 0.1, 0, None, 0, 0, 0.0, w.data_ptr(), 20, q, stream()) == 2
+    torch.cuda.synchronize()
+    assert torch.cuda.mem_get_info()[0] >= free - (64 << 20) and cache.offset == 20 and not w.any()
