@@ -1014,9 +1014,9 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, cons
         tiles[i] = (s.T + KT - 1) / KT;
     }
     // One quantized cache under many query tiles: its key tiles are dequantized once, into images
-    // (1.03 times its fp16 K and V), not once a query tile.
+    // (1.03 times its fp16 K and V: 2.2 GB at most), not once a query tile.
     const bool images = c[1] && !c[0] && !starts && c[1]->affine() && n_qt[1] >= kImageQueryTiles &&
-                        (int64_t)hkv * tail_rows * D <= (int64_t)1 << 29;
+                        (int64_t)c[1]->hkv * tail_rows * D <= (int64_t)1 << 29;
     // Tiles a split, for each launch: the count with the shortest estimate. A unit's us: a start and an
     // end that grow with its rows, and a time a tile (measured: 30 and 126 rows of 8-bit keys at D = 256
     // 23.6 and 38.4 us in 8 tiles, 126 rows 103 us in 32; few rows 14.5 us in 9); a partial row costs its

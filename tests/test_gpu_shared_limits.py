@@ -1,11 +1,9 @@
 """Sizes and values at the ends of what the shared, scored and evicting calls take."""
-import ctypes
-
 import numpy as np
 import pytest
 
 from conftest import rng
-from test_gpu_shared import dev, filled, queries
+from test_gpu_shared import attend, filled, queries
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -44,3 +42,31 @@ def test_too_many_turbo4_rows_refused():
     assert lib.qw_kv_attention_scored(cache._h, q, 8, n, 0.1, 0, None, 0, 0, 0.0, w.data_ptr(), 20, q, stream()) == 2
     torch.cuda.synchronize()
     assert torch.cuda.mem_get_info()[0] >= free - (64 << 20) and cache.offset == 20 and not w.any()
+
+
+def test_images_of_a_batch_stay_within_their_bound():
+    """A batch of prompts without a prefix: what the key tiles' images may take (2^29 halves of K) counts every
+    sequence's heads. 64 sequences of 70000 keys would take 2.4 GB for them."""
+    import qw_amd
+
+    B, T, L, hq = 64, 70000, 512, 8
+    prefix, tails = filled("affine4", 1, 128, 0, rng(1)), qw_amd.KVCache("affine4", B, 128, capacity=T)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for _ in range(7):
+        x = torch.empty((2, B, T // 7, 128), dtype=torch.float16, device="cuda").normal_(generator=g)
+        tails.update(x[0], x[1])
+    q = queries(rng(3), B, hq, L, 128)
+    qw_amd.release_workspaces()
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    out = prefix.shared_attention(q, tails, 0.09)
+    torch.cuda.synchronize()
+    taken = free - torch.cuda.mem_get_info()[0]
+    print(f"taken {taken / 1e9:.2f} GB", flush=True)
+    assert taken < 1.5e9
+    k, v = (x[0, B - 1].double().cpu().numpy() for x in tails.dequantize())
+    for j, i in ((0, 0), (5, 300), (7, L - 1)):
+        n = T - L + i + 1
+        ref, bar, _, _ = attend(q[B - 1, j, i].double().cpu().numpy(), k[:n], v[:n], 0.09)
+        assert np.all(np.abs(out[B - 1, j, i].double().cpu().numpy() - ref) <= bar), (j, i)
+    qw_amd.release_workspaces()
