@@ -494,27 +494,29 @@ class KVCache:
         if weights.dim() != 2 or weights.shape[0] != self.n_kv_heads or weights.shape[1] < n or \
                 weights.dtype is not torch.float32 or weights.device != self.device:
             raise QwError(1, f"{what}: weights must be [n_kv_heads, >= {n}] f32 on {self.device}")
-        return weights if weights.stride(1) == 1 and weights.stride(0) >= weights.shape[1] \
-            else weights.contiguous()
+        # (the strides of dimensions of one entry mean nothing, and contiguous() leaves them as they are)
+        rows, n = weights.shape
+        if n > 1 and weights.stride(1) != 1 or rows > 1 and weights.stride(0) < n:
+            weights = weights.contiguous()
+        return weights, weights.stride(0) if rows > 1 else n
 
     def _scored(self, q, keys, values, scale, weights, decay, causal, weights_out):
         qq, hq, L, D = _hld(q, "q")
         if D != self.head_dim or qq.device != self.device:
             raise QwError(1, "attention_scored: q must have the cache's head_dim and device")
         T = self.offset + (0 if keys is None else L)
-        w = None if weights is None else self._weights(weights, "attention_scored", 0)
+        w, ws = (None, 0) if weights is None else self._weights(weights, "attention_scored", 0)
         if weights_out is None:
-            wo = qq.new_empty((self.n_kv_heads, T), dtype=_torch().float32)
+            wo, wos = qq.new_empty((self.n_kv_heads, T), dtype=_torch().float32), T
         else:
-            wo = self._weights(weights_out, "attention_scored", T)
+            wo, wos = self._weights(weights_out, "attention_scored", T)
             if wo is not weights_out:
                 raise QwError(1, "attention_scored: weights_out must have unit key stride")
         out = _out_like(qq, hq, L, D)
         st = _stream(self.device)
         head = (self._h, qq.data_ptr(), hq, L)
         rest = (float(scale), int(causal), None if w is None else w.data_ptr(),
-                0 if w is None else w.stride(0), 0 if w is None else min(T, w.shape[1]), float(decay),
-                wo.data_ptr(), wo.stride(0), out.data_ptr(), st)
+                ws, 0 if w is None else min(T, w.shape[1]), float(decay), wo.data_ptr(), wos, out.data_ptr(), st)
         if keys is None:
             _check(lib().qw_kv_attention_scored(*head, *rest))
         else:
@@ -545,14 +547,14 @@ class KVCache:
         ties to the earlier key). The kept rows move, as they are stored, to ``into`` (a cache of the
         same mode and geometry, whose contents they replace) or stay here. Returns (kept
         positions [Hkv, n] int32 ascending, their weights [Hkv, n]), n = min(offset, budget)."""
-        w = self._weights(weights, "evict", self.offset)
+        w, ws = self._weights(weights, "evict", self.offset)
         if into is not None and not into._h:
             raise QwError(1, "evict: into is closed")
         budget, sink, recent = (min(int(x), 2 ** 31 - 1) for x in (budget, sink, recent))
         n = max(min(self.offset, budget), 0)
         kept = w.new_empty((self.n_kv_heads, n), dtype=_torch().int32)
         wo = w.new_empty((self.n_kv_heads, n))
-        _check(lib().qw_kv_evict(self._h, None if into is None else into._h, w.data_ptr(), w.stride(0),
+        _check(lib().qw_kv_evict(self._h, None if into is None else into._h, w.data_ptr(), ws,
                                  budget, sink, recent, kept.data_ptr(), wo.data_ptr(), n,
                                  None, _stream(self.device)))
         return kept, wo

@@ -329,7 +329,7 @@ int attention_scored(KVCache& c, const void* q, int n_q_heads, int n_rows, const
                "scored attention: empty cache, or fewer cached keys than causal query rows");
     QW_REQUIRE(weights_out_stride >= T && (!weights || (n_weights >= 0 && weights_stride >= n_weights)),
                QW_ERR_INVALID_ARGUMENT, "scored attention: a weights stride below its row's length");
-    if (weights && decay > 0.0f && !(weights == weights_out && weights_stride == weights_out_stride)) {
+    if (weights && decay > 0.0f && !(weights == weights_out && (weights_stride == weights_out_stride || c.hkv == 1))) {
         const uintptr_t a0 = (uintptr_t)weights, a1 = a0 + 4 * ((uint64_t)(c.hkv - 1) * weights_stride + n_weights);
         const uintptr_t b0 = (uintptr_t)weights_out, b1 = b0 + 4 * ((uint64_t)(c.hkv - 1) * weights_out_stride + T);
         QW_REQUIRE(a1 <= b0 || b1 <= a0, QW_ERR_INVALID_ARGUMENT,

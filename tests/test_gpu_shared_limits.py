@@ -70,3 +70,30 @@ def test_images_of_a_batch_stay_within_their_bound():
         ref, bar, _, _ = attend(q[B - 1, j, i].double().cpu().numpy(), k[:n], v[:n], 0.09)
         assert np.all(np.abs(out[B - 1, j, i].double().cpu().numpy() - ref) <= bar), (j, i)
     qw_amd.release_workspaces()
+
+
+def test_one_head_takes_weights_of_any_row_stride():
+    """With one KV head a row's stride means nothing: the transpose of an [n, 1] tensor is as good as any."""
+    r = rng(6)
+    cache, q = filled("fp16", 1, 128, 50, r), queries(r, 1, 4, 2, 128)
+    plain = torch.rand((1, 50), device="cuda")
+    column = torch.empty((50, 1), device="cuda").copy_(plain.t()).t()
+    assert column.stride() == (1, 1)
+    want = cache.attention_scored(q, 0.09, weights=plain, causal=True)
+    for w in (column, plain.as_strided((1, 50), (7, 1))):
+        got = cache.attention_scored(q, 0.09, weights=w, causal=True, weights_out=torch.zeros((50, 1), device="cuda").t())
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for a, b in zip(cache.evict(plain, 20, into=filled("fp16", 1, 128, 0, r)), cache.evict(column, 20, into=filled("fp16", 1, 128, 0, r))):
+        assert torch.equal(a, b)
+    # in place through two views of one array, one of them shorter
+    got = cache.attention_scored(q, 0.09, weights=column, causal=True, weights_out=column.as_strided((1, 50), (50, 1)))
+    assert torch.equal(got[1], want[1]) and torch.equal(column, want[1])
+    early = plain.clone()
+    want = cache.attention_scored(q, 0.09, weights=early[:, :40], causal=True)
+    got = cache.attention_scored(q, 0.09, weights=early[:, :40], causal=True, weights_out=early)
+    assert torch.equal(got[1], want[1]) and torch.equal(early, want[1])
+    # one key: its own stride means nothing either
+    one = filled("fp16", 2, 128, 1, r)
+    q, grid = queries(r, 1, 4, 1, 128), torch.zeros((2, 60), device="cuda")
+    one.attention_scored(q, 0.09, weights_out=grid[:, 5::30][:, :1])
+    assert torch.equal(grid[:, 5], torch.full((2,), 2.0, device="cuda")) and not grid[:, 6:].any()
