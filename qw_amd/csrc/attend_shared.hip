@@ -30,6 +30,7 @@
 // Whole calls against their floors (the keys once at 4.98 TB/s, the products at 1.15 PFLOP/s): 16
 // sequences over 32k 4-bit keys 34.1 us of 11.3, 64 over 64k fp16 keys 108 of 61.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <initializer_list>
 #include <type_traits>
@@ -994,8 +995,9 @@ int plan_shared(const KVCache* prefix, const KVCache* tails, int tail_rows, cons
     // (over Turbo4 caches q and the output pass through launches of a wave a row)
     QW_REQUIRE(!(prefix ? prefix : tails)->turbo4() || (int64_t)a.R * hkv <= UINT32_MAX / 64 - 3, QW_ERR_UNSUPPORTED,
                "attention over a Turbo4 cache: about 2^26 or more query rows in one call");
-    // (a scale of 0 stands as a tiny one, which leaves every score 0 and a hidden key's -inf itself)
-    a.scale2 = std::max(std::fabs(scale) * kLog2e, 1e-37f);
+    // (a scale of 0 stands as a tiny one, which leaves every score 0 and a hidden key's -inf itself; one that
+    // passes fp32 times log2 e as its largest number, which leaves a score of 0 itself)
+    a.scale2 = std::min(std::max(std::fabs(scale) * kLog2e, 1e-37f), FLT_MAX);
     a.q_flip = scale < 0.0f ? 0x80008000u : 0u;
     int tiles[2] = {0, 0}, n_qt[2] = {0, 0};
     for (int i = 0; i < 2; i++) {

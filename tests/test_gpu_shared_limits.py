@@ -3,7 +3,8 @@ import numpy as np
 import pytest
 
 from conftest import rng
-from test_gpu_shared import attend, filled, queries
+from test_gpu_key_weights import check_scored
+from test_gpu_shared import attend, check_shared, filled, queries
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -97,3 +98,16 @@ def test_one_head_takes_weights_of_any_row_stride():
     q, grid = queries(r, 1, 4, 1, 128), torch.zeros((2, 60), device="cuda")
     one.attention_scored(q, 0.09, weights_out=grid[:, 5::30][:, :1])
     assert torch.equal(grid[:, 5], torch.full((2,), 2.0, device="cuda")) and not grid[:, 6:].any()
+
+
+@pytest.mark.parametrize("L", [1, 40])
+@pytest.mark.parametrize("scale", [3e38, -3e38, 1e-38])
+def test_scales_at_the_ends_of_fp32(L, scale):
+    """Scores of 0 stay 0 under the largest scale (times log2 e it passes fp32): a mean of the keys seen."""
+    r = rng(7)
+    cache, prefix = filled("affine4", 2, 128, 90, r), filled("affine4", 1, 128, 33, r)
+    q = torch.zeros((1, 8, L, 128), dtype=torch.float16, device="cuda")
+    out, w = cache.attention_scored(q, scale, causal=True)
+    check_scored(out, w, q, cache, scale, True)
+    q = torch.zeros((2, 4, L, 128), dtype=torch.float16, device="cuda")
+    check_shared(prefix.shared_attention(q, cache, scale), q, prefix, cache, None, scale)
