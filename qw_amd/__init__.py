@@ -550,7 +550,9 @@ class KVCache:
         w, ws = self._weights(weights, "evict", self.offset)
         if into is not None and not into._h:
             raise QwError(1, "evict: into is closed")
-        budget, sink, recent = (min(int(x), 2 ** 31 - 1) for x in (budget, sink, recent))
+        budget, sink, recent = min(int(budget), 2 ** 31 - 1), int(sink), int(recent)
+        if min(sink, recent) < 0 or sink + recent > budget:  # (before any of them passes an int)
+            raise QwError(1, "evict: sink + recent <= budget, neither negative, expected")
         n = max(min(self.offset, budget), 0)
         kept = w.new_empty((self.n_kv_heads, n), dtype=_torch().int32)
         wo = w.new_empty((self.n_kv_heads, n))

@@ -111,3 +111,17 @@ def test_scales_at_the_ends_of_fp32(L, scale):
     check_scored(out, w, q, cache, scale, True)
     q = torch.zeros((2, 4, L, 128), dtype=torch.float16, device="cuda")
     check_shared(prefix.shared_attention(q, cache, scale), q, prefix, cache, None, scale)
+
+
+def test_evict_counts_beyond_an_int_are_not_wrapped():
+    """-2^32 + 3 is not 3: negative counts are refused whatever their size, and large ones are large."""
+    import qw_amd
+
+    cache, w = filled("affine8", 2, 128, 20, rng(8)), torch.rand((2, 20), device="cuda")
+    for a in ({"budget": 10, "sink": -2 ** 32 + 3}, {"budget": 10, "recent": -2 ** 32}, {"budget": -2 ** 32 + 5},
+              {"budget": 10, "sink": 2 ** 32}, {"budget": 2 ** 31 - 1, "sink": 2 ** 40}):
+        with pytest.raises(qw_amd.QwError) as e:
+            cache.evict(w, **a)
+        assert e.value.status == 1 and cache.offset == 20, a
+    kept, _ = cache.evict(w, 2 ** 40, sink=2 ** 30, recent=2 ** 30 - 1)
+    assert kept.shape == (2, 20) and cache.offset == 20
