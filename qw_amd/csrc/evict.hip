@@ -300,15 +300,16 @@ struct RowsCopy {
     const int32_t* kept;     // [hkv][n]
     const int* flag;         // the source's fast flag, copied where flag_to is not null
     int* flag_to;
-    int n, cap, cap_to, groups_v, kp_words;  // kp_words: words of a K row's params
+    int n, n_out;            // kept rows; rows written, zeros from n on (a multiple of 8)
+    int cap, cap_to, groups_v, kp_words;  // kp_words: words of a K row's params
     int row_major_v;         // Turbo4: V rows like K's, one params word a row
 };
 
 // BITS: of a code (or 16). Grid (groups, hkv), the first `groups_v` groups V's: a thread takes a
 // 16-byte piece of V of a block's 8 rows, or of K (and of a row-major V) the same piece of each of
-// the 8 rows. All its loads are issued before the first is used. Rows of the last block past row n - 1
-// become zeros (V's codes of them the last row's, under a scale and a bias of 0): what stands behind a
-// cache's offset has weight 0 in its attention, and has to be finite.
+// the 8 rows. All its loads are issued before the first is used. Rows n .. n_out - 1 become zeros (V's
+// codes in the last row's block that row's, under a scale and a bias of 0): what stands behind a
+// cache's offset, up to the end of a tile, has weight 0 in its attention, and has to be finite.
 template <int BITS, int D>
 __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
     constexpr int pieces = D * BITS / 16;  // of a block of V
@@ -319,7 +320,7 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
         const uint32_t id = (uint32_t)(group - (rows_of_v ? 0 : a.groups_v)) * 256u + threadIdx.x;
         const int b = (int)(id / ppr), c = (int)(id % ppr);
         if (id == 0 && h == 0 && !rows_of_v && a.flag_to) *a.flag_to = *a.flag;
-        if (8 * b >= a.n) return;
+        if (8 * b >= a.n_out) return;
         const u32x4* from = rows_of_v ? a.v : a.k;
         u32x4* to = rows_of_v ? a.v_to : a.k_to;
         const uint32_t* pf = rows_of_v ? a.vp : a.kp;
@@ -327,6 +328,14 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
         const int32_t* kept = a.kept + (int64_t)h * a.n + 8 * b;
         const int rows = min(8, a.n - 8 * b), pw = a.row_major_v ? 1 : a.kp_words;
         const int64_t dst = (int64_t)h * a.cap_to + 8 * b;
+        if (rows <= 0) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                to[(dst + k) * ppr + c] = u32x4{0, 0, 0, 0};
+                if (c < pw) pt[(dst + k) * pw + c] = 0;
+            }
+            return;
+        }
         int64_t src[8];
         u32x4 x[8];
         uint32_t p[8];
@@ -348,10 +357,15 @@ __global__ __launch_bounds__(256) void evict_rows_kernel(RowsCopy a) {
     const int pc = (int)(id % pieces);
     int b = (int)(id / pieces);
     if constexpr (pieces >= 64) b = __builtin_amdgcn_readfirstlane(b);  // a wave's pieces are one block's: its positions go through scalar loads
-    if (8 * b >= a.n) return;
+    if (8 * b >= a.n_out) return;
     const int32_t* kept = a.kept + (int64_t)h * a.n + 8 * b;
     const int rows = min(8, a.n - 8 * b);
     const int64_t sblk = (int64_t)h * (a.cap / 8), dblk = (int64_t)h * (a.cap_to / 8) + b;
+    if (rows <= 0) {
+        a.v_to[dblk * pieces + pc] = u32x4{0, 0, 0, 0};
+        if (BITS != 16 && pc < a.kp_words * 2) ((u32x4*)a.vp_to)[dblk * a.kp_words * 2 + pc] = u32x4{0, 0, 0, 0};
+        return;
+    }
     int t[8];
 #pragma unroll
     for (int k = 0; k < 8; k++) t[k] = kept[min(k, rows - 1)];
@@ -441,8 +455,9 @@ int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_str
         dst.offset = 0;
         return QW_OK;
     }
-    const int rows8 = (n + 7) / 8 * 8;
-    const int64_t of_v = (int64_t)(rows8 / 8) * (src.D * src.bits / 16), of_k = of_v / 8;  // threads of a head
+    // rows written: to a whole step of the capacity, which no tile of an attention kernel passes
+    const int n_out = (int)(((int64_t)n + 255) / 256 * 256);
+    const int64_t of_v = (int64_t)(n_out / 8) * (src.D * src.bits / 16), of_k = of_v / 8;  // threads of a head
     QW_REQUIRE(of_v + of_k + 512 <= UINT32_MAX, QW_ERR_UNSUPPORTED, "evict: too many rows for one call");
     DeviceGuard dg(src.device);
     QW_REQUIRE(dg.ok, QW_ERR_HIP, "evict: hipSetDevice failed");
@@ -453,15 +468,15 @@ int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_str
                    "evict: the destination has to grow and the stream is being captured; reserve it before");
         if (int rc = dst.reserve(n, stream)) return rc;
     }
-    // in place the rows that move are staged: planes of n rows a head, in whole 8-row blocks
+    // in place the rows that move are staged: planes of n_out rows a head
     char* ws = nullptr;
-    size_t at[4] = {0, src.k_data_bytes(rows8), 0, 0};
-    at[2] = at[1] + src.v_data_bytes(rows8);
-    at[3] = at[2] + (src.k_param_bytes(rows8) + 15) / 16 * 16;
+    size_t at[4] = {0, src.k_data_bytes(n_out), 0, 0};
+    at[2] = at[1] + src.v_data_bytes(n_out);
+    at[3] = at[2] + src.k_param_bytes(n_out);
     const bool staged = in_place && n < T;
     if (staged) {
         void* p = nullptr;
-        if (int rc = workspace(kWsEvict, src.device, stream, at[3] + src.v_param_bytes(rows8), &p)) return rc;
+        if (int rc = workspace(kWsEvict, src.device, stream, at[3] + src.v_param_bytes(n_out), &p)) return rc;
         ws = (char*)p;
     }
     const int first = std::min(sink, T), last = std::min(recent, T - first);  // (first + last <= n)
@@ -481,8 +496,9 @@ int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_str
     c.flag = src.fast_flag;
     c.flag_to = in_place ? nullptr : dst.fast_flag;
     c.n = n;
+    c.n_out = n_out;
     c.cap = src.cap;
-    c.cap_to = staged ? rows8 : dst.cap;
+    c.cap_to = staged ? n_out : dst.cap;
     c.kp_words = src.affine() ? src.D / kGroup : src.turbo4() ? 1 : 0;
     c.row_major_v = src.turbo4() ? 1 : 0;
     c.groups_v = (int)((src.turbo4() ? of_k + 255 : of_v + 255) / 256);
@@ -495,8 +511,8 @@ int evict(KVCache& src, KVCache* into, const float* weights, int64_t weights_str
     QW_HIP_CHECK(hipGetLastError());
     if (staged) {
         void* const to[4] = {src.k_data, src.v_data, src.k_params, src.v_params};
-        const size_t per[4] = {src.k_data_bytes(rows8), src.v_data_bytes(rows8), src.k_param_bytes(rows8),
-                               src.v_param_bytes(rows8)};
+        const size_t per[4] = {src.k_data_bytes(n_out), src.v_data_bytes(n_out), src.k_param_bytes(n_out),
+                               src.v_param_bytes(n_out)};
         const size_t full[4] = {src.k_data_bytes(src.cap), src.v_data_bytes(src.cap), src.k_param_bytes(src.cap),
                                 src.v_param_bytes(src.cap)};
         BackCopy b;

@@ -108,3 +108,34 @@ def test_evict_in_place_captured(mode, T, n):
         for name in want:
             assert torch.equal(got[name].view(torch.uint8), want[name].view(torch.uint8)), name
         same_as_fresh(cache, r, 8)
+
+
+def poisoned(mode, D, T, bad, r):
+    """A cache of T rows of which those in `bad` are NaN, and weights that are NaN for them."""
+    import qw_amd
+
+    cache = qw_amd.KVCache(mode, 2, D)
+    k, v = (r.standard_normal((2, T, D)).astype(np.float16) for _ in range(2))
+    k[:, bad] = v[:, bad] = np.nan
+    cache.update(dev(k), dev(v))
+    w = weights(r, 2, T, "log")
+    w[:, bad] = np.nan
+    return cache, dev(w)
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("D,T,n", [(128, 400, 300), (256, 300, 257), (128, 1000, 513), (256, 900, 64)])
+def test_evicted_rows_of_nan_are_gone(mode, D, T, n):
+    """Rows of NaN weight go first. What an eviction leaves behind the new end, in place or in a cache that held other
+    rows before, takes no part in the cache's attention."""
+    import qw_amd
+
+    r = rng(T + n)
+    bad = np.concatenate([np.arange(3, T - n, 7), np.arange(n, min(T, n + 40), 5)])
+    cache, w = poisoned(mode, D, T, bad[:T - n], r)
+    into, _ = poisoned(mode, D, n + 200, np.arange(n, n + 200), r)
+    cache.evict(w, n, into=into)
+    same_as_fresh(into, r, 8)
+    cache.evict(w, n)
+    assert cache.offset == n
+    same_as_fresh(cache, r, 8)
