@@ -240,7 +240,8 @@ int qw_kv_update_and_attention_general(qw_kv_cache* cache, const void* q, int n_
  * v_new [n_seq][n_kv_heads][n_rows][head_dim] first.
  *   q, out [n_seq][n_q_heads][n_rows][head_dim] fp16
  * Keys that a later row of its own sequence sees and this one does not must be
- * finite. Either cache may be empty, not both. Turbo4 caches go
+ * finite. Either cache may be empty, not both; fewer than 2^24 rows (n_seq * n_rows *
+ * heads of a group) a KV head, over Turbo4 caches also about 2^26 in all. Turbo4 caches go
  * together, with one seed: q rotated into the K basis (rounded to fp16), the values
  * f16(centroid * rescale), the output (rounded to fp16) rotated back out of the V
  * basis. */
@@ -259,7 +260,8 @@ int qw_kv_update_and_shared_attention(qw_kv_cache* prefix, qw_kv_cache* tails, i
  *     over the n_rows rows and the query heads of KV head h,   t < offset,
  * fp32 throughout (Turbo4 caches as there). weights (fp32 [n_kv_heads][>= n_weights], row stride in
  * elements; NULL, or decay 0: not read) counts as 0 from n_weights on, as for keys
- * appended since; weights_out [n_kv_heads][>= offset] may be the same array, else not overlap it. Keys
+ * appended since; weights_out [n_kv_heads][>= offset] may be the same array (of one head, under any
+ * stride), else not overlap it. Keys
  * that a later row sees and this one does not must be finite. The update form
  * appends k_new / v_new first. */
 int qw_kv_attention_scored(qw_kv_cache* cache, const void* q, int n_q_heads, int n_rows, float scale,
@@ -278,7 +280,8 @@ int qw_kv_update_and_attention_scored(qw_kv_cache* cache, const void* q, int n_q
  * of the largest weight, equal ones by the lower t, -0 equal to 0, a NaN below
  * every number. Their rows become rows 0 .. n - 1, ascending, code for code, of `into` (a
  * cache of the same mode, heads, head_dim, Turbo4 seed and device, whose contents
- * are replaced; NULL or `cache` itself: in place), whose offset is n. A key keeps
+ * are replaced; NULL or `cache` itself: in place), whose offset is n; rows n to the next
+ * multiple of 256 become zeros, but in place with n = offset. A key keeps
  * the rotation that it was stored with: the caller counts positions on from its own.
  *   kept [n_kv_heads][n] int32: the kept positions, ascending
  *   weights_out (or NULL) [n_kv_heads][>= n]: their weights; not inside weights

@@ -28,7 +28,7 @@
 // output, and over Turbo4 caches the rotated q and output.
 //
 // Whole calls against their floors (the keys once at 4.98 TB/s, the products at 1.15 PFLOP/s): 16
-// sequences over 32k 4-bit keys 34.1 us of 11.3, 64 over 64k fp16 keys 108 of 61.
+// sequences over 32k 4-bit keys 34.2 us of 11.3, 64 over 64k fp16 keys 105 of 61.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -47,12 +47,14 @@ namespace {
 
 constexpr int kWaves = 8, kFillWaves = 4;
 // Query tiles from which the key tiles of one quantized cache are laid out once. 256-row tiles of 8 heads,
-// D = 128, and 128-row ones of 4, D = 256, over 4k and 32k 4- and 8-bit keys: dequantized in each / laid
-// out, 2 tiles 33 / 34 and 62 / 93 us, 6 tiles 41 / 43 and 143 / 162, 10 tiles 52 / 54 and 216 / 228 (8-bit 233 /
-// 232); 72 tiles over 9.7k Int8 keys 513 / 421.
+// D = 128, and 128-row ones of 4, D = 256, over 4k, 9.7k and 32k 4-bit, 8-bit and Int8 keys, dequantized in each /
+// laid out: 8 tiles slower laid out by 0 to 8 %, 12 tiles 7 % faster to 5 % slower (32k 4-bit keys 420 / 416 and 229 /
+// 229 us), 16 tiles 6 % faster to 2 % slower (514 / 494, 293 / 286), 20 faster but for Int8 at D = 128 (109 / 115 at 4k),
+// 44 by 2 to 18 % (1461 / 1329, 813 / 748).
 constexpr int kImageQueryTiles = 16;
 constexpr int kFewRows = 16;  // of a unit of the kernel for few rows
-// 16-row tiles a computing wave of the other: what 168 registers hold (three waves a SIMD).
+// 16-row tiles a computing wave of the other, in 168 registers (three waves a SIMD). 4- and 8-bit instances spill one
+// at most, but fp16 and Turbo4 ones, whose filling waves stage more, 12 to 17.
 __host__ __device__ constexpr int many_tiles(int D) { return D == 256 ? 1 : 2; }
 
 // A unit: a split of a query tile of a head of one of the two caches.
@@ -287,6 +289,9 @@ struct TileFiller {
 //   (fp16 keeps 11 bits of p up to 2^8 as well; the accumulators are rescaled in few tiles),
 //   O += P . V in fp32.
 // Where the rows leave waves free these take parts of each tile's keys, joined at the end through LDS.
+// fp16: of K there is no such prefetch. Its loads compile to flat ones, which an LDS wait, so the one before each
+// tile's barrier, waits for, and the spilled registers are two of a thread's eight staged pieces, each waited for
+// behind its load.
 // One barrier a tile. (With 8 waves that dequantize and compute in turn, all of them were in the same
 // phase: LDS idle while they dequantize, the VALU while they read: 126 rows over 32k 8-bit keys, D =
 // 256, 42 against 38.4 us.)
@@ -574,8 +579,9 @@ __device__ __forceinline__ void many_body(const SharedArgs& a, char* lds) {
 // once this one's scores are formed, its V once this one's P . V is; the waves' sums join through
 // LDS. Bound by HBM latency and the dequantization between the loads: 6 rows over 32k 4-bit keys, D = 256,
 // 38 MB in 14.4 us, 2.6 TB/s (a second chunk in flight does not fit the registers: 19.2 us with its
-// spills). Turbo4: K and V through the table of centroid pairs in LDS; the call with weights takes 23.6 us where
-// the kernel for many rows and a second sight of K took 53.5, and 17.2 over 4-bit codes.
+// spills). fp16: K's loads flat ones, at D = 256 19 spilled registers. Turbo4: K and V through the table of
+// centroid pairs in LDS; the call with weights takes 23.6 us where the kernel for many rows and a second sight of
+// K took 53.5, and 17.2 over 4-bit codes.
 template <int KIND, int D, bool FAST, bool T4 = false>
 __device__ __forceinline__ void few_body(const SharedArgs& a, char* lds) {
     constexpr int NM = D / 32, NT = D / 16, NG = D / kGroup, DG = D / 4, DPL = D / 16;

@@ -89,9 +89,10 @@ int shared_turbo4_rotate_q(const KVCache& c, const void* q, int64_t q_rows, cons
 
 // Rows' partials joined by workgroups of 256, each partial row by TC threads and SG of them at a
 // time, four such in flight, their sums over LDS. A workgroup a row (TC = D / 4), but: few rows of
-// many slots are cut into 64 dims a workgroup (24 rows of 57 slots 7.0 -> 4.9 us beside the key
-// weights, 960 of 45 7.8 -> 10.1), and of many rows of few slots a workgroup takes 1024 / D
-// (36864 rows of 3 slots 34.7 -> 30.4 us, 64 of 3 3.2 -> 4.3).
+// many slots are cut into 64 dims a workgroup, and of many rows of few slots a workgroup takes 1024 / D.
+// D = 256, a row / cut: 24 rows of 45 slots 4.2 / 3.3 us, of 16 3.2 / 3.1, 512 of 45 6.9 / 7.4, of 128 21.7 / 18.8, 1024
+// of 128 26 / 34; a row / several: 4096 rows of 3 slots 5.9 / 4.6, of 8 9.6 / 8.6, 2048 of 3 3.9 / 3.7, of 8 5.5 / 5.7, 32768 of
+// 8 56 / 58, of 12 76 / 87.
 enum MergeForm { kMergeRow, kMergeCut, kMergeRows };
 __host__ __device__ inline MergeForm merge_form(int64_t rows, int n_slots) {
     return n_slots > 16 && rows <= 512 ? kMergeCut : n_slots <= 8 && rows >= 4096 ? kMergeRows : kMergeRow;

@@ -19,7 +19,8 @@
 // split's sums to a workspace, added up in order: no atomics, the same bits each time.
 // Bound by the MFMAs and the exponentials beside them (a product-and-sum, an exponential and a
 // product-and-sum a weight): 1536 rows over 9.7k Int8 keys, D = 256, 236 us, 0.72 PFLOP/s, the MFMAs busy
-// 0.35 of the profiler's window; K formed again for each step of rows took 1050 us a call.
+// 0.35 of the profiler's window; K formed again for each step of rows took 1050 us a call. A wave's K takes 128 of
+// some 212 registers at D = 256; over Turbo4 keys the lookups beside them spill 36.
 #include <algorithm>
 #include <cmath>
 
