@@ -529,6 +529,61 @@ int qw_kv_rope_update_and_attention(qw_kv_cache* cache, const void* qkv, int n_q
                                     float rope_scale, int position0, float scale, int causal,
                                     void* q_out, void* out, void* stream);
 
+/* ---------------------------------------------------------------- pages */
+
+/* No counterpart on the path above, whose caches hold one sequence each: a layer's keys and
+ * values of many sequences in pages of one pool. A page holds page_size tokens of every KV
+ * head; the caller owns the tables and gives pages to sequences. Token t of sequence b lies in
+ * slot t % page_size of page table[b][t / page_size].
+ *   table [n_seq][table_width] int32 device, row stride in elements: an entry outside
+ *     [0, n_pages) names no page: nothing is written there and its keys take no part. Two
+ *     sequences may share pages that neither call writes.
+ * Modes: fp16, the affine modes and Int8, with the codecs of a qw_kv_cache; head_dim 128 or 256;
+ * page_size 16, 32, 64, 128 or 256; at most 65535 KV heads. Rows start as zeros. */
+typedef struct qw_paged_cache qw_paged_cache;
+int qw_paged_create(int mode, int group_size, int n_kv_heads, int head_dim, int n_pages, int page_size, int device,
+                    qw_paged_cache** out);
+/* Frees the pool. Waits for the device first. */
+int qw_paged_destroy(qw_paged_cache* cache);
+int qw_paged_nbytes(const qw_paged_cache* cache, int64_t* nbytes);
+
+/* Writes n_tokens new tokens of n_seq sequences, quantized, into their pages: tokens
+ * offsets[b] .. offsets[b + 1] - 1 of k and v (offsets [n_seq + 1] int32 device, ascending from 0 to
+ * n_tokens; NULL: n_tokens / n_seq each) go to positions starts[b] .. (starts [n_seq] int32 device, >= 0).
+ *   k, v fp16, element (token, head, d) at k[token * k_token_stride + head * k_head_stride + d]; 8-byte
+ *     aligned with strides of whole 4 elements (a projection's output is taken as it lies)
+ * Slots that the call does not name stay as they were; a slot may be written again. Each page
+ * of a call belongs to one sequence. Tokens behind the table's last page are dropped. The call also keeps each
+ * page's bounds for qw_paged_select: the least and the largest key of each dim (as given, fp16) over what
+ * was written since slot 0 last was. n_tokens = 0: nothing happens. */
+int qw_paged_update(qw_paged_cache* cache, const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                    int64_t v_token_stride, int64_t v_head_stride, int n_tokens, int n_seq, const int32_t* offsets,
+                    const int32_t* starts, const int32_t* table, int64_t table_stride, int table_width, void* stream);
+
+/* Reads tokens back: positions starts[b] .. of each sequence, arguments as qw_paged_update, as the fp16
+ * values that their codes stand for (qw_kv_dequantize's). k_out, v_out [n_tokens][n_kv_heads][head_dim];
+ * positions without a page are zeros, rows of no sequence stay as they were. */
+int qw_paged_gather(const qw_paged_cache* cache, void* k_out, void* v_out, int n_tokens, int n_seq,
+                    const int32_t* offsets, const int32_t* starts, const int32_t* table, int64_t table_stride,
+                    int table_width, void* stream);
+
+/* Attention of each sequence's newest n_rows tokens over its first lengths[b] keys, the newest
+ * among them: row r sees keys t <= lengths[b] - n_rows + r.
+ *   out = softmax(scale q . k) . v   on code * scale + bias unrounded, in fp32 but for the weights'
+ *     rounding to fp16 in P . V; a row that sees no key is 0.
+ *   q [n_seq][n_q_heads][n_rows][head_dim] fp16 with element strides of whole 8, 16-byte aligned
+ *   lengths [n_seq] int32 device (clamped to 0 .. table_width * page_size)
+ *   picked (or NULL: all pages) [n_seq][n_kv_heads][n_picked] int32 device: the pages that a KV head
+ *     reads, as columns of its sequence's table row (entries outside it are skipped; of
+ *     each list the first min(n_picked, the sequence's pages) entries are read; qw_paged_select writes such)
+ *   out [n_seq][n_q_heads][n_rows][head_dim] fp16
+ * Keys that a later row sees and this one does not must be finite. |scale| <= 2^40; at most 16384 rows
+ * (n_rows * heads of a group) a KV head. n_seq = 0: nothing happens. */
+int qw_paged_attention(qw_paged_cache* cache, const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                       int64_t q_row_stride, int n_seq, int n_q_heads, int n_rows, const int32_t* lengths,
+                       const int32_t* table, int64_t table_stride, int table_width, const int32_t* picked,
+                       int n_picked, float scale, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,8 @@ and the tests use the reference's names:
   :meth:`KVCache.attention_general` take the same options over a cache.
 * :meth:`KVCache.shared_attention`, :meth:`KVCache.attention_scored` (with their
   update forms) and :meth:`KVCache.evict` have no counterpart in the reference.
+* :class:`PagedKVCache` (``qw_amd/paged.py``): many sequences in pages of one pool,
+  beyond the reference's full-attention path too.
 
 Torch is used only to hold device memory and to name the current stream.
 Tensors follow the reference's layouts: ``[1, H, L, D]`` (the batch of 1 may
@@ -33,7 +35,7 @@ __all__ = ["KVCacheMode", "KVCache", "QwError", "attention", "causal_attention",
            "sparse_attention", "sparse_attention_with",
            "fused_rope_qk_append", "dlsa_select", "dlsa_select_with", "turbo4_codebook",
            "turbo4_signs",
-           "release_workspaces", "lib", "LIB_PATH"]
+           "PagedKVCache", "release_workspaces", "lib", "LIB_PATH"]
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libqwattn.so")
 _lib = None
@@ -90,6 +92,12 @@ _SIGNATURES = {
     "qw_kv_update_and_attention_scored": (_i, [_p, _p, _i, _i, _p, _p, _f, _i, _p, _i64, _i, _f, _p,
                                                _i64, _p, _p]),
     "qw_kv_evict": (_i, [_p, _p, _p, _i64, _i, _i, _i, _p, _p, _i64, ctypes.POINTER(_i), _p]),
+    "qw_paged_create": (_i, [_i, _i, _i, _i, _i, _i, _i, ctypes.POINTER(_p)]),
+    "qw_paged_destroy": (_i, [_p]),
+    "qw_paged_nbytes": (_i, [_p, ctypes.POINTER(_i64)]),
+    "qw_paged_update": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _i, _i, _p, _p, _p, _i64, _i, _p]),
+    "qw_paged_gather": (_i, [_p, _p, _p, _i, _i, _p, _p, _p, _i64, _i, _p]),
+    "qw_paged_attention": (_i, [_p, _p, _i64, _i64, _i64, _i, _i, _i, _p, _p, _i64, _i, _p, _i, _f, _p, _p]),
     "qw_kv_trim": (_i, [_p, _i, ctypes.POINTER(_i)]),
     "qw_kv_dlsa_attention": (_i, [_p, _p, _i, _i, _p, _p, _i, _f, _p, _p]),
     "qw_kv_update_and_dlsa_attention": (_i, [_p, _p, _i, _i, _p, _p, _p, _p, _i, _f, _p, _p]),
@@ -904,3 +912,6 @@ def turbo4_signs(length: int, seed: int):
     out = np.zeros(length, np.float32)
     _check(lib().qw_turbo4_signs(length, seed & 0xFFFFFFFF, out.ctypes.data))
     return out
+
+
+from .paged import PagedKVCache  # noqa: E402  (it takes the helpers above)

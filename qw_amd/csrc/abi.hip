@@ -4,9 +4,13 @@
 #include <new>
 
 #include "kv_cache.hpp"
+#include "paged.hpp"
 
 struct qw_kv_cache {
     qw::KVCache impl;
+};
+struct qw_paged_cache {
+    qw::PagedCache impl;
 };
 
 
@@ -14,6 +18,14 @@ struct qw_kv_cache {
     do {                                                                      \
         if (!(c)) {                                                           \
             qw::set_error("null qw_kv_cache handle");                         \
+            return QW_ERR_INVALID_ARGUMENT;                                   \
+        }                                                                     \
+    } while (0)
+
+#define QW_PAGED_HANDLE(c)                                                    \
+    do {                                                                      \
+        if (!(c)) {                                                           \
+            qw::set_error("null qw_paged_cache handle");                      \
             return QW_ERR_INVALID_ARGUMENT;                                   \
         }                                                                     \
     } while (0)
@@ -485,6 +497,101 @@ int qw_kv_rope_update_and_attention(qw_kv_cache* cache, const void* qkv, int n_q
                                                      traditional, rope_base, rope_scale, position0,
                                                      scale, causal != 0, q_out, out,
                                                      (hipStream_t)stream));
+}
+
+int qw_paged_create(int mode, int group_size, int n_kv_heads, int head_dim, int n_pages, int page_size, int device,
+                    qw_paged_cache** out) {
+    if (!out) {
+        qw::set_error("qw_paged_create: null out pointer");
+        return QW_ERR_INVALID_ARGUMENT;
+    }
+    *out = nullptr;
+    qw_paged_cache* c = new (std::nothrow) qw_paged_cache();
+    if (!c) {
+        qw::set_error("qw_paged_create: host allocation failed");
+        return QW_ERR_OUT_OF_MEMORY;
+    }
+    int rc;
+    try {
+        rc = c->impl.init(mode, group_size, n_kv_heads, head_dim, n_pages, page_size, device);
+    } catch (...) {
+        rc = QW_ERR_STATE;
+        qw::set_error("qw_paged_create: unexpected C++ exception");
+    }
+    if (rc != QW_OK) {
+        c->impl.release();
+        delete c;
+        return rc;
+    }
+    *out = c;
+    return QW_OK;
+}
+
+int qw_paged_destroy(qw_paged_cache* cache) {
+    if (!cache) return QW_OK;
+    cache->impl.release();
+    delete cache;
+    return QW_OK;
+}
+
+int qw_paged_nbytes(const qw_paged_cache* cache, int64_t* nbytes) {
+    QW_PAGED_HANDLE(cache);
+    if (!nbytes) {
+        qw::set_error("qw_paged_nbytes: null out pointer");
+        return QW_ERR_INVALID_ARGUMENT;
+    }
+    *nbytes = cache->impl.nbytes();
+    return QW_OK;
+}
+
+static qw::PagedSeqs paged_seqs(int n_tokens, int n_seq, const int32_t* offsets, const int32_t* starts,
+                                const int32_t* table, int64_t table_stride, int table_width) {
+    qw::PagedSeqs s{};
+    s.table = table;
+    s.stride = table_stride;
+    s.width = table_width;
+    s.n_seq = n_seq;
+    s.offsets = offsets;
+    s.each = n_seq > 0 ? n_tokens / n_seq : 0;
+    s.starts = starts;
+    s.n_tokens = n_tokens;
+    return s;
+}
+
+int qw_paged_update(qw_paged_cache* cache, const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                    int64_t v_token_stride, int64_t v_head_stride, int n_tokens, int n_seq, const int32_t* offsets,
+                    const int32_t* starts, const int32_t* table, int64_t table_stride, int table_width, void* stream) {
+    QW_PAGED_HANDLE(cache);
+    QW_GUARDED(qw::paged_update(cache->impl, k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride,
+                                paged_seqs(n_tokens, n_seq, offsets, starts, table, table_stride, table_width),
+                                (hipStream_t)stream));
+}
+
+int qw_paged_gather(const qw_paged_cache* cache, void* k_out, void* v_out, int n_tokens, int n_seq,
+                    const int32_t* offsets, const int32_t* starts, const int32_t* table, int64_t table_stride,
+                    int table_width, void* stream) {
+    QW_PAGED_HANDLE(cache);
+    QW_GUARDED(qw::paged_gather(cache->impl, k_out, v_out,
+                                paged_seqs(n_tokens, n_seq, offsets, starts, table, table_stride, table_width),
+                                (hipStream_t)stream));
+}
+
+static qw::PagedQuery paged_query(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int64_t q_row_stride,
+                                  int n_seq, int n_q_heads, int n_rows, const int32_t* lengths, const int32_t* table,
+                                  int64_t table_stride, int table_width) {
+    return qw::PagedQuery{q,       q_seq_stride, q_head_stride, q_row_stride, n_seq,      n_q_heads,
+                          n_rows,  lengths,      table,         table_stride, table_width};
+}
+
+int qw_paged_attention(qw_paged_cache* cache, const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                       int64_t q_row_stride, int n_seq, int n_q_heads, int n_rows, const int32_t* lengths,
+                       const int32_t* table, int64_t table_stride, int table_width, const int32_t* picked,
+                       int n_picked, float scale, void* out, void* stream) {
+    QW_PAGED_HANDLE(cache);
+    QW_GUARDED(qw::paged_attention(cache->impl,
+                                   paged_query(q, q_seq_stride, q_head_stride, q_row_stride, n_seq, n_q_heads, n_rows,
+                                               lengths, table, table_stride, table_width),
+                                   picked, n_picked, scale, out, (hipStream_t)stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,146 @@
+// paged.hpp - a pool of KV pages shared by many sequences, and what its kernels have in common.
+//
+// A page holds page_size tokens of every KV head; a table [n_seq][table_width] of page indices says
+// where token t of a sequence lies: slot t % page_size of page table[b][t / page_size]. Indices
+// outside the pool name no page: nothing is written there, and keys there take no part. Layouts are
+// those the attention's matrix instructions take without a shuffle (E = 128 / bits codes in a
+// 16-byte piece):
+//   K  [page][head][slot][D * bits / 8 bytes]: the row's 32-dim steps c = d / 32, of each of which
+//      lane group g = d % 32 / 8 takes 8 dims; piece i of group g at 64 i + 16 g, holding the 8 dims
+//      of its 16 / bits steps one after another. fp16: dims in order. 8 bits: bytes in order. 4 bits: the
+//      8 codes at nibbles v4_nibble_pos.
+//   V  [page][head][slot / 8][D][8 codes]: for each dim the codes of 8 keys, 16, 8 or 4 bytes, in
+//      the same order.
+//   scales and biases of K and of V, [page][head][slot / 8][2][NG][8] fp16 (int8: the scales alone,
+//      [1][1][8]), NG = D / 64.
+// A 4- or 8-bit code in the low bits of a half is the subnormal code * 2^-24, which the matrix
+// instructions take as it is: codes need a mask, no conversion, and the scales go to the scores and
+// to the softmax weights.
+// Beside them, for each page and head: the least and the largest key of every dim over what was
+// written since slot 0 last was ([2][D] fp16), the same as 8-bit codes over the page's largest
+// magnitude ([2][D], largest first), that magnitude, and E >= 0 with every V scale below 2^E.
+#pragma once
+
+#include "kv_cache.hpp"
+
+namespace qw {
+
+struct PagedView {
+    char* k;
+    char* v;
+    f16* k_par;
+    f16* v_par;
+    f16* lohi;
+    int8_t* codes;
+    float* top;
+    int* v_exp;
+    int hkv, n_pages, lg;  // page_size = 1 << lg
+};
+
+struct PagedCache {
+    int mode = QW_KV_FP16, bits = 16, D = 0, hkv = 0, n_pages = 0, page_size = 0, device = 0;
+    PagedView view{};
+
+    bool int8() const { return mode == QW_KV_INT8; }
+    int par_halves() const { return bits == 16 ? 0 : int8() ? 8 : 2 * (D / kGroup) * 8; }  // of 8 slots
+    int64_t nbytes() const;
+    int init(int mode, int group_size, int n_kv_heads, int head_dim, int n_pages, int page_size, int device);
+    void release();
+};
+
+// The sequences' places: table, the first position of each, the tokens of each.
+struct PagedSeqs {
+    const int32_t* table;
+    int64_t stride;
+    int width, n_seq;
+    const int32_t* offsets;  // [n_seq + 1], or null: `each` tokens a sequence
+    int each;
+    const int32_t* starts;
+    int n_tokens;
+};
+
+int paged_update(PagedCache& c, const void* k, const void* v, int64_t k_token, int64_t k_head, int64_t v_token,
+                 int64_t v_head, const PagedSeqs& s, hipStream_t stream);
+int paged_gather(const PagedCache& c, void* k_out, void* v_out, const PagedSeqs& s, hipStream_t stream);
+int check_seqs(const PagedCache& c, const PagedSeqs& s, const char* what);
+
+// Queries [n_seq][n_q_heads][n_rows][D] of element strides, over the sequences' first lengths[b] keys.
+struct PagedQuery {
+    const void* q;
+    int64_t seq_stride, head_stride, row_stride;
+    int n_seq, n_q_heads, n_rows;
+    const int32_t* lengths;
+    const int32_t* table;
+    int64_t table_stride;
+    int table_width;
+};
+int check_query(const PagedCache& c, const PagedQuery& q, const char* what);
+// picked (or null): [n_seq][hkv][n_picked] positions in the sequences' rows of the table.
+int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, int n_picked, float scale, void* out,
+                    hipStream_t stream);
+
+// ------------------------------------------------------------------ device
+
+// Inclusive sums over a wave's lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    const int lane = (int)__lane_id();
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+// Which of n sequences holds unit `i` where sequence b has count(b) of them, and its index there; b = -1
+// behind the last. Every lane of a wave calls it and gets the same.
+struct PagedUnit {
+    int b;
+    uint32_t at, base;  // base: units before the sequence
+};
+template <class F>
+__device__ __forceinline__ PagedUnit find_unit(int n, uint32_t i, F count) {
+    const int lane = (int)__lane_id();
+    uint32_t base = 0;
+    for (int b0 = 0; b0 < n; b0 += 64) {
+        const uint32_t c = b0 + lane < n ? count(b0 + lane) : 0u;
+        const uint32_t s = wave_scan(c);
+        const uint64_t past = __ballot(base + s > i);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const uint32_t before = base + (uint32_t)__builtin_amdgcn_readlane((int)(s - c), l);
+            return {__builtin_amdgcn_readfirstlane(b0 + l), i - before, before};
+        }
+        base += (uint32_t)__builtin_amdgcn_readlane((int)s, 63);
+    }
+    return {-1, 0u, base};
+}
+
+// Where sequence b's new tokens go: positions start .. start + n - 1, from token `first` on.
+struct PagedSpan {
+    int start, n, first;
+};
+__device__ __forceinline__ PagedSpan span_of(const PagedSeqs& s, int b, int lg) {
+    PagedSpan p;
+    p.start = s.starts[b];
+    int64_t lo, hi;
+    if (s.offsets) {
+        lo = s.offsets[b], hi = s.offsets[b + 1];
+    } else {
+        lo = (int64_t)b * s.each, hi = lo + s.each;
+    }
+    lo = lo < 0 ? 0 : lo;
+    hi = hi > s.n_tokens ? s.n_tokens : hi;
+    int64_t n = hi - lo;
+    n = n < 0 || p.start < 0 ? 0 : n;
+    p.n = (int)n;
+    p.first = (int)(n > 0 ? lo : 0);
+    return p;
+}
+// (the tokens behind the table's last page have no place)
+__device__ __forceinline__ int span_in_table(const PagedSeqs& s, const PagedSpan& p, int lg) {
+    const int64_t room = ((int64_t)s.width << lg) - p.start;
+    return room < p.n ? (room > 0 ? (int)room : 0) : p.n;
+}
+
+}  // namespace qw

@@ -1,0 +1,539 @@
+// paged_store.hip - new tokens into their pages, quantized, and back out as fp16.
+//
+// The codecs are the caches' own: MLX affine in groups of 64 dims (quant.hpp), per-token int8, fp16.
+// A workgroup takes one page of one head, so that every word that holds several keys' codes, and the
+// page's bounds, have one writer. A wave takes 8 slots (two times 8 at D = 128): a lane holds 4 dims of
+// 8 tokens of K and V, 16 lanes a group, whose extremes come by DPP; V's words of 8 keys form in the
+// lane. Where a call covers part of such a word the rest is kept.
+#include <algorithm>
+
+#include "paged.hpp"
+#include "quant.hpp"
+
+namespace qw {
+
+namespace {
+
+size_t align16(size_t x) { return (x + 255) / 256 * 256; }
+
+}  // namespace
+
+int64_t PagedCache::nbytes() const {
+    const int64_t ph = (int64_t)n_pages * hkv, rows = ph * page_size;
+    return 2 * rows * D * bits / 8 + 2 * rows / 8 * par_halves() * 2 + ph * (4 * D + 2 * D + 8);
+}
+
+int PagedCache::init(int mode_, int group_size, int n_kv_heads, int head_dim, int n_pages_, int page_size_, int device_) {
+    QW_REQUIRE(mode_ == QW_KV_FP16 || mode_ == QW_KV_AFFINE8 || mode_ == QW_KV_AFFINE4 || mode_ == QW_KV_INT8 ||
+                   mode_ == QW_KV_TURBO4,
+               QW_ERR_INVALID_ARGUMENT, "qw_paged_create: unknown mode");
+    QW_REQUIRE(mode_ != QW_KV_TURBO4, QW_ERR_UNSUPPORTED, "qw_paged_create: turbo4 has no paged form");
+    QW_REQUIRE(n_kv_heads > 0 && n_kv_heads <= 65535 && n_pages_ > 0, QW_ERR_INVALID_ARGUMENT,
+               "qw_paged_create: 1 .. 65535 KV heads and at least one page expected");
+    QW_REQUIRE(head_dim == 128 || head_dim == 256, QW_ERR_UNSUPPORTED, "qw_paged_create: head_dim 128 or 256");
+    QW_REQUIRE((mode_ != QW_KV_AFFINE8 && mode_ != QW_KV_AFFINE4) || group_size == kGroup, QW_ERR_UNSUPPORTED,
+               "qw_paged_create: affine modes use group_size 64");
+    QW_REQUIRE(page_size_ >= 16 && page_size_ <= 256 && (page_size_ & (page_size_ - 1)) == 0, QW_ERR_UNSUPPORTED,
+               "qw_paged_create: page_size 16, 32, 64, 128 or 256");
+    mode = mode_;
+    bits = mode == QW_KV_AFFINE4 ? 4 : mode == QW_KV_FP16 ? 16 : 8;
+    D = head_dim;
+    hkv = n_kv_heads;
+    n_pages = n_pages_;
+    page_size = page_size_;
+    device = device_;
+    DeviceGuard dg(device);
+    QW_REQUIRE(dg.ok, QW_ERR_HIP, "qw_paged_create: hipSetDevice failed");
+    const size_t ph = (size_t)n_pages * hkv, rows = ph * page_size;
+    const size_t sizes[8] = {rows * D * bits / 8, rows * D * bits / 8, rows / 8 * par_halves() * 2, rows / 8 * par_halves() * 2,
+                             ph * 4 * D, ph * 2 * D, ph * 4, ph * 4};
+    void* at[8] = {};
+    for (int i = 0; i < 8; i++) {
+        const bool ok = sizes[i] == 0 || hipMalloc(&at[i], align16(sizes[i])) == hipSuccess;
+        if (!ok) {
+            (void)hipGetLastError();
+            for (void* p : at)
+                if (p) (void)hipFree(p);
+            set_error("qw_paged_create: hipMalloc of " + std::to_string(sizes[i]) + " bytes failed");
+            return QW_ERR_OUT_OF_MEMORY;
+        }
+    }
+    view = PagedView{(char*)at[0], (char*)at[1], (f16*)at[2], (f16*)at[3], (f16*)at[4], (int8_t*)at[5], (float*)at[6],
+                     (int*)at[7], hkv, n_pages, __builtin_ctz(page_size)};
+    for (int i = 0; i < 8; i++)
+        if (at[i]) QW_HIP_CHECK(hipMemset(at[i], 0, sizes[i]));
+    QW_HIP_CHECK(hipDeviceSynchronize());
+    return QW_OK;
+}
+
+void PagedCache::release() {
+    DeviceGuard dg(device);
+    (void)hipDeviceSynchronize();
+    void* ptrs[8] = {view.k, view.v, view.k_par, view.v_par, view.lohi, view.codes, view.top, view.v_exp};
+    for (void* p : ptrs)
+        if (p) (void)hipFree(p);
+    view = PagedView{};
+}
+
+int check_seqs(const PagedCache& c, const PagedSeqs& s, const char* what) {
+    const std::string w(what);
+    QW_REQUIRE(s.n_tokens >= 0 && s.n_seq >= 0 && (s.n_tokens == 0 || s.n_seq > 0), QW_ERR_INVALID_ARGUMENT,
+               w + ": n_tokens and n_seq >= 0, and a sequence for the tokens, expected");
+    QW_REQUIRE(s.n_tokens == 0 || (s.table && s.starts && s.width > 0), QW_ERR_INVALID_ARGUMENT, w + ": null table/starts, or a table without columns");
+    QW_REQUIRE(s.stride >= s.width, QW_ERR_INVALID_ARGUMENT, w + ": a table stride below its width");
+    QW_REQUIRE((int64_t)s.width * c.page_size <= 0x7fffff00, QW_ERR_INVALID_ARGUMENT, w + ": table_width * page_size < 2^31 expected");
+    QW_REQUIRE(s.n_seq <= 65535 && s.n_tokens <= (1 << 28), QW_ERR_UNSUPPORTED, w + ": at most 65535 sequences and 2^28 tokens a call");
+    QW_REQUIRE(s.n_tokens == 0 || s.offsets || s.n_tokens % s.n_seq == 0, QW_ERR_INVALID_ARGUMENT,
+               w + ": without offsets n_tokens is a multiple of n_seq");
+    return QW_OK;
+}
+
+namespace {
+
+// Extremes of a group: 16 lanes of 4 dims.
+template <class Op>
+__device__ __forceinline__ float reduce16(float x, Op op) {
+    x = op(x, dpp_mov<0xB1>(x));
+    x = op(x, dpp_mov<0x4E>(x));
+    x = op(x, dpp_mov<0x124>(x));
+    return op(x, dpp_mov<0x128>(x));
+}
+// And of a row: D / 4 lanes.
+template <int D, class Op>
+__device__ __forceinline__ float reduce_row(float x, Op op) {
+    const int lane = (int)__lane_id();
+    x = reduce16(x, op);
+    x = op(x, lane_xor<16>(x, lane));
+    return D == 256 ? op(x, lane_xor<32>(x, lane)) : x;
+}
+
+struct FMax {
+    __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct FMin {
+    __device__ float operator()(float a, float b) const { return fminf(a, b); }
+};
+
+// 4 dims' codes (a byte each) of a row, and the group's scale and bias.
+template <int BITS, bool INT8, int D>
+__device__ __forceinline__ uint32_t quantize4(half4v x, f16& scale, f16& bias) {
+    float f[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = (float)x[i];
+    uint32_t w = 0;
+    if constexpr (INT8) {
+        const float top = reduce_row<D>(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))), FMax());
+        scale = (f16)(top / 127.0f);
+        if ((float)scale == 0.0f) scale = (f16)1.0f;
+        bias = (f16)0.0f;
+        const float s = (float)scale;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float c = __builtin_rintf((float)(f16)(f[i] / s));
+            w |= (uint32_t)((int)fminf(fmaxf(c, -128.0f), 127.0f) + 128) << (8 * i);
+        }
+    } else {
+        const float mn = reduce16(fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), FMin());
+        const float mx = reduce16(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), FMax());
+        const AffineGroup q = affine_group(mn, mx, BITS);
+        const float inv = 1.0f / q.scale;
+        scale = (f16)q.scale;
+        bias = (f16)q.bias;
+#pragma unroll
+        for (int i = 0; i < 4; i++) w |= (uint32_t)affine_code_inv(f[i], q, inv, BITS) << (8 * i);
+    }
+    return w;
+}
+
+// Byte 64 i + 16 g + .. of a K row where a lane's 4 dims (of index li) begin.
+template <int BITS>
+__device__ __forceinline__ int k_at(int li) {
+    const int c = li >> 3, g = (li & 7) >> 1, hi = li & 1;
+    if (BITS == 16) return 8 * li;
+    if (BITS == 8) return (c >> 1) * 64 + g * 16 + (c & 1) * 8 + hi * 4;
+    return (c >> 2) * 64 + g * 16 + (c & 3) * 4;
+}
+
+constexpr int kStoreWaves = 4;
+
+struct StoreArgs {
+    const f16* k;
+    const f16* v;
+    int64_t k_token, k_head, v_token, v_head;
+    PagedSeqs s;
+};
+
+template <int BITS, bool INT8, int D>
+__global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedView c, StoreArgs a) {
+    constexpr int LPR = D / 4, SUB = 64 / LPR, NG = INT8 ? 1 : D / kGroup;
+    __shared__ float sm_lo[kStoreWaves][D], sm_hi[kStoreWaves][D], sm_s[kStoreWaves];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int nw = blockDim.x >> 6, h = blockIdx.y, ps = 1 << c.lg;
+    const PagedUnit u = find_unit(a.s.n_seq, blockIdx.x, [&](int b) {
+        const PagedSpan p = span_of(a.s, b, c.lg);
+        const int n = span_in_table(a.s, p, c.lg);
+        return n > 0 ? (uint32_t)(((p.start + n - 1) >> c.lg) - (p.start >> c.lg) + 1) : 0u;
+    });
+    if (u.b < 0) return;
+    const PagedSpan p = span_of(a.s, u.b, c.lg);
+    const int n = span_in_table(a.s, p, c.lg);
+    const int logical = (p.start >> c.lg) + (int)u.at;
+    const int page = a.s.table[u.b * a.s.stride + logical];
+    if (page < 0 || page >= c.n_pages) return;
+    const int pos0 = logical << c.lg;
+    const int s0 = max(p.start - pos0, 0), s1 = min(p.start + n - pos0, ps);
+    const int64_t ph = (int64_t)page * c.hkv + h;
+    const int li = lane % LPR, sub = lane / LPR, grp = li >> 4;
+
+    float lo[4], hi[4], smax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) lo[i] = INFINITY, hi[i] = -INFINITY;
+    const int first = s0 >> 3, last = (s1 - 1) >> 3;
+    for (int b0 = first; b0 <= last; b0 += nw * SUB) {
+        const int blk = b0 + wave * SUB + sub;
+        half4v xk[8], xv[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int slot = 8 * blk + k;
+            xk[k] = half4v{}, xv[k] = half4v{};
+            if (slot >= s0 && slot < s1) {
+                const int64_t t = (int64_t)p.first + (pos0 + slot - p.start);
+                xk[k] = *(const half4v*)(a.k + t * a.k_token + h * a.k_head + 4 * li);
+                xv[k] = *(const half4v*)(a.v + t * a.v_token + h * a.v_head + 4 * li);
+            }
+        }
+        const bool live = blk <= last;
+        const int64_t blk8 = ph * (ps >> 3) + blk;
+        char* krow = c.k + (ph * ps + 8 * blk) * (D * BITS / 8) + k_at<BITS>(li);
+        u32x4* vblk = (u32x4*)(c.v + blk8 * (D * BITS) + 4 * li * BITS);  // this lane's 4 dims
+        // what the words hold of keys that this call leaves alone
+        const bool whole = 8 * blk >= s0 && 8 * blk + 8 <= s1;
+        u32x4 old[BITS / 4];
+#pragma unroll
+        for (int j = 0; j < BITS / 4; j++) old[j] = live && !whole ? vblk[j] : u32x4{0, 0, 0, 0};
+        uint32_t vc[8];
+        half8 ks, kb, vs, vb;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int slot = 8 * blk + k;
+            const bool in = slot >= s0 && slot < s1;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float x = (float)xk[k][i];
+                lo[i] = in ? fminf(lo[i], x) : lo[i];
+                hi[i] = in ? fmaxf(hi[i], x) : hi[i];
+            }
+            if constexpr (BITS == 16) {
+                if (in) *(half4v*)(krow + k * (D * 2)) = xk[k];
+            } else {
+                f16 s, b;
+                uint32_t w = quantize4<BITS, INT8, D>(xk[k], s, b);
+                ks[k] = s, kb[k] = b;
+                if constexpr (BITS == 4) {
+                    // dims 8 j .. + 3 in an even lane (nibbles 0, 4, 1, 5), .. + 7 in the odd one (2, 6, 3, 7)
+                    const uint32_t x = (w & 15) | (w >> 8 & 15) << 16 | (w >> 16 & 15) << 4 | (w >> 24) << 20;
+                    w = __builtin_amdgcn_update_dpp(0u, x, 0xB1, 0xF, 0xF, false);  // the other lane's
+                    w = x | w << 8;
+                    if (in && (li & 1) == 0) *(uint32_t*)(krow + k * (D / 2)) = w;
+                } else {
+                    if (in) *(uint32_t*)(krow + k * D) = w;
+                }
+                vc[k] = quantize4<BITS, INT8, D>(xv[k], s, b);
+                vs[k] = s, vb[k] = b;
+                smax = in ? fmaxf(smax, fabsf((float)s)) : smax;
+            }
+        }
+        if (live) {
+            uint32_t key[4];  // of key pair j: all bits of the halves that this call writes
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int s = 8 * blk + 2 * j;
+                key[j] = (s >= s0 && s < s1 ? 0xFFFFu : 0u) | (s + 1 >= s0 && s + 1 < s1 ? 0xFFFF0000u : 0u);
+            }
+            if constexpr (BITS == 16) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    u32x4 w;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t x = __builtin_bit_cast(uint32_t, half2v{xv[2 * j][i], xv[2 * j + 1][i]});
+                        w[j] = (x & key[j]) | (old[i][j] & ~key[j]);
+                    }
+                    vblk[i] = w;
+                }
+            } else if constexpr (BITS == 8) {
+                uint32_t m[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    m[j] = (key[2 * j] & 0xFFu) | (key[2 * j] >> 8 & 0xFF00u) | (key[2 * j + 1] << 16 & 0xFF0000u) |
+                           (key[2 * j + 1] & 0xFF000000u);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        uint32_t x = 0;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) x |= (vc[4 * j + k] >> (8 * i) & 0xFFu) << (8 * k);
+                        const uint32_t o = old[i / 2][2 * (i & 1) + j];
+                        old[i / 2][2 * (i & 1) + j] = (x & m[j]) | (o & ~m[j]);
+                    }
+                vblk[0] = old[0];
+                vblk[1] = old[1];
+            } else {
+                uint32_t m = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) m |= (key[j] & 0x000F000Fu) << (4 * j);
+                u32x4 w;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t x = 0;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) x |= (vc[k] >> (8 * i) & 15u) << (4 * v4_nibble_pos(k));
+                    w[i] = (x & m) | (old[0][i] & ~m);
+                }
+                vblk[0] = w;
+            }
+            if constexpr (BITS != 16) {
+                if (INT8 ? li == 0 : (li & 15) == 0) {
+                    f16* kp = c.k_par + blk8 * (INT8 ? 8 : 16 * NG) + (INT8 ? 0 : 8 * grp);
+                    f16* vp = c.v_par + blk8 * (INT8 ? 8 : 16 * NG) + (INT8 ? 0 : 8 * grp);
+                    if (whole) {
+                        *(half8*)kp = ks;
+                        *(half8*)vp = vs;
+                        if (!INT8) *(half8*)(kp + 8 * NG) = kb, *(half8*)(vp + 8 * NG) = vb;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            if (8 * blk + k >= s0 && 8 * blk + k < s1) {
+                                kp[k] = ks[k], vp[k] = vs[k];
+                                if (!INT8) kp[8 * NG + k] = kb[k], vp[8 * NG + k] = vb[k];
+                            }
+                    }
+                }
+            }
+        }
+    }
+    // the page's bounds
+    if constexpr (SUB == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            lo[i] = fminf(lo[i], lane_xor<32>(lo[i], lane));
+            hi[i] = fmaxf(hi[i], lane_xor<32>(hi[i], lane));
+        }
+    }
+    smax = wave_reduce(smax, FMax());
+    if (nw > 1) {
+        if (sub == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) sm_lo[wave][4 * li + i] = lo[i], sm_hi[wave][4 * li + i] = hi[i];
+        }
+        if (lane == 0) sm_s[wave] = smax;
+        __syncthreads();
+        if (wave) return;
+        for (int w = 1; w < nw; w++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                lo[i] = fminf(lo[i], sm_lo[w][4 * li + i]);
+                hi[i] = fmaxf(hi[i], sm_hi[w][4 * li + i]);
+            }
+            smax = fmaxf(smax, sm_s[w]);
+        }
+    }
+    f16* lohi = c.lohi + ph * 2 * D + 4 * li;
+    if (s0 > 0) {
+        const half4v l = *(const half4v*)lohi, u4 = *(const half4v*)(lohi + D);
+#pragma unroll
+        for (int i = 0; i < 4; i++) lo[i] = fminf(lo[i], (float)l[i]), hi[i] = fmaxf(hi[i], (float)u4[i]);
+    }
+    half4v l, u4;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        lo[i] = fminf(fmaxf(lo[i], -65504.0f), 65504.0f);
+        hi[i] = fminf(fmaxf(hi[i], -65504.0f), 65504.0f);
+        if (lo[i] > hi[i]) lo[i] = hi[i] = 0.0f;  // nothing but NaN
+        l[i] = (f16)lo[i], u4[i] = (f16)hi[i];
+        top = fmaxf(top, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+    }
+    top = reduce_row<D>(top, FMax());
+    const float inv = top > 0.0f ? 127.0f / top : 0.0f;
+    uint32_t wl = 0, wh = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        wh |= ((uint32_t)(int)fminf(fmaxf(__builtin_ceilf(hi[i] * inv), -127.0f), 127.0f) & 0xFFu) << (8 * i);
+        wl |= ((uint32_t)(int)fminf(fmaxf(__builtin_floorf(lo[i] * inv), -127.0f), 127.0f) & 0xFFu) << (8 * i);
+    }
+    if (sub == 0) {
+        *(half4v*)lohi = l;
+        *(half4v*)(lohi + D) = u4;
+        *(uint32_t*)(c.codes + ph * 2 * D + 4 * li) = wh;
+        *(uint32_t*)(c.codes + ph * 2 * D + D + 4 * li) = wl;
+    }
+    if (lane == 0) {
+        c.top[ph] = top;
+        if (BITS != 16) {
+            int e = smax < 1.0f ? 0 : smax < 65536.0f ? (int)(__float_as_uint(smax) >> 23) - 126 : 17;
+            if (s0 > 0) e = max(e, c.v_exp[ph]);
+            c.v_exp[ph] = e;
+        }
+    }
+}
+
+// 4 dims' fp16 values of a code word (a byte each): f16(f16(code * scale) + bias).
+template <bool INT8>
+__device__ __forceinline__ half4v values4(uint32_t w, f16 s, f16 b) {
+    half4v y;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float c = (float)(int)(w >> (8 * i) & 0xFFu);
+        y[i] = INT8 ? (f16)((c - 128.0f) * (float)s) : (f16)affine_dequant(c, s, b);
+    }
+    return y;
+}
+
+template <int BITS, bool INT8, int D>
+__global__ __launch_bounds__(256) void paged_gather_kernel(PagedView c, PagedSeqs s, f16* k_out, f16* v_out) {
+    constexpr int LPR = D / 4, SUB = 64 / LPR, NG = INT8 ? 1 : D / kGroup;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int h = blockIdx.y, ps = 1 << c.lg;
+    const int li = lane % LPR, sub = lane / LPR, grp = INT8 ? 0 : li >> 4;
+    const uint32_t unit = (blockIdx.x * 4 + wave) * SUB;
+    auto blocks = [&](int b) {
+        const PagedSpan p = span_of(s, b, c.lg);
+        return p.n > 0 ? (uint32_t)((((int64_t)p.start + p.n - 1) >> 3) - (p.start >> 3) + 1) : 0u;
+    };
+    PagedUnit u = find_unit(s.n_seq, unit, blocks);
+    if (u.b < 0) return;
+    if constexpr (SUB == 2) {
+        const PagedUnit u1 = find_unit(s.n_seq, unit + 1, blocks);
+        if (sub) u = u1;
+        if (u.b < 0) return;
+    }
+    const PagedSpan p = span_of(s, u.b, c.lg);
+    const int64_t pos0 = ((int64_t)(p.start >> 3) + u.at) * 8, end = (int64_t)p.start + p.n;
+    const int64_t logical = pos0 >> c.lg;
+    int page = logical < s.width ? s.table[u.b * s.stride + logical] : -1;
+    const bool there = page >= 0 && page < c.n_pages;
+    page = there ? page : 0;
+    const int slot0 = (int)(pos0 & (ps - 1));
+    const int64_t ph = (int64_t)page * c.hkv + h, blk8 = ph * (ps >> 3) + (slot0 >> 3);
+    const char* krow = c.k + (ph * ps + slot0) * (D * BITS / 8) + k_at<BITS>(li);
+    const u32x4* vblk = (const u32x4*)(c.v + blk8 * (D * BITS) + 4 * li * BITS);
+    u32x4 vw[BITS / 4];
+#pragma unroll
+    for (int j = 0; j < BITS / 4; j++) vw[j] = vblk[j];
+    half8 ks{}, kb{}, vs{}, vb{};
+    if constexpr (BITS != 16) {
+        const f16* kp = c.k_par + blk8 * (INT8 ? 8 : 16 * NG) + 8 * grp;
+        const f16* vp = c.v_par + blk8 * (INT8 ? 8 : 16 * NG) + 8 * grp;
+        ks = *(const half8*)kp, vs = *(const half8*)vp;
+        if (!INT8) kb = *(const half8*)(kp + 8 * NG), vb = *(const half8*)(vp + 8 * NG);
+    }
+    half4v yk[8];
+    uint32_t kw[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        if constexpr (BITS == 16)
+            yk[k] = *(const half4v*)(krow + k * (D * 2));
+        else
+            kw[k] = *(const uint32_t*)(krow + k * (D * BITS / 8));
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const int64_t pos = pos0 + k;
+        half4v y;
+        if constexpr (BITS == 16) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t w = vw[i][k / 2];
+                y[i] = __builtin_bit_cast(f16, (uint16_t)(k & 1 ? w >> 16 : w));
+            }
+        } else {
+            uint32_t w = kw[k], x = 0;
+            if constexpr (BITS == 4) {
+                w >>= 8 * (li & 1);
+                w = (w & 15u) | (w >> 16 & 15u) << 8 | (w >> 4 & 15u) << 16 | (w >> 20 & 15u) << 24;
+#pragma unroll
+                for (int i = 0; i < 4; i++) x |= (vw[0][i] >> (4 * v4_nibble_pos(k)) & 15u) << (8 * i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) x |= (vw[i / 2][2 * (i & 1) + k / 4] >> (8 * (k & 3)) & 0xFFu) << (8 * i);
+            }
+            yk[k] = values4<INT8>(w, ks[k], kb[k]);
+            y = values4<INT8>(x, vs[k], vb[k]);
+        }
+        if (pos >= p.start && pos < end) {
+            const int64_t at = ((int64_t)(p.first + (pos - p.start)) * c.hkv + h) * D + 4 * li;
+            *(half4v*)(k_out + at) = there ? yk[k] : half4v{};
+            *(half4v*)(v_out + at) = there ? y : half4v{};
+        }
+    }
+}
+
+template <class F>
+void by_mode(const PagedCache& c, F f) {
+    auto of = [&](auto bits, auto i8) {
+        if (c.D == 256)
+            f(bits, i8, std::integral_constant<int, 256>());
+        else
+            f(bits, i8, std::integral_constant<int, 128>());
+    };
+    using std::integral_constant;
+    if (c.bits == 16)
+        of(integral_constant<int, 16>(), integral_constant<bool, false>());
+    else if (c.bits == 4)
+        of(integral_constant<int, 4>(), integral_constant<bool, false>());
+    else if (c.int8())
+        of(integral_constant<int, 8>(), integral_constant<bool, true>());
+    else
+        of(integral_constant<int, 8>(), integral_constant<bool, false>());
+}
+
+// Blocks of `size` tokens that n_tokens in n_seq runs can touch.
+int64_t most_units(const PagedSeqs& s, int size) {
+    return std::min<int64_t>(s.n_tokens, (int64_t)s.n_tokens / size + 2 * (int64_t)s.n_seq);
+}
+
+}  // namespace
+
+int paged_update(PagedCache& c, const void* k, const void* v, int64_t k_token, int64_t k_head, int64_t v_token,
+                 int64_t v_head, const PagedSeqs& s, hipStream_t stream) {
+    if (int rc = check_seqs(c, s, "paged update")) return rc;
+    if (s.n_tokens == 0) return QW_OK;
+    QW_REQUIRE(k && v, QW_ERR_INVALID_ARGUMENT, "paged update: null k/v");
+    QW_REQUIRE(((uintptr_t)k | (uintptr_t)v) % 8 == 0 && (k_token | k_head | v_token | v_head) % 4 == 0 && k_token >= 0 &&
+                   k_head >= 0 && v_token >= 0 && v_head >= 0,
+               QW_ERR_INVALID_ARGUMENT, "paged update: k and v 8-byte aligned with strides of whole 8 bytes expected");
+    DeviceGuard dg(c.device);
+    QW_REQUIRE(dg.ok, QW_ERR_HIP, "paged update: hipSetDevice failed");
+    const StoreArgs a{(const f16*)k, (const f16*)v, k_token, k_head, v_token, v_head, s};
+    // waves for the blocks of 8 slots that an average sequence touches in a page, two a wave at D = 128
+    const int blocks = std::min(c.page_size / 8, s.n_tokens / s.n_seq / 8 + 1);
+    const int waves = std::max(1, std::min(kStoreWaves, blocks * c.D / 256));
+    const dim3 grid((unsigned)most_units(s, c.page_size), c.hkv);
+    by_mode(c, [&](auto bits, auto i8, auto d) {
+        hipLaunchKernelGGL((paged_update_kernel<decltype(bits)::value, decltype(i8)::value, decltype(d)::value>), grid,
+                           dim3(64 * waves), 0, stream, c.view, a);
+    });
+    QW_HIP_CHECK(hipGetLastError());
+    return QW_OK;
+}
+
+int paged_gather(const PagedCache& c, void* k_out, void* v_out, const PagedSeqs& s, hipStream_t stream) {
+    if (int rc = check_seqs(c, s, "paged gather")) return rc;
+    if (s.n_tokens == 0) return QW_OK;
+    QW_REQUIRE(k_out && v_out, QW_ERR_INVALID_ARGUMENT, "paged gather: null k_out/v_out");
+    QW_REQUIRE(((uintptr_t)k_out | (uintptr_t)v_out) % 8 == 0, QW_ERR_INVALID_ARGUMENT, "paged gather: outputs 8-byte aligned expected");
+    DeviceGuard dg(c.device);
+    QW_REQUIRE(dg.ok, QW_ERR_HIP, "paged gather: hipSetDevice failed");
+    const int64_t per = 4 * 256 / c.D;  // units a workgroup
+    const dim3 grid((unsigned)((most_units(s, 8) + per - 1) / per), c.hkv);
+    by_mode(c, [&](auto bits, auto i8, auto d) {
+        hipLaunchKernelGGL((paged_gather_kernel<decltype(bits)::value, decltype(i8)::value, decltype(d)::value>), grid,
+                           dim3(256), 0, stream, c.view, s, (f16*)k_out, (f16*)v_out);
+    });
+    QW_HIP_CHECK(hipGetLastError());
+    return QW_OK;
+}
+
+}  // namespace qw

@@ -271,6 +271,7 @@ enum Workspace {
     kWsRowSums,  // the rows' softmax statistics for the key weights (key_weights.hip)
     kWsSelect,   // an eviction's digit counts (evict.hip)
     kWsEvict,    // the rows that an eviction in place moves (evict.hip)
+    kWsPaged,    // partials of attention over pages (paged_attend.hip)
     kWorkspaces
 };
 int workspace(Workspace kind, int device, hipStream_t stream, size_t need, void** out);

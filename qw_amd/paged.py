@@ -1,0 +1,139 @@
+"""Caches of many sequences in pages of one pool (``qw_paged_*`` of ``include/qwattn.h``).
+
+A layer's keys and values lie in pages of ``page_size`` tokens of every KV head. The caller owns the
+tables: ``table`` [B, W] int32 on the device gives the pool's page of each ``page_size`` tokens of each
+sequence, anything outside the pool (-1) where it has none.
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import KVCacheMode, QwError, _check, _stream, _torch, lib
+
+
+def _ints(t, what: str, device, n: int):
+    """A [n] int32 tensor on the device, contiguous."""
+    torch = _torch()
+    if t.shape != (n,) or t.dtype is not torch.int32 or t.device != device:
+        raise QwError(1, f"{what} must be a [{n}] int32 tensor on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _table(t, device, what: str):
+    """(tensor, B, W, row stride) of a table [B, W] int32 on the device."""
+    torch = _torch()
+    if t.dim() != 2 or t.dtype is not torch.int32 or t.device != device:
+        raise QwError(1, f"{what}: table must be a [B, W] int32 tensor on {device}")
+    B, W = t.shape
+    if W > 1 and t.stride(1) != 1 or B > 1 and t.stride(0) < W:
+        t = t.contiguous()
+    return t, B, W, t.stride(0) if B > 1 else W
+
+
+class PagedKVCache:
+    """One layer's keys and values of many sequences, in pages (``qw_paged_create``). Modes
+    ``"fp16"``, ``"affine8"``, ``"affine4"`` and ``"int8"``, with the codecs of :class:`KVCache`;
+    head_dim 128 or 256; ``page_size`` 16, 32, 64, 128 or 256."""
+
+    def __init__(self, mode: int | str, n_kv_heads: int, head_dim: int, n_pages: int, page_size: int = 64,
+                 group_size: int = 64, device=None):
+        torch = _torch()
+        if isinstance(mode, str):
+            mode = KVCacheMode.from_str(mode)
+        self.mode, self.n_kv_heads, self.head_dim = mode, n_kv_heads, head_dim
+        self.n_pages, self.page_size = n_pages, page_size
+        self.bits = KVCacheMode.BITS[mode]
+        self.device = torch.device("cuda", torch.cuda.current_device() if device is None else
+                                   torch.device(device).index or 0)
+        self._h = None
+        h = ctypes.c_void_p()
+        _check(lib().qw_paged_create(mode, group_size, n_kv_heads, head_dim, n_pages, page_size,
+                                     self.device.index, ctypes.byref(h)))
+        self._h = h
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            lib().qw_paged_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def nbytes(self) -> int:
+        v = ctypes.c_int64()
+        _check(lib().qw_paged_nbytes(self._h, ctypes.byref(v)))
+        return v.value
+
+    # -- new tokens in, tokens back out
+    def _seqs(self, n: int, table, starts, offsets, what: str):
+        t, B, W, stride = _table(table, self.device, what)
+        s = _ints(starts, f"{what}: starts", self.device, B)
+        o = None if offsets is None else _ints(offsets, f"{what}: offsets", self.device, B + 1)
+        if o is None and B and n % B:
+            raise QwError(1, f"{what}: without offsets the tokens must be as many for each sequence")
+        return (n, B, None if o is None else o.data_ptr(), s.data_ptr(), t.data_ptr(), stride, W), (t, s, o)
+
+    def _rows(self, t, what: str):
+        """New rows [n, Hkv, D] of any token and head strides: (tensor, n, token stride, head stride)."""
+        torch = _torch()
+        if t.dim() != 3 or t.shape[1] != self.n_kv_heads or t.shape[2] != self.head_dim or \
+                t.dtype is not torch.float16 or t.device != self.device:
+            raise QwError(1, f"{what} must be [n, {self.n_kv_heads}, {self.head_dim}] fp16 on {self.device}")
+        if t.stride(2) != 1 or t.stride(0) % 4 or t.stride(1) % 4 or t.data_ptr() % 8:
+            t = t.clone(memory_format=torch.contiguous_format)
+        return t, t.shape[0], t.stride(0), t.stride(1)
+
+    def update(self, keys, values, table, starts, offsets=None) -> None:
+        """New tokens ``keys``, ``values`` [n, Hkv, D] fp16 into their pages: those of sequence b,
+        ``offsets[b]`` .. ``offsets[b + 1]`` - 1 (int32 [B + 1]; None: n / B each), to positions
+        ``starts[b]`` .. (int32 [B])."""
+        k, n, kt, kh = self._rows(keys, "update: keys")
+        v, nv, vt, vh = self._rows(values, "update: values")
+        if nv != n:
+            raise QwError(1, "update: keys and values must be as many")
+        args, _keep = self._seqs(n, table, starts, offsets, "update")
+        _check(lib().qw_paged_update(self._h, k.data_ptr(), v.data_ptr(), kt, kh, vt, vh, *args, _stream(self.device)))
+
+    def gather(self, table, starts, n: int, offsets=None):
+        """The tokens at those positions back: (keys, values) [n, Hkv, D] fp16, zeros where a
+        position has no page."""
+        args, _keep = self._seqs(n, table, starts, offsets, "gather")
+        shape = (n, self.n_kv_heads, self.head_dim)
+        k, v = (_torch().empty(shape, dtype=_torch().float16, device=self.device) for _ in range(2))
+        _check(lib().qw_paged_gather(self._h, k.data_ptr(), v.data_ptr(), *args, _stream(self.device)))
+        return k, v
+
+    # -- attention
+    def _query(self, q, table, lengths, what: str):
+        torch = _torch()
+        if q.dim() != 4 or q.shape[3] != self.head_dim or q.dtype is not torch.float16 or q.device != self.device:
+            raise QwError(1, f"{what}: q must be [B, Hq, L, {self.head_dim}] fp16 on {self.device}")
+        if q.stride(3) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.stride(2) % 8 or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+        t, B, W, stride = _table(table, self.device, what)
+        if q.shape[0] != B:
+            raise QwError(1, f"{what}: q and table must have as many sequences")
+        n = _ints(lengths, f"{what}: lengths", self.device, B)
+        return (q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), B, q.shape[1], q.shape[2], n.data_ptr(),
+                t.data_ptr(), stride, W), (q, t, n)
+
+    def attention(self, q, table, lengths, scale: float, picked=None):
+        """Attention of each sequence's newest L tokens ``q`` [B, Hq, L, D] over its first
+        ``lengths[b]`` keys (int32 [B], the newest among them), causal among the last L; ``picked``
+        ([B, Hkv, n] int32, as :meth:`select_pages` gives): over those pages alone. Returns [B, Hq, L, D]."""
+        torch = _torch()
+        args, keep = self._query(q, table, lengths, "attention")
+        n = 0
+        if picked is not None:
+            if picked.dim() != 3 or picked.shape[0] != args[4] or picked.shape[1] != self.n_kv_heads or \
+                    picked.shape[2] < 1 or picked.dtype is not torch.int32 or picked.device != self.device:
+                raise QwError(1, f"attention: picked must be [B, {self.n_kv_heads}, n] int32 on {self.device}")
+            picked = picked.contiguous()
+            n = picked.shape[2]
+        out = torch.empty(keep[0].shape, dtype=torch.float16, device=self.device)
+        _check(lib().qw_paged_attention(self._h, *args, None if picked is None else picked.data_ptr(), n, float(scale),
+                                        out.data_ptr(), _stream(self.device)))
+        return out
