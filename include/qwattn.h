@@ -584,6 +584,41 @@ int qw_paged_attention(qw_paged_cache* cache, const void* q, int64_t q_seq_strid
                        const int32_t* table, int64_t table_stride, int table_width, const int32_t* picked,
                        int n_picked, float scale, void* out, void* stream);
 
+/* The pages that each KV head reads for those queries (arguments as qw_paged_attention): the first `sink`
+ * and the last `recent` of its sequence's pages and, of the others, those of the largest score, equal ones by the
+ * lower page, `budget` in all; all pages where there are no more.
+ *   score(page) = top * max over the head's rows of sum_d max(q_d hi_d, q_d lo_d), in whole numbers
+ *     but for one product in fp32: top the largest magnitude of the page's keys, hi_d = ceil(max_d * (127 / top))
+ *     and lo_d = floor(min_d * (127 / top)) the bounds kept by qw_paged_update, within -127 .. 127, q_d =
+ *     rint(q * (127 / largest |q| of the head's rows)); factors in fp32
+ *   picked [n_seq][n_kv_heads][budget] int32: ascending columns of the table row, -1 behind the last
+ * Entries of the table that name no page score below every other. q finite. sink + recent <= budget; a
+ * table of at most 65536 columns. */
+int qw_paged_select(qw_paged_cache* cache, const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                    int64_t q_row_stride, int n_seq, int n_q_heads, int n_rows, const int32_t* lengths,
+                    const int32_t* table, int64_t table_stride, int table_width, int budget, int sink, int recent,
+                    int32_t* picked, void* stream);
+
+/* Rotary positions of several axes, for tokens of images and video: as qw_fused_rope_qk_append, but
+ * each token has a position on each axis and each pair turns by one axis:
+ *   pair p of a head's first rope_dims dims, (p, p + rope_dims / 2) or (2p, 2p + 1) if traditional, turns by
+ *   positions[axes[p]][token] * rope_scale * rope_base^(-2 p / rope_dims), the angle in 64 bits
+ *   qkv [n_tokens][(n_q_heads + 2 n_kv_heads) head_dim] fp16, packed
+ *   positions [n_axes][n_tokens] int32 device, row stride in elements; axes [rope_dims / 2] (host)
+ *   q_out [n_tokens][n_q_heads][head_dim], k_out [n_tokens][n_kv_heads][head_dim] fp16; dims
+ *     behind rope_dims are copied, v stays where it is
+ * head_dim even; rope_dims even, at most head_dim and 512. n_tokens = 0: nothing happens. */
+int qw_rope_axes(const void* qkv, int n_tokens, int n_q_heads, int n_kv_heads, int head_dim, int rope_dims,
+                 int traditional, float rope_base, float rope_scale, const int32_t* positions,
+                 int64_t positions_stride, int n_axes, const uint8_t* axes, void* q_out, void* k_out, void* stream);
+
+/* qw_rope_axes, then qw_paged_update of the rotated keys and the projection's values; the rotated q to q_out. */
+int qw_paged_rope_update(qw_paged_cache* cache, const void* qkv, int n_q_heads, int rope_dims, int traditional,
+                         float rope_base, float rope_scale, const int32_t* positions, int64_t positions_stride,
+                         int n_axes, const uint8_t* axes, void* q_out, int n_tokens, int n_seq, const int32_t* offsets,
+                         const int32_t* starts, const int32_t* table, int64_t table_stride, int table_width,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

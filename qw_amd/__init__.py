@@ -18,8 +18,9 @@ and the tests use the reference's names:
   :meth:`KVCache.attention_general` take the same options over a cache.
 * :meth:`KVCache.shared_attention`, :meth:`KVCache.attention_scored` (with their
   update forms) and :meth:`KVCache.evict` have no counterpart in the reference.
-* :class:`PagedKVCache` (``qw_amd/paged.py``): many sequences in pages of one pool,
-  beyond the reference's full-attention path too.
+* :class:`PagedKVCache` and :func:`rope_axes` (``qw_amd/paged.py``): many sequences in
+  pages of one pool and rotary positions of several axes, beyond the reference's
+  full-attention path too.
 
 Torch is used only to hold device memory and to name the current stream.
 Tensors follow the reference's layouts: ``[1, H, L, D]`` (the batch of 1 may
@@ -35,7 +36,7 @@ __all__ = ["KVCacheMode", "KVCache", "QwError", "attention", "causal_attention",
            "sparse_attention", "sparse_attention_with",
            "fused_rope_qk_append", "dlsa_select", "dlsa_select_with", "turbo4_codebook",
            "turbo4_signs",
-           "PagedKVCache", "release_workspaces", "lib", "LIB_PATH"]
+           "PagedKVCache", "rope_axes", "release_workspaces", "lib", "LIB_PATH"]
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libqwattn.so")
 _lib = None
@@ -98,6 +99,10 @@ _SIGNATURES = {
     "qw_paged_update": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _i, _i, _p, _p, _p, _i64, _i, _p]),
     "qw_paged_gather": (_i, [_p, _p, _p, _i, _i, _p, _p, _p, _i64, _i, _p]),
     "qw_paged_attention": (_i, [_p, _p, _i64, _i64, _i64, _i, _i, _i, _p, _p, _i64, _i, _p, _i, _f, _p, _p]),
+    "qw_paged_select": (_i, [_p, _p, _i64, _i64, _i64, _i, _i, _i, _p, _p, _i64, _i, _i, _i, _i, _p, _p]),
+    "qw_rope_axes": (_i, [_p, _i, _i, _i, _i, _i, _i, _f, _f, _p, _i64, _i, ctypes.c_char_p, _p, _p, _p]),
+    "qw_paged_rope_update": (_i, [_p, _p, _i, _i, _i, _f, _f, _p, _i64, _i, ctypes.c_char_p, _p, _i, _i, _p, _p, _p,
+                                  _i64, _i, _p]),
     "qw_kv_trim": (_i, [_p, _i, ctypes.POINTER(_i)]),
     "qw_kv_dlsa_attention": (_i, [_p, _p, _i, _i, _p, _p, _i, _f, _p, _p]),
     "qw_kv_update_and_dlsa_attention": (_i, [_p, _p, _i, _i, _p, _p, _p, _p, _i, _f, _p, _p]),
@@ -914,4 +919,4 @@ def turbo4_signs(length: int, seed: int):
     return out
 
 
-from .paged import PagedKVCache  # noqa: E402  (it takes the helpers above)
+from .paged import PagedKVCache, rope_axes  # noqa: E402  (it takes the helpers above)

@@ -594,4 +594,34 @@ int qw_paged_attention(qw_paged_cache* cache, const void* q, int64_t q_seq_strid
                                    picked, n_picked, scale, out, (hipStream_t)stream));
 }
 
+int qw_paged_select(qw_paged_cache* cache, const void* q, int64_t q_seq_stride, int64_t q_head_stride,
+                    int64_t q_row_stride, int n_seq, int n_q_heads, int n_rows, const int32_t* lengths,
+                    const int32_t* table, int64_t table_stride, int table_width, int budget, int sink, int recent,
+                    int32_t* picked, void* stream) {
+    QW_PAGED_HANDLE(cache);
+    QW_GUARDED(qw::paged_select(cache->impl,
+                                paged_query(q, q_seq_stride, q_head_stride, q_row_stride, n_seq, n_q_heads, n_rows,
+                                            lengths, table, table_stride, table_width),
+                                budget, sink, recent, picked, (hipStream_t)stream));
+}
+
+int qw_rope_axes(const void* qkv, int n_tokens, int n_q_heads, int n_kv_heads, int head_dim, int rope_dims,
+                 int traditional, float rope_base, float rope_scale, const int32_t* positions,
+                 int64_t positions_stride, int n_axes, const uint8_t* axes, void* q_out, void* k_out, void* stream) {
+    const qw::RopeAxes r{positions, positions_stride, n_axes, axes, rope_dims, traditional, rope_base, rope_scale};
+    QW_GUARDED(qw::rope_axes(r, qkv, n_tokens, n_q_heads, n_kv_heads, head_dim, q_out, k_out, (hipStream_t)stream));
+}
+
+int qw_paged_rope_update(qw_paged_cache* cache, const void* qkv, int n_q_heads, int rope_dims, int traditional,
+                         float rope_base, float rope_scale, const int32_t* positions, int64_t positions_stride,
+                         int n_axes, const uint8_t* axes, void* q_out, int n_tokens, int n_seq, const int32_t* offsets,
+                         const int32_t* starts, const int32_t* table, int64_t table_stride, int table_width,
+                         void* stream) {
+    QW_PAGED_HANDLE(cache);
+    const qw::RopeAxes r{positions, positions_stride, n_axes, axes, rope_dims, traditional, rope_base, rope_scale};
+    QW_GUARDED(qw::paged_rope_update(cache->impl, r, qkv, n_q_heads, q_out,
+                                     paged_seqs(n_tokens, n_seq, offsets, starts, table, table_stride, table_width),
+                                     (hipStream_t)stream));
+}
+
 }  // extern "C"

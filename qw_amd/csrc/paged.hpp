@@ -79,6 +79,23 @@ int check_query(const PagedCache& c, const PagedQuery& q, const char* what);
 int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, int n_picked, float scale, void* out,
                     hipStream_t stream);
 
+// The budget pages of each sequence and KV head that its queries' bounds rank first (paged_select.hip).
+int paged_select(PagedCache& c, const PagedQuery& q, int budget, int sink, int recent, int32_t* picked, hipStream_t stream);
+
+// Rotary positions of several axes (rope_axes.hip): positions [n_axes][n_tokens] (device), the axis of each pair (host).
+struct RopeAxes {
+    const int32_t* positions;
+    int64_t stride;
+    int n_axes;
+    const uint8_t* axes;
+    int rope_dims, traditional;
+    float base, scale;
+};
+int rope_axes(const RopeAxes& r, const void* qkv, int n_tokens, int hq, int hkv, int D, void* q_out, void* k_out,
+              hipStream_t stream);
+int paged_rope_update(PagedCache& c, const RopeAxes& r, const void* qkv, int hq, void* q_out, const PagedSeqs& s,
+                      hipStream_t stream);
+
 // ------------------------------------------------------------------ device
 
 // Inclusive sums over a wave's lanes.

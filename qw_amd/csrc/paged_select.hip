@@ -1,0 +1,303 @@
+// paged_select.hip - which pages of a sequence each KV head reads for its newest tokens.
+//
+// No key of a page scores more than sum_d max(q_d hi_d, q_d lo_d), with hi and lo the page's largest and
+// least key of each dim. The bounds are kept as 8-bit codes over the page's largest magnitude (paged.hpp),
+// q becomes 8-bit codes over its rows' largest magnitude, and the sum is of whole numbers:
+//   score(page) = top(page) * max over rows of sum_d (max(q_d, 0) hi_d + min(q_d, 0) lo_d)
+// with one rounding, so that the picks do not depend on any order of summation. It is a product of
+// matrices of 2 D codes (v_mfma_i32_16x16x64_i8: 16 pages by 16 rows), bound by reading 2 D + 4 bytes a page.
+// A second launch finds the score of the last page that stays, two bits a step over keys held in
+// registers, and writes the picks in ascending order.
+#include <algorithm>
+
+#include "paged.hpp"
+
+namespace qw {
+
+namespace {
+
+typedef int int4v __attribute__((ext_vector_type(4)));
+
+constexpr int kMaxPages = 65536;
+
+struct SelectArgs {
+    PagedView c;
+    const f16* q;
+    int64_t q_seq, q_head, q_row;
+    const int32_t* lengths;
+    const int32_t* table;
+    int64_t table_stride;
+    int width, G, n_rows, R;
+    int budget, sink, recent;
+    int tiles;      // tiles of 16 pages a wave
+    float* scores;  // [n_seq][hkv][width]
+    int32_t* picked;  // [n_seq][hkv][budget]
+};
+
+__device__ __forceinline__ int pages_of(const SelectArgs& a, int b) {
+    const int len = min(max(a.lengths[b], 0), a.width << a.c.lg);
+    return (len + (1 << a.c.lg) - 1) >> a.c.lg;
+}
+
+template <int CTRL>
+__device__ __forceinline__ int dpp_max(int x) {
+    return max(x, __builtin_amdgcn_update_dpp(x, x, CTRL, 0xF, 0xF, false));
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void paged_score_kernel(SelectArgs a) {
+    constexpr int STEPS = D / 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const int h = blockIdx.y, b = blockIdx.z;
+    const int pages = pages_of(a, b);
+    const int first = ((int)blockIdx.x * 4 + wave) * a.tiles * 16;
+    if (pages <= a.budget || first >= pages) return;  // (they all stay; no barrier follows)
+    auto row_at = [&](int tile) {
+        const int row = min(16 * tile + col, a.R - 1);
+        return a.q + b * a.q_seq + (int64_t)(h * a.G + row / a.n_rows) * a.q_head + row % a.n_rows * a.q_row + 16 * g;
+    };
+    const int row_tiles = (a.R + 15) / 16;
+    float big = 0.0f;
+    for (int t = 0; t < row_tiles; t++) {
+        const f16* q = row_at(t);
+#pragma unroll
+        for (int j = 0; j < STEPS; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const half8 x = *(const half8*)(q + 64 * j + 8 * e);
+#pragma unroll
+                for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf((float)x[i]));
+            }
+    }
+    big = wave_reduce(big, [](float x, float y) { return fmaxf(x, y); });
+    const float inv = big > 0.0f ? 127.0f / big : 0.0f;
+    const int last = min(first + a.tiles * 16, pages);
+    float* scores = a.scores + ((int64_t)b * a.c.hkv + h) * a.width;
+    for (int t = 0; t < row_tiles; t++) {
+        const f16* q = row_at(t);
+        int4v up[STEPS], down[STEPS];
+#pragma unroll
+        for (int j = 0; j < STEPS; j++)
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const half4v x = *(const half4v*)(q + 64 * j + 4 * w);
+                uint32_t u = 0, d = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int c = (int)fminf(fmaxf(__builtin_rintf((float)x[i] * inv), -127.0f), 127.0f);
+                    u |= (uint32_t)max(c, 0) << (8 * i);
+                    d |= ((uint32_t)min(c, 0) & 0xFFu) << (8 * i);
+                }
+                up[j][w] = (int)u, down[j][w] = (int)d;
+            }
+        const bool real = 16 * t + col < a.R;
+        for (int p0 = first; p0 < last; p0 += 16) {
+            const int page = a.table[b * a.table_stride + min(p0 + col, pages - 1)];
+            const bool there = (uint32_t)page < (uint32_t)a.c.n_pages;
+            const int64_t ph = (int64_t)(there ? page : 0) * a.c.hkv + h;
+            const int8_t* codes = a.c.codes + ph * 2 * D + 16 * g;
+            const float top = a.c.top[ph];
+            int4v x[2 * STEPS];
+#pragma unroll
+            for (int j = 0; j < 2 * STEPS; j++) x[j] = *(const int4v*)(codes + 64 * j);
+            int4v acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < STEPS; j++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[j], up[j], acc, 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < STEPS; j++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[STEPS + j], down[j], acc, 0, 0, 0);
+            // pages p0 + 4 g + i: the largest of the 16 rows
+            int best[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                int m = real ? acc[i] : INT32_MIN;
+                m = dpp_max<0xB1>(m);
+                m = dpp_max<0x4E>(m);
+                m = dpp_max<0x124>(m);
+                best[i] = dpp_max<0x128>(m);
+            }
+            // lane col writes page p0 + col: its rows' largest lie in lanes 16 (col / 4) ..
+            const int from = 16 * (col >> 2);
+            const int b0 = __shfl(best[0], from), b1 = __shfl(best[1], from), b2 = __shfl(best[2], from), b3 = __shfl(best[3], from);
+            const int m = col & 2 ? (col & 1 ? b3 : b2) : (col & 1 ? b1 : b0);
+            if (g == 0 && p0 + col < last) {
+                float s = there ? top * (float)m + 0.0f : -INFINITY;  // (-0 becomes 0)
+                if (t > 0) s = fmaxf(s, scores[p0 + col]);
+                scores[p0 + col] = s;
+            }
+        }
+    }
+}
+
+// Whole numbers that order as the scores do; 0 for no page.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+template <int NT, int KPT>
+__global__ __launch_bounds__(NT) void paged_pick_kernel(SelectArgs a) {
+    constexpr int NW = NT / 64;
+    __shared__ uint32_t sm[2][NW][4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int h = blockIdx.x, b = blockIdx.y;
+    const int n = pages_of(a, b);
+    int32_t* picked = a.picked + ((int64_t)b * a.c.hkv + h) * a.budget;
+    if (n <= a.budget) {
+        for (int i = threadIdx.x; i < a.budget; i += NT) picked[i] = i < n ? i : -1;
+        return;
+    }
+    const float* scores = a.scores + ((int64_t)b * a.c.hkv + h) * a.width;
+    const int lo = a.sink, hi = n - a.recent;
+    const uint32_t need = (uint32_t)(a.budget - a.sink - a.recent);
+    const int first = wave * 64 * KPT + lane;
+    uint32_t key[KPT], least = ~0u, most = 0;
+#pragma unroll
+    for (int i = 0; i < KPT; i++) {
+        const int p = first + 64 * i;
+        const bool in = p >= lo && p < hi;
+        key[i] = in ? ordered(scores[p]) : 0u;
+        if (in) least = min(least, key[i]), most = max(most, key[i]);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        least = min(least, (uint32_t)__shfl_xor((int)least, d));
+        most = max(most, (uint32_t)__shfl_xor((int)most, d));
+    }
+    if (lane == 0) sm[0][wave][0] = least, sm[0][wave][1] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; w++) least = min(least, sm[0][w][0]), most = max(most, sm[0][w][1]);
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+    // the largest value that `need` keys reach: bits above the highest that differs are common to all
+    uint32_t cut = ~0u;
+    if (need > 0) {
+        const int top = least == most ? 0 : 32 - __builtin_clz(least ^ most);  // bits to find
+        int shift = (top + 1) & ~1;
+        cut = shift >= 32 ? 0u : most >> shift << shift;
+        int turn = 1;
+        while (shift > 0) {
+            shift -= 2;
+            const uint32_t t1 = cut | 1u << shift, t2 = cut | 2u << shift, t3 = cut | 3u << shift;
+            uint32_t c1 = 0, c2 = 0, c3 = 0;  // a lane's, then the wave's
+#pragma unroll
+            for (int i = 0; i < KPT; i++) {
+                c1 += key[i] >= t1;
+                c2 += key[i] >= t2;
+                c3 += key[i] >= t3;
+            }
+            // (a lane counts 64 at most, so that two sums share a register)
+            uint32_t c12 = c1 | c2 << 16;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                c12 += (uint32_t)__shfl_xor((int)c12, d);
+                c3 += (uint32_t)__shfl_xor((int)c3, d);
+            }
+            c1 = c12 & 0xFFFFu, c2 = c12 >> 16;
+            if (lane == 0) sm[turn][wave][0] = c1, sm[turn][wave][1] = c2, sm[turn][wave][2] = c3;
+            __syncthreads();
+            c1 = c2 = c3 = 0;
+#pragma unroll
+            for (int w = 0; w < NW; w++) c1 += sm[turn][w][0], c2 += sm[turn][w][1], c3 += sm[turn][w][2];
+            cut = c3 >= need ? t3 : c2 >= need ? t2 : c1 >= need ? t1 : cut;
+            cut = __builtin_amdgcn_readfirstlane(cut);
+            turn ^= 1;
+        }
+    }
+    // those above the cut, the protected ones, and of the equal ones the first that there is room for
+    uint32_t above = 0, equal = 0, higher = 0;
+#pragma unroll
+    for (int i = 0; i < KPT; i++) {
+        const int p = first + 64 * i;
+        const bool kept = p < n && (p < lo || p >= hi), more = need > 0 && key[i] > cut;
+        above += kept || more;
+        higher += more;
+        equal += need > 0 && key[i] == cut;
+    }
+    uint32_t both = above | equal << 16;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        both += (uint32_t)__shfl_xor((int)both, d);
+        higher += (uint32_t)__shfl_xor((int)higher, d);
+    }
+    above = both & 0xFFFFu, equal = both >> 16;
+    __syncthreads();  // (the steps' counts are read)
+    if (lane == 0) sm[0][wave][0] = above, sm[0][wave][1] = equal, sm[0][wave][2] = higher;
+    __syncthreads();
+    uint32_t room = need;
+#pragma unroll
+    for (int w = 0; w < NW; w++) room -= sm[0][w][2];
+    uint32_t at = 0, ties = 0;
+    for (int w = 0; w < wave; w++) {
+        const uint32_t e = sm[0][w][1], take = ties < room ? min(e, room - ties) : 0u;
+        at += sm[0][w][0] + take;
+        ties += e;
+    }
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < KPT; i++) {
+        const int p = first + 64 * i;
+        const bool tie = need > 0 && key[i] == cut;
+        const uint64_t tied = __ballot(tie);
+        const bool in = (p < n && (p < lo || p >= hi)) || (need > 0 && key[i] > cut) ||
+                        (tie && ties + (uint32_t)__builtin_popcountll(tied & below) < room);
+        const uint64_t all = __ballot(in);
+        if (in) picked[at + (uint32_t)__builtin_popcountll(all & below)] = p;
+        at += (uint32_t)__builtin_popcountll(all);
+        ties += (uint32_t)__builtin_popcountll(tied);
+        if (KPT > 8) __builtin_amdgcn_sched_barrier(0);  // (masks of all steps at once spill)
+    }
+}
+
+}  // namespace
+
+int paged_select(PagedCache& c, const PagedQuery& q, int budget, int sink, int recent, int32_t* picked, hipStream_t stream) {
+    if (int rc = check_query(c, q, "paged select")) return rc;
+    QW_REQUIRE(budget > 0 && sink >= 0 && recent >= 0 && (int64_t)sink + recent <= budget, QW_ERR_INVALID_ARGUMENT,
+               "paged select: budget > 0 and sink + recent <= budget, neither negative, expected");
+    QW_REQUIRE((int64_t)budget * c.page_size <= 0x7fffff00, QW_ERR_INVALID_ARGUMENT, "paged select: budget * page_size < 2^31 expected");
+    QW_REQUIRE(q.table_width <= kMaxPages, QW_ERR_UNSUPPORTED, "paged select: at most 65536 pages a sequence");
+    if (q.n_seq == 0) return QW_OK;
+    QW_REQUIRE(picked, QW_ERR_INVALID_ARGUMENT, "paged select: null picked");
+    QW_REQUIRE(stream != hipStreamPerThread, QW_ERR_UNSUPPORTED, "paged select: hipStreamPerThread; name a stream");
+    DeviceGuard dg(c.device);
+    QW_REQUIRE(dg.ok, QW_ERR_HIP, "paged select: hipSetDevice failed");
+    SelectArgs a{};
+    a.c = c.view;
+    a.q = (const f16*)q.q;
+    a.q_seq = q.seq_stride, a.q_head = q.head_stride, a.q_row = q.row_stride;
+    a.lengths = q.lengths;
+    a.table = q.table;
+    a.table_stride = q.table_stride;
+    a.width = q.table_width;
+    a.G = q.n_q_heads / c.hkv;
+    a.n_rows = q.n_rows;
+    a.R = a.G * q.n_rows;
+    a.budget = budget, a.sink = sink, a.recent = recent;
+    a.picked = picked;
+    if (q.table_width > budget) {
+        void* ws = nullptr;
+        if (int rc = workspace(kWsPagedScores, c.device, stream, (size_t)q.n_seq * c.hkv * q.table_width * 4, &ws)) return rc;
+        a.scores = (float*)ws;
+        // tiles of 16 pages: one a wave while that leaves CUs idle, else up to four (q's codes form once a wave)
+        const int64_t tiles = (int64_t)(q.table_width + 15) / 16 * c.hkv * q.n_seq;
+        a.tiles = (int)std::max<int64_t>(1, std::min<int64_t>(4, tiles / 4096));
+        const dim3 grid((unsigned)((q.table_width + 64 * a.tiles - 1) / (64 * a.tiles)), c.hkv, q.n_seq);
+        if (c.D == 256)
+            hipLaunchKernelGGL(paged_score_kernel<256>, grid, dim3(256), 0, stream, a);
+        else
+            hipLaunchKernelGGL(paged_score_kernel<128>, grid, dim3(256), 0, stream, a);
+        QW_HIP_CHECK(hipGetLastError());
+    }
+    const dim3 grid(c.hkv, q.n_seq);
+    if (q.table_width <= 1024)
+        hipLaunchKernelGGL((paged_pick_kernel<256, 4>), grid, dim3(256), 0, stream, a);
+    else if (q.table_width <= 8192)
+        hipLaunchKernelGGL((paged_pick_kernel<1024, 8>), grid, dim3(1024), 0, stream, a);
+    else
+        hipLaunchKernelGGL((paged_pick_kernel<1024, 64>), grid, dim3(1024), 0, stream, a);
+    QW_HIP_CHECK(hipGetLastError());
+    return QW_OK;
+}
+
+}  // namespace qw

@@ -272,6 +272,8 @@ enum Workspace {
     kWsSelect,   // an eviction's digit counts (evict.hip)
     kWsEvict,    // the rows that an eviction in place moves (evict.hip)
     kWsPaged,    // partials of attention over pages (paged_attend.hip)
+    kWsPagedScores,  // the pages' scores (paged_select.hip)
+    kWsPagedKeys,    // rotated keys on their way into pages (rope_axes.hip)
     kWorkspaces
 };
 int workspace(Workspace kind, int device, hipStream_t stream, size_t need, void** out);

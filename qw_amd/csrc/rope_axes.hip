@@ -1,0 +1,150 @@
+// rope_axes.hip - rotary positions of several axes (time, height, width) for packed tokens.
+//
+// Pair p of a head's first rope_dims dims turns by positions[axes[p]][token] * scale * base^(-p / half):
+//   r1 = x1 cos - x2 sin,  r2 = x1 sin + x2 cos
+// with the angle reduced in 64 bits (turns modulo one), so that far positions keep theirs: in fp32 a
+// position of 10^6 is off by up to 0.06 radians. A workgroup forms its tokens' cosines and sines once, in
+// LDS, for all heads; then it is a copy, bound by reading and writing q and k.
+#include <algorithm>
+#include <cmath>
+
+#include "paged.hpp"
+#include "rope.hpp"
+
+namespace qw {
+
+namespace {
+
+constexpr int kMaxHalf = 256;   // pairs
+constexpr int kAngles = 2048;   // (cos, sin) of a workgroup
+
+struct RopeAxesArgs {
+    const f16* qkv;
+    f16* q_out;
+    f16* k_out;
+    const int32_t* positions;
+    int64_t stride;  // of an axis
+    int n, hq, hkv, D, half, traditional, tokens;  // tokens of a workgroup
+    double log2_base, scale;  // scale over 2 pi
+    uint8_t axes[kMaxHalf];
+};
+
+// VEC: 8 dims a thread (head_dim and half multiples of 8), else one.
+template <bool VEC>
+__global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
+    __shared__ float2 sm[kAngles];
+    const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.n - t0);
+    for (int p = threadIdx.x % 64; p < a.half; p += 64) {
+        const double f = exp2(-((double)p / a.half) * a.log2_base) * a.scale;
+        const int32_t* pos = a.positions + a.axes[p] * a.stride + t0;
+        for (int t = threadIdx.x / 64; t < nt; t += 4) {
+            double x = (double)pos[t] * f;
+            x -= rint(x);
+            float s, c;
+            sincospif(2.0f * (float)x, &s, &c);
+            sm[t * a.half + p] = float2{c, s};
+        }
+    }
+    __syncthreads();
+    constexpr int N = VEC ? 8 : 1;
+    const int per = a.D / N, heads = a.hq + a.hkv, R = 2 * a.half;
+    const int total = nt * heads * per;
+    for (int i = threadIdx.x; i < total; i += 256) {
+        const int d = i % per * N, row = i / per, t = row / heads, h = row - t * heads;
+        const int64_t token = t0 + t;
+        const f16* in = a.qkv + (token * (heads + a.hkv) + h) * a.D;
+        f16* out = h < a.hq ? a.q_out + (token * a.hq + h) * a.D : a.k_out + (token * a.hkv + h - a.hq) * a.D;
+        alignas(16) f16 x[N], y[N];
+        if constexpr (VEC)
+            *(half8*)x = *(const half8*)(in + d);
+        else
+            x[0] = in[d];
+        if (d >= R) {
+#pragma unroll
+            for (int e = 0; e < N; e++) y[e] = x[e];
+        } else {
+            const bool first = a.traditional ? true : d < a.half;
+            alignas(16) f16 z[N];  // the other dims of its pairs
+            if (a.traditional) {
+#pragma unroll
+                for (int e = 0; e < N; e++) z[e] = VEC ? x[e ^ (N > 1)] : in[d ^ 1];
+            } else if constexpr (VEC) {
+                *(half8*)z = *(const half8*)(in + (first ? d + a.half : d - a.half));
+            } else {
+                z[0] = in[first ? d + a.half : d - a.half];
+            }
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const bool one = a.traditional ? ((d + e) & 1) == 0 : first;
+                const int p = a.traditional ? (d + e) >> 1 : first ? d + e : d + e - a.half;
+                const float2 cs = sm[t * a.half + p];
+                float r1, r2;
+                rope_rot((float)(one ? x[e] : z[e]), (float)(one ? z[e] : x[e]), cs.x, cs.y, r1, r2);
+                y[e] = (f16)(one ? r1 : r2);
+            }
+        }
+        if constexpr (VEC)
+            *(half8*)(out + d) = *(const half8*)y;
+        else
+            out[d] = y[0];
+    }
+}
+
+}  // namespace
+
+int rope_axes(const RopeAxes& r, const void* qkv, int n_tokens, int hq, int hkv, int D, void* q_out, void* k_out,
+              hipStream_t stream) {
+    QW_REQUIRE(n_tokens >= 0 && n_tokens <= (1 << 28) && hq > 0 && hkv > 0 && D > 0 && (int64_t)hq + 2 * (int64_t)hkv <= (1 << 24) / D,
+               QW_ERR_INVALID_ARGUMENT, "rope axes: 0 .. 2^28 tokens, n_q_heads, n_kv_heads and head_dim > 0, a row of at most 2^24 values expected");
+    QW_REQUIRE(r.rope_dims > 0 && r.rope_dims % 2 == 0 && r.rope_dims <= D && r.rope_dims <= 2 * kMaxHalf && D % 2 == 0,
+               QW_ERR_INVALID_ARGUMENT, "rope axes: rope_dims even, positive, at most head_dim and 512, head_dim even");
+    QW_REQUIRE(r.base > 0.0f && std::isfinite(r.base) && std::isfinite(r.scale), QW_ERR_INVALID_ARGUMENT,
+               "rope axes: a finite base > 0 and a finite scale expected");
+    QW_REQUIRE(r.n_axes > 0 && r.axes && r.stride >= n_tokens, QW_ERR_INVALID_ARGUMENT,
+               "rope axes: n_axes > 0, an axis for each pair, and a positions stride of n_tokens at least expected");
+    RopeAxesArgs a{};
+    for (int p = 0; p < r.rope_dims / 2; p++) {
+        QW_REQUIRE(r.axes[p] < r.n_axes, QW_ERR_INVALID_ARGUMENT, "rope axes: a pair's axis is not below n_axes");
+        a.axes[p] = r.axes[p];
+    }
+    if (n_tokens == 0) return QW_OK;
+    QW_REQUIRE(qkv && q_out && k_out && r.positions, QW_ERR_INVALID_ARGUMENT, "rope axes: null qkv/positions/output");
+    a.qkv = (const f16*)qkv;
+    a.q_out = (f16*)q_out;
+    a.k_out = (f16*)k_out;
+    a.positions = r.positions;
+    a.stride = r.stride;
+    a.n = n_tokens, a.hq = hq, a.hkv = hkv, a.D = D;
+    a.half = r.rope_dims / 2;
+    a.traditional = r.traditional;
+    a.log2_base = std::log2((double)r.base);
+    a.scale = (double)r.scale / 6.283185307179586476925;
+    // a token a workgroup while there are few, else as many as its angles' place holds, up to 8
+    a.tokens = std::max(1, std::min({8, n_tokens / 1024, kAngles / a.half}));
+    const dim3 grid((unsigned)((n_tokens + a.tokens - 1) / a.tokens));
+    const bool vec = D % 8 == 0 && a.half % 8 == 0 && ((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_out) % 16 == 0;
+    if (vec)
+        hipLaunchKernelGGL(rope_axes_kernel<true>, grid, dim3(256), 0, stream, a);
+    else
+        hipLaunchKernelGGL(rope_axes_kernel<false>, grid, dim3(256), 0, stream, a);
+    QW_HIP_CHECK(hipGetLastError());
+    return QW_OK;
+}
+
+int paged_rope_update(PagedCache& c, const RopeAxes& r, const void* qkv, int hq, void* q_out, const PagedSeqs& s,
+                      hipStream_t stream) {
+    if (int rc = check_seqs(c, s, "paged rope update")) return rc;
+    QW_REQUIRE((uintptr_t)qkv % 8 == 0, QW_ERR_INVALID_ARGUMENT, "paged rope update: qkv 8-byte aligned expected");
+    QW_REQUIRE(stream != hipStreamPerThread, QW_ERR_UNSUPPORTED, "paged rope update: hipStreamPerThread; name a stream");
+    DeviceGuard dg(c.device);
+    QW_REQUIRE(dg.ok, QW_ERR_HIP, "paged rope update: hipSetDevice failed");
+    if (s.n_tokens == 0) return rope_axes(r, qkv, 0, hq, c.hkv, c.D, q_out, nullptr, stream);
+    // the rotated keys pass through a workspace on their way into the pages
+    void* k = nullptr;
+    if (int rc = workspace(kWsPagedKeys, c.device, stream, (size_t)s.n_tokens * c.hkv * c.D * sizeof(f16), &k)) return rc;
+    if (int rc = rope_axes(r, qkv, s.n_tokens, hq, c.hkv, c.D, q_out, k, stream)) return rc;
+    const int64_t row = (int64_t)(hq + 2 * c.hkv) * c.D;
+    return paged_update(c, k, (const f16*)qkv + (int64_t)(hq + c.hkv) * c.D, (int64_t)c.hkv * c.D, c.D, row, c.D, s, stream);
+}
+
+}  // namespace qw

@@ -7,6 +7,7 @@ sequence, anything outside the pool (-1) where it has none.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 from . import KVCacheMode, QwError, _check, _stream, _torch, lib
 
@@ -28,6 +29,48 @@ def _table(t, device, what: str):
     if W > 1 and t.stride(1) != 1 or B > 1 and t.stride(0) < W:
         t = t.contiguous()
     return t, B, W, t.stride(0) if B > 1 else W
+
+
+@functools.lru_cache(maxsize=64)
+def _axes(sections: tuple, interleaved: bool) -> bytes:
+    """The axis of each pair: runs of the sections' lengths, or the axes in turn, each while it has pairs
+    left, the first for the rest."""
+    n = len(sections)
+    if not 1 <= n <= 8 or any(int(s) != s or s < 0 for s in sections) or not 0 < sum(sections) <= 256:
+        raise QwError(1, "rope_axes: 1 to 8 sections of pairs, none negative, 1 to 256 in all, expected")
+    if not interleaved:
+        return bytes(a for a, s in enumerate(sections) for _ in range(s))
+    return bytes(p % n if p < n * sections[p % n] else 0 for p in range(sum(sections)))
+
+
+def _turned(qkv, positions, sections, width: int, what: str):
+    """Checked (qkv, its tokens, positions, their stride)."""
+    torch = _torch()
+    if qkv.dim() != 2 or qkv.shape[1] != width or qkv.dtype is not torch.float16 or not qkv.is_cuda:
+        raise QwError(1, f"{what}: qkv must be [n, {width}] fp16 on the device")
+    n = qkv.shape[0]
+    if positions.dim() != 2 or positions.shape != (len(sections), n) or positions.dtype is not torch.int32 or \
+            positions.device != qkv.device:
+        raise QwError(1, f"{what}: positions must be [{len(sections)}, {n}] int32 on {qkv.device}")
+    if n > 1 and positions.stride(1) != 1 or len(sections) > 1 and positions.stride(0) < n:
+        positions = positions.contiguous()
+    return qkv.contiguous(), n, positions, positions.stride(0) if len(sections) > 1 else n
+
+
+def rope_axes(qkv, positions, sections, n_q_heads: int, n_kv_heads: int, head_dim: int, rope_base: float,
+              rope_scale: float = 1.0, interleaved: bool = False, traditional: bool = False):
+    """Rotary positions of several axes (time, height, width) out of the packed projection ``qkv``
+    [n, (Hq + 2 Hkv) D] fp16: ``positions`` [axes, n] int32, ``sections`` the pairs of each axis
+    (2 * their sum dims of a head turn), one run after another or, ``interleaved``, in turn. Returns
+    (q [n, Hq, D], k [n, Hkv, D]), rotated; the values stay in ``qkv``."""
+    axes = _axes(tuple(sections), bool(interleaved))
+    x, n, pos, stride = _turned(qkv, positions, sections, (n_q_heads + 2 * n_kv_heads) * head_dim, "rope_axes")
+    q, k = x.new_empty((n, n_q_heads, head_dim)), x.new_empty((n, n_kv_heads, head_dim))
+    with _torch().cuda.device(x.device):
+        _check(lib().qw_rope_axes(x.data_ptr(), n, n_q_heads, n_kv_heads, head_dim, 2 * len(axes), int(traditional),
+                                  float(rope_base), float(rope_scale), pos.data_ptr(), stride, len(sections), axes,
+                                  q.data_ptr(), k.data_ptr(), _stream(x.device)))
+    return q, k
 
 
 class PagedKVCache:
@@ -106,6 +149,21 @@ class PagedKVCache:
         _check(lib().qw_paged_gather(self._h, k.data_ptr(), v.data_ptr(), *args, _stream(self.device)))
         return k, v
 
+    def rope_update(self, qkv, positions, sections, n_q_heads: int, rope_base: float, table, starts, offsets=None,
+                    rope_scale: float = 1.0, interleaved: bool = False, traditional: bool = False):
+        """:func:`rope_axes` of the new tokens' projection ``qkv`` [n, (Hq + 2 Hkv) D], its rotated keys and
+        values into their pages as :meth:`update` takes them. Returns q [n, Hq, D], rotated."""
+        axes = _axes(tuple(sections), bool(interleaved))
+        x, n, pos, stride = _turned(qkv, positions, sections, (n_q_heads + 2 * self.n_kv_heads) * self.head_dim, "rope_update")
+        if x.device != self.device:
+            raise QwError(1, f"rope_update: qkv must be on {self.device}")
+        args, _keep = self._seqs(n, table, starts, offsets, "rope_update")
+        q = x.new_empty((n, n_q_heads, self.head_dim))
+        _check(lib().qw_paged_rope_update(self._h, x.data_ptr(), n_q_heads, 2 * len(axes), int(traditional),
+                                          float(rope_base), float(rope_scale), pos.data_ptr(), stride, len(sections),
+                                          axes, q.data_ptr(), *args, _stream(self.device)))
+        return q
+
     # -- attention
     def _query(self, q, table, lengths, what: str):
         torch = _torch()
@@ -137,3 +195,15 @@ class PagedKVCache:
         _check(lib().qw_paged_attention(self._h, *args, None if picked is None else picked.data_ptr(), n, float(scale),
                                         out.data_ptr(), _stream(self.device)))
         return out
+
+    def select_pages(self, q, table, lengths, budget: int, sink: int = 0, recent: int = 0):
+        """The pages that each KV head should read for those queries: the first ``sink``, the last
+        ``recent`` and, of the others, those whose keys' bounds promise the largest scores, ``budget`` in all.
+        Returns [B, Hkv, budget] int32, ascending columns of the table, -1 behind the last."""
+        args, _keep = self._query(q, table, lengths, "select_pages")
+        budget, sink, recent = int(budget), int(sink), int(recent)
+        if not 0 < budget < 2 ** 27 or min(sink, recent) < 0 or sink + recent > budget:  # (before any of them passes an int)
+            raise QwError(1, "select_pages: 0 < budget < 2^27 and sink + recent <= budget, neither negative, expected")
+        picked = _torch().empty((args[4], self.n_kv_heads, budget), dtype=_torch().int32, device=self.device)
+        _check(lib().qw_paged_select(self._h, *args, budget, sink, recent, picked.data_ptr(), _stream(self.device)))
+        return picked

@@ -200,3 +200,39 @@ def test_dlsa_union_line_limits(qwlib):
     assert 0 < f(1, 1, 1 << 20, 1 << 16, 24, 4, 256, 1 << 30) < 1 << 30  # (no overflow on the way)
     assert f(0, 0, 1 << 20, 1 << 20, 16, 1, 64, (1 << 31) - 1) >= 0
     assert f(0, 0, 0, 64, 16, 1, 64, 100) == 0 and f(0, 0, 9999, 64, 17, 1, 64, 100) == 0
+
+
+def test_paged_contract_fails_before_device_work(qwlib):
+    """qw_paged_* and qw_rope_axes: what is refused before any device call."""
+    h = ctypes.c_void_p()
+    create = qwlib.qw_paged_create
+    assert create(0, 64, 2, 128, 4, 64, 0, None) == 1
+    assert create(9, 64, 2, 128, 4, 64, 0, ctypes.byref(h)) == 1
+    assert create(4, 64, 2, 128, 4, 64, 0, ctypes.byref(h)) == 2    # turbo4
+    assert create(0, 64, 0, 128, 4, 64, 0, ctypes.byref(h)) == 1
+    assert create(0, 64, 2, 128, 0, 64, 0, ctypes.byref(h)) == 1
+    assert create(0, 64, 2, 64, 4, 64, 0, ctypes.byref(h)) == 2     # head_dim
+    assert create(2, 32, 2, 128, 4, 64, 0, ctypes.byref(h)) == 2    # group
+    for ps in (0, 8, 24, 512, -16):
+        assert create(0, 64, 2, 128, 4, ps, 0, ctypes.byref(h)) == 2
+    assert not h.value
+    one = ctypes.c_void_p(16)
+    assert qwlib.qw_paged_destroy(None) == 0
+    assert qwlib.qw_paged_nbytes(None, None) == 1
+    assert qwlib.qw_paged_update(None, one, one, 256, 128, 256, 128, 1, 1, None, one, one, 4, 4, None) == 1
+    assert qwlib.qw_paged_gather(None, one, one, 1, 1, None, one, one, 4, 4, None) == 1
+    assert qwlib.qw_paged_attention(None, one, 1024, 128, 128, 1, 8, 1, one, one, 4, 4, None, 0, 0.1, one, None) == 1
+    assert qwlib.qw_paged_select(None, one, 1024, 128, 128, 1, 8, 1, one, one, 4, 4, 2, 0, 0, one, None) == 1
+    assert b"null" in qwlib.qw_last_error()
+
+    def rope(**kw):
+        a = dict(qkv=one, n=4, hq=4, hkv=2, D=128, R=8, base=1e4, scale=1.0, pos=one, stride=4, n_axes=3, axes=bytes([0, 1, 2, 0]))
+        a.update(kw)
+        return qwlib.qw_rope_axes(a["qkv"], a["n"], a["hq"], a["hkv"], a["D"], a["R"], 0, a["base"], a["scale"], a["pos"],
+                                  a["stride"], a["n_axes"], a["axes"], one, one, None)
+
+    assert rope(n=0) == 0  # nothing to do: no launch
+    for kw in (dict(qkv=None), dict(n=-1), dict(hq=0), dict(hkv=-1), dict(D=0), dict(D=127), dict(R=0), dict(R=7), dict(R=130),
+               dict(D=1024, R=514), dict(base=0.0), dict(base=float("inf")), dict(scale=float("nan")), dict(pos=None),
+               dict(stride=3), dict(n_axes=0), dict(n_axes=2), dict(axes=None), dict(hq=2 ** 30)):
+        assert rope(**kw) == 1, kw
