@@ -100,12 +100,13 @@ int paged_rope_update(PagedCache& c, const RopeAxes& r, const void* qkv, int hq,
 
 // Inclusive sums over a wave's lanes.
 __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-    const int lane = (int)__lane_id();
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
+    // within rows of 16 lanes, then the rows' last lanes to the rows behind
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xA, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xC, 0xF, false);
     return x;
 }
 

@@ -71,7 +71,7 @@ __device__ __forceinline__ uint32_t workers_of(const AttendArgs& a, uint64_t tot
 
 // 32 keys' place: of each 16 the pool's page, the slot, and the position of the first; the pages' V exponent.
 struct Place {
-    int page0, page1, slot0, slot1, pos0, pos1, e;
+    int page0, page1, slot0, slot1, pos0, pos1, e0, e1;
 };
 // Tables, picks and exponents are read by scalar loads: a vector load would wait for the keys requested before it.
 typedef const int32_t __attribute__((address_space(4))) * Scalars;
@@ -204,7 +204,10 @@ __global__ __launch_bounds__(256 * RT, D == 256 ? 2 : 3) void paged_attend_kerne
             const int key = (int)(r * kRound) + 32 * kw;
             half_at(key, p.page0, p.slot0, p.pos0);
             half_at(key + 16, p.page1, p.slot1, p.pos1);
-            if (BITS != 16) p.e = max(v_exp[(int64_t)p.page0 * a.c.hkv + h], v_exp[(int64_t)p.page1 * a.c.hkv + h]);
+            if (BITS != 16) {  // (left as they come: a use here would wait for them)
+                p.e0 = v_exp[(int64_t)p.page0 * a.c.hkv + h];
+                p.e1 = v_exp[(int64_t)p.page1 * a.c.hkv + h];
+            }
             return p;
         };
 
@@ -301,7 +304,7 @@ __global__ __launch_bounds__(256 * RT, D == 256 ? 2 : 3) void paged_attend_kerne
                 for (int i = 0; i < D / 16; i++) o[i] *= alpha;
             }
             if constexpr (BITS != 16) {
-                const int e = cur.e;
+                const int e = max(cur.e0, cur.e1);
                 if (e > E) {  // V scales of 1 and more: P gives way, so that P times a scale fits a half
                     const float f = __builtin_amdgcn_exp2f((float)(E - e));
                     E = e;

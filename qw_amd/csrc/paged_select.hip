@@ -128,6 +128,10 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectArgs a) {
     }
 }
 
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(x), 63);
+}
+
 // Whole numbers that order as the scores do; 0 for no page.
 __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t u = __float_as_uint(x);
@@ -150,19 +154,17 @@ __global__ __launch_bounds__(NT) void paged_pick_kernel(SelectArgs a) {
     const int lo = a.sink, hi = n - a.recent;
     const uint32_t need = (uint32_t)(a.budget - a.sink - a.recent);
     const int first = wave * 64 * KPT + lane;
-    uint32_t key[KPT], least = ~0u, most = 0;
+    uint32_t key[KPT];
+    float least_f = INFINITY, most_f = -INFINITY;
 #pragma unroll
     for (int i = 0; i < KPT; i++) {
         const int p = first + 64 * i;
         const bool in = p >= lo && p < hi;
-        key[i] = in ? ordered(scores[p]) : 0u;
-        if (in) least = min(least, key[i]), most = max(most, key[i]);
+        const float s = in ? scores[p] : 0.0f;
+        key[i] = in ? ordered(s) : 0u;
+        if (in) least_f = OpMin()(least_f, s), most_f = OpMax()(most_f, s);
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        least = min(least, (uint32_t)__shfl_xor((int)least, d));
-        most = max(most, (uint32_t)__shfl_xor((int)most, d));
-    }
+    uint32_t least = ordered(wave_reduce(least_f, OpMin())), most = ordered(wave_reduce(most_f, OpMax()));
     if (lane == 0) sm[0][wave][0] = least, sm[0][wave][1] = most;
     __syncthreads();
 #pragma unroll
@@ -179,21 +181,25 @@ __global__ __launch_bounds__(NT) void paged_pick_kernel(SelectArgs a) {
         while (shift > 0) {
             shift -= 2;
             const uint32_t t1 = cut | 1u << shift, t2 = cut | 2u << shift, t3 = cut | 3u << shift;
-            uint32_t c1 = 0, c2 = 0, c3 = 0;  // a lane's, then the wave's
+            uint32_t c1 = 0, c2 = 0, c3 = 0;
+            if constexpr (KPT <= 8) {
 #pragma unroll
-            for (int i = 0; i < KPT; i++) {
-                c1 += key[i] >= t1;
-                c2 += key[i] >= t2;
-                c3 += key[i] >= t3;
-            }
-            // (a lane counts 64 at most, so that two sums share a register)
-            uint32_t c12 = c1 | c2 << 16;
+                for (int i = 0; i < KPT; i++) {
+                    c1 += __builtin_popcountll(__ballot(key[i] >= t1));
+                    c2 += __builtin_popcountll(__ballot(key[i] >= t2));
+                    c3 += __builtin_popcountll(__ballot(key[i] >= t3));
+                }
+            } else {
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                c12 += (uint32_t)__shfl_xor((int)c12, d);
-                c3 += (uint32_t)__shfl_xor((int)c3, d);
+                for (int i = 0; i < KPT; i++) {
+                    c1 += key[i] >= t1;
+                    c2 += key[i] >= t2;
+                    c3 += key[i] >= t3;
+                }
+                c1 = wave_sum(c1 | c2 << 16);  // (a wave counts 4096 at most)
+                c2 = c1 >> 16, c1 &= 0xFFFFu;
+                c3 = wave_sum(c3);
             }
-            c1 = c12 & 0xFFFFu, c2 = c12 >> 16;
             if (lane == 0) sm[turn][wave][0] = c1, sm[turn][wave][1] = c2, sm[turn][wave][2] = c3;
             __syncthreads();
             c1 = c2 = c3 = 0;
@@ -214,13 +220,9 @@ __global__ __launch_bounds__(NT) void paged_pick_kernel(SelectArgs a) {
         higher += more;
         equal += need > 0 && key[i] == cut;
     }
-    uint32_t both = above | equal << 16;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        both += (uint32_t)__shfl_xor((int)both, d);
-        higher += (uint32_t)__shfl_xor((int)higher, d);
-    }
+    const uint32_t both = wave_sum(above | equal << 16);
     above = both & 0xFFFFu, equal = both >> 16;
+    higher = wave_sum(higher);
     __syncthreads();  // (the steps' counts are read)
     if (lane == 0) sm[0][wave][0] = above, sm[0][wave][1] = equal, sm[0][wave][2] = higher;
     __syncthreads();
@@ -290,8 +292,8 @@ int paged_select(PagedCache& c, const PagedQuery& q, int budget, int sink, int r
         QW_HIP_CHECK(hipGetLastError());
     }
     const dim3 grid(c.hkv, q.n_seq);
-    if (q.table_width <= 1024)
-        hipLaunchKernelGGL((paged_pick_kernel<256, 4>), grid, dim3(256), 0, stream, a);
+    if (q.table_width <= 2048)
+        hipLaunchKernelGGL((paged_pick_kernel<256, 8>), grid, dim3(256), 0, stream, a);
     else if (q.table_width <= 8192)
         hipLaunchKernelGGL((paged_pick_kernel<1024, 8>), grid, dim3(1024), 0, stream, a);
     else
