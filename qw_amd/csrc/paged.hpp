@@ -33,7 +33,6 @@ struct PagedView {
     f16* lohi;
     int8_t* codes;
     float* top;
-    int* v_exp;
     int hkv, n_pages, lg;  // page_size = 1 << lg
 };
 

@@ -28,7 +28,7 @@ namespace {
 constexpr int kRound = 128;             // keys of a round: 4 waves of 32
 constexpr float kNone = -0x1p100f;      // a maximum below every score
 constexpr float kLazy = 4.0f;           // scores pass the reference by so much (log2) before it follows
-constexpr float kLift = 11.0f;          // log2 of P at the reference: P <= 2^15 fits a half, and 2^-25 of it too
+constexpr float kLift = 10.0f;          // log2 of P at the reference: P <= 2^14, times a scale below 2, fits a half
 
 struct AttendArgs {
     PagedView c;
@@ -43,103 +43,210 @@ struct AttendArgs {
     int n_picked;
     float scale2;  // scale * log2 e
     int workers;
-    float* part_o;    // [workers][2][hkv][R][D]
-    float2* part_ml;  // [workers][2][hkv][R]
+    float* part_o;    // [2 workers][hkv][R][D]
+    float2* part_ml;  // [2 workers][hkv][R]
 };
 
 // A sequence's keys as the kernel walks them: the whole of it, or its picked pages side by side.
-__device__ __forceinline__ int keys_of(const AttendArgs& a, int b) {
-    const int len = min(max(a.lengths[b], 0), a.width << a.c.lg);
+__device__ __forceinline__ int keys_of(const AttendArgs& a, int len) {
     if (!a.picked) return len;
     const int pages = (len + (1 << a.c.lg) - 1) >> a.c.lg;
     return min(pages, a.n_picked) << a.c.lg;
 }
 __device__ __forceinline__ uint32_t rounds_of(const AttendArgs& a, int b) {
-    return (uint32_t)(keys_of(a, b) + kRound - 1) / kRound;
-}
-__device__ __forceinline__ uint32_t total_rounds(const AttendArgs& a) {
-    const int lane = (int)__lane_id();
-    uint32_t n = 0;
-    for (int b = lane; b < a.n_seq; b += 64) n += rounds_of(a, b);
-    return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
+    return (uint32_t)(keys_of(a, min(max(a.lengths[b], 0), a.width << a.c.lg)) + kRound - 1) / kRound;
 }
 
-// (a round at least for each that works)
-__device__ __forceinline__ uint32_t workers_of(const AttendArgs& a, uint64_t total) {
-    return (uint64_t)a.workers < total ? (uint32_t)a.workers : (uint32_t)total;
-}
-
-// 32 keys' place: of each 16 the pool's page, the slot, and the position of the first; the pages' V exponent.
-struct Place {
-    int page0, page1, slot0, slot1, pos0, pos1, e0, e1;
+// How the rounds are dealt, the same for every wave of a call. Up to 64 sequences (a lane each): pieces of
+// one sequence each, of at most `most` rounds, one a worker, if there is such a length not much above the
+// average; a second piece would begin with its own loads, one behind the other. Else equal runs of all rounds.
+struct Plan {
+    int len;                            // lane b's sequence (up to 64)
+    uint32_t rounds, through;           // its rounds, and all up to it
+    uint32_t total, workers, per, rest; // the first `rest` runs have per + 1 rounds
+    uint32_t most, pieces, last;        // piece by piece: its pieces, and all up to it; else most = 0
 };
-// Tables, picks and exponents are read by scalar loads: a vector load would wait for the keys requested before it.
-typedef const int32_t __attribute__((address_space(4))) * Scalars;
-__device__ __forceinline__ Scalars scalars(const int32_t* p) { return (Scalars)(uintptr_t)p; }
+__device__ __forceinline__ uint32_t wave_last(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
+__device__ __forceinline__ Plan plan_of(const AttendArgs& a) {
+    const int lane = (int)__lane_id();
+    Plan p{};
+    if (a.n_seq <= 64) {
+        if (lane < a.n_seq) {
+            p.len = min(max(a.lengths[lane], 0), a.width << a.c.lg);
+            p.rounds = (uint32_t)(keys_of(a, p.len) + kRound - 1) / kRound;
+        }
+        p.through = wave_scan(p.rounds);
+        p.total = wave_last(p.through);
+    } else {
+        uint32_t n = 0;
+        for (int b = lane; b < a.n_seq; b += 64) n += rounds_of(a, b);
+        p.total = wave_last(wave_scan(n));
+    }
+    p.workers = min((uint32_t)a.workers, p.total);  // (a round at least for each that works)
+    if (p.total == 0) return p;
+    p.per = __builtin_amdgcn_readfirstlane(p.total / p.workers);
+    p.rest = p.total - p.per * p.workers;
+    if (a.n_seq <= 64) {
+        uint32_t most = p.per + (p.rest > 0);
+        for (int i = 0; i < 4; i++, most += 1 + most / 16) {
+            p.pieces = (p.rounds + most - 1) / most;
+            p.last = wave_scan(p.pieces);
+            if (wave_last(p.last) <= (uint32_t)a.workers) {
+                p.most = most;
+                break;
+            }
+        }
+    }
+    return p;
+}
+// Rounds r0 .. r1 - 1 of sequence b's `all`, whose partials have their place; b = -1: none.
+struct Piece {
+    int b, len;
+    uint32_t r0, r1, all, slot;
+};
+// Worker w's piece that begins at round `at` of its run.
+__device__ __forceinline__ Piece piece_of(const AttendArgs& a, uint32_t per, uint32_t rest, uint32_t w, uint32_t at, int b, int len,
+                                          uint32_t all, uint32_t before) {
+    const uint32_t begin = w * per + min(w, rest), end = begin + per + (w < rest);
+    return Piece{b, len, at - before, min(all, end - before), all, 2 * w + (at == before && at != begin ? 1 : 0)};
+}
+__device__ __forceinline__ Piece piece_at(const AttendArgs& a, uint32_t per, uint32_t rest, uint32_t w, uint32_t at) {
+    const PagedUnit u = find_unit(a.n_seq, at, [&](int b) { return rounds_of(a, b); });
+    if (u.b < 0) return Piece{-1, 0, 0, 0, 0, 0};
+    return piece_of(a, per, rest, w, at, u.b, min(max(a.lengths[u.b], 0), a.width << a.c.lg), rounds_of(a, u.b), u.base);
+}
+// Its first piece (piece by piece: its only one); at: the round that it begins with.
+__device__ __forceinline__ Piece first_piece(const AttendArgs& a, const Plan& p, uint32_t w, uint32_t at) {
+    if (a.n_seq > 64) return piece_at(a, p.per, p.rest, w, at);
+    const uint64_t past = __ballot(p.most ? p.last > w : p.through > at);
+    if (!past) return Piece{-1, 0, 0, 0, 0, 0};
+    const int b = __builtin_ctzll(past);
+    const int len = __builtin_amdgcn_readlane(p.len, b);
+    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)p.rounds, b);
+    if (p.most) {
+        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)p.pieces, b);
+        const uint32_t i = w - ((uint32_t)__builtin_amdgcn_readlane((int)p.last, b) - n);
+        const uint32_t each = __builtin_amdgcn_readfirstlane(all / n), more = all - each * n;
+        const uint32_t r0 = i * each + min(i, more);
+        return Piece{b, len, r0, r0 + each + (i < more), all, 2 * w};
+    }
+    return piece_of(a, p.per, p.rest, w, at, b, len, all, (uint32_t)__builtin_amdgcn_readlane((int)p.through, b) - all);
+}
+
+// 32 keys' place: of each 16 the pool's page, the slot, and the position of the first.
+struct Place {
+    int page0, page1, slot0, slot1, pos0, pos1;
+};
+// The places of a wave's keys in 32 rounds, a lane each 16 keys: a round's come by two lane reads. (As scalar loads round
+// by round they shared a counter with the queries' LDS reads, which then waited for them.)
+struct Places {
+    int page, pos;
+};
 constexpr int kNoKey = 0x7fffff00;  // a position behind every key
 
+// Waves a SIMD that the registers are cut for.
+constexpr int waves_of(int bits, int D, int RT) {
+    return D == 256 && RT == 2 ? 1 : bits == 16 && D == 128 && RT == 1 ? 3 : 2;
+}
+
 template <int BITS, int D, bool INT8>
-struct Chunk {
+struct Shape {
     static constexpr int NG = INT8 ? 1 : D / kGroup;
-    static constexpr int NK = D * BITS / 512;      // 16-byte pieces of a K row a lane group
+    static constexpr int NK = D * BITS / 512;               // 16-byte pieces of a K row a lane group
     static constexpr int DPP = BITS == 16 ? 1 : 16 / BITS;  // dims of a V piece
     static constexpr int NV = D / 16 / DPP;
     static constexpr int PAR = INT8 ? 8 : 16 * NG;  // halves of 8 keys' scales and biases
-    u32x4 k[2][NK];
-    u32x4 v[NV];
-    half8 ks[NG], kb[NG], vs[NG], vb;
+    // A wave's 32 keys in LDS, each of its loads' 1 KB as the lanes hold it: K, V, scales and biases.
+    static constexpr int V0 = 2 * NK * 1024, P0 = V0 + NV * 1024, SLOT = P0 + 1024, LOADS = SLOT / 1024;
 };
 
-template <int BITS, int D, bool INT8>
-__device__ __forceinline__ void load_k(Chunk<BITS, D, INT8>& x, const PagedView& c, const Place& p, int h, int lane) {
-    using C = Chunk<BITS, D, INT8>;
-    const int i = lane & 15, g = lane >> 4;
+// One load of 64 times 16 bytes to LDS. M0, which gives the place, is saved and restored so that the compiler's
+// view of it holds; the offset counts for both addresses. The compiler knows nothing of the load: what reads the
+// place waits by wait_loads first.
+template <int OFFSET>
+__device__ __forceinline__ void to_lds(const char* from, uint32_t place) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, off offset:%3\n\t"
+        "s_nop 0\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(from), "s"(__builtin_amdgcn_readfirstlane(place - OFFSET)), "n"(OFFSET)
+        : "memory");
+}
+template <int N, int STEP, int J = 0>
+__device__ __forceinline__ void run_to_lds(const char* from, uint32_t place) {
+    if constexpr (J < N) {
+        to_lds<J * STEP>(from, place + J * 1024);
+        run_to_lds<N, STEP, J + 1>(from, place);
+    }
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // until at most N of the wave's loads are on their way
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ const char* k_row(const PagedView& c, const Place& p, int h, int lane, int row_bytes) {
     const int64_t page = lane & 8 ? p.page1 : p.page0;
-    const int slot = (lane & 8 ? p.slot1 : p.slot0) + 8 * (i >> 2 & 1) + (i & 3);
-    const char* row = c.k + (((page * c.hkv + h) << c.lg) + slot) * (D * BITS / 8) + 16 * g;
+    const int slot = (lane & 8 ? p.slot1 : p.slot0) + 8 * (lane >> 2 & 1) + (lane & 3);
+    return c.k + (((page * c.hkv + h) << c.lg) + slot) * row_bytes + 16 * (lane >> 4);
+}
+// The 8 keys of a lane group: their place among the pool's blocks of 8.
+__device__ __forceinline__ int64_t block_of(const PagedView& c, const Place& p, int h, int g) {
+    const int64_t page = g & 2 ? p.page1 : p.page0;
+    return ((page * c.hkv + h) << (c.lg - 3)) + ((g & 2 ? p.slot1 : p.slot0) >> 3) + (g & 1);
+}
+
+template <int BITS, int D, bool INT8>
+__device__ __forceinline__ void request(const PagedView& c, const Place& p, int h, int lane, uint32_t slot) {
+    using S = Shape<BITS, D, INT8>;
+    constexpr int ROW = D * BITS / 8;
+    const char* row = k_row(c, p, h, lane, ROW);
+    run_to_lds<S::NK, 64>(row, slot);
+    run_to_lds<S::NK, 64>(row + 4 * ROW, slot + S::NK * 1024);
+    run_to_lds<S::NV, 256>(c.v + block_of(c, p, h, lane >> 4) * (D * BITS) + 16 * (lane & 15), slot + S::V0);
+    // K's and V's scales and biases of the 4 blocks, one behind the other (the lanes behind them repeat the last)
+    constexpr int LPB = S::PAR / 8;
+    const int i = min(lane, 8 * LPB - 1), blk = i / LPB & 3;
+    const f16* par = (i < 4 * LPB ? c.k_par : c.v_par) + block_of(c, p, h, blk) * S::PAR;
+    to_lds<0>((const char*)par + i % LPB * 16, slot + S::P0);
+}
+
+// fp16 keys stay in registers.
+template <int D>
+struct Chunk {
+    u32x4 k[2][D / 32];
+    u32x4 v[D / 16];
+};
+template <int D>
+__device__ __forceinline__ void load_k(Chunk<D>& x, const PagedView& c, const Place& p, int h, int lane) {
+    const char* row = k_row(c, p, h, lane, 2 * D);
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int j = 0; j < C::NK; j++) x.k[t][j] = *(const u32x4*)(row + t * 4 * (D * BITS / 8) + 64 * j);
-    if constexpr (BITS != 16) {
-        const int64_t pg = g & 2 ? p.page1 : p.page0;
-        const int blk = ((g & 2 ? p.slot1 : p.slot0) >> 3) + (g & 1);
-        const f16* par = c.k_par + (((pg * c.hkv + h) << (c.lg - 3)) + blk) * C::PAR;
-#pragma unroll
-        for (int m = 0; m < C::NG; m++) {
-            x.ks[m] = *(const half8*)(par + 8 * m);
-            if (!INT8) x.kb[m] = *(const half8*)(par + 8 * (C::NG + m));
-        }
-    }
+        for (int j = 0; j < D / 32; j++) x.k[t][j] = *(const u32x4*)(row + t * 8 * D + 64 * j);
 }
-template <int BITS, int D, bool INT8>
-__device__ __forceinline__ void load_v(Chunk<BITS, D, INT8>& x, const PagedView& c, const Place& p, int h, int lane) {
-    using C = Chunk<BITS, D, INT8>;
-    const int n = lane & 15, g = lane >> 4;
-    const int64_t pg = g & 2 ? p.page1 : p.page0;
-    const int64_t blk = (((pg * c.hkv + h) << (c.lg - 3)) + ((g & 2 ? p.slot1 : p.slot0) >> 3) + (g & 1));
-    const char* at = c.v + blk * (D * BITS) + 16 * n;
+template <int D>
+__device__ __forceinline__ void load_v(Chunk<D>& x, const PagedView& c, const Place& p, int h, int lane) {
+    const char* at = c.v + block_of(c, p, h, lane >> 4) * (D * 16) + 16 * (lane & 15);
 #pragma unroll
-    for (int j = 0; j < C::NV; j++) x.v[j] = *(const u32x4*)(at + 256 * j);
-    if constexpr (BITS != 16) {
-        const f16* par = c.v_par + blk * C::PAR;
-#pragma unroll
-        for (int m = 0; m < C::NG; m++) x.vs[m] = *(const half8*)(par + 8 * m);
-        if (!INT8) x.vb = *(const half8*)(par + 8 * (C::NG + min(n, C::NG - 1)));
-    }
+    for (int j = 0; j < D / 16; j++) x.v[j] = *(const u32x4*)(at + 256 * j);
 }
 
-// 8 codes of a K piece as halves code * 2^-24.
+// 8 codes of a K piece, its step e, as halves code * 2^-24.
 template <int BITS>
-__device__ __forceinline__ half8 k_codes(const u32x4* k, int m) {
+__device__ __forceinline__ half8 k_codes(u32x4 k, int e) {
     if constexpr (BITS == 16) {
-        return as_h8(k[m]);
+        return as_h8(k);
     } else if constexpr (BITS == 8) {
-        const uint32_t w0 = k[m / 2][2 * (m & 1)], w1 = k[m / 2][2 * (m & 1) + 1];
+        const uint32_t w0 = k[2 * e], w1 = k[2 * e + 1];
         return as_h8(u32x4{__builtin_amdgcn_perm(0u, w0, 0x0C010C00u), __builtin_amdgcn_perm(0u, w0, 0x0C030C02u),
                            __builtin_amdgcn_perm(0u, w1, 0x0C010C00u), __builtin_amdgcn_perm(0u, w1, 0x0C030C02u)});
     } else {
-        const uint32_t w = k[m / 4][m & 3], f = 0x000F000Fu;
+        const uint32_t w = k[e], f = 0x000F000Fu;
         return as_h8(u32x4{w & f, w >> 4 & f, w >> 8 & f, w >> 12 & f});
     }
 }
@@ -158,286 +265,431 @@ __device__ __forceinline__ half8 v_codes(u32x4 v, int e) {
     }
 }
 
+// The same number, of which the compiler keeps nothing from one use to the next: what is formed of it costs a few
+// instructions each time, where kept in registers it drove others to memory.
+__device__ __forceinline__ int afresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 __device__ __forceinline__ float4v mfma(half8 a, half8 b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// RT row tiles of 16 in a workgroup, 4 waves each.
+// Columns of a piece's rows that are joined over LDS at a time.
+constexpr int kJoin = 128;
+// Floats of LDS that hold four waves' keys, two chunks each, or their rows being joined [4][rows][kJoin + 4].
+template <int BITS, int D, bool INT8>
+__host__ __device__ constexpr int key_floats(int rows) {
+    const int join = 4 * rows * (kJoin + 4), ring = BITS == 16 ? 0 : 8 * Shape<BITS, D, INT8>::SLOT / 4;
+    return join > ring ? join : ring;
+}
+
+// RT row tiles of 16: a wave takes its keys once for all of them. The queries wait in LDS.
 template <int BITS, int D, bool INT8, int RT>
-__global__ __launch_bounds__(256 * RT, D == 256 ? 2 : 3) void paged_attend_kernel(AttendArgs a) {
-    using C = Chunk<BITS, D, INT8>;
-    constexpr int NG = C::NG, STEPS = D / 32, DPP = C::DPP;
-    extern __shared__ __attribute__((aligned(16))) float lds[];  // [RT][4][rows][D + 4], then (max, sum) [RT][4][16]
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int kw = wave & 3, rt = wave >> 2, h = blockIdx.y;
+__global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kernel(AttendArgs a) {
+    using C = Shape<BITS, D, INT8>;
+    constexpr bool RING = BITS != 16;  // keys come through LDS
+    constexpr int NG = C::NG, STEPS = D / 32, DPP = C::DPP, QS = D + 8, PPS = 16 / BITS;  // K steps of a piece
+    extern __shared__ __attribute__((aligned(16))) float lds[];  // keys or joins, (max, sum) [RT][4][16], q [RT * 16][QS]
+    const int lane = threadIdx.x & 63, kw = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = blockIdx.y;
     const int col = lane & 15, g = lane >> 4;
-    const int row0 = ((int)blockIdx.z * RT + rt) * 16, rows = max(min(a.R - row0, 16), 0);
-    const int tile_rows = min(a.R - (int)blockIdx.z * RT * 16, 16);  // of the workgroup's first tile: the LDS row count
+    const int row0 = (int)blockIdx.z * RT * 16;
+    const int tile_rows = min(a.R - row0, 16);  // of the first tile
+    const int q_col = RT == 1 ? min(col, tile_rows - 1) : col;
+    float2* sml = (float2*)(lds + key_floats<BITS, D, INT8>(tile_rows));
+    f16* sq = (f16*)(sml + RT * 64);
 
-    const uint64_t total = total_rounds(a);
-    const uint32_t w = blockIdx.x, workers = workers_of(a, total);
-    if (w >= workers) return;
-    const uint32_t begin = (uint32_t)(w * total / workers), end = (uint32_t)((w + 1) * total / workers);
-    uint32_t at = begin;
-    bool first = true;
-    while (at < end) {
-        const PagedUnit u = find_unit(a.n_seq, at, [&](int b) { return rounds_of(a, b); });
-        if (u.b < 0) return;
-        const int b = u.b, keys = keys_of(a, b), len = min(max(a.lengths[b], 0), a.width << a.c.lg);
-        const uint32_t all = (uint32_t)(keys + kRound - 1) / kRound;
-        const uint32_t r0 = u.at, r1 = min(all, u.at + (end - at));
-        const Scalars table = scalars(a.table + b * a.table_stride), v_exp = scalars(a.c.v_exp);
-        const Scalars picked = scalars(a.picked ? a.picked + ((int64_t)b * a.c.hkv + h) * a.n_picked : nullptr);
-
-        auto half_at = [&](int key, int& page, int& slot, int& pos) {  // (uniform) 16 keys from `key` on
-            const int j = key >> a.c.lg;
-            slot = key & ((1 << a.c.lg) - 1);
+    const uint32_t w = blockIdx.x;
+    uint32_t at = 0, end = 0, per, rest;  // (one piece: end stays below)
+    Piece piece;
+    {
+        const Plan plan = plan_of(a);
+        per = plan.per, rest = plan.rest;
+        if (!plan.most) {
+            if (w >= plan.workers) return;
+            at = w * per + min(w, rest);
+            end = at + per + (w < rest);
+        }
+        piece = first_piece(a, plan, w, at);
+    }
+    for (bool first = true; piece.b >= 0; first = false) {
+        const int b = piece.b, len = piece.len, keys = keys_of(a, len);
+        const uint32_t r0 = piece.r0, r1 = piece.r1;
+        const int32_t* table = a.table + b * a.table_stride;
+        const int32_t* picked = a.picked ? a.picked + ((int64_t)b * a.c.hkv + h) * a.n_picked : nullptr;
+        Places ahead;
+        auto look = [&](uint32_t r) {
+            const int ln = afresh(lane);
+            const int64_t key = (int64_t)(r + (ln >> 1)) * kRound + 32 * kw + 16 * (ln & 1);
+            const int j = (int)(key >> a.c.lg);
             int logical = key < keys ? (picked ? picked[j] : j) : -1;
-            page = (uint32_t)logical < (uint32_t)a.width ? table[logical] : -1;
+            const int page = (uint32_t)logical < (uint32_t)a.width ? table[logical] : -1;
             const bool there = (uint32_t)page < (uint32_t)a.c.n_pages;
-            pos = there ? (logical << a.c.lg) + slot : kNoKey;
-            page = there ? page : 0;
+            ahead.page = there ? page : 0;
+            ahead.pos = there ? (logical << a.c.lg) + (int)(key & ((1 << a.c.lg) - 1)) : kNoKey;
         };
         auto place_of = [&](uint32_t r) {
             Place p{};
             if (r >= r1) return p;  // (behind the piece: page 0, which every wave then requests and none uses)
-            const int key = (int)(r * kRound) + 32 * kw;
-            half_at(key, p.page0, p.slot0, p.pos0);
-            half_at(key + 16, p.page1, p.slot1, p.pos1);
-            if (BITS != 16) {  // (left as they come: a use here would wait for them)
-                p.e0 = v_exp[(int64_t)p.page0 * a.c.hkv + h];
-                p.e1 = v_exp[(int64_t)p.page1 * a.c.hkv + h];
-            }
+            const int i = (int)((r - r0) & 31) * 2;
+            if (i == 0) look(r);
+            p.page0 = __builtin_amdgcn_readlane(ahead.page, i);
+            p.page1 = __builtin_amdgcn_readlane(ahead.page, i + 1);
+            p.pos0 = __builtin_amdgcn_readlane(ahead.pos, i);
+            p.pos1 = __builtin_amdgcn_readlane(ahead.pos, i + 1);
+            const int key = (int)(r * kRound) + 32 * kw, last = (1 << a.c.lg) - 1;
+            p.slot0 = key & last;
+            p.slot1 = (key + 16) & last;
             return p;
         };
 
-        // the query rows
-        half8 q[STEPS];
-        float qsum[NG];
-        const int row = row0 + min(col, rows - 1);
-        const int rr = row % a.n_rows;
-        {
-            const f16* qr = a.q + b * a.q_seq + (int64_t)(h * a.G + row / a.n_rows) * a.q_head + rr * a.q_row;
+        Chunk<D> x;  // (not RING)
+        const char* ring = (const char*)lds + kw * 2 * C::SLOT;
+        const uint32_t ring0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)ring;
+        // the query rows: requested, with the first pages, before the keys, behind which they would wait
+        constexpr int QN = RT * 16 * (D / 8) / 256;
+        half8 qr[QN];
+        const int tid = afresh(threadIdx.x);
+        const int q_rows = RT == 1 ? tile_rows : 16 * RT;
 #pragma unroll
-            for (int m = 0; m < STEPS; m++) q[m] = rows > 0 ? *(const half8*)(qr + 32 * m + 8 * g) : half8{};
+        for (int i = 0; i < QN; i++) {
+            const int c = (tid + 256 * i) / (D / 8), d = tid % (D / 8) * 8, row = min(row0 + c, a.R - 1);
+            const f16* from = a.q + b * a.q_seq + (int64_t)(h * a.G + row / a.n_rows) * a.q_head + row % a.n_rows * a.q_row;
+            if (c < q_rows) qr[i] = *(const half8*)(from + d);
+        }
+        Place cur = place_of(r0), next{};
+        if (!first) __syncthreads();  // (the last piece's rows and sums are read)
+#pragma unroll
+        for (int i = 0; i < QN; i++) {
+            const int c = (tid + 256 * i) / (D / 8), d = tid % (D / 8) * 8;
+            if (c < q_rows) *(half8*)(sq + c * QS + d) = qr[i];
+        }
+        if constexpr (RING) {
+            request<BITS, D, INT8>(a.c, cur, h, lane, ring0);
+            next = place_of(r0 + 1);
+            if (r0 + 1 < r1) request<BITS, D, INT8>(a.c, next, h, lane, ring0 + C::SLOT);
+        } else {
+            load_k(x, a.c, cur, h, afresh(lane));
+            load_v(x, a.c, cur, h, afresh(lane));
+        }
+        __syncthreads();
+        float qsum[RT][NG];
+        int seen[RT];  // keys before it are the row's
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            seen[t] = len - a.n_rows + min(row0 + 16 * t + col, a.R - 1) % a.n_rows + 1;
             if constexpr (BITS != 16) {
 #pragma unroll
                 for (int m = 0; m < NG; m++) {
-                    float s = 0.0f;
+                    float y = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < STEPS / NG; j++)
+                    for (int j = 0; j < STEPS / NG; j++) {
+                        const half8 q = *(const half8*)(sq + (16 * t + q_col) * QS + 32 * (m * (STEPS / NG) + j) + 8 * g);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) s += (float)q[m * (STEPS / NG) + j][e];
-                    s += lane_xor<16>(s, lane);
-                    s += lane_xor<32>(s, lane);
-                    qsum[m] = s * (INT8 ? -128.0f * 0x1p-24f : 0x1p-24f);  // in the codes' units
+                        for (int e = 0; e < 8; e++) y += (float)q[e];
+                    }
+                    y += lane_xor<16>(y, lane);
+                    y += lane_xor<32>(y, lane);
+                    qsum[t][m] = y * (INT8 ? -128.0f * 0x1p-24f : 0x1p-24f);  // in the codes' units
                 }
             }
         }
         const float sc = a.scale2 * (BITS == 16 ? 1.0f : 0x1p24f);
-        const int seen = len - a.n_rows + rr + 1;     // keys before it are this row's
-        const int seen_all = len - a.n_rows + 1;      // and all rows'
+        const int seen_all = len - a.n_rows + 1;  // keys before it are all rows'
 
-        float4v o[D / 16], ob = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < D / 16; i++) o[i] = float4v{0, 0, 0, 0};
-        float M = kNone, l = 0.0f, lp = 0.0f;
+        float4v o[RT][D / 16], ob[RT];
+        float M[RT], l[RT], lp[RT];
         int E = 0;
-
-        C x;
-        Place cur = place_of(r0);
-        load_k(x, a.c, cur, h, lane);
-        load_v(x, a.c, cur, h, lane);
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            M[t] = kNone, l[t] = lp[t] = 0.0f;
+            ob[t] = float4v{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) o[t][i] = float4v{0, 0, 0, 0};
+        }
         for (uint32_t r = r0; r < r1; r++) {
-            const Place next = place_of(r + 1);
+            const char* slot = ring + ((r - r0) & 1) * C::SLOT;
+            if constexpr (RING) {
+                if (r + 1 < r1)
+                    wait_loads<C::LOADS>();
+                else
+                    wait_loads<0>();
+            } else {
+                next = place_of(r + 1);
+            }
+            const f16* kpar = (const f16*)(slot + C::P0) + g * C::PAR;
             const int top = max(cur.pos0, cur.pos1) + 15;
-            // scores: lane group g has keys 8 g + 4 t + i
-            float s[8];
+            // scores: lane group g has keys 8 g + 4 u + i
+            float s[RT][8];
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                float4v acc[NG];
+            for (int v = 0; v < 2; v++) {
+                float4v acc[RT][NG];
 #pragma unroll
-                for (int m = 0; m < NG; m++) acc[m] = float4v{0, 0, 0, 0};
+                for (int t = 0; t < RT; t++)
 #pragma unroll
-                for (int m = 0; m < STEPS; m++)
-                    acc[m / (STEPS / NG)] = mfma(k_codes<BITS>(x.k[t], m), q[m], acc[m / (STEPS / NG)]);
+                    for (int m = 0; m < NG; m++) acc[t][m] = float4v{0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if constexpr (BITS == 16) {
-                        float y = acc[0][i];
+                for (int m = 0; m < STEPS; m++) {
+                    half8 k;
+                    if constexpr (RING)
+                        k = k_codes<BITS>(*(const u32x4*)(slot + (v * C::NK + m / PPS) * 1024 + 16 * lane), m % PPS);
+                    else
+                        k = k_codes<BITS>(x.k[v][m], 0);
 #pragma unroll
-                        for (int m = 1; m < NG; m++) y += acc[m][i];
-                        s[4 * t + i] = y;
-                    } else if constexpr (INT8) {
-                        s[4 * t + i] = (float)x.ks[0][4 * t + i] * (acc[0][i] + qsum[0]);
-                    } else {
+                    for (int t = 0; t < RT; t++) {
+                        const half8 q = *(const half8*)(sq + (16 * t + q_col) * QS + 32 * m + 8 * g);
+                        acc[t][m / (STEPS / NG)] = mfma(k, q, acc[t][m / (STEPS / NG)]);
+                    }
+                }
+                half4v ks[NG], kb[NG];
+                if constexpr (RING) {
+#pragma unroll
+                    for (int m = 0; m < NG; m++) {
+                        ks[m] = *(const half4v*)(kpar + 8 * m + 4 * v);
+                        if (!INT8) kb[m] = *(const half4v*)(kpar + 8 * (NG + m) + 4 * v);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < RT; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
                         float y = 0.0f;
+                        if constexpr (BITS == 16) {
+                            y = acc[t][0][i];
 #pragma unroll
-                        for (int m = 0; m < NG; m++) {
-                            y = __builtin_fmaf((float)x.ks[m][4 * t + i], acc[m][i], y);
-                            y = __builtin_fmaf((float)x.kb[m][4 * t + i], qsum[m], y);
+                            for (int m = 1; m < NG; m++) y += acc[t][m][i];
+                        } else if constexpr (INT8) {
+                            y = (float)ks[0][i] * (acc[t][0][i] + qsum[t][0]);
+                        } else {
+#pragma unroll
+                            for (int m = 0; m < NG; m++) {
+                                y = __builtin_fmaf((float)ks[m][i], acc[t][m][i], y);
+                                y = __builtin_fmaf((float)kb[m][i], qsum[t][m], y);
+                            }
                         }
-                        s[4 * t + i] = y;
+                        s[t][4 * v + i] = y;
+                    }
+            }
+            if constexpr (!RING) {
+                __builtin_amdgcn_sched_barrier(0);
+                load_k(x, a.c, next, h, afresh(lane));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const bool masked = top >= seen_all;
+            const int pos = (g & 2 ? cur.pos1 : cur.pos0) + 8 * (g & 1);
+            u32x4 km;  // the keys before the sequence's end: what stands behind it takes no part, whatever it is
+            if (masked) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) km[j] = (pos + 2 * j < len ? 0xFFFFu : 0u) | (pos + 2 * j + 1 < len ? 0xFFFF0000u : 0u);
+            }
+            half8 vs[NG], vb{};
+            if constexpr (RING) {
+#pragma unroll
+                for (int m = 0; m < NG; m++) vs[m] = *(const half8*)(kpar + 4 * C::PAR + 8 * m);
+                if constexpr (!INT8) vb = *(const half8*)(kpar + 4 * C::PAR + 8 * (NG + min(col, NG - 1)));
+                if (masked) {
+#pragma unroll
+                    for (int m = 0; m < NG; m++) vs[m] = as_h8(__builtin_bit_cast(u32x4, vs[m]) & km);
+                    vb = as_h8(__builtin_bit_cast(u32x4, vb) & km);
+                }
+            }
+            if constexpr (RING) {
+                uint32_t high = 0;
+#pragma unroll
+                for (int m = 0; m < NG; m++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) high |= __builtin_bit_cast(u32x4, vs[m])[j];
+                if (__any((high & 0x40004000u) != 0)) {  // V scales of 2 and more: P gives way, so that P times a scale fits a half
+                    float big = 0.0f;
+#pragma unroll
+                    for (int m = 0; m < NG; m++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf((float)vs[m][i]));
+                    big = wave_reduce(big, OpMax());
+                    const int e = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(big) >> 23) - 127);
+                    if (e > E) {
+                        const float f = __builtin_amdgcn_exp2f((float)(E - e));
+                        E = e;
+#pragma unroll
+                        for (int t = 0; t < RT; t++) {
+                            l[t] *= f, lp[t] *= f;
+                            ob[t] *= f;
+#pragma unroll
+                            for (int i = 0; i < D / 16; i++) o[t][i] *= f;
+                        }
                     }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
-            load_k(x, a.c, next, h, lane);
-            __builtin_amdgcn_sched_barrier(0);
-            const bool masked = top >= seen_all;
 #pragma unroll
-            for (int i = 0; i < 8; i++) s[i] *= sc;
-            if (masked) {
-                const int pos = (g & 2 ? cur.pos1 : cur.pos0) + 8 * (g & 1);
+            for (int t = 0; t < RT; t++) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) s[i] = pos + i < seen ? s[i] : -INFINITY;
-            }
-            float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-            if (__any(mx > M + kLazy)) {
-                mx = fmaxf(mx, lane_xor<16>(mx, lane));
-                mx = fmaxf(mx, lane_xor<32>(mx, lane));
-                const float m1 = fmaxf(M, mx), alpha = __builtin_amdgcn_exp2f(M - m1);
-                M = m1;
-                l *= alpha, lp *= alpha;
-                ob *= alpha;
+                for (int i = 0; i < 8; i++) s[t][i] *= sc;
+                if (masked) {
 #pragma unroll
-                for (int i = 0; i < D / 16; i++) o[i] *= alpha;
-            }
-            if constexpr (BITS != 16) {
-                const int e = max(cur.e0, cur.e1);
-                if (e > E) {  // V scales of 1 and more: P gives way, so that P times a scale fits a half
-                    const float f = __builtin_amdgcn_exp2f((float)(E - e));
-                    E = e;
-                    l *= f, lp *= f;
-                    ob *= f;
+                    for (int i = 0; i < 8; i++) s[t][i] = pos + i < seen[t] ? s[t][i] : -INFINITY;
+                }
+                float mx = fmaxf(fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])),
+                                 fmaxf(fmaxf(s[t][4], s[t][5]), fmaxf(s[t][6], s[t][7])));
+                if (__any(mx > M[t] + kLazy)) {
+                    mx = fmaxf(mx, lane_xor<16>(mx, lane));
+                    mx = fmaxf(mx, lane_xor<32>(mx, lane));
+                    const float m1 = fmaxf(M[t], mx), alpha = __builtin_amdgcn_exp2f(M[t] - m1);
+                    M[t] = m1;
+                    l[t] *= alpha, lp[t] *= alpha;
+                    ob[t] *= alpha;
 #pragma unroll
-                    for (int i = 0; i < D / 16; i++) o[i] *= f;
+                    for (int i = 0; i < D / 16; i++) o[t][i] *= alpha;
+                }
+                const float ref = M[t] + ((float)E - kLift);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - ref);
+                    l[t] += s[t][i];
                 }
             }
-            const float ref = M + ((float)E - kLift);
-            float p[8];
+            half8 ph[RT];
+            if constexpr (BITS == 16 || !INT8) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
-                l += p[i];
-            }
-            uint32_t key[4] = {~0u, ~0u, ~0u, ~0u};
-            if (masked) {  // what stands behind the sequence's end takes no part, whatever it is
-                const int pos = (g & 2 ? cur.pos1 : cur.pos0) + 8 * (g & 1);
+                for (int t = 0; t < RT; t++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) key[j] = (pos + 2 * j < len ? 0xFFFFu : 0u) | (pos + 2 * j + 1 < len ? 0xFFFF0000u : 0u);
+                    for (int i = 0; i < 8; i++) ph[t][i] = (f16)s[t][i];
             }
-            const u32x4 km = {key[0], key[1], key[2], key[3]};
             if constexpr (BITS == 16) {
-                half8 ph;
-#pragma unroll
-                for (int i = 0; i < 8; i++) ph[i] = (f16)p[i];
                 if (masked) {
 #pragma unroll
                     for (int j = 0; j < C::NV; j++) x.v[j] &= km;
                 }
 #pragma unroll
-                for (int j = 0; j < C::NV; j++) o[j] = mfma(v_codes<16>(x.v[j], 0), ph, o[j]);
+                for (int j = 0; j < C::NV; j++)
+#pragma unroll
+                    for (int t = 0; t < RT; t++) o[t][j] = mfma(v_codes<16>(x.v[j], 0), ph[t], o[t][j]);
             } else {
-                if (masked) {
-#pragma unroll
-                    for (int m = 0; m < NG; m++) x.vs[m] = as_h8(__builtin_bit_cast(u32x4, x.vs[m]) & km);
-                    if (!INT8) x.vb = as_h8(__builtin_bit_cast(u32x4, x.vb) & km);
-                }
                 if constexpr (!INT8) {
-                    half8 ph;
+                    if (col >= NG) vb = half8{};
 #pragma unroll
-                    for (int i = 0; i < 8; i++) ph[i] = (f16)p[i];
-                    ob = mfma(col < NG ? x.vb : half8{}, ph, ob);
+                    for (int t = 0; t < RT; t++) ob[t] = mfma(vb, ph[t], ob[t]);
                 }
-                if constexpr (BITS == 4) p[2] *= 0.0625f, p[3] *= 0.0625f, p[6] *= 0.0625f, p[7] *= 0.0625f;
+                if constexpr (BITS == 4) {
+#pragma unroll
+                    for (int t = 0; t < RT; t++)
+                        s[t][2] *= 0.0625f, s[t][3] *= 0.0625f, s[t][6] *= 0.0625f, s[t][7] *= 0.0625f;
+                }
                 constexpr int PER = C::NV / NG;
 #pragma unroll
                 for (int m = 0; m < NG; m++) {
-                    half8 ph;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) ph[i] = (f16)(p[i] * (float)x.vs[m][i]);
-                    if constexpr (INT8) {
+                    for (int t = 0; t < RT; t++) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) lp += (float)ph[i];
+                        for (int i = 0; i < 8; i++) ph[t][i] = (f16)(s[t][i] * (float)vs[m][i]);
+                        if constexpr (INT8) {
+#pragma unroll
+                            for (int i = 0; i < 8; i++) lp[t] += (float)ph[t][i];
+                        }
                     }
 #pragma unroll
-                    for (int j = m * PER; j < (m + 1) * PER; j++)
+                    for (int j = m * PER; j < (m + 1) * PER; j++) {
+                        const u32x4 piece = *(const u32x4*)(slot + C::V0 + j * 1024 + 16 * lane);
 #pragma unroll
-                        for (int e = 0; e < DPP; e++) o[j * DPP + e] = mfma(v_codes<BITS>(x.v[j], e), ph, o[j * DPP + e]);
+                        for (int e = 0; e < DPP; e++) {
+                            const half8 v = v_codes<BITS>(piece, e);
+#pragma unroll
+                            for (int t = 0; t < RT; t++) o[t][j * DPP + e] = mfma(v, ph[t], o[t][j * DPP + e]);
+                        }
+                    }
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
-            load_v(x, a.c, next, h, lane);
-            __builtin_amdgcn_sched_barrier(0);
-            cur = next;
-        }
-
-        // the wave's row: sum over the lane groups, biases, the codes' units
-        l += lane_xor<16>(l, lane);
-        l += lane_xor<32>(l, lane);
-        if constexpr (INT8) {
-            lp += lane_xor<16>(lp, lane);
-            lp += lane_xor<32>(lp, lane);
-        }
-        float* so = lds + ((rt * 4 + kw) * tile_rows + col) * (D + 4);
-        float2* sml = (float2*)(lds + RT * 4 * tile_rows * (D + 4));
-        if (!first) __syncthreads();  // (the last piece's sums are read)
-        first = false;
-        if (g == 0) sml[(rt * 4 + kw) * 16 + col] = float2{M + (float)E, l};
-        float bias[NG];
-#pragma unroll
-        for (int m = 0; m < NG; m++)
-            bias[m] = BITS == 16 ? 0.0f : INT8 ? -128.0f * lp : __shfl(ob[m & 3], col);
-        if (col < rows) {
-#pragma unroll
-            for (int j = 0; j < C::NV; j++) {
-                float f[4 * DPP];  // dims DPP (16 j + 4 g) ..
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int e = 0; e < DPP; e++) {
-                        const float y = o[j * DPP + e][i];
-                        f[i * DPP + e] = BITS == 16 ? y : __builtin_fmaf(y, 0x1p24f, bias[INT8 ? 0 : j / (C::NV / NG)]);
-                    }
-#pragma unroll
-                for (int i = 0; i < DPP; i++)
-                    *(float4v*)(so + DPP * (16 * j + 4 * g) + 4 * i) = float4v{f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]};
-            }
-        }
-        __syncthreads();
-        // the four waves' rows joined by the tile's 256 threads
-        const bool done = r0 == 0 && r1 == all;
-        const int slot = 2 * (int)w + (u.at == 0 && at != begin ? 1 : 0);
-        for (int i = kw * 64 + lane; i < rows * (D / 4); i += 256) {
-            const int c = i / (D / 4), d = i % (D / 4) * 4;
-            float2 ml[4];
-            float mm = kNone;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                ml[k] = sml[(rt * 4 + k) * 16 + c];
-                mm = fmaxf(mm, ml[k].x);
-            }
-            float4v y = {0, 0, 0, 0};
-            float sum = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float f = __builtin_amdgcn_exp2f(ml[k].x - mm);
-                y += f * *(const float4v*)(lds + ((rt * 4 + k) * tile_rows + c) * (D + 4) + d);
-                sum = __builtin_fmaf(f, ml[k].y, sum);
-            }
-            const int64_t rw = row0 + c;
-            if (done) {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const int64_t to = ((b * (int64_t)a.c.hkv + h) * a.R + rw) * D + d;
-                *(half4v*)(a.out + to) = half4v{(f16)(y[0] * inv), (f16)(y[1] * inv), (f16)(y[2] * inv), (f16)(y[3] * inv)};
+            if constexpr (RING) {
+                cur = next;
+                if (r + 2 < r1) {  // this chunk is read: its place takes the one behind the next
+                    next = place_of(r + 2);
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    request<BITS, D, INT8>(a.c, next, h, afresh(lane), ring0 + ((r - r0) & 1) * C::SLOT);
+                }
             } else {
-                const int64_t to = ((int64_t)slot * a.c.hkv + h) * a.R + rw;
-                *(float4v*)(a.part_o + to * D + d) = y;
-                if (d == 0) a.part_ml[to] = float2{mm, sum};
+                __builtin_amdgcn_sched_barrier(0);
+                load_v(x, a.c, next, h, afresh(lane));
+                __builtin_amdgcn_sched_barrier(0);
+                cur = next;
+            }
+        }
+        if constexpr (RING) __syncthreads();  // (every wave has read its keys: their place takes the rows)
+
+        // the rows' sums over the lane groups, biases, and the four waves joined
+        const bool done = r0 == 0 && r1 == piece.all;
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            l[t] += lane_xor<16>(l[t], lane);
+            l[t] += lane_xor<32>(l[t], lane);
+            if constexpr (INT8) {
+                lp[t] += lane_xor<16>(lp[t], lane);
+                lp[t] += lane_xor<32>(lp[t], lane);
+            }
+            if (g == 0) sml[(t * 4 + kw) * 16 + col] = float2{M[t] + (float)E, l[t]};
+        }
+        float* so = lds + (kw * tile_rows + col) * (kJoin + 4);
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const int rows = min(a.R - row0 - 16 * t, 16);  // (none or fewer: nothing is written)
+            float bias[NG];
+#pragma unroll
+            for (int m = 0; m < NG; m++)
+                bias[m] = BITS == 16 ? 0.0f : INT8 ? -128.0f * lp[t] : __shfl(ob[t][m & 3], col);
+#pragma unroll
+            for (int part = 0; part < D / kJoin; part++) {
+                constexpr int PJ = C::NV * kJoin / D;  // V pieces of a part
+                if (t > 0 || part > 0) __syncthreads();  // (the last part is read)
+                if (col < rows) {
+#pragma unroll
+                    for (int jj = 0; jj < PJ; jj++) {
+                        const int j = part * PJ + jj;
+                        float f[4 * DPP];  // dims DPP (16 jj + 4 g) .. of the part
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+#pragma unroll
+                            for (int e = 0; e < DPP; e++) {
+                                const float y = o[t][j * DPP + e][i];
+                                f[i * DPP + e] = BITS == 16 ? y : __builtin_fmaf(y, 0x1p24f, bias[INT8 ? 0 : j / (C::NV / NG)]);
+                            }
+#pragma unroll
+                        for (int i = 0; i < DPP; i++)
+                            *(float4v*)(so + DPP * (16 * jj + 4 * g) + 4 * i) = float4v{f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]};
+                    }
+                }
+                __syncthreads();
+                for (int i = afresh(threadIdx.x); i < rows * (kJoin / 4); i += 256) {
+                    const int c = i / (kJoin / 4), d = i % (kJoin / 4) * 4;
+                    float2 ml[4];
+                    float mm = kNone;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        ml[k] = sml[(t * 4 + k) * 16 + c];
+                        mm = fmaxf(mm, ml[k].x);
+                    }
+                    float4v y = {0, 0, 0, 0};
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float f = __builtin_amdgcn_exp2f(ml[k].x - mm);
+                        y += f * *(const float4v*)(lds + (k * tile_rows + c) * (kJoin + 4) + d);
+                        sum = __builtin_fmaf(f, ml[k].y, sum);
+                    }
+                    const int64_t rw = row0 + 16 * t + c;
+                    if (done) {
+                        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                        const int64_t to = ((b * (int64_t)a.c.hkv + h) * a.R + rw) * D + part * kJoin + d;
+                        *(half4v*)(a.out + to) = half4v{(f16)(y[0] * inv), (f16)(y[1] * inv), (f16)(y[2] * inv), (f16)(y[3] * inv)};
+                    } else {
+                        const int64_t to = ((int64_t)piece.slot * a.c.hkv + h) * a.R + rw;
+                        *(float4v*)(a.part_o + to * D + part * kJoin + d) = y;
+                        if (part == 0 && d == 0) a.part_ml[to] = float2{mm, sum};
+                    }
+                }
             }
         }
         at += r1 - r0;
+        if (at >= end) return;
+        piece = piece_at(a, per, rest, w, at);
     }
 }
 
@@ -449,14 +701,18 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
     __shared__ float4v sm_o[256];
     __shared__ float sm_l[SG];
     const int tid = threadIdx.x, b = blockIdx.y, h = (int)blockIdx.x / a.R, row = (int)blockIdx.x % a.R;
-    const uint64_t total = total_rounds(a);
-    const uint32_t mine = rounds_of(a, b);
-    uint32_t base = 0;
-    {
-        uint32_t n = 0;
-        const int lane = tid & 63;
-        for (int i = lane; i < b; i += 64) n += rounds_of(a, i);
-        base = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
+    const Plan plan = plan_of(a);
+    const int lane = tid & 63;
+    uint32_t mine, before = 0, n, slot0;  // the sequence's rounds; its pieces, the first one's slot
+    int64_t step = 2;
+    if (a.n_seq <= 64) {
+        mine = (uint32_t)__builtin_amdgcn_readlane((int)plan.rounds, b);
+        before = (uint32_t)__builtin_amdgcn_readlane((int)plan.through, b) - mine;
+    } else {
+        mine = rounds_of(a, b);
+        uint32_t x = 0;
+        for (int i = lane; i < b; i += 64) x += rounds_of(a, i);
+        before = wave_last(wave_scan(x));
     }
     const int d = tid % TC * 4, sg = tid / TC;
     f16* to = a.out + ((b * (int64_t)a.c.hkv + h) * a.R + row) * D + d;
@@ -464,24 +720,45 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
         if (sg == 0) *(half4v*)to = half4v{};
         return;
     }
-    const uint32_t workers = workers_of(a, total);
-    auto worker_of = [&](uint64_t x) { return (int)(((x + 1) * workers - 1) / total); };
-    const int w0 = worker_of(base), w1 = worker_of(base + mine - 1);
-    if (w0 == w1) return;
-    // its first piece is the last of its worker's run, unless that begins with it
-    const int s0 = (uint32_t)((uint64_t)w0 * total / workers) == base ? 2 * w0 : 2 * w0 + 1;
-    auto slot_of = [&](int w) { return ((int64_t)(w == w0 ? s0 : 2 * w) * a.c.hkv + h) * a.R + row; };
+    if (plan.most) {
+        n = (uint32_t)__builtin_amdgcn_readlane((int)plan.pieces, b);
+        slot0 = 2 * ((uint32_t)__builtin_amdgcn_readlane((int)plan.last, b) - n);
+        step = slot0;
+    } else {
+        // the worker of a round, and where its run begins; a sequence's first piece is the last of its worker's run,
+        // unless that begins with it
+        const uint32_t longer = plan.rest * (plan.per + 1);
+        auto worker_of = [&](uint32_t x) {
+            return x < longer ? x / (plan.per + 1) : plan.rest + (x - longer) / plan.per;
+        };
+        const uint32_t w0 = worker_of(before), w1 = worker_of(before + mine - 1);
+        n = w1 - w0 + 1;
+        slot0 = w0 * plan.per + min(w0, plan.rest) == before ? 2 * w0 : 2 * w0 + 1;
+        step = 2 * w0;
+    }
+    if (n == 1) return;
+    auto slot_of = [&](uint32_t i) { return ((int64_t)(i == 0 ? slot0 : step + 2 * i) * a.c.hkv + h) * a.R + row; };
     float mm = kNone;
-    for (int w = w0 + (tid & 63); w <= w1; w += 64) mm = fmaxf(mm, a.part_ml[slot_of(w)].x);
+    for (uint32_t i = lane; i < n; i += 64) mm = fmaxf(mm, a.part_ml[slot_of(i)].x);
     mm = wave_reduce(mm, OpMax());
     float4v y = {0, 0, 0, 0};
     float sum = 0.0f;
-    for (int w = w0 + sg; w <= w1; w += SG) {
-        const int64_t s = slot_of(w);
-        const float2 ml = a.part_ml[s];
-        const float f = __builtin_amdgcn_exp2f(ml.x - mm);
-        y += f * *(const float4v*)(a.part_o + s * D + d);
-        sum = __builtin_fmaf(f, ml.y, sum);
+    constexpr int AHEAD = 8;  // pieces in flight
+    for (uint32_t i = sg; i < n; i += SG * AHEAD) {
+        float2 ml[AHEAD];
+        float4v x[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            const int64_t s = slot_of(min(i + k * SG, n - 1));
+            ml[k] = a.part_ml[s];
+            x[k] = *(const float4v*)(a.part_o + s * D + d);
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            const float f = i + k * SG < n ? __builtin_amdgcn_exp2f(ml[k].x - mm) : 0.0f;
+            y += f * x[k];
+            sum = __builtin_fmaf(f, ml[k].y, sum);
+        }
     }
     sm_o[tid] = y;
     if (tid % TC == 0) sm_l[sg] = sum;
@@ -497,20 +774,34 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
 }
 
 template <int BITS, int D, bool INT8, int RT>
-int launch_attend(const AttendArgs& a, int groups, hipStream_t stream) {
-    const int rows = std::min(a.R, 16);
-    const size_t lds = (size_t)RT * 4 * (rows * (D + 4) * 4 + 16 * 8);
+size_t attend_lds(int R) {
+    const int rows = std::min(R, 16), q_rows = RT == 1 ? rows : 16 * RT;
+    return (size_t)key_floats<BITS, D, INT8>(rows) * 4 + RT * 64 * 8 + (size_t)q_rows * (D + 8) * 2;
+}
+template <int BITS, int D, bool INT8, int RT>
+int launch_attend(const AttendArgs& a, hipStream_t stream) {
+    const size_t lds = attend_lds<BITS, D, INT8, RT>(a.R);
     const void* f = (const void*)paged_attend_kernel<BITS, D, INT8, RT>;
     if (int rc = ensure_dynamic_lds(f, lds)) return rc;
-    hipLaunchKernelGGL((paged_attend_kernel<BITS, D, INT8, RT>), dim3(a.workers, a.c.hkv, groups), dim3(256 * RT), lds, stream, a);
+    const dim3 grid(a.workers, a.c.hkv, (a.R + 16 * RT - 1) / (16 * RT));
+    hipLaunchKernelGGL((paged_attend_kernel<BITS, D, INT8, RT>), grid, dim3(256), lds, stream, a);
     QW_HIP_CHECK(hipGetLastError());
     return QW_OK;
 }
-template <int BITS, bool INT8>
-int launch_rows(const AttendArgs& a, int D, hipStream_t stream) {
-    const int tiles = (a.R + 15) / 16;
-    if (tiles == 1) return D == 256 ? launch_attend<BITS, 256, INT8, 1>(a, 1, stream) : launch_attend<BITS, 128, INT8, 1>(a, 1, stream);
-    return D == 256 ? launch_attend<BITS, 256, INT8, 2>(a, (tiles + 1) / 2, stream) : launch_attend<BITS, 128, INT8, 2>(a, (tiles + 1) / 2, stream);
+// f(row tiles of a workgroup) for the call's rows
+template <class F>
+int by_shape(int bits, bool int8, int D, int R, F f) {
+    using std::integral_constant;
+    auto tiles = [&](auto b, auto i8, auto d) {
+        return R <= 16 ? f(b, i8, d, integral_constant<int, 1>()) : f(b, i8, d, integral_constant<int, 2>());
+    };
+    auto dims = [&](auto b, auto i8) {
+        return D == 256 ? tiles(b, i8, integral_constant<int, 256>()) : tiles(b, i8, integral_constant<int, 128>());
+    };
+    if (bits == 16) return dims(integral_constant<int, 16>(), integral_constant<bool, false>());
+    if (bits == 4) return dims(integral_constant<int, 4>(), integral_constant<bool, false>());
+    if (int8) return dims(integral_constant<int, 8>(), integral_constant<bool, true>());
+    return dims(integral_constant<int, 8>(), integral_constant<bool, false>());
 }
 
 }  // namespace
@@ -561,18 +852,22 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     a.picked = picked;
     a.n_picked = n_picked;
     a.scale2 = scale * kLog2e;
-    const int groups = a.R <= 16 ? 1 : ((a.R + 15) / 16 + 1) / 2;
-    a.workers = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, 512 / ((int64_t)c.hkv * groups)));
+    // as many workers as the card holds at a time, all heads and row tiles counted
+    const int held = by_shape(c.bits, c.int8(), c.D, a.R, [&](auto b, auto i8, auto d, auto rt) {
+        constexpr int B = decltype(b)::value, DD = decltype(d)::value, RT = decltype(rt)::value;
+        return std::max(1, std::min<int>(waves_of(B, DD, RT), (int)(160 * 1024 / attend_lds<B, DD, decltype(i8)::value, RT>(a.R))));
+    });
+    const int groups = a.R <= 16 ? 1 : (a.R + 31) / 32;
+    a.workers = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, 256 * held / ((int64_t)c.hkv * groups)));
     const int64_t parts = (int64_t)a.workers * 2 * c.hkv * a.R;
     void* ws = nullptr;
     if (int rc = workspace(kWsPaged, c.device, stream, (size_t)(parts * (c.D * 4 + 8)), &ws)) return rc;
     a.part_o = (float*)ws;
     a.part_ml = (float2*)(a.part_o + parts * c.D);
     if (rounds > 0) {
-        const int rc = c.bits == 16 ? launch_rows<16, false>(a, c.D, stream)
-                       : c.bits == 4 ? launch_rows<4, false>(a, c.D, stream)
-                       : c.int8()    ? launch_rows<8, true>(a, c.D, stream)
-                                     : launch_rows<8, false>(a, c.D, stream);
+        const int rc = by_shape(c.bits, c.int8(), c.D, a.R, [&](auto b, auto i8, auto d, auto rt) {
+            return launch_attend<decltype(b)::value, decltype(d)::value, decltype(i8)::value, decltype(rt)::value>(a, stream);
+        });
         if (rc) return rc;
     }
     const dim3 grid((unsigned)(c.hkv * a.R), q.n_seq);

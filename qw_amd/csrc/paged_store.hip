@@ -20,7 +20,7 @@ size_t align16(size_t x) { return (x + 255) / 256 * 256; }
 
 int64_t PagedCache::nbytes() const {
     const int64_t ph = (int64_t)n_pages * hkv, rows = ph * page_size;
-    return 2 * rows * D * bits / 8 + 2 * rows / 8 * par_halves() * 2 + ph * (4 * D + 2 * D + 8);
+    return 2 * rows * D * bits / 8 + 2 * rows / 8 * par_halves() * 2 + ph * (4 * D + 2 * D + 4);
 }
 
 int PagedCache::init(int mode_, int group_size, int n_kv_heads, int head_dim, int n_pages_, int page_size_, int device_) {
@@ -45,10 +45,10 @@ int PagedCache::init(int mode_, int group_size, int n_kv_heads, int head_dim, in
     DeviceGuard dg(device);
     QW_REQUIRE(dg.ok, QW_ERR_HIP, "qw_paged_create: hipSetDevice failed");
     const size_t ph = (size_t)n_pages * hkv, rows = ph * page_size;
-    const size_t sizes[8] = {rows * D * bits / 8, rows * D * bits / 8, rows / 8 * par_halves() * 2, rows / 8 * par_halves() * 2,
-                             ph * 4 * D, ph * 2 * D, ph * 4, ph * 4};
-    void* at[8] = {};
-    for (int i = 0; i < 8; i++) {
+    const size_t sizes[7] = {rows * D * bits / 8, rows * D * bits / 8, rows / 8 * par_halves() * 2, rows / 8 * par_halves() * 2,
+                             ph * 4 * D, ph * 2 * D, ph * 4};
+    void* at[7] = {};
+    for (int i = 0; i < 7; i++) {
         const bool ok = sizes[i] == 0 || hipMalloc(&at[i], align16(sizes[i])) == hipSuccess;
         if (!ok) {
             (void)hipGetLastError();
@@ -59,8 +59,8 @@ int PagedCache::init(int mode_, int group_size, int n_kv_heads, int head_dim, in
         }
     }
     view = PagedView{(char*)at[0], (char*)at[1], (f16*)at[2], (f16*)at[3], (f16*)at[4], (int8_t*)at[5], (float*)at[6],
-                     (int*)at[7], hkv, n_pages, __builtin_ctz(page_size)};
-    for (int i = 0; i < 8; i++)
+                     hkv, n_pages, __builtin_ctz(page_size)};
+    for (int i = 0; i < 7; i++)
         if (at[i]) QW_HIP_CHECK(hipMemset(at[i], 0, sizes[i]));
     QW_HIP_CHECK(hipDeviceSynchronize());
     return QW_OK;
@@ -69,7 +69,7 @@ int PagedCache::init(int mode_, int group_size, int n_kv_heads, int head_dim, in
 void PagedCache::release() {
     DeviceGuard dg(device);
     (void)hipDeviceSynchronize();
-    void* ptrs[8] = {view.k, view.v, view.k_par, view.v_par, view.lohi, view.codes, view.top, view.v_exp};
+    void* ptrs[7] = {view.k, view.v, view.k_par, view.v_par, view.lohi, view.codes, view.top};
     for (void* p : ptrs)
         if (p) (void)hipFree(p);
     view = PagedView{};
@@ -166,7 +166,7 @@ struct StoreArgs {
 template <int BITS, bool INT8, int D>
 __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedView c, StoreArgs a) {
     constexpr int LPR = D / 4, SUB = 64 / LPR, NG = INT8 ? 1 : D / kGroup;
-    __shared__ float sm_lo[kStoreWaves][D], sm_hi[kStoreWaves][D], sm_s[kStoreWaves];
+    __shared__ float sm_lo[kStoreWaves][D], sm_hi[kStoreWaves][D];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int nw = blockDim.x >> 6, h = blockIdx.y, ps = 1 << c.lg;
     const PagedUnit u = find_unit(a.s.n_seq, blockIdx.x, [&](int b) {
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
     const int64_t ph = (int64_t)page * c.hkv + h;
     const int li = lane % LPR, sub = lane / LPR, grp = li >> 4;
 
-    float lo[4], hi[4], smax = 0.0f;
+    float lo[4], hi[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) lo[i] = INFINITY, hi[i] = -INFINITY;
     const int first = s0 >> 3, last = (s1 - 1) >> 3;
@@ -240,7 +240,6 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
                 }
                 vc[k] = quantize4<BITS, INT8, D>(xv[k], s, b);
                 vs[k] = s, vb[k] = b;
-                smax = in ? fmaxf(smax, fabsf((float)s)) : smax;
             }
         }
         if (live) {
@@ -321,13 +320,11 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
             hi[i] = fmaxf(hi[i], lane_xor<32>(hi[i], lane));
         }
     }
-    smax = wave_reduce(smax, FMax());
     if (nw > 1) {
         if (sub == 0) {
 #pragma unroll
             for (int i = 0; i < 4; i++) sm_lo[wave][4 * li + i] = lo[i], sm_hi[wave][4 * li + i] = hi[i];
         }
-        if (lane == 0) sm_s[wave] = smax;
         __syncthreads();
         if (wave) return;
         for (int w = 1; w < nw; w++) {
@@ -336,7 +333,6 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
                 lo[i] = fminf(lo[i], sm_lo[w][4 * li + i]);
                 hi[i] = fmaxf(hi[i], sm_hi[w][4 * li + i]);
             }
-            smax = fmaxf(smax, sm_s[w]);
         }
     }
     f16* lohi = c.lohi + ph * 2 * D + 4 * li;
@@ -369,14 +365,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
         *(uint32_t*)(c.codes + ph * 2 * D + 4 * li) = wh;
         *(uint32_t*)(c.codes + ph * 2 * D + D + 4 * li) = wl;
     }
-    if (lane == 0) {
-        c.top[ph] = top;
-        if (BITS != 16) {
-            int e = smax < 1.0f ? 0 : smax < 65536.0f ? (int)(__float_as_uint(smax) >> 23) - 126 : 17;
-            if (s0 > 0) e = max(e, c.v_exp[ph]);
-            c.v_exp[ph] = e;
-        }
-    }
+    if (lane == 0) c.top[ph] = top;
 }
 
 // 4 dims' fp16 values of a code word (a byte each): f16(f16(code * scale) + bias).
