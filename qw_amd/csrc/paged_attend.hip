@@ -3,7 +3,7 @@
 // out = softmax(scale q . k) v for each row over its sequence's keys, causal among the last n_rows of
 // them, in one pass with the running maximum and sum. Bound by reading the codes once from HBM.
 //
-// Work is dealt in rounds of 128 keys: the rounds of all sequences, one behind the other, in equal runs
+// Work is dealt in rounds of 128 or 256 keys: the rounds of all sequences, one behind the other, in equal runs
 // to the workers of a head (a grid sized for the card, lengths read on the device), so that sequences of
 // any lengths keep the chip busy. A worker's piece of a sequence that is not all of it goes to a
 // workspace as fp32 partials that a second launch joins.
@@ -25,7 +25,6 @@ namespace qw {
 
 namespace {
 
-constexpr int kRound = 128;             // keys of a round: 4 waves of 32
 constexpr float kNone = -0x1p100f;      // a maximum below every score
 constexpr float kLazy = 4.0f;           // scores pass the reference by so much (log2) before it follows
 constexpr float kLift = 10.0f;          // log2 of P at the reference: P <= 2^14, times a scale below 2, fits a half
@@ -42,7 +41,7 @@ struct AttendArgs {
     const int32_t* picked;
     int n_picked;
     float scale2;  // scale * log2 e
-    int workers;
+    int workers, round;  // keys of a round: 32 a wave
     float* part_o;    // [2 workers][hkv][R][D]
     float2* part_ml;  // [2 workers][hkv][R]
 };
@@ -54,7 +53,7 @@ __device__ __forceinline__ int keys_of(const AttendArgs& a, int len) {
     return min(pages, a.n_picked) << a.c.lg;
 }
 __device__ __forceinline__ uint32_t rounds_of(const AttendArgs& a, int b) {
-    return (uint32_t)(keys_of(a, min(max(a.lengths[b], 0), a.width << a.c.lg)) + kRound - 1) / kRound;
+    return (uint32_t)(keys_of(a, min(max(a.lengths[b], 0), a.width << a.c.lg)) + a.round - 1) / a.round;
 }
 
 // How the rounds are dealt, the same for every wave of a call. Up to 64 sequences (a lane each): pieces of
@@ -73,7 +72,7 @@ __device__ __forceinline__ Plan plan_of(const AttendArgs& a) {
     if (a.n_seq <= 64) {
         if (lane < a.n_seq) {
             p.len = min(max(a.lengths[lane], 0), a.width << a.c.lg);
-            p.rounds = (uint32_t)(keys_of(a, p.len) + kRound - 1) / kRound;
+            p.rounds = (uint32_t)(keys_of(a, p.len) + a.round - 1) / a.round;
         }
         p.through = wave_scan(p.rounds);
         p.total = wave_last(p.through);
@@ -144,10 +143,17 @@ struct Places {
 };
 constexpr int kNoKey = 0x7fffff00;  // a position behind every key
 
-// Waves a SIMD that the registers are cut for.
-constexpr int waves_of(int bits, int D, int RT) {
-    return D == 256 && RT == 2 ? 1 : bits == 16 && D == 128 && RT == 1 ? 3 : 2;
-}
+// How a call's row tiles of 16 go to waves: up to 16 rows a tile and 4 waves a workgroup; above, two tiles, for both of
+// which a wave takes its keys once, and 8 waves that share the queries. fp16 keys go through registers, but for two tiles
+// at D = 256: there 4 waves fill LDS.
+template <int BITS, int D, int TILES>
+struct Form {
+    static constexpr bool WIDE = BITS == 16 && D == 256 && TILES == 2;
+    static constexpr bool RING = BITS != 16 || WIDE;         // keys come through LDS
+    static constexpr int WAVES = WIDE ? 4 : 4 * TILES;
+    static constexpr int SIMD = WIDE ? 1 : D == 128 && TILES == 1 ? (RING ? 4 : 3) : 2;  // waves a SIMD that the registers are cut for
+    static constexpr int ROUND = 32 * WAVES;
+};
 
 template <int BITS, int D, bool INT8>
 struct Shape {
@@ -155,9 +161,10 @@ struct Shape {
     static constexpr int NK = D * BITS / 512;               // 16-byte pieces of a K row a lane group
     static constexpr int DPP = BITS == 16 ? 1 : 16 / BITS;  // dims of a V piece
     static constexpr int NV = D / 16 / DPP;
-    static constexpr int PAR = INT8 ? 8 : 16 * NG;  // halves of 8 keys' scales and biases
-    // A wave's 32 keys in LDS, each of its loads' 1 KB as the lanes hold it: K, V, scales and biases.
-    static constexpr int V0 = 2 * NK * 1024, P0 = V0 + NV * 1024, SLOT = P0 + 1024, LOADS = SLOT / 1024;
+    static constexpr int PAR = BITS == 16 ? 0 : INT8 ? 8 : 16 * NG;  // halves of 8 keys' scales and biases
+    // A wave's 32 keys in LDS, each of its loads' 1 KB as the lanes hold it: K, V, K's and V's scales and biases.
+    static constexpr int V0 = 2 * NK * 1024, P0 = V0 + NV * 1024, SLOT = P0 + (PAR ? 1024 : 0);
+    static constexpr int K_LOADS = 2 * NK + (PAR ? 1 : 0), V_LOADS = NV + (PAR ? 1 : 0);
 };
 
 // One load of 64 times 16 bytes to LDS. M0, which gives the place, is saved and restored so that the compiler's
@@ -201,18 +208,27 @@ __device__ __forceinline__ int64_t block_of(const PagedView& c, const Place& p, 
 }
 
 template <int BITS, int D, bool INT8>
-__device__ __forceinline__ void request(const PagedView& c, const Place& p, int h, int lane, uint32_t slot) {
+__device__ __forceinline__ void params_to_lds(const PagedView& c, const f16* par, const Place& p, int h, int lane, uint32_t place) {
+    constexpr int LPB = Shape<BITS, D, INT8>::PAR / 8;  // lanes of 8 keys' scales and biases
+    if constexpr (LPB > 0) {
+        if (lane < 4 * LPB)
+            to_lds<0>((const char*)(par + block_of(c, p, h, lane / LPB) * (8 * LPB)) + lane % LPB * 16, place);
+    }
+}
+template <int BITS, int D, bool INT8>
+__device__ __forceinline__ void request_k(const PagedView& c, const Place& p, int h, int lane, uint32_t slot) {
     using S = Shape<BITS, D, INT8>;
     constexpr int ROW = D * BITS / 8;
     const char* row = k_row(c, p, h, lane, ROW);
     run_to_lds<S::NK, 64>(row, slot);
     run_to_lds<S::NK, 64>(row + 4 * ROW, slot + S::NK * 1024);
+    params_to_lds<BITS, D, INT8>(c, c.k_par, p, h, lane, slot + S::P0);
+}
+template <int BITS, int D, bool INT8>
+__device__ __forceinline__ void request_v(const PagedView& c, const Place& p, int h, int lane, uint32_t slot) {
+    using S = Shape<BITS, D, INT8>;
     run_to_lds<S::NV, 256>(c.v + block_of(c, p, h, lane >> 4) * (D * BITS) + 16 * (lane & 15), slot + S::V0);
-    // K's and V's scales and biases of the 4 blocks, one behind the other (the lanes behind them repeat the last)
-    constexpr int LPB = S::PAR / 8;
-    const int i = min(lane, 8 * LPB - 1), blk = i / LPB & 3;
-    const f16* par = (i < 4 * LPB ? c.k_par : c.v_par) + block_of(c, p, h, blk) * S::PAR;
-    to_lds<0>((const char*)par + i % LPB * 16, slot + S::P0);
+    params_to_lds<BITS, D, INT8>(c, c.v_par, p, h, lane, slot + S::P0 + 512);
 }
 
 // fp16 keys stay in registers.
@@ -278,27 +294,29 @@ __device__ __forceinline__ float4v mfma(half8 a, half8 b, float4v c) {
 
 // Columns of a piece's rows that are joined over LDS at a time.
 constexpr int kJoin = 128;
-// Floats of LDS that hold four waves' keys, two chunks each, or their rows being joined [4][rows][kJoin + 4].
-template <int BITS, int D, bool INT8>
+// Floats of LDS that hold the waves' keys, or their rows being joined [WAVES][rows][kJoin + 4].
+template <int BITS, int D, bool INT8, int TILES>
 __host__ __device__ constexpr int key_floats(int rows) {
-    const int join = 4 * rows * (kJoin + 4), ring = BITS == 16 ? 0 : 8 * Shape<BITS, D, INT8>::SLOT / 4;
-    return join > ring ? join : ring;
+    const int waves = Form<BITS, D, TILES>::WAVES;
+    const int join = waves * rows * (kJoin + 4), keys = Form<BITS, D, TILES>::RING ? waves * Shape<BITS, D, INT8>::SLOT / 4 : 0;
+    return join > keys ? join : keys;
 }
 
-// RT row tiles of 16: a wave takes its keys once for all of them. The queries wait in LDS.
-template <int BITS, int D, bool INT8, int RT>
-__global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kernel(AttendArgs a) {
+template <int BITS, int D, bool INT8, int TILES>
+__global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, TILES>::SIMD)) void paged_attend_kernel(AttendArgs a) {
     using C = Shape<BITS, D, INT8>;
-    constexpr bool RING = BITS != 16;  // keys come through LDS
+    using F = Form<BITS, D, TILES>;
+    constexpr bool RING = F::RING;
+    constexpr int RT = TILES, KW = F::WAVES, NT = 64 * KW;
     constexpr int NG = C::NG, STEPS = D / 32, DPP = C::DPP, QS = D + 8, PPS = 16 / BITS;  // K steps of a piece
-    extern __shared__ __attribute__((aligned(16))) float lds[];  // keys or joins, (max, sum) [RT][4][16], q [RT * 16][QS]
-    const int lane = threadIdx.x & 63, kw = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = blockIdx.y;
+    extern __shared__ __attribute__((aligned(16))) float lds[];  // keys or joins, (max, sum) [TILES][KW][16], q [rows][QS]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = blockIdx.y;
     const int col = lane & 15, g = lane >> 4;
-    const int row0 = (int)blockIdx.z * RT * 16;
-    const int tile_rows = min(a.R - row0, 16);  // of the first tile
-    const int q_col = RT == 1 ? min(col, tile_rows - 1) : col;
-    float2* sml = (float2*)(lds + key_floats<BITS, D, INT8>(tile_rows));
-    f16* sq = (f16*)(sml + RT * 64);
+    const int row0 = (int)blockIdx.z * TILES * 16;  // the workgroup's first
+    const int tile_rows = min(a.R - row0, 16);      // of the first tile
+    const int q_rows = TILES == 1 ? tile_rows : 16 * TILES, q_col = TILES == 1 ? min(col, tile_rows - 1) : col;
+    float2* sml = (float2*)(lds + key_floats<BITS, D, INT8, TILES>(tile_rows));
+    f16* sq = (f16*)(sml + TILES * KW * 16);
 
     const uint32_t w = blockIdx.x;
     uint32_t at = 0, end = 0, per, rest;  // (one piece: end stays below)
@@ -321,7 +339,7 @@ __global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kerne
         Places ahead;
         auto look = [&](uint32_t r) {
             const int ln = afresh(lane);
-            const int64_t key = (int64_t)(r + (ln >> 1)) * kRound + 32 * kw + 16 * (ln & 1);
+            const int64_t key = (int64_t)(r + (ln >> 1)) * F::ROUND + 32 * wave + 16 * (ln & 1);
             const int j = (int)(key >> a.c.lg);
             int logical = key < keys ? (picked ? picked[j] : j) : -1;
             const int page = (uint32_t)logical < (uint32_t)a.width ? table[logical] : -1;
@@ -338,23 +356,22 @@ __global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kerne
             p.page1 = __builtin_amdgcn_readlane(ahead.page, i + 1);
             p.pos0 = __builtin_amdgcn_readlane(ahead.pos, i);
             p.pos1 = __builtin_amdgcn_readlane(ahead.pos, i + 1);
-            const int key = (int)(r * kRound) + 32 * kw, last = (1 << a.c.lg) - 1;
+            const int key = (int)(r * F::ROUND) + 32 * wave, last = (1 << a.c.lg) - 1;
             p.slot0 = key & last;
             p.slot1 = (key + 16) & last;
             return p;
         };
 
         Chunk<D> x;  // (not RING)
-        const char* ring = (const char*)lds + kw * 2 * C::SLOT;
-        const uint32_t ring0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)ring;
+        const char* slot = (const char*)lds + wave * C::SLOT;
+        const uint32_t slot0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)slot;
         // the query rows: requested, with the first pages, before the keys, behind which they would wait
-        constexpr int QN = RT * 16 * (D / 8) / 256;
+        constexpr int QN = TILES * 16 * (D / 8) / NT;
         half8 qr[QN];
         const int tid = afresh(threadIdx.x);
-        const int q_rows = RT == 1 ? tile_rows : 16 * RT;
 #pragma unroll
         for (int i = 0; i < QN; i++) {
-            const int c = (tid + 256 * i) / (D / 8), d = tid % (D / 8) * 8, row = min(row0 + c, a.R - 1);
+            const int c = (tid + NT * i) / (D / 8), d = tid % (D / 8) * 8, row = min(row0 + c, a.R - 1);
             const f16* from = a.q + b * a.q_seq + (int64_t)(h * a.G + row / a.n_rows) * a.q_head + row % a.n_rows * a.q_row;
             if (c < q_rows) qr[i] = *(const half8*)(from + d);
         }
@@ -362,13 +379,12 @@ __global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kerne
         if (!first) __syncthreads();  // (the last piece's rows and sums are read)
 #pragma unroll
         for (int i = 0; i < QN; i++) {
-            const int c = (tid + 256 * i) / (D / 8), d = tid % (D / 8) * 8;
+            const int c = (tid + NT * i) / (D / 8), d = tid % (D / 8) * 8;
             if (c < q_rows) *(half8*)(sq + c * QS + d) = qr[i];
         }
         if constexpr (RING) {
-            request<BITS, D, INT8>(a.c, cur, h, lane, ring0);
-            next = place_of(r0 + 1);
-            if (r0 + 1 < r1) request<BITS, D, INT8>(a.c, next, h, lane, ring0 + C::SLOT);
+            request_k<BITS, D, INT8>(a.c, cur, h, afresh(lane), slot0);
+            request_v<BITS, D, INT8>(a.c, cur, h, afresh(lane), slot0);
         } else {
             load_k(x, a.c, cur, h, afresh(lane));
             load_v(x, a.c, cur, h, afresh(lane));
@@ -409,73 +425,72 @@ __global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kerne
             for (int i = 0; i < D / 16; i++) o[t][i] = float4v{0, 0, 0, 0};
         }
         for (uint32_t r = r0; r < r1; r++) {
-            const char* slot = ring + ((r - r0) & 1) * C::SLOT;
-            if constexpr (RING) {
-                if (r + 1 < r1)
-                    wait_loads<C::LOADS>();
-                else
-                    wait_loads<0>();
-            } else {
-                next = place_of(r + 1);
-            }
+            next = place_of(r + 1);
+            if constexpr (RING) wait_loads<C::V_LOADS>();
             const f16* kpar = (const f16*)(slot + C::P0) + g * C::PAR;
             const int top = max(cur.pos0, cur.pos1) + 15;
             // scores: lane group g has keys 8 g + 4 u + i
             float s[RT][8];
+            constexpr int QG = BITS == 16 ? 1 : NG, PER_G = STEPS / QG;
 #pragma unroll
-            for (int v = 0; v < 2; v++) {
-                float4v acc[RT][NG];
+            for (int m = 0; m < QG; m++) {
+                float4v acc[2][RT];
+#pragma unroll
+                for (int v = 0; v < 2; v++)
+#pragma unroll
+                    for (int t = 0; t < RT; t++) acc[v][t] = float4v{0, 0, 0, 0};
+#pragma unroll
+                for (int j = m * PER_G; j < (m + 1) * PER_G; j++) {
+                    half8 q[RT];
+#pragma unroll
+                    for (int t = 0; t < RT; t++) q[t] = *(const half8*)(sq + (16 * t + q_col) * QS + 32 * j + 8 * g);
+#pragma unroll
+                    for (int v = 0; v < 2; v++) {
+                        half8 k;
+                        if constexpr (RING)
+                            k = k_codes<BITS>(*(const u32x4*)(slot + (v * C::NK + j / PPS) * 1024 + 16 * lane), j % PPS);
+                        else
+                            k = k_codes<BITS>(x.k[v][j], 0);
+#pragma unroll
+                        for (int t = 0; t < RT; t++) acc[v][t] = mfma(k, q[t], acc[v][t]);
+                    }
+                }
+                half8 ks, kb;
+                if constexpr (BITS != 16) {
+                    ks = *(const half8*)(kpar + 8 * m);
+                    if (!INT8) kb = *(const half8*)(kpar + 8 * (NG + m));
+                }
 #pragma unroll
                 for (int t = 0; t < RT; t++)
 #pragma unroll
-                    for (int m = 0; m < NG; m++) acc[t][m] = float4v{0, 0, 0, 0};
-#pragma unroll
-                for (int m = 0; m < STEPS; m++) {
-                    half8 k;
-                    if constexpr (RING)
-                        k = k_codes<BITS>(*(const u32x4*)(slot + (v * C::NK + m / PPS) * 1024 + 16 * lane), m % PPS);
-                    else
-                        k = k_codes<BITS>(x.k[v][m], 0);
-#pragma unroll
-                    for (int t = 0; t < RT; t++) {
-                        const half8 q = *(const half8*)(sq + (16 * t + q_col) * QS + 32 * m + 8 * g);
-                        acc[t][m / (STEPS / NG)] = mfma(k, q, acc[t][m / (STEPS / NG)]);
-                    }
-                }
-                half4v ks[NG], kb[NG];
-                if constexpr (RING) {
-#pragma unroll
-                    for (int m = 0; m < NG; m++) {
-                        ks[m] = *(const half4v*)(kpar + 8 * m + 4 * v);
-                        if (!INT8) kb[m] = *(const half4v*)(kpar + 8 * (NG + m) + 4 * v);
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < RT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        float y = 0.0f;
+                    for (int i = 0; i < 8; i++) {
+                        const float y = acc[i / 4][t][i % 4];
                         if constexpr (BITS == 16) {
-                            y = acc[t][0][i];
-#pragma unroll
-                            for (int m = 1; m < NG; m++) y += acc[t][m][i];
+                            s[t][i] = y;
                         } else if constexpr (INT8) {
-                            y = (float)ks[0][i] * (acc[t][0][i] + qsum[t][0]);
+                            s[t][i] = (float)ks[i] * (y + qsum[t][0]);
                         } else {
-#pragma unroll
-                            for (int m = 0; m < NG; m++) {
-                                y = __builtin_fmaf((float)ks[m][i], acc[t][m][i], y);
-                                y = __builtin_fmaf((float)kb[m][i], qsum[t][m], y);
-                            }
+                            s[t][i] = __builtin_fmaf((float)ks[i], y, m ? s[t][i] : 0.0f);
+                            s[t][i] = __builtin_fmaf((float)kb[i], qsum[t][m], s[t][i]);
                         }
-                        s[t][4 * v + i] = y;
                     }
+                // (formed here: put off behind a branch, the compiler's choice, they keep four times as many registers)
+                if constexpr (BITS != 16) {
+#pragma unroll
+                    for (int t = 0; t < RT; t++)
+#pragma unroll
+                        for (int i = 0; i < 8; i++) asm volatile("" : "+v"(s[t][i]));
+                }
+                if (RT > 1 && QG > 1) __builtin_amdgcn_sched_barrier(0);
             }
-            if constexpr (!RING) {
-                __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (RING) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read: its place takes the next
+                if (r + 1 < r1) request_k<BITS, D, INT8>(a.c, next, h, afresh(lane), slot0);
+            } else {
                 load_k(x, a.c, next, h, afresh(lane));
-                __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_sched_barrier(0);
             const bool masked = top >= seen_all;
             const int pos = (g & 2 ? cur.pos1 : cur.pos0) + 8 * (g & 1);
             u32x4 km;  // the keys before the sequence's end: what stands behind it takes no part, whatever it is
@@ -483,29 +498,32 @@ __global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kerne
 #pragma unroll
                 for (int j = 0; j < 4; j++) km[j] = (pos + 2 * j < len ? 0xFFFFu : 0u) | (pos + 2 * j + 1 < len ? 0xFFFF0000u : 0u);
             }
-            half8 vs[NG], vb{};
             if constexpr (RING) {
-#pragma unroll
-                for (int m = 0; m < NG; m++) vs[m] = *(const half8*)(kpar + 4 * C::PAR + 8 * m);
-                if constexpr (!INT8) vb = *(const half8*)(kpar + 4 * C::PAR + 8 * (NG + min(col, NG - 1)));
-                if (masked) {
-#pragma unroll
-                    for (int m = 0; m < NG; m++) vs[m] = as_h8(__builtin_bit_cast(u32x4, vs[m]) & km);
-                    vb = as_h8(__builtin_bit_cast(u32x4, vb) & km);
-                }
+                if (r + 1 < r1)
+                    wait_loads<C::K_LOADS>();
+                else
+                    wait_loads<0>();
             }
-            if constexpr (RING) {
+            const f16* vpar = kpar + 256;
+            auto v_scales = [&](const f16* par, int m) {  // of 8 keys in group m
+                const half8 x = *(const half8*)(par + 8 * m);
+                return masked ? as_h8(__builtin_bit_cast(u32x4, x) & km) : x;
+            };
+            if constexpr (BITS != 16) {
                 uint32_t high = 0;
 #pragma unroll
-                for (int m = 0; m < NG; m++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) high |= __builtin_bit_cast(u32x4, vs[m])[j];
+                for (int m = 0; m < NG; m++) {
+                    const u32x4 x = __builtin_bit_cast(u32x4, v_scales(vpar, m));
+                    high |= x[0] | x[1] | x[2] | x[3];
+                }
                 if (__any((high & 0x40004000u) != 0)) {  // V scales of 2 and more: P gives way, so that P times a scale fits a half
                     float big = 0.0f;
+#pragma unroll 1
+                    for (int m = 0; m < NG; m++) {
+                        const half8 x = v_scales(vpar, m);
 #pragma unroll
-                    for (int m = 0; m < NG; m++)
-#pragma unroll
-                        for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf((float)vs[m][i]));
+                        for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf((float)x[i]));
+                    }
                     big = wave_reduce(big, OpMax());
                     const int e = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(big) >> 23) - 127);
                     if (e > E) {
@@ -520,6 +538,7 @@ __global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kerne
                         }
                     }
                 }
+                vpar += afresh(0);  // (read again below, not held)
             }
 #pragma unroll
             for (int t = 0; t < RT; t++) {
@@ -556,16 +575,20 @@ __global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kerne
                     for (int i = 0; i < 8; i++) ph[t][i] = (f16)s[t][i];
             }
             if constexpr (BITS == 16) {
-                if (masked) {
 #pragma unroll
-                    for (int j = 0; j < C::NV; j++) x.v[j] &= km;
+                for (int j = 0; j < C::NV; j++) {
+                    u32x4 v;
+                    if constexpr (RING)
+                        v = *(const u32x4*)(slot + C::V0 + j * 1024 + 16 * lane);
+                    else
+                        v = x.v[j];
+                    if (masked) v &= km;
+#pragma unroll
+                    for (int t = 0; t < RT; t++) o[t][j] = mfma(as_h8(v), ph[t], o[t][j]);
                 }
-#pragma unroll
-                for (int j = 0; j < C::NV; j++)
-#pragma unroll
-                    for (int t = 0; t < RT; t++) o[t][j] = mfma(v_codes<16>(x.v[j], 0), ph[t], o[t][j]);
             } else {
                 if constexpr (!INT8) {
+                    half8 vb = v_scales(vpar, NG + min(col, NG - 1));
                     if (col >= NG) vb = half8{};
 #pragma unroll
                     for (int t = 0; t < RT; t++) ob[t] = mfma(vb, ph[t], ob[t]);
@@ -578,10 +601,11 @@ __global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kerne
                 constexpr int PER = C::NV / NG;
 #pragma unroll
                 for (int m = 0; m < NG; m++) {
+                    const half8 vs = v_scales(vpar, m);
 #pragma unroll
                     for (int t = 0; t < RT; t++) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) ph[t][i] = (f16)(s[t][i] * (float)vs[m][i]);
+                        for (int i = 0; i < 8; i++) ph[t][i] = (f16)__builtin_fmaf(s[t][i], (float)vs[i], 0.0f);
                         if constexpr (INT8) {
 #pragma unroll
                             for (int i = 0; i < 8; i++) lp[t] += (float)ph[t][i];
@@ -597,25 +621,22 @@ __global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kerne
                             for (int t = 0; t < RT; t++) o[t][j * DPP + e] = mfma(v, ph[t], o[t][j * DPP + e]);
                         }
                     }
+                    if (RT > 1) __builtin_amdgcn_sched_barrier(0);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
             if constexpr (RING) {
-                cur = next;
-                if (r + 2 < r1) {  // this chunk is read: its place takes the one behind the next
-                    next = place_of(r + 2);
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    request<BITS, D, INT8>(a.c, next, h, afresh(lane), ring0 + ((r - r0) & 1) * C::SLOT);
-                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (r + 1 < r1) request_v<BITS, D, INT8>(a.c, next, h, afresh(lane), slot0);
             } else {
-                __builtin_amdgcn_sched_barrier(0);
                 load_v(x, a.c, next, h, afresh(lane));
-                __builtin_amdgcn_sched_barrier(0);
-                cur = next;
             }
+            __builtin_amdgcn_sched_barrier(0);
+            cur = next;
         }
         if constexpr (RING) __syncthreads();  // (every wave has read its keys: their place takes the rows)
 
-        // the rows' sums over the lane groups, biases, and the four waves joined
+        // the rows' sums over the lane groups, biases, and the waves of a tile joined
         const bool done = r0 == 0 && r1 == piece.all;
 #pragma unroll
         for (int t = 0; t < RT; t++) {
@@ -625,9 +646,9 @@ __global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kerne
                 lp[t] += lane_xor<16>(lp[t], lane);
                 lp[t] += lane_xor<32>(lp[t], lane);
             }
-            if (g == 0) sml[(t * 4 + kw) * 16 + col] = float2{M[t] + (float)E, l[t]};
+            if (g == 0) sml[(t * KW + wave) * 16 + col] = float2{M[t] + (float)E, l[t]};
         }
-        float* so = lds + (kw * tile_rows + col) * (kJoin + 4);
+        float* so = lds + (wave * tile_rows + col) * (kJoin + 4);
 #pragma unroll
         for (int t = 0; t < RT; t++) {
             const int rows = min(a.R - row0 - 16 * t, 16);  // (none or fewer: nothing is written)
@@ -657,22 +678,19 @@ __global__ __launch_bounds__(256, waves_of(BITS, D, RT)) void paged_attend_kerne
                     }
                 }
                 __syncthreads();
-                for (int i = afresh(threadIdx.x); i < rows * (kJoin / 4); i += 256) {
+                for (int i = afresh(threadIdx.x); i < rows * (kJoin / 4); i += NT) {
                     const int c = i / (kJoin / 4), d = i % (kJoin / 4) * 4;
-                    float2 ml[4];
                     float mm = kNone;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        ml[k] = sml[(t * 4 + k) * 16 + c];
-                        mm = fmaxf(mm, ml[k].x);
-                    }
+                    for (int k = 0; k < KW; k++) mm = fmaxf(mm, sml[(t * KW + k) * 16 + c].x);
                     float4v y = {0, 0, 0, 0};
                     float sum = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float f = __builtin_amdgcn_exp2f(ml[k].x - mm);
+                    for (int k = 0; k < KW; k++) {
+                        const float2 ml = sml[(t * KW + k) * 16 + c];
+                        const float f = __builtin_amdgcn_exp2f(ml.x - mm);
                         y += f * *(const float4v*)(lds + (k * tile_rows + c) * (kJoin + 4) + d);
-                        sum = __builtin_fmaf(f, ml[k].y, sum);
+                        sum = __builtin_fmaf(f, ml.y, sum);
                     }
                     const int64_t rw = row0 + 16 * t + c;
                     if (done) {
@@ -773,27 +791,27 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
     *(half4v*)to = half4v{(f16)(y[0] * inv), (f16)(y[1] * inv), (f16)(y[2] * inv), (f16)(y[3] * inv)};
 }
 
-template <int BITS, int D, bool INT8, int RT>
+template <int BITS, int D, bool INT8, int TILES>
 size_t attend_lds(int R) {
-    const int rows = std::min(R, 16), q_rows = RT == 1 ? rows : 16 * RT;
-    return (size_t)key_floats<BITS, D, INT8>(rows) * 4 + RT * 64 * 8 + (size_t)q_rows * (D + 8) * 2;
+    const int rows = std::min(R, 16), q_rows = TILES == 1 ? rows : 16 * TILES;
+    return (size_t)key_floats<BITS, D, INT8, TILES>(rows) * 4 + TILES * Form<BITS, D, TILES>::WAVES * 16 * 8 + (size_t)q_rows * (D + 8) * 2;
 }
-template <int BITS, int D, bool INT8, int RT>
+template <int BITS, int D, bool INT8, int TILES>
 int launch_attend(const AttendArgs& a, hipStream_t stream) {
-    const size_t lds = attend_lds<BITS, D, INT8, RT>(a.R);
-    const void* f = (const void*)paged_attend_kernel<BITS, D, INT8, RT>;
+    const size_t lds = attend_lds<BITS, D, INT8, TILES>(a.R);
+    static_assert(BITS == 16 || 8 * Shape<BITS, D, INT8>::PAR <= 512, "K's and V's scales and biases of 32 keys have 512 bytes each");
+    const void* f = (const void*)paged_attend_kernel<BITS, D, INT8, TILES>;
     if (int rc = ensure_dynamic_lds(f, lds)) return rc;
-    const dim3 grid(a.workers, a.c.hkv, (a.R + 16 * RT - 1) / (16 * RT));
-    hipLaunchKernelGGL((paged_attend_kernel<BITS, D, INT8, RT>), grid, dim3(256), lds, stream, a);
+    const dim3 grid(a.workers, a.c.hkv, (a.R + 16 * TILES - 1) / (16 * TILES));
+    hipLaunchKernelGGL((paged_attend_kernel<BITS, D, INT8, TILES>), grid, dim3(64 * Form<BITS, D, TILES>::WAVES), lds, stream, a);
     QW_HIP_CHECK(hipGetLastError());
     return QW_OK;
 }
-// f(row tiles of a workgroup) for the call's rows
 template <class F>
-int by_shape(int bits, bool int8, int D, int R, F f) {
+int by_shape(int bits, bool int8, int D, int n_tiles, F f) {
     using std::integral_constant;
     auto tiles = [&](auto b, auto i8, auto d) {
-        return R <= 16 ? f(b, i8, d, integral_constant<int, 1>()) : f(b, i8, d, integral_constant<int, 2>());
+        return n_tiles == 1 ? f(b, i8, d, integral_constant<int, 1>()) : f(b, i8, d, integral_constant<int, 2>());
     };
     auto dims = [&](auto b, auto i8) {
         return D == 256 ? tiles(b, i8, integral_constant<int, 256>()) : tiles(b, i8, integral_constant<int, 128>());
@@ -830,7 +848,18 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     if (q.n_seq == 0) return QW_OK;
     QW_REQUIRE(out && (uintptr_t)out % 8 == 0, QW_ERR_INVALID_ARGUMENT, "paged attention: out null or off 8 bytes");
     const int64_t most = std::min<int64_t>(q.table_width, picked ? n_picked : q.table_width) * c.page_size;  // keys of a sequence
-    const int64_t rounds = (most + kRound - 1) / kRound * q.n_seq;
+    const int tiles = (q.n_q_heads / c.hkv) * q.n_rows <= 16 ? 1 : 2;
+    // as many workers as the card holds at a time, all heads and row tiles counted
+    int held = 0, round = 0;
+    by_shape(c.bits, c.int8(), c.D, tiles, [&](auto b, auto i8, auto d, auto t) {
+        using F = Form<decltype(b)::value, decltype(d)::value, decltype(t)::value>;
+        const size_t lds = attend_lds<decltype(b)::value, decltype(d)::value, decltype(i8)::value, decltype(t)::value>(
+            (q.n_q_heads / c.hkv) * q.n_rows);
+        held = std::max(1, std::min<int>(4 * F::SIMD / F::WAVES, (int)(160 * 1024 / lds)));
+        round = F::ROUND;
+        return QW_OK;
+    });
+    const int64_t rounds = (most + round - 1) / round * q.n_seq;
     QW_REQUIRE(rounds < (1ll << 31), QW_ERR_UNSUPPORTED, "paged attention: n_seq * table_width * page_size below 2^38 expected");
     // (one handle, a stream a thread: they would share a workspace)
     QW_REQUIRE(stream != hipStreamPerThread, QW_ERR_UNSUPPORTED, "paged attention: hipStreamPerThread; name a stream");
@@ -852,12 +881,8 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     a.picked = picked;
     a.n_picked = n_picked;
     a.scale2 = scale * kLog2e;
-    // as many workers as the card holds at a time, all heads and row tiles counted
-    const int held = by_shape(c.bits, c.int8(), c.D, a.R, [&](auto b, auto i8, auto d, auto rt) {
-        constexpr int B = decltype(b)::value, DD = decltype(d)::value, RT = decltype(rt)::value;
-        return std::max(1, std::min<int>(waves_of(B, DD, RT), (int)(160 * 1024 / attend_lds<B, DD, decltype(i8)::value, RT>(a.R))));
-    });
-    const int groups = a.R <= 16 ? 1 : (a.R + 31) / 32;
+    const int groups = (a.R + 16 * tiles - 1) / (16 * tiles);
+    a.round = round;
     a.workers = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, 256 * held / ((int64_t)c.hkv * groups)));
     const int64_t parts = (int64_t)a.workers * 2 * c.hkv * a.R;
     void* ws = nullptr;
@@ -865,8 +890,8 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     a.part_o = (float*)ws;
     a.part_ml = (float2*)(a.part_o + parts * c.D);
     if (rounds > 0) {
-        const int rc = by_shape(c.bits, c.int8(), c.D, a.R, [&](auto b, auto i8, auto d, auto rt) {
-            return launch_attend<decltype(b)::value, decltype(d)::value, decltype(i8)::value, decltype(rt)::value>(a, stream);
+        const int rc = by_shape(c.bits, c.int8(), c.D, tiles, [&](auto b, auto i8, auto d, auto t) {
+            return launch_attend<decltype(b)::value, decltype(d)::value, decltype(i8)::value, decltype(t)::value>(a, stream);
         });
         if (rc) return rc;
     }
