@@ -6,8 +6,9 @@
 //   score(page) = top(page) * max over rows of sum_d (max(q_d, 0) hi_d + min(q_d, 0) lo_d)
 // with one rounding, so that the picks do not depend on any order of summation. It is a product of
 // matrices of 2 D codes (v_mfma_i32_16x16x64_i8: 16 pages by 16 rows), bound by reading 2 D + 4 bytes a page.
-// A second launch finds the score of the last page that stays, two bits a step over keys held in
-// registers, and writes the picks in ascending order.
+// A second launch finds the score of the last page that stays: a histogram of the scores in LDS gives its bin, the
+// bin's few members are ranked one against the other (where they are many, as with ties, the score is found two
+// bits a step over the keys, which wait in registers), and the picks are written in ascending order.
 #include <algorithm>
 
 #include "paged.hpp"
@@ -49,9 +50,27 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectArgs a) {
     constexpr int STEPS = D / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
     const int h = blockIdx.y, b = blockIdx.z;
-    const int pages = pages_of(a, b);
     const int first = ((int)blockIdx.x * 4 + wave) * a.tiles * 16;
-    if (pages <= a.budget || first >= pages) return;  // (they all stay; no barrier follows)
+    if (first >= a.width) return;  // (no barrier follows)
+    // the bounds of 16 pages: requested before the queries' codes form
+    struct Bounds {
+        int4v x[2 * STEPS];
+        float top;
+        bool there;
+    } cur, next;
+    auto page_at = [&](int p0) { return a.table[b * a.table_stride + min(p0 + col, a.width - 1)]; };
+    auto load = [&](Bounds& to, int page) {
+        to.there = (uint32_t)page < (uint32_t)a.c.n_pages;
+        const int64_t ph = (int64_t)(to.there ? page : 0) * a.c.hkv + h;
+        const int8_t* codes = a.c.codes + ph * 2 * D + 16 * g;
+        to.top = a.c.top[ph];
+#pragma unroll
+        for (int j = 0; j < 2 * STEPS; j++) to.x[j] = *(const int4v*)(codes + 64 * j);
+    };
+    const int page0 = page_at(first), page1 = page_at(first + 16);
+    load(cur, page0);
+    const int pages = pages_of(a, b);
+    if (pages <= a.budget || first >= pages) return;  // (they all stay)
     auto row_at = [&](int tile) {
         const int row = min(16 * tile + col, a.R - 1);
         return a.q + b * a.q_seq + (int64_t)(h * a.G + row / a.n_rows) * a.q_head + row % a.n_rows * a.q_row + 16 * g;
@@ -91,20 +110,18 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectArgs a) {
                 up[j][w] = (int)u, down[j][w] = (int)d;
             }
         const bool real = 16 * t + col < a.R;
+        if (t > 0) load(cur, page0);
+        int ahead = page1;  // the page behind the next 16's bounds, which are on their way
         for (int p0 = first; p0 < last; p0 += 16) {
-            const int page = a.table[b * a.table_stride + min(p0 + col, pages - 1)];
-            const bool there = (uint32_t)page < (uint32_t)a.c.n_pages;
-            const int64_t ph = (int64_t)(there ? page : 0) * a.c.hkv + h;
-            const int8_t* codes = a.c.codes + ph * 2 * D + 16 * g;
-            const float top = a.c.top[ph];
-            int4v x[2 * STEPS];
-#pragma unroll
-            for (int j = 0; j < 2 * STEPS; j++) x[j] = *(const int4v*)(codes + 64 * j);
+            if (p0 + 16 < last) {
+                load(next, ahead);
+                ahead = page_at(p0 + 32);
+            }
             int4v acc = {0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < STEPS; j++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[j], up[j], acc, 0, 0, 0);
+            for (int j = 0; j < STEPS; j++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.x[j], up[j], acc, 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < STEPS; j++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[STEPS + j], down[j], acc, 0, 0, 0);
+            for (int j = 0; j < STEPS; j++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(cur.x[STEPS + j], down[j], acc, 0, 0, 0);
             // pages p0 + 4 g + i: the largest of the 16 rows
             int best[4];
 #pragma unroll
@@ -120,10 +137,11 @@ __global__ __launch_bounds__(256) void paged_score_kernel(SelectArgs a) {
             const int b0 = __shfl(best[0], from), b1 = __shfl(best[1], from), b2 = __shfl(best[2], from), b3 = __shfl(best[3], from);
             const int m = col & 2 ? (col & 1 ? b3 : b2) : (col & 1 ? b1 : b0);
             if (g == 0 && p0 + col < last) {
-                float s = there ? top * (float)m + 0.0f : -INFINITY;  // (-0 becomes 0)
+                float s = cur.there ? cur.top * (float)m + 0.0f : -INFINITY;  // (-0 becomes 0)
                 if (t > 0) s = fmaxf(s, scores[p0 + col]);
                 scores[p0 + col] = s;
             }
+            cur = next;
         }
     }
 }
@@ -132,48 +150,147 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
     return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(x), 63);
 }
 
-// Whole numbers that order as the scores do; 0 for no page.
+// Whole numbers that order as the scores do; 0 for none.
 __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t u = __float_as_uint(x);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+__device__ __forceinline__ float unordered(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+constexpr uint32_t kNoPage = 0x007FFFFFu;  // ordered(-infinity): a column that names no page
+constexpr int kBins = 2048, kMembers = 256;
+
+// KPT scores a thread in registers, or (0) as many as there are, read again where they are looked at.
 template <int NT, int KPT>
 __global__ __launch_bounds__(NT) void paged_pick_kernel(SelectArgs a) {
     constexpr int NW = NT / 64;
-    __shared__ uint32_t sm[2][NW][4];
+    __shared__ uint32_t sm[2][NW][4], hist[kBins], found[4];
+    __shared__ uint2 member[kMembers];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int h = blockIdx.x, b = blockIdx.y;
+    const float* scores = a.scores + ((int64_t)b * a.c.hkv + h) * a.width;
+    const int per_thread = KPT ? KPT : (a.width + NT - 1) / NT;
+    const int first = wave * 64 * per_thread + lane;
+    constexpr int U = KPT ? KPT : 1;
+    float score[U];
+    if constexpr (KPT > 0) {  // (with the lengths; what stands behind a sequence's pages is not looked at)
+#pragma unroll
+        for (int i = 0; i < KPT; i++) score[i] = a.width > a.budget && first + 64 * i < a.width ? scores[first + 64 * i] : 0.0f;
+    }
     const int n = pages_of(a, b);
     int32_t* picked = a.picked + ((int64_t)b * a.c.hkv + h) * a.budget;
     if (n <= a.budget) {
         for (int i = threadIdx.x; i < a.budget; i += NT) picked[i] = i < n ? i : -1;
         return;
     }
-    const float* scores = a.scores + ((int64_t)b * a.c.hkv + h) * a.width;
     const int lo = a.sink, hi = n - a.recent;
     const uint32_t need = (uint32_t)(a.budget - a.sink - a.recent);
-    const int first = wave * 64 * KPT + lane;
-    uint32_t key[KPT];
-    float least_f = INFINITY, most_f = -INFINITY;
+    uint32_t key[U];
+    if constexpr (KPT > 0) {
 #pragma unroll
-    for (int i = 0; i < KPT; i++) {
-        const int p = first + 64 * i;
-        const bool in = p >= lo && p < hi;
-        const float s = in ? scores[p] : 0.0f;
-        key[i] = in ? ordered(s) : 0u;
-        if (in) least_f = OpMin()(least_f, s), most_f = OpMax()(most_f, s);
+        for (int i = 0; i < KPT; i++) {
+            const int p = first + 64 * i;
+            key[i] = p >= lo && p < hi ? ordered(score[i]) : 0u;
+        }
     }
-    uint32_t least = ordered(wave_reduce(least_f, OpMin())), most = ordered(wave_reduce(most_f, OpMax()));
-    if (lane == 0) sm[0][wave][0] = least, sm[0][wave][1] = most;
+    auto key_at = [&](int i) {
+        if constexpr (KPT > 0) return key[i];
+        const int p = first + 64 * i;
+        return p >= lo && p < hi ? ordered(scores[p]) : 0u;
+    };
+    float least_f = INFINITY, most_f = -INFINITY;  // of the scores of pages that there are
+#pragma unroll U
+    for (int i = 0; i < per_thread; i++) {
+        const uint32_t k = key_at(i);
+        if (k > kNoPage) least_f = OpMin()(least_f, unordered(k)), most_f = OpMax()(most_f, unordered(k));
+    }
+    least_f = wave_reduce(least_f, OpMin());
+    most_f = wave_reduce(most_f, OpMax());
+    if (lane == 0) sm[0][wave][0] = __float_as_uint(least_f), sm[0][wave][1] = __float_as_uint(most_f);
+    for (int i = threadIdx.x; i < kBins; i += NT) hist[i] = 0;
+    if (threadIdx.x == 0) found[2] = 0;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; w++) least = min(least, sm[0][w][0]), most = max(most, sm[0][w][1]);
-    least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
-    // the largest value that `need` keys reach: bits above the highest that differs are common to all
+    for (int w = 0; w < NW; w++) {
+        least_f = OpMin()(least_f, __uint_as_float(sm[0][w][0]));
+        most_f = OpMax()(most_f, __uint_as_float(sm[0][w][1]));
+    }
     uint32_t cut = ~0u;
+    bool few = true;
     if (need > 0) {
+        // bins grow with the scores (differences, products and whole parts keep an order), the lowest for what has none
+        const float per = (float)kBins / (most_f - least_f);
+        auto bin_of = [&](uint32_t k) { return (int)fminf(fmaxf((unordered(k) - least_f) * per, 0.0f), (float)(kBins - 1)); };
+#pragma unroll U
+        for (int i = 0; i < per_thread; i++) {
+            const uint32_t k = key_at(i);
+            if (k) atomicAdd(&hist[bin_of(k)], 1u);
+        }
+        __syncthreads();
+        // the bin in which the sum from the top reaches `need`
+        constexpr int PER = kBins / NT;
+        uint32_t mine[PER], sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) sum += mine[i] = hist[kBins - 1 - ((int)threadIdx.x * PER + i)];
+        uint32_t through = wave_scan(sum);
+        if (lane == 63) sm[1][wave][0] = through;
+        __syncthreads();
+        for (int w = 0; w < wave; w++) through += sm[1][w][0];
+        if (through >= need && through - sum < need) {
+            uint32_t above = through - sum;
+            int i = 0;
+#pragma unroll
+            for (int k = 0; k < PER - 1; k++)
+                if (i == k && above + mine[k] < need) above += mine[k], i++;
+            found[0] = kBins - 1 - (threadIdx.x * PER + i);
+            found[1] = above;
+            found[3] = hist[kBins - 1 - (threadIdx.x * PER + i)];
+        }
+        __syncthreads();
+        const int bin = (int)found[0];
+        few = found[3] <= kMembers;
+        if (few) {
+#pragma unroll U
+            for (int i = 0; i < per_thread; i++) {
+                const uint32_t k = key_at(i);
+                if (k && bin_of(k) == bin) member[atomicAdd(&found[2], 1u)] = uint2{k, (uint32_t)(first + 64 * i)};
+            }
+            __syncthreads();
+            const uint32_t members = found[3], room = need - found[1];
+            if (threadIdx.x < members) {
+                const uint2 me = member[threadIdx.x];
+                uint32_t before = 0;
+                for (uint32_t i = 0; i < members; i++) {
+                    const uint2 x = member[i];
+                    before += x.x > me.x || (x.x == me.x && x.y < me.y);
+                }
+                if (before + 1 == room) found[0] = me.x;
+            }
+            __syncthreads();
+            cut = __builtin_amdgcn_readfirstlane(found[0]);
+        }
+    }
+    // many members: the largest value that `need` keys reach; bits above the highest that differs are common to all
+    if (!few) {
+        uint32_t least = ~0u, most = 0;
+#pragma unroll U
+        for (int i = 0; i < per_thread; i++) {
+            const uint32_t k = key_at(i);
+            if (k) least = min(least, k), most = max(most, k);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            least = min(least, (uint32_t)__shfl_xor((int)least, d));
+            most = max(most, (uint32_t)__shfl_xor((int)most, d));
+        }
+        if (lane == 0) sm[0][wave][0] = least, sm[0][wave][1] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; w++) least = min(least, sm[0][w][0]), most = max(most, sm[0][w][1]);
+        least = __builtin_amdgcn_readfirstlane(least);
+        most = __builtin_amdgcn_readfirstlane(most);
         const int top = least == most ? 0 : 32 - __builtin_clz(least ^ most);  // bits to find
         int shift = (top + 1) & ~1;
         cut = shift >= 32 ? 0u : most >> shift << shift;
@@ -182,23 +299,12 @@ __global__ __launch_bounds__(NT) void paged_pick_kernel(SelectArgs a) {
             shift -= 2;
             const uint32_t t1 = cut | 1u << shift, t2 = cut | 2u << shift, t3 = cut | 3u << shift;
             uint32_t c1 = 0, c2 = 0, c3 = 0;
-            if constexpr (KPT <= 8) {
-#pragma unroll
-                for (int i = 0; i < KPT; i++) {
-                    c1 += __builtin_popcountll(__ballot(key[i] >= t1));
-                    c2 += __builtin_popcountll(__ballot(key[i] >= t2));
-                    c3 += __builtin_popcountll(__ballot(key[i] >= t3));
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < KPT; i++) {
-                    c1 += key[i] >= t1;
-                    c2 += key[i] >= t2;
-                    c3 += key[i] >= t3;
-                }
-                c1 = wave_sum(c1 | c2 << 16);  // (a wave counts 4096 at most)
-                c2 = c1 >> 16, c1 &= 0xFFFFu;
-                c3 = wave_sum(c3);
+#pragma unroll U
+            for (int i = 0; i < per_thread; i++) {
+                const uint32_t k = key_at(i);
+                c1 += __builtin_popcountll(__ballot(k >= t1));
+                c2 += __builtin_popcountll(__ballot(k >= t2));
+                c3 += __builtin_popcountll(__ballot(k >= t3));
             }
             if (lane == 0) sm[turn][wave][0] = c1, sm[turn][wave][1] = c2, sm[turn][wave][2] = c3;
             __syncthreads();
@@ -212,13 +318,14 @@ __global__ __launch_bounds__(NT) void paged_pick_kernel(SelectArgs a) {
     }
     // those above the cut, the protected ones, and of the equal ones the first that there is room for
     uint32_t above = 0, equal = 0, higher = 0;
-#pragma unroll
-    for (int i = 0; i < KPT; i++) {
+#pragma unroll U
+    for (int i = 0; i < per_thread; i++) {
         const int p = first + 64 * i;
-        const bool kept = p < n && (p < lo || p >= hi), more = need > 0 && key[i] > cut;
+        const uint32_t k = key_at(i);
+        const bool kept = p < n && (p < lo || p >= hi), more = need > 0 && k > cut;
         above += kept || more;
         higher += more;
-        equal += need > 0 && key[i] == cut;
+        equal += need > 0 && k == cut;
     }
     const uint32_t both = wave_sum(above | equal << 16);
     above = both & 0xFFFFu, equal = both >> 16;
@@ -236,18 +343,18 @@ __global__ __launch_bounds__(NT) void paged_pick_kernel(SelectArgs a) {
         ties += e;
     }
     const uint64_t below = (1ull << lane) - 1;
-#pragma unroll
-    for (int i = 0; i < KPT; i++) {
+#pragma unroll U
+    for (int i = 0; i < per_thread; i++) {
         const int p = first + 64 * i;
-        const bool tie = need > 0 && key[i] == cut;
+        const uint32_t k = key_at(i);
+        const bool tie = need > 0 && k == cut;
         const uint64_t tied = __ballot(tie);
-        const bool in = (p < n && (p < lo || p >= hi)) || (need > 0 && key[i] > cut) ||
+        const bool in = (p < n && (p < lo || p >= hi)) || (need > 0 && k > cut) ||
                         (tie && ties + (uint32_t)__builtin_popcountll(tied & below) < room);
         const uint64_t all = __ballot(in);
         if (in) picked[at + (uint32_t)__builtin_popcountll(all & below)] = p;
         at += (uint32_t)__builtin_popcountll(all);
         ties += (uint32_t)__builtin_popcountll(tied);
-        if (KPT > 8) __builtin_amdgcn_sched_barrier(0);  // (masks of all steps at once spill)
     }
 }
 
@@ -297,7 +404,7 @@ int paged_select(PagedCache& c, const PagedQuery& q, int budget, int sink, int r
     else if (q.table_width <= 8192)
         hipLaunchKernelGGL((paged_pick_kernel<1024, 8>), grid, dim3(1024), 0, stream, a);
     else
-        hipLaunchKernelGGL((paged_pick_kernel<1024, 64>), grid, dim3(1024), 0, stream, a);
+        hipLaunchKernelGGL((paged_pick_kernel<1024, 0>), grid, dim3(1024), 0, stream, a);
     QW_HIP_CHECK(hipGetLastError());
     return QW_OK;
 }
