@@ -3,8 +3,11 @@
 // The codecs are the caches' own: MLX affine in groups of 64 dims (quant.hpp), per-token int8, fp16.
 // A workgroup takes one page of one head, so that every word that holds several keys' codes, and the
 // page's bounds, have one writer. A wave takes 8 slots (two times 8 at D = 128): a lane holds 4 dims of
-// 8 tokens of K and V, 16 lanes a group, whose extremes come by DPP; V's words of 8 keys form in the
-// lane. Where a call covers part of such a word the rest is kept.
+// 8 tokens of K and V, 16 lanes a group, whose extremes come by DPP. Those 16 lanes then each form the
+// step and base of one of the 16 rows (8 tokens' K and V), with its divisions, and hand them round; codes come
+// by a product and one correction of its remainder, and are packed as bytes as they are converted (two
+// keys' 4-bit codes as one number), so that V's words of 8 keys need no transposition. Where a call
+// covers part of such a word the rest is kept; tokens that a call does not have cost nothing.
 #include <algorithm>
 
 #include "paged.hpp"
@@ -114,35 +117,57 @@ struct FMin {
     __device__ float operator()(float a, float b) const { return fminf(a, b); }
 };
 
-// 4 dims' codes (a byte each) of a row, and the group's scale and bias.
-template <int BITS, bool INT8, int D>
-__device__ __forceinline__ uint32_t quantize4(half4v x, f16& scale, f16& bias) {
-    float f[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) f[i] = (float)x[i];
-    uint32_t w = 0;
-    if constexpr (INT8) {
-        const float top = reduce_row<D>(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))), FMax());
-        scale = (f16)(top / 127.0f);
+// f of 0 .. 7, as constants.
+template <class F>
+__device__ __forceinline__ void each8(F f) {
+    using std::integral_constant;
+    f(integral_constant<int, 0>()), f(integral_constant<int, 1>()), f(integral_constant<int, 2>()), f(integral_constant<int, 3>());
+    f(integral_constant<int, 4>()), f(integral_constant<int, 5>()), f(integral_constant<int, 6>()), f(integral_constant<int, 7>());
+}
+
+// Lane J's value to all 16 lanes of its row.
+template <int J>
+__device__ __forceinline__ float of_lane(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(x), 0x150 + J, 0xF, 0xF, false));
+}
+// x into lane J of each row of 16.
+template <int J>
+__device__ __forceinline__ void to_lane(float& at, float x, int r16) {
+    at = r16 == J ? x : at;
+}
+
+// Steps of the rows' codes: value = code * step + base, inv = 1 / step.
+struct Steps {
+    float step, base, inv;
+};
+template <int BITS, bool INT8>
+__device__ __forceinline__ Steps steps_of(float mn, float mx, f16& scale, f16& bias) {
+    if constexpr (INT8) {  // mx: the row's largest magnitude
+        scale = (f16)(mx / 127.0f);
         if ((float)scale == 0.0f) scale = (f16)1.0f;
         bias = (f16)0.0f;
-        const float s = (float)scale;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float c = __builtin_rintf((float)(f16)(f[i] / s));
-            w |= (uint32_t)((int)fminf(fmaxf(c, -128.0f), 127.0f) + 128) << (8 * i);
-        }
+        return Steps{(float)scale, 0.0f, 1.0f / (float)scale};
     } else {
-        const float mn = reduce16(fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), FMin());
-        const float mx = reduce16(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), FMax());
         const AffineGroup q = affine_group(mn, mx, BITS);
-        const float inv = 1.0f / q.scale;
         scale = (f16)q.scale;
         bias = (f16)q.bias;
-#pragma unroll
-        for (int i = 0; i < 4; i++) w |= (uint32_t)affine_code_inv(f[i], q, inv, BITS) << (8 * i);
+        return Steps{q.scale, q.bias, 1.0f / q.scale};
     }
-    return w;
+}
+// A code as a whole number in a float, int8's 128 above itself. The quotient: inv is the step's reciprocal, rounded
+// once; the product of it and its remainder, which an fma has exactly, correct it to the rounded quotient
+// (Markstein, 1990), as the codec's division gives it. x finite.
+template <int BITS, bool INT8>
+__device__ __forceinline__ float code_of(float x, const Steps& q) {
+    const float t = INT8 ? x : x - q.base;
+    float p = t * q.inv;
+    p = __builtin_fmaf(__builtin_fmaf(-p, q.step, t), q.inv, p);
+    if constexpr (INT8) return __builtin_amdgcn_fmed3f(__builtin_rintf((float)(f16)p), -128.0f, 127.0f) + 128.0f;
+    return __builtin_amdgcn_fmed3f(__builtin_rintf(p), 0.0f, (float)((1 << BITS) - 1));
+}
+template <int BYTE>
+__device__ __forceinline__ uint32_t put_byte(uint32_t w, float c) {
+    return __builtin_amdgcn_cvt_pk_u8_f32(c, BYTE, w);
 }
 
 // Byte 64 i + 16 g + .. of a K row where a lane's 4 dims (of index li) begin.
@@ -154,7 +179,7 @@ __device__ __forceinline__ int k_at(int li) {
     return (c >> 2) * 64 + g * 16 + (c & 3) * 4;
 }
 
-constexpr int kStoreWaves = 4;
+constexpr int kStoreWaves = 8;
 
 struct StoreArgs {
     const f16* k;
@@ -166,10 +191,11 @@ struct StoreArgs {
 template <int BITS, bool INT8, int D>
 __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedView c, StoreArgs a) {
     constexpr int LPR = D / 4, SUB = 64 / LPR, NG = INT8 ? 1 : D / kGroup;
-    __shared__ float sm_lo[kStoreWaves][D], sm_hi[kStoreWaves][D];
+    __shared__ half4v sm_lo[kStoreWaves][LPR], sm_hi[kStoreWaves][LPR];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int nw = blockDim.x >> 6, h = blockIdx.y, ps = 1 << c.lg;
-    const PagedUnit u = find_unit(a.s.n_seq, blockIdx.x, [&](int b) {
+    // (heads side by side: a token's row of all heads is read at about the same time)
+    const int nw = blockDim.x >> 6, h = (int)(blockIdx.x % c.hkv), ps = 1 << c.lg;
+    const PagedUnit u = find_unit(a.s.n_seq, blockIdx.x / c.hkv, [&](int b) {
         const PagedSpan p = span_of(a.s, b, c.lg);
         const int n = span_in_table(a.s, p, c.lg);
         return n > 0 ? (uint32_t)(((p.start + n - 1) >> c.lg) - (p.start >> c.lg) + 1) : 0u;
@@ -179,15 +205,14 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
     const int n = span_in_table(a.s, p, c.lg);
     const int logical = (p.start >> c.lg) + (int)u.at;
     const int page = a.s.table[u.b * a.s.stride + logical];
-    if (page < 0 || page >= c.n_pages) return;
     const int pos0 = logical << c.lg;
     const int s0 = max(p.start - pos0, 0), s1 = min(p.start + n - pos0, ps);
     const int64_t ph = (int64_t)page * c.hkv + h;
     const int li = lane % LPR, sub = lane / LPR, grp = li >> 4;
 
-    float lo[4], hi[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) lo[i] = INFINITY, hi[i] = -INFINITY;
+    const int r16 = lane & 15;
+    const f16 inf = (f16)INFINITY;
+    half4v lo = {inf, inf, inf, inf}, hi = -lo;
     const int first = s0 >> 3, last = (s1 - 1) >> 3;
     for (int b0 = first; b0 <= last; b0 += nw * SUB) {
         const int blk = b0 + wave * SUB + sub;
@@ -202,6 +227,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
                 xv[k] = *(const half4v*)(a.v + t * a.v_token + h * a.v_head + 4 * li);
             }
         }
+        if (page < 0 || page >= c.n_pages) return;  // (the whole workgroup's; the tokens were requested beside the table's entry)
         const bool live = blk <= last;
         const int64_t blk8 = ph * (ps >> 3) + blk;
         char* krow = c.k + (ph * ps + 8 * blk) * (D * BITS / 8) + k_at<BITS>(li);
@@ -211,44 +237,75 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
         u32x4 old[BITS / 4];
 #pragma unroll
         for (int j = 0; j < BITS / 4; j++) old[j] = live && !whole ? vblk[j] : u32x4{0, 0, 0, 0};
-        uint32_t vc[8];
-        half8 ks, kb, vs, vb;
+        auto in = [&](int k) { return 8 * blk + k >= s0 && 8 * blk + k < s1; };
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const int slot = 8 * blk + k;
-            const bool in = slot >= s0 && slot < s1;
+            lo = in(k) ? __builtin_elementwise_min(lo, xk[k]) : lo;
+            hi = in(k) ? __builtin_elementwise_max(hi, xk[k]) : hi;
+        }
+        float cv[8][4];  // V's codes
+        if constexpr (BITS == 16) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float x = (float)xk[k][i];
-                lo[i] = in ? fminf(lo[i], x) : lo[i];
-                hi[i] = in ? fmaxf(hi[i], x) : hi[i];
-            }
-            if constexpr (BITS == 16) {
-                if (in) *(half4v*)(krow + k * (D * 2)) = xk[k];
-            } else {
-                f16 s, b;
-                uint32_t w = quantize4<BITS, INT8, D>(xk[k], s, b);
-                ks[k] = s, kb[k] = b;
+            for (int k = 0; k < 8; k++)
+                if (in(k)) *(half4v*)(krow + k * (D * 2)) = xk[k];
+        } else {
+            // the rows' extremes: K's of token k in lane k of a group, V's in lane 8 + k
+            float mn = 0.0f, mx = 0.0f;
+            auto extremes = [&](auto item, half4v x) {
+                constexpr int J = decltype(item)::value;
+                const float f0 = (float)x[0], f1 = (float)x[1], f2 = (float)x[2], f3 = (float)x[3];
+                if constexpr (INT8) {
+                    to_lane<J>(mx, reduce_row<D>(fmaxf(fmaxf(fabsf(f0), fabsf(f1)), fmaxf(fabsf(f2), fabsf(f3))), FMax()), r16);
+                } else {
+                    to_lane<J>(mn, reduce16(fminf(fminf(f0, f1), fminf(f2, f3)), FMin()), r16);
+                    to_lane<J>(mx, reduce16(fmaxf(fmaxf(f0, f1), fmaxf(f2, f3)), FMax()), r16);
+                }
+            };
+            each8([&](auto k) {
+                constexpr int K = decltype(k)::value;
+                if (__any(in(K))) {
+                    extremes(std::integral_constant<int, K>(), xk[K]);
+                    extremes(std::integral_constant<int, 8 + K>(), xv[K]);
+                }
+            });
+            f16 scale, bias;
+            const Steps mine = steps_of<BITS, INT8>(mn, mx, scale, bias);
+            each8([&](auto k) {
+                constexpr int K = decltype(k)::value;
+                if (!__any(in(K))) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) cv[K][i] = 0.0f;
+                    return;
+                }
+                const Steps qk{of_lane<K>(mine.step), of_lane<K>(mine.base), of_lane<K>(mine.inv)};
+                const Steps qv{of_lane<8 + K>(mine.step), of_lane<8 + K>(mine.base), of_lane<8 + K>(mine.inv)};
+                float c[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    c[i] = code_of<BITS, INT8>((float)xk[K][i], qk);
+                    cv[K][i] = code_of<BITS, INT8>((float)xv[K][i], qv);
+                }
                 if constexpr (BITS == 4) {
                     // dims 8 j .. + 3 in an even lane (nibbles 0, 4, 1, 5), .. + 7 in the odd one (2, 6, 3, 7)
-                    const uint32_t x = (w & 15) | (w >> 8 & 15) << 16 | (w >> 16 & 15) << 4 | (w >> 24) << 20;
-                    w = __builtin_amdgcn_update_dpp(0u, x, 0xB1, 0xF, 0xF, false);  // the other lane's
-                    w = x | w << 8;
-                    if (in && (li & 1) == 0) *(uint32_t*)(krow + k * (D / 2)) = w;
+                    uint32_t w = put_byte<0>(0u, __builtin_fmaf(16.0f, c[2], c[0]));
+                    w = put_byte<2>(w, __builtin_fmaf(16.0f, c[3], c[1]));
+                    w |= __builtin_amdgcn_update_dpp(0u, w, 0xB1, 0xF, 0xF, false) << 8;  // the other lane's
+                    if (in(K) && (li & 1) == 0) *(uint32_t*)(krow + K * (D / 2)) = w;
                 } else {
-                    if (in) *(uint32_t*)(krow + k * D) = w;
+                    const uint32_t w = put_byte<3>(put_byte<2>(put_byte<1>(put_byte<0>(0u, c[0]), c[1]), c[2]), c[3]);
+                    if (in(K)) *(uint32_t*)(krow + K * D) = w;
                 }
-                vc[k] = quantize4<BITS, INT8, D>(xv[k], s, b);
-                vs[k] = s, vb[k] = b;
+            });
+            if (in(r16 & 7) && (!INT8 || li < 16)) {
+                f16* par = (r16 < 8 ? c.k_par : c.v_par) + blk8 * (INT8 ? 8 : 16 * NG) + (INT8 ? 0 : 8 * grp) + (r16 & 7);
+                par[0] = scale;
+                if (!INT8) par[8 * NG] = bias;
             }
         }
         if (live) {
             uint32_t key[4];  // of key pair j: all bits of the halves that this call writes
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int s = 8 * blk + 2 * j;
-                key[j] = (s >= s0 && s < s1 ? 0xFFFFu : 0u) | (s + 1 >= s0 && s + 1 < s1 ? 0xFFFF0000u : 0u);
-            }
+            for (int j = 0; j < 4; j++) key[j] = (in(2 * j) ? 0xFFFFu : 0u) | (in(2 * j + 1) ? 0xFFFF0000u : 0u);
             if constexpr (BITS == 16) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
@@ -270,9 +327,10 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
                 for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        uint32_t x = 0;
-#pragma unroll
-                        for (int k = 0; k < 4; k++) x |= (vc[4 * j + k] >> (8 * i) & 0xFFu) << (8 * k);
+                        uint32_t x = put_byte<0>(0u, cv[4 * j][i]);
+                        x = put_byte<1>(x, cv[4 * j + 1][i]);
+                        x = put_byte<2>(x, cv[4 * j + 2][i]);
+                        x = put_byte<3>(x, cv[4 * j + 3][i]);
                         const uint32_t o = old[i / 2][2 * (i & 1) + j];
                         old[i / 2][2 * (i & 1) + j] = (x & m[j]) | (o & ~m[j]);
                     }
@@ -284,84 +342,63 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
                 for (int j = 0; j < 4; j++) m |= (key[j] & 0x000F000Fu) << (4 * j);
                 u32x4 w;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    uint32_t x = 0;
-#pragma unroll
-                    for (int k = 0; k < 8; k++) x |= (vc[k] >> (8 * i) & 15u) << (4 * v4_nibble_pos(k));
+                for (int i = 0; i < 4; i++) {  // nibbles of keys 0 2 | 4 6 | 1 3 | 5 7
+                    uint32_t x = put_byte<0>(0u, __builtin_fmaf(16.0f, cv[2][i], cv[0][i]));
+                    x = put_byte<1>(x, __builtin_fmaf(16.0f, cv[6][i], cv[4][i]));
+                    x = put_byte<2>(x, __builtin_fmaf(16.0f, cv[3][i], cv[1][i]));
+                    x = put_byte<3>(x, __builtin_fmaf(16.0f, cv[7][i], cv[5][i]));
                     w[i] = (x & m) | (old[0][i] & ~m);
                 }
                 vblk[0] = w;
             }
-            if constexpr (BITS != 16) {
-                if (INT8 ? li == 0 : (li & 15) == 0) {
-                    f16* kp = c.k_par + blk8 * (INT8 ? 8 : 16 * NG) + (INT8 ? 0 : 8 * grp);
-                    f16* vp = c.v_par + blk8 * (INT8 ? 8 : 16 * NG) + (INT8 ? 0 : 8 * grp);
-                    if (whole) {
-                        *(half8*)kp = ks;
-                        *(half8*)vp = vs;
-                        if (!INT8) *(half8*)(kp + 8 * NG) = kb, *(half8*)(vp + 8 * NG) = vb;
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            if (8 * blk + k >= s0 && 8 * blk + k < s1) {
-                                kp[k] = ks[k], vp[k] = vs[k];
-                                if (!INT8) kp[8 * NG + k] = kb[k], vp[8 * NG + k] = vb[k];
-                            }
-                    }
-                }
-            }
         }
     }
     // the page's bounds
+    f16* lohi = c.lohi + ph * 2 * D + 4 * li;
+    half4v was_lo = lo, was_hi = hi;
+    if (s0 > 0 && wave == 0) was_lo = *(const half4v*)lohi, was_hi = *(const half4v*)(lohi + D);
+    auto other_half = [&](half4v x) {
+        const u32x2 u = __builtin_bit_cast(u32x2, x);
+        return __builtin_bit_cast(half4v, u32x2{__float_as_uint(lane_xor<32>(__uint_as_float(u[0]), lane)),
+                                                __float_as_uint(lane_xor<32>(__uint_as_float(u[1]), lane))});
+    };
     if constexpr (SUB == 2) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            lo[i] = fminf(lo[i], lane_xor<32>(lo[i], lane));
-            hi[i] = fmaxf(hi[i], lane_xor<32>(hi[i], lane));
-        }
+        lo = __builtin_elementwise_min(lo, other_half(lo));
+        hi = __builtin_elementwise_max(hi, other_half(hi));
     }
     if (nw > 1) {
-        if (sub == 0) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) sm_lo[wave][4 * li + i] = lo[i], sm_hi[wave][4 * li + i] = hi[i];
-        }
+        if (sub == 0) sm_lo[wave][li] = lo, sm_hi[wave][li] = hi;
         __syncthreads();
         if (wave) return;
         for (int w = 1; w < nw; w++) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                lo[i] = fminf(lo[i], sm_lo[w][4 * li + i]);
-                hi[i] = fmaxf(hi[i], sm_hi[w][4 * li + i]);
-            }
+            lo = __builtin_elementwise_min(lo, sm_lo[w][li]);
+            hi = __builtin_elementwise_max(hi, sm_hi[w][li]);
         }
     }
-    f16* lohi = c.lohi + ph * 2 * D + 4 * li;
     if (s0 > 0) {
-        const half4v l = *(const half4v*)lohi, u4 = *(const half4v*)(lohi + D);
-#pragma unroll
-        for (int i = 0; i < 4; i++) lo[i] = fminf(lo[i], (float)l[i]), hi[i] = fmaxf(hi[i], (float)u4[i]);
+        lo = __builtin_elementwise_min(lo, was_lo);
+        hi = __builtin_elementwise_max(hi, was_hi);
     }
-    half4v l, u4;
+    const f16 most = (f16)65504.0f;
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        lo[i] = fminf(fmaxf(lo[i], -65504.0f), 65504.0f);
-        hi[i] = fminf(fmaxf(hi[i], -65504.0f), 65504.0f);
-        if (lo[i] > hi[i]) lo[i] = hi[i] = 0.0f;  // nothing but NaN
-        l[i] = (f16)lo[i], u4[i] = (f16)hi[i];
-        top = fmaxf(top, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+        lo[i] = lo[i] < -most ? -most : lo[i] > most ? most : lo[i];
+        hi[i] = hi[i] < -most ? -most : hi[i] > most ? most : hi[i];
+        if (!(lo[i] <= hi[i])) lo[i] = hi[i] = (f16)0.0f;  // nothing but NaN
+        top = fmaxf(top, fmaxf(fabsf((float)lo[i]), fabsf((float)hi[i])));
     }
     top = reduce_row<D>(top, FMax());
     const float inv = top > 0.0f ? 127.0f / top : 0.0f;
     uint32_t wl = 0, wh = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        wh |= ((uint32_t)(int)fminf(fmaxf(__builtin_ceilf(hi[i] * inv), -127.0f), 127.0f) & 0xFFu) << (8 * i);
-        wl |= ((uint32_t)(int)fminf(fmaxf(__builtin_floorf(lo[i] * inv), -127.0f), 127.0f) & 0xFFu) << (8 * i);
+        wh |= ((uint32_t)(int)__builtin_amdgcn_fmed3f(__builtin_ceilf((float)hi[i] * inv), -127.0f, 127.0f) & 0xFFu) << (8 * i);
+        wl |= ((uint32_t)(int)__builtin_amdgcn_fmed3f(__builtin_floorf((float)lo[i] * inv), -127.0f, 127.0f) & 0xFFu) << (8 * i);
     }
     if (sub == 0) {
-        *(half4v*)lohi = l;
-        *(half4v*)(lohi + D) = u4;
+        *(half4v*)lohi = lo;
+        *(half4v*)(lohi + D) = hi;
         *(uint32_t*)(c.codes + ph * 2 * D + 4 * li) = wh;
         *(uint32_t*)(c.codes + ph * 2 * D + D + 4 * li) = wl;
     }
@@ -384,9 +421,9 @@ template <int BITS, bool INT8, int D>
 __global__ __launch_bounds__(256) void paged_gather_kernel(PagedView c, PagedSeqs s, f16* k_out, f16* v_out) {
     constexpr int LPR = D / 4, SUB = 64 / LPR, NG = INT8 ? 1 : D / kGroup;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int h = blockIdx.y, ps = 1 << c.lg;
+    const int h = (int)(blockIdx.x % c.hkv), ps = 1 << c.lg;
     const int li = lane % LPR, sub = lane / LPR, grp = INT8 ? 0 : li >> 4;
-    const uint32_t unit = (blockIdx.x * 4 + wave) * SUB;
+    const uint32_t unit = (blockIdx.x / c.hkv * 4 + wave) * SUB;
     auto blocks = [&](int b) {
         const PagedSpan p = span_of(s, b, c.lg);
         return p.n > 0 ? (uint32_t)((((int64_t)p.start + p.n - 1) >> 3) - (p.start >> 3) + 1) : 0u;
@@ -499,7 +536,9 @@ int paged_update(PagedCache& c, const void* k, const void* v, int64_t k_token, i
     // waves for the blocks of 8 slots that an average sequence touches in a page, two a wave at D = 128
     const int blocks = std::min(c.page_size / 8, s.n_tokens / s.n_seq / 8 + 1);
     const int waves = std::max(1, std::min(kStoreWaves, blocks * c.D / 256));
-    const dim3 grid((unsigned)most_units(s, c.page_size), c.hkv);
+    const int64_t groups = most_units(s, c.page_size) * c.hkv;
+    QW_REQUIRE(groups * 64 * waves <= UINT32_MAX, QW_ERR_UNSUPPORTED, "paged update: too many tokens for one call");
+    const dim3 grid((unsigned)groups);
     by_mode(c, [&](auto bits, auto i8, auto d) {
         hipLaunchKernelGGL((paged_update_kernel<decltype(bits)::value, decltype(i8)::value, decltype(d)::value>), grid,
                            dim3(64 * waves), 0, stream, c.view, a);
@@ -516,7 +555,9 @@ int paged_gather(const PagedCache& c, void* k_out, void* v_out, const PagedSeqs&
     DeviceGuard dg(c.device);
     QW_REQUIRE(dg.ok, QW_ERR_HIP, "paged gather: hipSetDevice failed");
     const int64_t per = 4 * 256 / c.D;  // units a workgroup
-    const dim3 grid((unsigned)((most_units(s, 8) + per - 1) / per), c.hkv);
+    const int64_t groups = (most_units(s, 8) + per - 1) / per * c.hkv;
+    QW_REQUIRE(groups * 256 <= UINT32_MAX, QW_ERR_UNSUPPORTED, "paged gather: too many tokens for one call");
+    const dim3 grid((unsigned)groups);
     by_mode(c, [&](auto bits, auto i8, auto d) {
         hipLaunchKernelGGL((paged_gather_kernel<decltype(bits)::value, decltype(i8)::value, decltype(d)::value>), grid,
                            dim3(256), 0, stream, c.view, s, (f16*)k_out, (f16*)v_out);

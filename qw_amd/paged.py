@@ -12,23 +12,29 @@ import functools
 from . import KVCacheMode, QwError, _check, _stream, _torch, lib
 
 
+# (A decoding step is a few of these calls, each about as long on the host as on the device: attributes that cost a
+# call are read once.)
+
+
 def _ints(t, what: str, device, n: int):
     """A [n] int32 tensor on the device, contiguous."""
-    torch = _torch()
-    if t.shape != (n,) or t.dtype is not torch.int32 or t.device != device:
+    if t.shape != (n,) or t.dtype is not _torch().int32 or t.device != device:
         raise QwError(1, f"{what} must be a [{n}] int32 tensor on {device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _table(t, device, what: str):
     """(tensor, B, W, row stride) of a table [B, W] int32 on the device."""
-    torch = _torch()
-    if t.dim() != 2 or t.dtype is not torch.int32 or t.device != device:
+    shape = t.shape
+    if len(shape) != 2 or t.dtype is not _torch().int32 or t.device != device:
         raise QwError(1, f"{what}: table must be a [B, W] int32 tensor on {device}")
-    B, W = t.shape
-    if W > 1 and t.stride(1) != 1 or B > 1 and t.stride(0) < W:
-        t = t.contiguous()
-    return t, B, W, t.stride(0) if B > 1 else W
+    B, W = shape
+    if t.is_contiguous():
+        return t, B, W, W
+    row, col = t.stride()
+    if W > 1 and col != 1 or B > 1 and row < W:
+        return t.contiguous(), B, W, W
+    return t, B, W, row if B > 1 else W
 
 
 @functools.lru_cache(maxsize=64)
@@ -88,6 +94,7 @@ class PagedKVCache:
         self.bits = KVCacheMode.BITS[mode]
         self.device = torch.device("cuda", torch.cuda.current_device() if device is None else
                                    torch.device(device).index or 0)
+        self._row = (n_kv_heads, head_dim)
         self._h = None
         h = ctypes.c_void_p()
         _check(lib().qw_paged_create(mode, group_size, n_kv_heads, head_dim, n_pages, page_size,
@@ -121,13 +128,14 @@ class PagedKVCache:
 
     def _rows(self, t, what: str):
         """New rows [n, Hkv, D] of any token and head strides: (tensor, n, token stride, head stride)."""
-        torch = _torch()
-        if t.dim() != 3 or t.shape[1] != self.n_kv_heads or t.shape[2] != self.head_dim or \
-                t.dtype is not torch.float16 or t.device != self.device:
+        torch, shape = _torch(), t.shape
+        if len(shape) != 3 or shape[1:] != self._row or t.dtype is not torch.float16 or t.device != self.device:
             raise QwError(1, f"{what} must be [n, {self.n_kv_heads}, {self.head_dim}] fp16 on {self.device}")
-        if t.stride(2) != 1 or t.stride(0) % 4 or t.stride(1) % 4 or t.data_ptr() % 8:
+        token, head, d = t.stride()
+        if d != 1 or token % 4 or head % 4 or t.data_ptr() % 8:
             t = t.clone(memory_format=torch.contiguous_format)
-        return t, t.shape[0], t.stride(0), t.stride(1)
+            token, head, d = t.stride()
+        return t, shape[0], token, head
 
     def update(self, keys, values, table, starts, offsets=None) -> None:
         """New tokens ``keys``, ``values`` [n, Hkv, D] fp16 into their pages: those of sequence b,
@@ -143,9 +151,10 @@ class PagedKVCache:
     def gather(self, table, starts, n: int, offsets=None):
         """The tokens at those positions back: (keys, values) [n, Hkv, D] fp16, zeros where a
         position has no page."""
+        if n < 0:
+            raise QwError(1, "gather: n >= 0 expected")
         args, _keep = self._seqs(n, table, starts, offsets, "gather")
-        shape = (n, self.n_kv_heads, self.head_dim)
-        k, v = (_torch().empty(shape, dtype=_torch().float16, device=self.device) for _ in range(2))
+        k, v = _torch().empty((2, n, *self._row), dtype=_torch().float16, device=self.device).unbind()
         _check(lib().qw_paged_gather(self._h, k.data_ptr(), v.data_ptr(), *args, _stream(self.device)))
         return k, v
 
@@ -166,34 +175,35 @@ class PagedKVCache:
 
     # -- attention
     def _query(self, q, table, lengths, what: str):
-        torch = _torch()
-        if q.dim() != 4 or q.shape[3] != self.head_dim or q.dtype is not torch.float16 or q.device != self.device:
+        torch, shape = _torch(), q.shape
+        if len(shape) != 4 or shape[3] != self.head_dim or q.dtype is not torch.float16 or q.device != self.device:
             raise QwError(1, f"{what}: q must be [B, Hq, L, {self.head_dim}] fp16 on {self.device}")
-        if q.stride(3) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.stride(2) % 8 or q.data_ptr() % 16:
+        seq, head, row, d = q.stride()
+        if d != 1 or (seq | head | row) % 8 or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
+            seq, head, row, d = q.stride()
         t, B, W, stride = _table(table, self.device, what)
-        if q.shape[0] != B:
+        if shape[0] != B:
             raise QwError(1, f"{what}: q and table must have as many sequences")
         n = _ints(lengths, f"{what}: lengths", self.device, B)
-        return (q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), B, q.shape[1], q.shape[2], n.data_ptr(),
-                t.data_ptr(), stride, W), (q, t, n)
+        return (q.data_ptr(), seq, head, row, B, shape[1], shape[2], n.data_ptr(), t.data_ptr(), stride, W), (q, t, n)
 
     def attention(self, q, table, lengths, scale: float, picked=None):
         """Attention of each sequence's newest L tokens ``q`` [B, Hq, L, D] over its first
         ``lengths[b]`` keys (int32 [B], the newest among them), causal among the last L; ``picked``
         ([B, Hkv, n] int32, as :meth:`select_pages` gives): over those pages alone. Returns [B, Hq, L, D]."""
         torch = _torch()
-        args, keep = self._query(q, table, lengths, "attention")
-        n = 0
+        args, _keep = self._query(q, table, lengths, "attention")
+        n, at = 0, None
         if picked is not None:
-            if picked.dim() != 3 or picked.shape[0] != args[4] or picked.shape[1] != self.n_kv_heads or \
-                    picked.shape[2] < 1 or picked.dtype is not torch.int32 or picked.device != self.device:
+            shape = picked.shape
+            if len(shape) != 3 or shape[0] != args[4] or shape[1] != self.n_kv_heads or shape[2] < 1 or \
+                    picked.dtype is not torch.int32 or picked.device != self.device:
                 raise QwError(1, f"attention: picked must be [B, {self.n_kv_heads}, n] int32 on {self.device}")
             picked = picked.contiguous()
-            n = picked.shape[2]
-        out = torch.empty(keep[0].shape, dtype=torch.float16, device=self.device)
-        _check(lib().qw_paged_attention(self._h, *args, None if picked is None else picked.data_ptr(), n, float(scale),
-                                        out.data_ptr(), _stream(self.device)))
+            n, at = shape[2], picked.data_ptr()
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        _check(lib().qw_paged_attention(self._h, *args, at, n, float(scale), out.data_ptr(), _stream(self.device)))
         return out
 
     def select_pages(self, q, table, lengths, budget: int, sink: int = 0, recent: int = 0):
