@@ -154,7 +154,8 @@ __device__ __forceinline__ Steps steps_of(float mn, float mx, f16& scale, f16& b
         return Steps{q.scale, q.bias, 1.0f / q.scale};
     }
 }
-// A code as a whole number in a float, int8's 128 above itself. The quotient: inv is the step's reciprocal, rounded
+// A code in a float: of 4 bits a whole number, of 8 bits before its rounding, int8's 128 above itself (put_byte rounds to the
+// nearest, to even, and ends at 0 and 255). The quotient: inv is the step's reciprocal, rounded
 // once; the product of it and its remainder, which an fma has exactly, correct it to the rounded quotient
 // (Markstein, 1990), as the codec's division gives it. x finite.
 template <int BITS, bool INT8>
@@ -162,8 +163,8 @@ __device__ __forceinline__ float code_of(float x, const Steps& q) {
     const float t = INT8 ? x : x - q.base;
     float p = t * q.inv;
     p = __builtin_fmaf(__builtin_fmaf(-p, q.step, t), q.inv, p);
-    if constexpr (INT8) return __builtin_amdgcn_fmed3f(__builtin_rintf((float)(f16)p), -128.0f, 127.0f) + 128.0f;
-    return __builtin_amdgcn_fmed3f(__builtin_rintf(p), 0.0f, (float)((1 << BITS) - 1));
+    if constexpr (INT8) return (float)(f16)p + 128.0f;
+    return BITS == 8 ? p : __builtin_amdgcn_fmed3f(__builtin_rintf(p), 0.0f, 15.0f);
 }
 template <int BYTE>
 __device__ __forceinline__ uint32_t put_byte(uint32_t w, float c) {

@@ -72,10 +72,14 @@ def rope_axes(qkv, positions, sections, n_q_heads: int, n_kv_heads: int, head_di
     axes = _axes(tuple(sections), bool(interleaved))
     x, n, pos, stride = _turned(qkv, positions, sections, (n_q_heads + 2 * n_kv_heads) * head_dim, "rope_axes")
     q, k = x.new_empty((n, n_q_heads, head_dim)), x.new_empty((n, n_kv_heads, head_dim))
-    with _torch().cuda.device(x.device):
-        _check(lib().qw_rope_axes(x.data_ptr(), n, n_q_heads, n_kv_heads, head_dim, 2 * len(axes), int(traditional),
-                                  float(rope_base), float(rope_scale), pos.data_ptr(), stride, len(sections), axes,
-                                  q.data_ptr(), k.data_ptr(), _stream(x.device)))
+    args = (x.data_ptr(), n, n_q_heads, n_kv_heads, head_dim, 2 * len(axes), int(traditional), float(rope_base),
+            float(rope_scale), pos.data_ptr(), stride, len(sections), axes, q.data_ptr(), k.data_ptr(), _stream(x.device))
+    cuda = _torch().cuda
+    if x.get_device() == cuda.current_device():
+        _check(lib().qw_rope_axes(*args))
+    else:
+        with cuda.device(x.device):
+            _check(lib().qw_rope_axes(*args))
     return q, k
 
 
