@@ -42,6 +42,7 @@ struct AttendArgs {
     int n_picked;
     float scale2;  // scale * log2 e
     int workers, round;  // keys of a round: 32 a wave
+    int whole;           // sequences stay whole, and no second launch follows
     float* part_o;    // [2 workers][hkv][R][D]
     float2* part_ml;  // [2 workers][hkv][R]
 };
@@ -86,7 +87,7 @@ __device__ __forceinline__ Plan plan_of(const AttendArgs& a) {
     p.per = __builtin_amdgcn_readfirstlane(p.total / p.workers);
     p.rest = p.total - p.per * p.workers;
     if (a.n_seq <= 64) {
-        uint32_t most = p.per + (p.rest > 0);
+        uint32_t most = a.whole ? p.total : p.per + (p.rest > 0);
         for (int i = 0; i < 4; i++, most += 1 + most / 16) {
             p.pieces = (p.rounds + most - 1) / most;
             p.last = wave_scan(p.pieces);
@@ -324,6 +325,14 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
     {
         const Plan plan = plan_of(a);
         per = plan.per, rest = plan.rest;
+        if (a.whole) {  // sequences without keys are zeros (else the second launch's)
+            for (int b = w; b < a.n_seq; b += gridDim.x) {
+                const uint32_t n = a.n_seq <= 64 ? (uint32_t)__builtin_amdgcn_readlane((int)plan.rounds, b) : rounds_of(a, b);
+                if (n == 0)
+                    for (int i = threadIdx.x; i < min(a.R - row0, 16 * RT) * (D / 4); i += NT)
+                        *(half4v*)(a.out + ((b * (int64_t)a.c.hkv + h) * a.R + row0) * D + 4 * i) = half4v{};
+            }
+        }
         if (!plan.most) {
             if (w >= plan.workers) return;
             at = w * per + min(w, rest);
@@ -884,7 +893,13 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     const int groups = (a.R + 16 * tiles - 1) / (16 * tiles);
     a.round = round;
     a.workers = (int)std::max<int64_t>(1, std::min<int64_t>(rounds, 256 * held / ((int64_t)c.hkv * groups)));
-    const int64_t parts = (int64_t)a.workers * 2 * c.hkv * a.R;
+    // A sequence of few rounds is read by one worker where the rounds one after another cost less than the second launch,
+    // which joins pieces (of one round none is cut anyway). Whole / cut, a pass in us, 1 sequence: D = 256, 8 bits, 3 rounds
+    // 11.7 / 12.0, 5 rounds 15.6 / 12.1, fp16 12.8 / 12.8 and 17.2 / 13.1; D = 128, 8 bits, 3 rounds 9.0 / 11.2, 5
+    // rounds 11.7 / 11.2, fp16 8.0 / 11.2 and 9.9 / 11.2. 16 sequences, D = 128, 5 rounds 12.4 / 13.9 and 11.0 / 16.3.
+    const int few = c.D == 256 ? 3 : c.bits == 16 ? 5 : 4;
+    a.whole = rounds > 0 && (most <= round || (most <= few * round && q.n_seq <= 64 && q.n_seq <= a.workers));
+    const int64_t parts = a.whole ? 0 : (int64_t)a.workers * 2 * c.hkv * a.R;
     void* ws = nullptr;
     if (int rc = workspace(kWsPaged, c.device, stream, (size_t)(parts * (c.D * 4 + 8)), &ws)) return rc;
     a.part_o = (float*)ws;
@@ -895,6 +910,7 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
         });
         if (rc) return rc;
     }
+    if (a.whole) return QW_OK;
     const dim3 grid((unsigned)(c.hkv * a.R), q.n_seq);
     if (c.D == 256)
         hipLaunchKernelGGL(paged_merge_kernel<256>, grid, dim3(256), 0, stream, a);

@@ -414,3 +414,118 @@ def test_refusals():
     assert s.cache.attention(q[:0], e, z, 0.1).shape == (0, 4, 1, 128)
     s.cache.update(k[:0], k[:0], e, z)
     assert torch.all(s.cache.attention(q, t[:, :0], n, 0.1) == 0)  # a table without columns
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_odd_rows_are_stored_as_a_cache_stores_them(mode):
+    """Zeros, constants, the smallest and the largest numbers, one number among zeros, negative rows."""
+    import qw_amd
+
+    r = rng(70)
+    hkv, D, ps = 2, 128, 16
+    x = rows(r, 40, hkv, D)
+    x[0] = 0
+    x[1] = 1.5
+    x[2] = 2.0 ** -24
+    x[3] = r.integers(0, 9, x[3].shape) * 2.0 ** -24
+    x[4] = 65504
+    x[5] = 65504 * np.sign(r.standard_normal(x[5].shape))
+    x[6] = 0
+    x[6, :, 77] = -3e-5
+    x[7] = -np.abs(x[7])
+    x[8] = np.abs(x[8]) * 1e-6
+    x[9, :, :64] = 0
+    x[10] = np.float16(2.0 ** -14) * (1 + r.integers(0, 3, x[10].shape))
+    x[11:30] = (r.standard_normal((19, hkv, D)) * 10.0 ** r.uniform(-6, 4, (19, 1, 1))).astype(np.float16)
+    y = x[::-1].copy()
+    cache = qw_amd.PagedKVCache(mode, hkv, D, 3, page_size=ps)
+    t = ints([[2, 0, 1]])
+    cache.update(dev(x), dev(y), t, ints([0]))
+    got = cache.gather(t, ints([0]), 40)
+    for a, b in zip(got, stored(mode, x, y, hkv, D)):
+        assert np.array_equal(a.cpu().numpy().view(np.uint16), b.view(np.uint16))
+
+
+@pytest.mark.parametrize("mode", ["affine8", "fp16"])
+@pytest.mark.parametrize("hq,hkv,n_seq,most,L", [(2, 2, 64, 700, 1), (2, 2, 65, 400, 1), (32, 32, 40, 300, 1), (16, 2, 3, 900, 9), (3, 1, 70, 120, 1)])
+def test_attention_of_ragged_batches(mode, hq, hkv, n_seq, most, L):
+    """Batches at the line of the lane-held plan, with sequences without keys among them; rows in many tiles; short ones."""
+    r = rng(n_seq + most)
+    lengths = [int(x) for x in r.integers(0, most, n_seq)]
+    lengths[::7] = [0] * len(lengths[::7])
+    lengths[-1] = most
+    s = Sequences(r, mode, hkv, 128, 16, lengths)
+    q = queries(r, n_seq, hq, L, 128)
+    s.check(s.cache.attention(q, ints(s.table), ints(lengths), 0.09), q, 0.09)
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("D", [128, 256])
+def test_short_sequences_stay_whole(mode, D):
+    """Around the lengths up to which no sequence is cut."""
+    r = rng(D)
+    for lengths in ([5, 0, 128], [129, 256, 0], [384, 385, 1], [512, 100], [513], [640, 0], [641]):
+        s = Sequences(r, mode, 2, D, 16, lengths)
+        q = queries(r, len(lengths), 8, 1, D)
+        s.check(s.cache.attention(q, ints(s.table), ints(lengths), 0.09), q, 0.09)
+
+
+@pytest.mark.parametrize("mode", ["fp16", "affine8"])
+def test_a_pool_past_32_bits(mode):
+    """Pages whose bytes, and whose rows, lie past 2^32 in the pool's planes."""
+    import qw_amd
+
+    r = rng(71)
+    hkv, D, ps = 8, 256, 256
+    n_pages = 4300 if mode == "fp16" else 8500  # 1 MB, or half of it, a page in each plane
+    cache = qw_amd.PagedKVCache(mode, hkv, D, n_pages, page_size=ps)
+    small = qw_amd.PagedKVCache(mode, hkv, D, 3, page_size=ps)
+    k, v = rows(r, 700, hkv, D), rows(r, 700, hkv, D)
+    far, near, zero = ints([[n_pages - 1, n_pages - 3, n_pages - 2]]), ints([[0, 2, 1]]), ints([0])
+    q, n = queries(r, 1, 16, 1, D), ints([700])
+    for c, t in ((cache, far), (small, near)):
+        c.update(dev(k), dev(v), t, zero)
+    for x, y in zip(cache.gather(far, zero, 700), small.gather(near, zero, 700)):
+        assert torch.equal(x, y)
+    assert torch.equal(cache.attention(q, far, n, 1 / 16), small.attention(q, near, n, 1 / 16))
+    assert torch.equal(cache.select_pages(q, far, n, 2), small.select_pages(q, near, n, 2))
+    assert all(torch.all(x == 0) for x in cache.gather(ints([[0, 1]]), zero, 512))
+
+
+def test_stream_per_thread_is_refused():
+    """One handle for a stream a thread: the calls that keep a workspace of their stream name it as unsupported."""
+    import qw_amd
+
+    r = rng(72)
+    s = Sequences(r, "fp16", 2, 128, 16, [40])
+    q, out = queries(r, 1, 4, 1, 128), torch.empty((1, 4, 1, 128), dtype=torch.float16, device="cuda")
+    t, n = ints(s.table), ints([40])
+    picked = ints(np.zeros((1, 2, 3)))
+    args = (s.cache._h, q.data_ptr(), 512, 128, 128, 1, 4, 1, n.data_ptr(), t.data_ptr(), 3, 3)
+    assert qw_amd.lib().qw_paged_attention(*args, None, 0, 0.1, out.data_ptr(), 2) == 2
+    assert qw_amd.lib().qw_paged_select(*args, 2, 0, 0, picked.data_ptr(), 2) == 2
+
+
+def test_first_use_inside_a_capture():
+    """A call that has to make its workspace is refused while its stream is captured, and the capture goes on."""
+    import qw_amd
+
+    r = rng(73)
+    s = Sequences(r, "affine4", 2, 128, 16, [3000])
+    q, t, n = queries(r, 1, 8, 1, 128), ints(s.table), ints([3000])
+    want = s.cache.attention(q, t, n, 0.1)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    refused = False
+    x = torch.zeros(8, device="cuda")
+    with torch.cuda.graph(g, stream=stream):
+        try:
+            s.cache.attention(q, t, n, 0.1)
+        except qw_amd.QwError as e:
+            refused = e.status == 5
+        x.add_(1)
+    g.replay()
+    torch.cuda.synchronize()
+    assert refused and torch.all(x == 1)
+    assert torch.equal(s.cache.attention(q, t, n, 0.1), want)
