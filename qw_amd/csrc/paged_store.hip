@@ -93,29 +93,17 @@ int check_seqs(const PagedCache& c, const PagedSeqs& s, const char* what) {
 
 namespace {
 
-// Extremes of a group: 16 lanes of 4 dims.
-template <class Op>
-__device__ __forceinline__ float reduce16(float x, Op op) {
-    x = op(x, dpp_mov<0xB1>(x));
-    x = op(x, dpp_mov<0x4E>(x));
-    x = op(x, dpp_mov<0x124>(x));
-    return op(x, dpp_mov<0x128>(x));
-}
-// And of a row: D / 4 lanes.
-template <int D, class Op>
-__device__ __forceinline__ float reduce_row(float x, Op op) {
+// The greatest of a row: D / 4 lanes.
+template <int D>
+__device__ __forceinline__ float row_max(float x) {
     const int lane = (int)__lane_id();
-    x = reduce16(x, op);
-    x = op(x, lane_xor<16>(x, lane));
-    return D == 256 ? op(x, lane_xor<32>(x, lane)) : x;
+    x = fmaxf(x, dpp_mov<0xB1>(x));
+    x = fmaxf(x, dpp_mov<0x4E>(x));
+    x = fmaxf(x, dpp_mov<0x124>(x));
+    x = fmaxf(x, dpp_mov<0x128>(x));
+    x = fmaxf(x, lane_xor<16>(x, lane));
+    return D == 256 ? fmaxf(x, lane_xor<32>(x, lane)) : x;
 }
-
-struct FMax {
-    __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
-};
-struct FMin {
-    __device__ float operator()(float a, float b) const { return fminf(a, b); }
-};
 
 // f of 0 .. 7, as constants.
 template <class F>
@@ -128,12 +116,65 @@ __device__ __forceinline__ void each8(F f) {
 // Lane J's value to all 16 lanes of its row.
 template <int J>
 __device__ __forceinline__ float of_lane(float x) {
-    return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(x), 0x150 + J, 0xF, 0xF, false));
+    return dpp_mov<0x150 + J>(x);
 }
-// x into lane J of each row of 16.
-template <int J>
-__device__ __forceinline__ void to_lane(float& at, float x, int r16) {
-    at = r16 == J ? x : at;
+
+// Rows' extremes as pairs of halves, both of which the least is taken of (exact: the rows are halves): an affine row's least
+// and negative greatest, or the negative magnitudes of a K and a V row.
+// As written: the compiler puts an instruction before it for each operand, against signalling NaNs.
+__device__ __forceinline__ half2v least(half2v a, half2v b) {
+    half2v y;
+    asm("v_pk_min_f16 %0, %1, %2" : "=v"(y) : "v"(a), "v"(b));
+    return y;
+}
+__device__ __forceinline__ half2v least_negated(half2v a, half2v b) {  // of -a and -b
+    half2v y;
+    asm("v_pk_min_f16 %0, %1, %2 neg_lo:[1,1] neg_hi:[1,1]" : "=v"(y) : "v"(a), "v"(b));
+    return y;
+}
+__device__ __forceinline__ half2v least_of_negative(half2v a, half2v b) {  // of a and -b
+    half2v y;
+    asm("v_pk_min_f16 %0, %1, %2 neg_lo:[0,1] neg_hi:[0,1]" : "=v"(y) : "v"(a), "v"(b));
+    return y;
+}
+__device__ __forceinline__ half2v ends_of(half4v x) {
+    const half2v a = least(x.lo, x.hi), b = least_negated(x.lo, x.hi);
+    return least(half2v{a[0], b[0]}, half2v{a[1], b[1]});
+}
+__device__ __forceinline__ half2v sizes_of(half4v k, half4v v) {
+    auto negative = [](half2v x) { return __builtin_bit_cast(half2v, __builtin_bit_cast(uint32_t, x) | 0x80008000u); };
+    const half2v a = least(negative(k.lo), negative(k.hi)), b = least(negative(v.lo), negative(v.hi));
+    return least(half2v{a[0], b[0]}, half2v{a[1], b[1]});
+}
+template <int CTRL>
+__device__ __forceinline__ half2v moved(half2v x) {
+    asm volatile("s_nop 1" : "+v"(x));  // (two waits between a write of x, which may be in assembly, and a lane move of it)
+    return __builtin_bit_cast(half2v, dpp_mov<CTRL>(__builtin_bit_cast(float, x)));
+}
+template <int S>
+__device__ __forceinline__ half2v lane_least(half2v x, int lane) {
+    asm volatile("s_nop 1" : "+v"(x));
+    return least(x, __builtin_bit_cast(half2v, lane_xor<S>(__builtin_bit_cast(float, x), lane)));
+}
+// The first N of x over as many lanes of 16: lane i ends with x[i]'s least. Each step leaves a lane half of its rows, and
+// gives the other half to a lane that differs in the next bit (by mirrors for bits 3 and 2).
+template <int N>
+__device__ __forceinline__ half2v spread_least(half2v* x, int r16) {
+    auto step = [&](auto half, auto ctrl) {
+        constexpr int H = decltype(half)::value;
+        const bool up = (r16 & H) != 0;
+#pragma unroll
+        for (int j = 0; j < H; j++) {
+            const half2v keep = up ? x[j + H] : x[j], give = up ? x[j] : x[j + H];
+            x[j] = least(keep, moved<decltype(ctrl)::value>(give));
+        }
+    };
+    using std::integral_constant;
+    if constexpr (N == 16) step(integral_constant<int, 8>(), integral_constant<int, 0x140>());
+    step(integral_constant<int, 4>(), integral_constant<int, 0x141>());
+    step(integral_constant<int, 2>(), integral_constant<int, 0x4E>());
+    step(integral_constant<int, 1>(), integral_constant<int, 0xB1>());
+    return x[0];
 }
 
 // Steps of the rows' codes: value = code * step + base, inv = 1 / step.
@@ -213,7 +254,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
 
     const int r16 = lane & 15;
     const f16 inf = (f16)INFINITY;
-    half4v lo = {inf, inf, inf, inf}, hi = -lo;
+    half4v lo = {inf, inf, inf, inf}, negative_hi = lo;
     const int first = s0 >> 3, last = (s1 - 1) >> 3;
     for (int b0 = first; b0 <= last; b0 += nw * SUB) {
         const int blk = b0 + wave * SUB + sub;
@@ -239,10 +280,18 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
 #pragma unroll
         for (int j = 0; j < BITS / 4; j++) old[j] = live && !whole ? vblk[j] : u32x4{0, 0, 0, 0};
         auto in = [&](int k) { return 8 * blk + k >= s0 && 8 * blk + k < s1; };
+        auto bounds = [&](half4v x, bool with) {
+            const half2v l0 = least(lo.lo, x.lo), l1 = least(lo.hi, x.hi);
+            const half2v h0 = least_of_negative(negative_hi.lo, x.lo), h1 = least_of_negative(negative_hi.hi, x.hi);
+            lo.lo = with ? l0 : lo.lo, lo.hi = with ? l1 : lo.hi;
+            negative_hi.lo = with ? h0 : negative_hi.lo, negative_hi.hi = with ? h1 : negative_hi.hi;
+        };
+        if (__all(whole)) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            lo = in(k) ? __builtin_elementwise_min(lo, xk[k]) : lo;
-            hi = in(k) ? __builtin_elementwise_max(hi, xk[k]) : hi;
+            for (int k = 0; k < 8; k++) bounds(xk[k], true);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) bounds(xk[k], in(k));
         }
         float cv[8][4];  // V's codes
         if constexpr (BITS == 16) {
@@ -251,24 +300,23 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
                 if (in(k)) *(half4v*)(krow + k * (D * 2)) = xk[k];
         } else {
             // the rows' extremes: K's of token k in lane k of a group, V's in lane 8 + k
-            float mn = 0.0f, mx = 0.0f;
-            auto extremes = [&](auto item, half4v x) {
-                constexpr int J = decltype(item)::value;
-                const float f0 = (float)x[0], f1 = (float)x[1], f2 = (float)x[2], f3 = (float)x[3];
-                if constexpr (INT8) {
-                    to_lane<J>(mx, reduce_row<D>(fmaxf(fmaxf(fabsf(f0), fabsf(f1)), fmaxf(fabsf(f2), fabsf(f3))), FMax()), r16);
-                } else {
-                    to_lane<J>(mn, reduce16(fminf(fminf(f0, f1), fminf(f2, f3)), FMin()), r16);
-                    to_lane<J>(mx, reduce16(fmaxf(fmaxf(f0, f1), fmaxf(f2, f3)), FMax()), r16);
-                }
-            };
-            each8([&](auto k) {
-                constexpr int K = decltype(k)::value;
-                if (__any(in(K))) {
-                    extremes(std::integral_constant<int, K>(), xk[K]);
-                    extremes(std::integral_constant<int, 8 + K>(), xv[K]);
-                }
-            });
+            float mn = 0.0f, mx;
+            if constexpr (INT8) {
+                half2v x[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = sizes_of(xk[k], xv[k]);
+                half2v y = spread_least<8>(x, r16);
+                y = least(y, moved<0x128>(y));
+                y = lane_least<16>(y, lane);
+                if (D == 256) y = lane_least<32>(y, lane);
+                mx = -(float)(r16 < 8 ? y[0] : y[1]);
+            } else {
+                half2v x[16];
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = ends_of(xk[k]), x[8 + k] = ends_of(xv[k]);
+                const half2v y = spread_least<16>(x, r16);
+                mn = (float)y[0], mx = -(float)y[1];
+            }
             f16 scale, bias;
             const Steps mine = steps_of<BITS, INT8>(mn, mx, scale, bias);
             each8([&](auto k) {
@@ -356,7 +404,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
     }
     // the page's bounds
     f16* lohi = c.lohi + ph * 2 * D + 4 * li;
-    half4v was_lo = lo, was_hi = hi;
+    half4v hi = -negative_hi, was_lo = lo, was_hi = hi;
     if (s0 > 0 && wave == 0) was_lo = *(const half4v*)lohi, was_hi = *(const half4v*)(lohi + D);
     auto other_half = [&](half4v x) {
         const u32x2 u = __builtin_bit_cast(u32x2, x);
@@ -389,7 +437,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
         if (!(lo[i] <= hi[i])) lo[i] = hi[i] = (f16)0.0f;  // nothing but NaN
         top = fmaxf(top, fmaxf(fabsf((float)lo[i]), fabsf((float)hi[i])));
     }
-    top = reduce_row<D>(top, FMax());
+    top = row_max<D>(top);
     const float inv = top > 0.0f ? 127.0f / top : 0.0f;
     uint32_t wl = 0, wh = 0;
 #pragma unroll
