@@ -195,17 +195,29 @@ __device__ __forceinline__ Steps steps_of(float mn, float mx, f16& scale, f16& b
         return Steps{q.scale, q.bias, 1.0f / q.scale};
     }
 }
-// A code in a float: of 4 bits a whole number, of 8 bits before its rounding, int8's 128 above itself (put_byte rounds to the
+// A code in a float: of 4 bits a whole number, of 8 bits before its rounding (put_byte rounds to the
 // nearest, to even, and ends at 0 and 255). The quotient: inv is the step's reciprocal, rounded
 // once; the product of it and its remainder, which an fma has exactly, correct it to the rounded quotient
-// (Markstein, 1990), as the codec's division gives it. x finite.
-template <int BITS, bool INT8>
-__device__ __forceinline__ float code_of(float x, const Steps& q) {
-    const float t = INT8 ? x : x - q.base;
+// (Markstein, 1990), as the codec's division gives it. x finite. one: 1.0 that the compiler doesn't know, for a
+// difference that takes x as a half.
+template <int BITS>
+__device__ __forceinline__ float code_of(f16 x, const Steps& q, float one) {
+    const float t = __builtin_fmaf((float)x, one, -q.base);
     float p = t * q.inv;
     p = __builtin_fmaf(__builtin_fmaf(-p, q.step, t), q.inv, p);
-    if constexpr (INT8) return (float)(f16)p + 128.0f;
     return BITS == 8 ? p : __builtin_amdgcn_fmed3f(__builtin_rintf(p), 0.0f, 15.0f);
+}
+// int8's, 128 above themselves, in the low bytes of two halves: the codec rounds the quotient to a half, and a half in
+// 1024 .. 2047 ends at its ones, so that the sum with 1152 rounds it to the nearest, to even.
+__device__ __forceinline__ uint32_t codes_of(half2v x, const Steps& q) {
+    half2v y;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const float p = __builtin_fmaf((float)x[i], q.inv, 0.0f);
+        y[i] = (f16)__builtin_fmaf(__builtin_fmaf(-p, q.step, (float)x[i]), q.inv, p);
+    }
+    y = __builtin_elementwise_min(__builtin_elementwise_max(y, half2v{} - (f16)128.0f), half2v{} + (f16)127.0f);
+    return __builtin_bit_cast(uint32_t, y + (f16)1152.0f);
 }
 template <int BYTE>
 __device__ __forceinline__ uint32_t put_byte(uint32_t w, float c) {
@@ -259,14 +271,19 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
     for (int b0 = first; b0 <= last; b0 += nw * SUB) {
         const int blk = b0 + wave * SUB + sub;
         half4v xk[8], xv[8];
+        auto in = [&](int k) { return 8 * blk + k >= s0 && 8 * blk + k < s1; };
+        const bool whole = 8 * blk >= s0 && 8 * blk + 8 <= s1;
+        const int64_t t0 = (int64_t)p.first + (pos0 + 8 * blk - p.start);  // slot 8 blk's token, if that is the call's
+        const f16* kt = a.k + t0 * a.k_token + h * a.k_head + 4 * li;
+        const f16* vt = a.v + t0 * a.v_token + h * a.v_head + 4 * li;
+        if (__all(whole)) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const int slot = 8 * blk + k;
-            xk[k] = half4v{}, xv[k] = half4v{};
-            if (slot >= s0 && slot < s1) {
-                const int64_t t = (int64_t)p.first + (pos0 + slot - p.start);
-                xk[k] = *(const half4v*)(a.k + t * a.k_token + h * a.k_head + 4 * li);
-                xv[k] = *(const half4v*)(a.v + t * a.v_token + h * a.v_head + 4 * li);
+            for (int k = 0; k < 8; k++) xk[k] = *(const half4v*)(kt + k * a.k_token), xv[k] = *(const half4v*)(vt + k * a.v_token);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                xk[k] = half4v{}, xv[k] = half4v{};
+                if (in(k)) xk[k] = *(const half4v*)(kt + k * a.k_token), xv[k] = *(const half4v*)(vt + k * a.v_token);
             }
         }
         if (page < 0 || page >= c.n_pages) return;  // (the whole workgroup's; the tokens were requested beside the table's entry)
@@ -275,11 +292,9 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
         char* krow = c.k + (ph * ps + 8 * blk) * (D * BITS / 8) + k_at<BITS>(li);
         u32x4* vblk = (u32x4*)(c.v + blk8 * (D * BITS) + 4 * li * BITS);  // this lane's 4 dims
         // what the words hold of keys that this call leaves alone
-        const bool whole = 8 * blk >= s0 && 8 * blk + 8 <= s1;
         u32x4 old[BITS / 4];
 #pragma unroll
         for (int j = 0; j < BITS / 4; j++) old[j] = live && !whole ? vblk[j] : u32x4{0, 0, 0, 0};
-        auto in = [&](int k) { return 8 * blk + k >= s0 && 8 * blk + k < s1; };
         auto bounds = [&](half4v x, bool with) {
             const half2v l0 = least(lo.lo, x.lo), l1 = least(lo.hi, x.hi);
             const half2v h0 = least_of_negative(negative_hi.lo, x.lo), h1 = least_of_negative(negative_hi.hi, x.hi);
@@ -293,7 +308,10 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
 #pragma unroll
             for (int k = 0; k < 8; k++) bounds(xk[k], in(k));
         }
-        float cv[8][4];  // V's codes
+        float cv[8][4];      // V's codes
+        uint32_t cv2[8][2];  // int8's, of dims 0 1 and 2 3
+        float one = 1.0f;
+        asm volatile("" : "+v"(one));
         if constexpr (BITS == 16) {
 #pragma unroll
             for (int k = 0; k < 8; k++)
@@ -324,17 +342,25 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
                 if (!__any(in(K))) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) cv[K][i] = 0.0f;
+                    cv2[K][0] = cv2[K][1] = 0;
                     return;
                 }
                 const Steps qk{of_lane<K>(mine.step), of_lane<K>(mine.base), of_lane<K>(mine.inv)};
                 const Steps qv{of_lane<8 + K>(mine.step), of_lane<8 + K>(mine.base), of_lane<8 + K>(mine.inv)};
                 float c[4];
+                if constexpr (INT8) {
+                    cv2[K][0] = codes_of(xv[K].lo, qv), cv2[K][1] = codes_of(xv[K].hi, qv);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    c[i] = code_of<BITS, INT8>((float)xk[K][i], qk);
-                    cv[K][i] = code_of<BITS, INT8>((float)xv[K][i], qv);
+                    for (int i = 0; i < 4; i++) {
+                        c[i] = code_of<BITS>(xk[K][i], qk, one);
+                        cv[K][i] = code_of<BITS>(xv[K][i], qv, one);
+                    }
                 }
-                if constexpr (BITS == 4) {
+                if constexpr (INT8) {
+                    const uint32_t w = __builtin_amdgcn_perm(codes_of(xk[K].hi, qk), codes_of(xk[K].lo, qk), 0x06040200u);
+                    if (in(K)) *(uint32_t*)(krow + K * D) = w;
+                } else if constexpr (BITS == 4) {
                     // dims 8 j .. + 3 in an even lane (nibbles 0, 4, 1, 5), .. + 7 in the odd one (2, 6, 3, 7)
                     uint32_t w = put_byte<0>(0u, __builtin_fmaf(16.0f, c[2], c[0]));
                     w = put_byte<2>(w, __builtin_fmaf(16.0f, c[3], c[1]));
@@ -376,10 +402,17 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
                 for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        uint32_t x = put_byte<0>(0u, cv[4 * j][i]);
-                        x = put_byte<1>(x, cv[4 * j + 1][i]);
-                        x = put_byte<2>(x, cv[4 * j + 2][i]);
-                        x = put_byte<3>(x, cv[4 * j + 3][i]);
+                        uint32_t x;
+                        if constexpr (INT8) {
+                            const uint32_t a = __builtin_amdgcn_perm(cv2[4 * j + 1][i / 2], cv2[4 * j][i / 2], 0x06020400u);
+                            const uint32_t b = __builtin_amdgcn_perm(cv2[4 * j + 3][i / 2], cv2[4 * j + 2][i / 2], 0x06020400u);
+                            x = __builtin_amdgcn_perm(b, a, i & 1 ? 0x07060302u : 0x05040100u);
+                        } else {
+                            x = put_byte<0>(0u, cv[4 * j][i]);
+                            x = put_byte<1>(x, cv[4 * j + 1][i]);
+                            x = put_byte<2>(x, cv[4 * j + 2][i]);
+                            x = put_byte<3>(x, cv[4 * j + 3][i]);
+                        }
                         const uint32_t o = old[i / 2][2 * (i & 1) + j];
                         old[i / 2][2 * (i & 1) + j] = (x & m[j]) | (o & ~m[j]);
                     }
