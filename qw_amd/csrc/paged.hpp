@@ -18,7 +18,7 @@
 // to the softmax weights.
 // Beside them, for each page and head: the least and the largest key of every dim over what was
 // written since slot 0 last was ([2][D] fp16), the same as 8-bit codes over the page's largest
-// magnitude ([2][D], largest first), that magnitude, and E >= 0 with every V scale below 2^E.
+// magnitude ([2][D], largest first), and that magnitude.
 #pragma once
 
 #include "kv_cache.hpp"
@@ -56,6 +56,9 @@ struct PagedSeqs {
     int each;
     const int32_t* starts;
     int n_tokens;
+
+    // Runs of `size` slots that a sequence's tokens can touch, where each has as many of them.
+    __host__ __device__ int runs(int size) const { return each == 1 ? 1 : (int)(((int64_t)each + size - 2) / size) + 1; }
 };
 
 int paged_update(PagedCache& c, const void* k, const void* v, int64_t k_token, int64_t k_head, int64_t v_token,
@@ -115,22 +118,38 @@ struct PagedUnit {
     int b;
     uint32_t at, base;  // base: units before the sequence
 };
+// (from sequence b0 on, before which lie `base` units)
 template <class F>
-__device__ __forceinline__ PagedUnit find_unit(int n, uint32_t i, F count) {
+__device__ __forceinline__ PagedUnit find_unit(int n, uint32_t i, F count, int b0 = 0, uint32_t base = 0) {
     const int lane = (int)__lane_id();
-    uint32_t base = 0;
-    for (int b0 = 0; b0 < n; b0 += 64) {
-        const uint32_t c = b0 + lane < n ? count(b0 + lane) : 0u;
+    PagedUnit u{-1, 0u, 0u};
+    auto in = [&](int at, uint32_t c) {  // (c: sequence at + lane's)
         const uint32_t s = wave_scan(c);
         const uint64_t past = __ballot(base + s > i);
         if (past) {
             const int l = __builtin_ctzll(past);
-            const uint32_t before = base + (uint32_t)__builtin_amdgcn_readlane((int)(s - c), l);
-            return {__builtin_amdgcn_readfirstlane(b0 + l), i - before, before};
+            u.base = base + (uint32_t)__builtin_amdgcn_readlane((int)(s - c), l);
+            u.b = __builtin_amdgcn_readfirstlane(at + l);
+            u.at = i - u.base;
         }
         base += (uint32_t)__builtin_amdgcn_readlane((int)s, 63);
+        return past != 0;
+    };
+    constexpr int AHEAD = 4;  // of many, these times 64 at once
+    for (; n - b0 > 64; b0 += 64 * AHEAD) {
+        uint32_t c[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            const int b = b0 + 64 * k + lane;
+            c[k] = count(min(b, n - 1));
+            c[k] = b < n ? c[k] : 0u;
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++)
+            if (in(b0 + 64 * k, c[k])) return u;
     }
-    return {-1, 0u, base};
+    if (b0 < n) in(b0, b0 + lane < n ? count(b0 + lane) : 0u);
+    return u;
 }
 
 // Where sequence b's new tokens go: positions start .. start + n - 1, from token `first` on.

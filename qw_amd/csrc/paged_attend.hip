@@ -48,6 +48,8 @@ struct AttendArgs {
     int whole;           // sequences stay whole, and no second launch follows
     float* part_o;    // [2 workers][hkv][R][D]
     float2* part_ml;  // [2 workers][hkv][R]
+    uint4* cut;       // above 64 sequences, for each worker: the one whose first piece ends its run, unfinished (or -1),
+                      // the rounds before it, its own, and all
 };
 
 // A sequence's keys as the kernel walks them: the whole of it, or its picked pages side by side.
@@ -82,7 +84,11 @@ __device__ __forceinline__ Plan plan_of(const AttendArgs& a) {
         p.total = wave_last(p.through);
     } else {
         uint32_t n = 0;
-        for (int b = lane; b < a.n_seq; b += 64) n += rounds_of(a, b);
+#pragma unroll 8
+        for (int b0 = 0; b0 < a.n_seq; b0 += 64) {
+            const uint32_t c = rounds_of(a, min(b0 + lane, a.n_seq - 1));
+            n += b0 + lane < a.n_seq ? c : 0u;
+        }
         p.total = wave_last(wave_scan(n));
     }
     p.workers = min((uint32_t)a.workers, p.total);  // (a round at least for each that works)
@@ -113,14 +119,15 @@ __device__ __forceinline__ Piece piece_of(const AttendArgs& a, uint32_t per, uin
     const uint32_t begin = w * per + min(w, rest), end = begin + per + (w < rest);
     return Piece{b, len, at - before, min(all, end - before), all, 2 * w + (at == before && at != begin ? 1 : 0)};
 }
-__device__ __forceinline__ Piece piece_at(const AttendArgs& a, uint32_t per, uint32_t rest, uint32_t w, uint32_t at) {
-    const PagedUnit u = find_unit(a.n_seq, at, [&](int b) { return rounds_of(a, b); });
+// (among the sequences from b0 on, before which lie `base` rounds)
+__device__ __forceinline__ Piece piece_from(const AttendArgs& a, uint32_t per, uint32_t rest, uint32_t w, uint32_t at, int b0, uint32_t base) {
+    const PagedUnit u = find_unit(a.n_seq, at, [&](int b) { return rounds_of(a, b); }, b0, base);
     if (u.b < 0) return Piece{-1, 0, 0, 0, 0, 0};
     return piece_of(a, per, rest, w, at, u.b, min(max(a.lengths[u.b], 0), a.width << a.c.lg), rounds_of(a, u.b), u.base);
 }
 // Its first piece (piece by piece: its only one); at: the round that it begins with.
 __device__ __forceinline__ Piece first_piece(const AttendArgs& a, const Plan& p, uint32_t w, uint32_t at) {
-    if (a.n_seq > 64) return piece_at(a, p.per, p.rest, w, at);
+    if (a.n_seq > 64) return piece_from(a, p.per, p.rest, w, at, 0, 0u);
     const uint64_t past = __ballot(p.most ? p.last > w : p.through > at);
     if (!past) return Piece{-1, 0, 0, 0, 0, 0};
     const int b = __builtin_ctzll(past);
@@ -330,19 +337,23 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
     f16* sq = (f16*)(sml + TILES * KW * 16);
 
     const uint32_t w = blockIdx.x;
-    uint32_t at = 0, end = 0, per, rest;  // (one piece: end stays below)
+    uint32_t at = 0, end = 0, per, rest, total;  // (one piece: end stays below)
     Piece piece;
     {
         const Plan plan = plan_of(a);
         per = plan.per, rest = plan.rest;
-        if (a.whole) {  // sequences without keys are zeros (else the second launch's)
-            for (int b = w; b < a.n_seq; b += gridDim.x) {
-                const uint32_t n = a.n_seq <= 64 ? (uint32_t)__builtin_amdgcn_readlane((int)plan.rounds, b) : rounds_of(a, b);
-                if (n == 0)
-                    for (int i = threadIdx.x; i < min(a.R - row0, 16 * RT) * (D / 4); i += NT)
-                        *(half4v*)(a.out + ((b * (int64_t)a.c.hkv + h) * a.R + row0) * D + 4 * i) = half4v{};
+        const bool many = a.n_seq > 64;
+        if (a.whole || many) {  // sequences without keys are zeros (else the second launch's)
+            for (int b0 = 64 * w; b0 < a.n_seq; b0 += 64 * gridDim.x) {
+                const uint32_t n = b0 + lane >= a.n_seq ? 1u : many ? rounds_of(a, b0 + lane) : plan.rounds;
+                for (uint64_t none = __ballot(n == 0); none; none &= none - 1) {
+                    const int64_t at = ((b0 + __builtin_ctzll(none)) * (int64_t)a.c.hkv + h) * a.R + row0;
+                    for (int i = threadIdx.x; i < min(a.R - row0, 16 * RT) * (D / 4); i += NT) *(half4v*)(a.out + at * D + 4 * i) = half4v{};
+                }
             }
         }
+        total = plan.total;
+        if (many && !a.whole && (threadIdx.x | h | row0) == 0) a.cut[w].x = ~0u;
         if (!plan.most) {
             if (w >= plan.workers) return;
             at = w * per + min(w, rest);
@@ -718,33 +729,44 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
                 }
             }
         }
+        if (a.n_seq > 64 && !a.whole && r0 == 0 && r1 < piece.all && (threadIdx.x | h | row0) == 0)
+            a.cut[w] = uint4{(uint32_t)b, at, piece.all, total};
         at += r1 - r0;
         if (at >= end) return;
-        piece = piece_at(a, per, rest, w, at);
+        piece = piece_from(a, per, rest, w, at, b + 1, at);
     }
 }
 
 // Joins a row's pieces: grid (rows of all heads, n_seq). A sequence within one worker's run was written
-// by it; one without keys is zeros.
+// by it; one without keys is zeros. Above 64 sequences grid (rows of all heads, workers): a worker's part of
+// it is the sequence that its run leaves unfinished, if it begins there (by sequences, each looking for its place: 1024 of up
+// to 256 keys, D = 128, 8 bits, 297 us for 130).
 template <int D>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttendArgs a) {
     constexpr int TC = D / 4, SG = 256 / TC;
     __shared__ float4v sm_o[256];
     __shared__ float sm_l[SG];
-    const int tid = threadIdx.x, b = blockIdx.y, h = (int)blockIdx.x / a.R, row = (int)blockIdx.x % a.R;
-    const Plan plan = plan_of(a);
+    const int tid = threadIdx.x, h = (int)blockIdx.x / a.R, row = (int)blockIdx.x % a.R;
     const int lane = tid & 63;
-    uint32_t mine, before = 0, n, slot0;  // the sequence's rounds; its pieces, the first one's slot
-    int64_t step = 2;
-    if (a.n_seq <= 64) {
-        mine = (uint32_t)__builtin_amdgcn_readlane((int)plan.rounds, b);
-        before = (uint32_t)__builtin_amdgcn_readlane((int)plan.through, b) - mine;
+    int b = blockIdx.y;
+    Plan plan;
+    uint32_t mine, before; // the sequence's rounds, and those before it
+    if (a.cut) {
+        const uint4 x = a.cut[b];
+        b = (int)x.x;
+        if (b < 0) return;
+        before = x.y, mine = x.z;
+        plan.workers = min((uint32_t)a.workers, x.w);
+        plan.per = x.w / plan.workers;
+        plan.rest = x.w - plan.per * plan.workers;
+        plan.most = 0;
     } else {
-        mine = rounds_of(a, b);
-        uint32_t x = 0;
-        for (int i = lane; i < b; i += 64) x += rounds_of(a, i);
-        before = wave_last(wave_scan(x));
+        plan = plan_of(a);  // (above 64: tables without columns)
+        mine = a.n_seq > 64 ? 0u : (uint32_t)__builtin_amdgcn_readlane((int)plan.rounds, b);
+        before = a.n_seq > 64 ? 0u : (uint32_t)__builtin_amdgcn_readlane((int)plan.through, b) - mine;
     }
+    uint32_t n, slot0;  // its pieces, the first one's slot
+    int64_t step;
     const int d = tid % TC * 4, sg = tid / TC;
     f16* to = a.out + ((b * (int64_t)a.c.hkv + h) * a.R + row) * D + d;
     if (mine == 0) {
@@ -905,9 +927,11 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     a.whole = rounds > 0 && (most <= round || (most <= few * round && q.n_seq <= 64 && q.n_seq <= a.workers));
     const int64_t parts = a.whole ? 0 : (int64_t)a.workers * 2 * c.hkv * a.R;
     void* ws = nullptr;
-    if (int rc = workspace(kWsPaged, c.device, stream, (size_t)(parts * (c.D * 4 + 8)), &ws)) return rc;
+    const bool cuts = q.n_seq > 64 && rounds > 0 && !a.whole;
+    if (int rc = workspace(kWsPaged, c.device, stream, (size_t)(parts * (c.D * 4 + 8) + (cuts ? a.workers * 16 : 0)), &ws)) return rc;
     a.part_o = (float*)ws;
     a.part_ml = (float2*)(a.part_o + parts * c.D);
+    a.cut = cuts ? (uint4*)(a.part_ml + parts) : nullptr;
     if (rounds > 0) {
         const int rc = by_shape(c.bits, c.int8(), c.D, tiles, [&](auto b, auto i8, auto d, auto t) {
             return launch_attend<decltype(b)::value, decltype(d)::value, decltype(i8)::value, decltype(t)::value>(a, stream);
@@ -915,7 +939,7 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
         if (rc) return rc;
     }
     if (a.whole) return QW_OK;
-    const dim3 grid((unsigned)(c.hkv * a.R), q.n_seq);
+    const dim3 grid((unsigned)(c.hkv * a.R), cuts ? a.workers : q.n_seq);
     if (c.D == 256)
         hipLaunchKernelGGL(paged_merge_kernel<256>, grid, dim3(256), 0, stream, a);
     else

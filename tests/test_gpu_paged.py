@@ -529,3 +529,69 @@ def test_first_use_inside_a_capture():
     torch.cuda.synchronize()
     assert refused and torch.all(x == 1)
     assert torch.equal(s.cache.attention(q, t, n, 0.1), want)
+
+
+@pytest.mark.parametrize("mode,hq,hkv,n_seq", [("int8", 4, 2, 130), ("affine4", 2, 2, 300), ("fp16", 40, 2, 65)])
+def test_many_sequences_of_which_few_are_long(mode, hq, hkv, n_seq):
+    """More than a wave's lanes: runs that end in a long sequence, begin with one, or hold many, empty ones among them."""
+    r = rng(n_seq)
+    lengths = [int(x) for x in r.integers(0, 40, n_seq)]
+    lengths[3], lengths[64], lengths[n_seq - 1] = 5000, 2611, 1500
+    lengths[4:20] = [0] * 16
+    lengths[5] = 256
+    s = Sequences(r, mode, hkv, 128, 16, lengths)
+    q = queries(r, n_seq, hq, 1, 128)
+    out = s.cache.attention(q, ints(s.table), ints(lengths), 0.09)
+    s.check(out, q, 0.09)
+    assert torch.equal(s.cache.attention(q, ints(s.table), ints(lengths), 0.09), out)
+    none = s.cache.attention(q, ints(s.table), ints([0] * n_seq), 0.09)
+    assert torch.all(none == 0)
+    none = s.cache.attention(q, ints(s.table)[:, :0], ints(lengths), 0.09)
+    assert torch.all(none == 0)
+
+
+@pytest.mark.parametrize("n_seq", [65, 127, 200, 1000])
+def test_stores_of_many_sequences(n_seq):
+    """More sequences than a wave's lanes, most of them with no token."""
+    import qw_amd
+
+    r = rng(n_seq)
+    hkv, D, ps = 2, 128, 16
+    n = [int(x) if r.random() < 0.3 else 0 for x in r.integers(1, 25, n_seq)]
+    n[-1] = 17
+    starts = [int(x) for x in r.integers(0, 20, n_seq)]
+    width = 3
+    cache = qw_amd.PagedKVCache("affine8", hkv, D, n_seq * width, page_size=ps)
+    table = ints(r.permutation(n_seq * width).reshape(n_seq, width))
+    k, v = rows(r, sum(n), hkv, D), rows(r, sum(n), hkv, D)
+    offsets = ints(np.concatenate([[0], np.cumsum(n)]))
+    cache.update(dev(k), dev(v), table, ints(starts), offsets)
+    got = cache.gather(table, ints(starts), sum(n), offsets)
+    for a, b in zip(got, stored("affine8", k, v, hkv, D)):
+        assert np.array_equal(a.cpu().numpy(), b)
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_values_of_one_sign(mode):
+    """Values of 0 and more: a V group's middle lies far from many of them. Its weights' rounding meets a code's distance from
+    the middle, at most c0 scale <= 1.004 * the group's largest value / 2 * 2, and the middle itself twice (the weights'
+    rounding and its own): 3.02 U of the group's largest value for each key, and the result's rounding."""
+    r = rng(90)
+    D, n = 128, 300
+    s = Sequences(r, mode, 1, D, 16, [n])
+    v = np.maximum(rows(r, n, 1, D), 0)
+    v[:, :, 5] = 0
+    s.cache.update(dev(s.k[0]), dev(v), ints(s.table), ints([0]))
+    s.v = [v]
+    q = queries(r, 1, 4, 1, D)
+    out = s.cache.attention(q, ints(s.table), ints([n]), 0.09).double().cpu().numpy()
+    k, vv = unrounded(mode, s.k[0], 1, D), unrounded(mode, v, 1, D)
+    big = np.repeat(np.abs(v[:, 0]).astype(np.float64).reshape(n, D // 64, 64).max(2), 64, axis=1)
+    for j in range(4):
+        x = q[0, j, 0].double().cpu().numpy()
+        sc = (k[0][0] @ x) * 0.09
+        p = np.exp(sc - sc.max())
+        g = (D + 40) * E * 0.09 * (k[2][0] @ np.abs(x)).max()
+        ref = p @ vv[0][0] / p.sum()
+        bar = (3.02 * U + 2 * g + 60 * E) * (p @ big) / p.sum() + U * np.abs(ref) + 2.0 ** -25 + n * 2.0 ** -28 / p.sum()
+        assert (np.abs(out[0, j, 0] - ref) <= bar).all()
