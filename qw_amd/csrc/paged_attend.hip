@@ -45,7 +45,7 @@ struct AttendArgs {
     int n_picked;
     float scale2;  // scale * log2 e
     int workers, round;  // keys of a round: 32 a wave
-    int whole;           // sequences stay whole, and no second launch follows
+    int whole;           // sequence by sequence, worker b % workers' each, and no second launch follows
     float* part_o;    // [2 workers][hkv][R][D]
     float2* part_ml;  // [2 workers][hkv][R]
     uint4* cut;       // above 64 sequences, for each worker: the one whose first piece ends its run, unfinished (or -1),
@@ -96,7 +96,7 @@ __device__ __forceinline__ Plan plan_of(const AttendArgs& a) {
     p.per = __builtin_amdgcn_readfirstlane(p.total / p.workers);
     p.rest = p.total - p.per * p.workers;
     if (a.n_seq <= 64) {
-        uint32_t most = a.whole ? p.total : p.per + (p.rest > 0);
+        uint32_t most = p.per + (p.rest > 0);
         for (int i = 0; i < 4; i++, most += 1 + most / 16) {
             p.pieces = (p.rounds + most - 1) / most;
             p.last = wave_scan(p.pieces);
@@ -339,21 +339,32 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
     const uint32_t w = blockIdx.x;
     uint32_t at = 0, end = 0, per, rest, total;  // (one piece: end stays below)
     Piece piece;
-    {
-        const Plan plan = plan_of(a);
-        per = plan.per, rest = plan.rest;
-        const bool many = a.n_seq > 64;
-        if (a.whole || many) {  // sequences without keys are zeros (else the second launch's)
-            for (int b0 = 64 * w; b0 < a.n_seq; b0 += 64 * gridDim.x) {
-                const uint32_t n = b0 + lane >= a.n_seq ? 1u : many ? rounds_of(a, b0 + lane) : plan.rounds;
-                for (uint64_t none = __ballot(n == 0); none; none &= none - 1) {
-                    const int64_t at = ((b0 + __builtin_ctzll(none)) * (int64_t)a.c.hkv + h) * a.R + row0;
-                    for (int i = threadIdx.x; i < min(a.R - row0, 16 * RT) * (D / 4); i += NT) *(half4v*)(a.out + at * D + 4 * i) = half4v{};
-                }
-            }
+    auto zeros = [&](int b) {  // of a sequence without keys
+        const int64_t at = (b * (int64_t)a.c.hkv + h) * a.R + row0;
+        for (int i = threadIdx.x; i < min(a.R - row0, 16 * RT) * (D / 4); i += NT) *(half4v*)(a.out + at * D + 4 * i) = half4v{};
+    };
+    auto whole_from = [&](int b) {
+        for (; b < a.n_seq; b += gridDim.x) {
+            const int len = min(max(a.lengths[b], 0), a.width << a.c.lg);
+            const uint32_t all = (uint32_t)(keys_of(a, len) + a.round - 1) / a.round;
+            if (all) return Piece{b, len, 0, all, all, 0};
+            zeros(b);
         }
-        total = plan.total;
-        if (many && !a.whole && (threadIdx.x | h | row0) == 0) a.cut[w].x = ~0u;
+        return Piece{-1, 0, 0, 0, 0, 0};
+    };
+    if (a.whole) {
+        per = rest = total = 0;
+        piece = whole_from(w);
+    } else {
+        const Plan plan = plan_of(a);
+        per = plan.per, rest = plan.rest, total = plan.total;
+        if (a.n_seq > 64) {  // (else the second launch's)
+            for (int b0 = 64 * w; b0 < a.n_seq; b0 += 64 * gridDim.x) {
+                const uint32_t n = b0 + lane < a.n_seq ? rounds_of(a, b0 + lane) : 1u;
+                for (uint64_t none = __ballot(n == 0); none; none &= none - 1) zeros(b0 + __builtin_ctzll(none));
+            }
+            if ((threadIdx.x | h | row0) == 0) a.cut[w].x = ~0u;
+        }
         if (!plan.most) {
             if (w >= plan.workers) return;
             at = w * per + min(w, rest);
@@ -729,7 +740,11 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
                 }
             }
         }
-        if (a.n_seq > 64 && !a.whole && r0 == 0 && r1 < piece.all && (threadIdx.x | h | row0) == 0)
+        if (a.whole) {
+            piece = whole_from(b + gridDim.x);
+            continue;
+        }
+        if (a.n_seq > 64 && r0 == 0 && r1 < piece.all && (threadIdx.x | h | row0) == 0)
             a.cut[w] = uint4{(uint32_t)b, at, piece.all, total};
         at += r1 - r0;
         if (at >= end) return;
@@ -922,9 +937,11 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     // A sequence of few rounds is read by one worker where the rounds one after another cost less than the second launch,
     // which joins pieces (of one round none is cut anyway). Whole / cut, a pass in us, 1 sequence: D = 256, 8 bits, 3 rounds
     // 11.7 / 12.0, 5 rounds 15.6 / 12.1, fp16 12.8 / 12.8 and 17.2 / 13.1; D = 128, 8 bits, 3 rounds 9.0 / 11.2, 5
-    // rounds 11.7 / 11.2, fp16 8.0 / 11.2 and 9.9 / 11.2. 16 sequences, D = 128, 5 rounds 12.4 / 13.9 and 11.0 / 16.3.
-    const int few = c.D == 256 ? 3 : c.bits == 16 ? 5 : 4;
-    a.whole = rounds > 0 && (most <= round || (most <= few * round && q.n_seq <= 64 && q.n_seq <= a.workers));
+    // rounds 11.7 / 11.2, fp16 8.0 / 11.2 and 9.9 / 11.2. 16 sequences, D = 128, 5 rounds 12.4 / 13.9 and 11.0 / 16.3. With
+    // more than 64, whose cuts take a search, up to 8: D = 128, 8 bits, 65 sequences 32.0 / 34.9, 128 41.0 / 50.8, 256 97.7 /
+    // 102, 1024 374 / 368; D = 256, 4 bits, 128 32.9 / 49.8, 1024 246 / 255.
+    const int few = q.n_seq > 64 ? 8 : c.D == 256 ? 3 : c.bits == 16 ? 5 : 4;
+    a.whole = rounds > 0 && most <= few * round;
     const int64_t parts = a.whole ? 0 : (int64_t)a.workers * 2 * c.hkv * a.R;
     void* ws = nullptr;
     const bool cuts = q.n_seq > 64 && rounds > 0 && !a.whole;

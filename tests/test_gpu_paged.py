@@ -595,3 +595,15 @@ def test_values_of_one_sign(mode):
         ref = p @ vv[0][0] / p.sum()
         bar = (3.02 * U + 2 * g + 60 * E) * (p @ big) / p.sum() + U * np.abs(ref) + 2.0 ** -25 + n * 2.0 ** -28 / p.sum()
         assert (np.abs(out[0, j, 0] - ref) <= bar).all()
+
+
+@pytest.mark.parametrize("mode,D,n_seq,most", [("affine8", 128, 300, 1024), ("affine4", 256, 270, 640), ("fp16", 128, 129, 1100)])
+def test_more_sequences_than_workers(mode, D, n_seq, most):
+    """A worker's several sequences, one behind the other, whole (up to 8 rounds) or in runs."""
+    r = rng(n_seq + D)
+    lengths = [int(x) for x in r.integers(0, 60, n_seq)]
+    lengths[0], lengths[128], lengths[n_seq - 1] = most, most - 3, 129
+    lengths[7:11] = [0] * 4
+    s = Sequences(r, mode, 4, D, 16, lengths)
+    q = queries(r, n_seq, 4, 1, D)
+    s.check(s.cache.attention(q, ints(s.table), ints(lengths), 0.07), q, 0.07)
