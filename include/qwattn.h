@@ -570,12 +570,14 @@ int qw_paged_gather(const qw_paged_cache* cache, void* k_out, void* v_out, int n
 /* Attention of each sequence's newest n_rows tokens over its first lengths[b] keys, the newest
  * among them: row r sees keys t <= lengths[b] - n_rows + r.
  *   out = softmax(scale q . k) . v   on code * scale + bias unrounded, in fp32 but for the weights'
- *     rounding to fp16 in P . V; a row that sees no key is 0.
+ *     rounding to fp16 in P . V and, in the affine modes, that of a V group's middle (bias + 8 or 128
+ *     scales); a row that sees no key is 0.
  *   q [n_seq][n_q_heads][n_rows][head_dim] fp16 with element strides of whole 8, 16-byte aligned
  *   lengths [n_seq] int32 device (clamped to 0 .. table_width * page_size)
  *   picked (or NULL: all pages) [n_seq][n_kv_heads][n_picked] int32 device: the pages that a KV head
  *     reads, as columns of its sequence's table row (entries outside it are skipped; of
- *     each list the first min(n_picked, the sequence's pages) entries are read; qw_paged_select writes such)
+ *     each list the first min(n_picked, the sequence's pages) entries are read, and a page that is named twice
+ *     counts twice, here as in the table; qw_paged_select writes such)
  *   out [n_seq][n_q_heads][n_rows][head_dim] fp16
  * Keys that a later row sees and this one does not must be finite. |scale| <= 2^40; at most 16384 rows
  * (n_rows * heads of a group) a KV head. n_seq = 0: nothing happens. */

@@ -236,3 +236,10 @@ def test_paged_contract_fails_before_device_work(qwlib):
                dict(D=1024, R=514), dict(base=0.0), dict(base=float("inf")), dict(scale=float("nan")), dict(pos=None),
                dict(stride=3), dict(n_axes=0), dict(n_axes=2), dict(axes=None), dict(hq=2 ** 30)):
         assert rope(**kw) == 1, kw
+
+
+def test_rope_axes_grid_limit(qwlib):
+    """More workgroups than a launch takes are refused before it."""
+    one = ctypes.c_void_p(16)
+    assert qwlib.qw_rope_axes(one, 1 << 28, 1, 1, 2, 2, 0, 1e4, 1.0, one, 1 << 28, 1, bytes([0]), one, one, None) == 2
+    assert b"too many tokens" in qwlib.qw_last_error()

@@ -82,6 +82,12 @@ def rows(r, n, hkv, D, sigma=1.0):
     return (sigma * r.standard_normal((n, hkv, D))).astype(np.float16)
 
 
+def side_stream():
+    """A stream of torch's, which hands its 32 out in turn. A workspace that a graph holds stays its stream's: a whole turn
+    leaves the tests behind this one the streams that they had."""
+    return [torch.cuda.Stream() for _ in range(32)][0]
+
+
 class Sequences:
     """Random sequences of the given lengths in a pool, with a spare page of NaN-free rubbish."""
 
@@ -514,7 +520,7 @@ def test_first_use_inside_a_capture():
     s = Sequences(r, "affine4", 2, 128, 16, [3000])
     q, t, n = queries(r, 1, 8, 1, 128), ints(s.table), ints([3000])
     want = s.cache.attention(q, t, n, 0.1)
-    stream = torch.cuda.Stream()
+    stream = side_stream()
     stream.wait_stream(torch.cuda.current_stream())
     g = torch.cuda.CUDAGraph()
     refused = False
@@ -607,3 +613,24 @@ def test_more_sequences_than_workers(mode, D, n_seq, most):
     s = Sequences(r, mode, 4, D, 16, lengths)
     q = queries(r, n_seq, 4, 1, D)
     s.check(s.cache.attention(q, ints(s.table), ints(lengths), 0.07), q, 0.07)
+
+
+@pytest.mark.parametrize("mode", ["int8", "affine4"])
+def test_a_page_named_twice_counts_twice(mode):
+    """In a list of pages and in the table, as the same keys stored twice would."""
+    r = rng(91)
+    hkv, D, ps, scale = 2, 128, 16, 0.09
+    s = Sequences(r, mode, hkv, D, ps, [6 * ps])
+    q = queries(r, 1, 4, 1, D)
+    twice = np.array([[1, 4, 1, 0, 1]] * hkv)[None]
+    table = ints(np.concatenate([s.table[:, :6], s.table[:, twice[0, 0]]], axis=1))  # the same columns, once more
+    out = s.cache.attention(q, ints(s.table), ints([6 * ps]), scale, picked=ints(twice))
+    # (unmasked: every key of the first 6 pages is before the end)
+    keys = np.concatenate([np.arange(ps) + ps * p for p in twice[0, 0]])
+    again = Sequences(r, mode, hkv, D, ps, [5 * ps])
+    again.k[0], again.v[0] = s.k[0][keys], s.v[0][keys]
+    again.check(out, q, scale)
+    out = s.cache.attention(q, table, ints([11 * ps]), scale)
+    both = Sequences(r, mode, hkv, D, ps, [11 * ps])
+    both.k[0], both.v[0] = np.concatenate([s.k[0], s.k[0][keys]]), np.concatenate([s.v[0], s.v[0][keys]])
+    both.check(out, q, scale)

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from conftest import rng
-from test_gpu_paged import MODES, Sequences, dev, ints, queries, rows
+from test_gpu_paged import MODES, Sequences, dev, ints, queries, rows, side_stream
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -249,7 +249,7 @@ def test_a_step_in_a_graph(mode):
     spare = [p for p in range(s.n_pages) if p not in s.table]
     s.table[0, 19], s.table[1, 6] = spare[:2]
     table.copy_(ints(s.table))
-    stream = torch.cuda.Stream()
+    stream = side_stream()
     stream.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(stream):
         n.add_(1)
@@ -283,11 +283,11 @@ def test_two_streams_and_threads():
         t, n = ints(s.table[b:b + 1]), ints([s.lengths[b]])
         args.append((q, t, n, s.cache.select_pages(q, t, n, 9, recent=1), s.cache.attention(q, t, n, 1 / 16)))
     torch.cuda.synchronize()
-    wrong = []
+    wrong, streams = [], [side_stream(), side_stream()]
 
     def work(b):
         q, t, n, picked, out = args[b]
-        stream = torch.cuda.Stream()
+        stream = streams[b]
         with torch.cuda.stream(stream):
             for _ in range(30):
                 p = s.cache.select_pages(q, t, n, 9, recent=1)
