@@ -120,8 +120,9 @@ int rope_axes(const RopeAxes& r, const void* qkv, int n_tokens, int hq, int hkv,
     a.traditional = r.traditional;
     a.log2_base = std::log2((double)r.base);
     a.scale = (double)r.scale / 6.283185307179586476925;
-    // a token a workgroup while there are few, else as many as its angles' place holds, up to 8
-    a.tokens = std::max(1, std::min({8, n_tokens / 1024, kAngles / a.half}));
+    // a token a workgroup while there are few, else as many as its angles' place holds, up to 8. One / 8, 32 + 8 heads of
+    // D = 128, us: 64 tokens 5.3 / 19.5, 1500 10.5 / 22.2, 4099 19.2 / 26.9, 32768 154 / 145
+    a.tokens = std::max(1, std::min({8, n_tokens / 4096, kAngles / a.half}));
     const int64_t groups = ((int64_t)n_tokens + a.tokens - 1) / a.tokens;
     QW_REQUIRE(groups * 256 <= UINT32_MAX, QW_ERR_UNSUPPORTED, "rope axes: too many tokens for one call");
     const dim3 grid((unsigned)groups);

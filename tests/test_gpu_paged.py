@@ -634,3 +634,13 @@ def test_a_page_named_twice_counts_twice(mode):
     both = Sequences(r, mode, hkv, D, ps, [11 * ps])
     both.k[0], both.v[0] = np.concatenate([s.k[0], s.k[0][keys]]), np.concatenate([s.v[0], s.v[0][keys]])
     both.check(out, q, scale)
+
+
+@pytest.mark.parametrize("mode,D,L", [("affine4", 256, 90), ("fp16", 128, 260), ("int8", 256, 33)])
+def test_many_rows(mode, D, L):
+    """Row tiles over many workgroups, tiles that end in a head, rows before a sequence's first key."""
+    r = rng(L)
+    lengths = [L + 70, L, 100 if L > 100 else 20]
+    s = Sequences(r, mode, 1, D, 32, lengths)
+    q = queries(r, 3, 3, L, D)
+    s.check(s.cache.attention(q, ints(s.table), ints(lengths), 0.07), q, 0.07)
