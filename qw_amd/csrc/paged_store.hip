@@ -259,8 +259,8 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
     __shared__ half4v sm_lo[kStoreWaves][LPR], sm_hi[kStoreWaves][LPR];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     // (heads side by side: a token's row of all heads is read at about the same time)
-    const int nw = blockDim.x >> 6, h = (int)(blockIdx.x % c.hkv), ps = 1 << c.lg;
-    const PagedUnit u = unit_of(a.s, blockIdx.x / c.hkv, ps, [&](int b) {
+    const int nw = blockDim.x >> 6, h = (int)((blockIdx.x >> 3) % c.hkv), ps = 1 << c.lg;
+    const PagedUnit u = unit_of(a.s, (blockIdx.x >> 3) / c.hkv * 8 + (blockIdx.x & 7), ps, [&](int b) {
         const PagedSpan p = span_of(a.s, b, c.lg);
         const int n = span_in_table(a.s, p, c.lg);
         return n > 0 ? (uint32_t)(((p.start + n - 1) >> c.lg) - (p.start >> c.lg) + 1) : 0u;
@@ -514,9 +514,9 @@ template <int BITS, bool INT8, int D>
 __global__ __launch_bounds__(256) void paged_gather_kernel(PagedView c, PagedSeqs s, f16* k_out, f16* v_out) {
     constexpr int LPR = D / 4, SUB = 64 / LPR, NG = INT8 ? 1 : D / kGroup;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int h = (int)(blockIdx.x % c.hkv), ps = 1 << c.lg;
+    const int h = (int)((blockIdx.x >> 3) % c.hkv), ps = 1 << c.lg;
     const int li = lane % LPR, sub = lane / LPR, grp = INT8 ? 0 : li >> 4;
-    const uint32_t unit = (blockIdx.x / c.hkv * 4 + wave) * SUB;
+    const uint32_t unit = (((blockIdx.x >> 3) / c.hkv * 8 + (blockIdx.x & 7)) * 4 + wave) * SUB;
     auto blocks = [&](int b) {
         const PagedSpan p = span_of(s, b, c.lg);
         return p.n > 0 ? (uint32_t)((((int64_t)p.start + p.n - 1) >> 3) - (p.start >> 3) + 1) : 0u;
@@ -632,7 +632,7 @@ int paged_update(PagedCache& c, const void* k, const void* v, int64_t k_token, i
     // 19.5 / 32.0; 13107 each of 5, pages of 32, D = 128 65 / 163 / 66
     const int blocks = std::min(c.page_size / 8, s.n_tokens / s.n_seq / 8 + 1);
     const int waves = std::max(1, std::min(kStoreWaves, blocks * c.D / 256));
-    const int64_t groups = most_units(s, c.page_size) * c.hkv;
+    const int64_t groups = (most_units(s, c.page_size) + 7) / 8 * 8 * c.hkv;
     QW_REQUIRE(groups * 64 * waves <= UINT32_MAX, QW_ERR_UNSUPPORTED, "paged update: too many tokens for one call");
     const dim3 grid((unsigned)groups);
     by_mode(c, [&](auto bits, auto i8, auto d) {
@@ -651,7 +651,7 @@ int paged_gather(const PagedCache& c, void* k_out, void* v_out, const PagedSeqs&
     DeviceGuard dg(c.device);
     QW_REQUIRE(dg.ok, QW_ERR_HIP, "paged gather: hipSetDevice failed");
     const int64_t per = 4 * 256 / c.D;  // units a workgroup
-    const int64_t groups = (most_units(s, 8) + per - 1) / per * c.hkv;
+    const int64_t groups = (most_units(s, 8) + 8 * per - 1) / (8 * per) * 8 * c.hkv;
     QW_REQUIRE(groups * 256 <= UINT32_MAX, QW_ERR_UNSUPPORTED, "paged gather: too many tokens for one call");
     const dim3 grid((unsigned)groups);
     by_mode(c, [&](auto bits, auto i8, auto d) {
