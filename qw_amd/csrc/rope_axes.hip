@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
             }
         }
         if constexpr (VEC)
-            *(half8*)(out + d) = *(const half8*)y;
+            __builtin_nontemporal_store(*(const half8*)y, (half8*)(out + d));
         else
             out[d] = y[0];
     }
