@@ -185,25 +185,31 @@ struct Shape {
 // One load of 64 times 16 bytes to LDS. M0, which gives the place, is saved and restored so that the compiler's
 // view of it holds; the offset counts for both addresses. The compiler knows nothing of the load: what reads the
 // place waits by wait_loads first.
-template <int OFFSET>
+#define QW_TO_LDS(CACHE)                                            \
+    asm volatile(                                                   \
+        "s_mov_b32 %0, m0\n\t"                                      \
+        "s_mov_b32 m0, %2\n\t"                                      \
+        "s_nop 0\n\t"                                               \
+        "global_load_lds_dwordx4 %1, off offset:%3" CACHE "\n\t"    \
+        "s_nop 0\n\t"                                               \
+        "s_mov_b32 m0, %0"                                          \
+        : "=&s"(saved)                                              \
+        : "v"(from), "s"(__builtin_amdgcn_readfirstlane(place - OFFSET)), "n"(OFFSET) \
+        : "memory")
+template <int OFFSET, bool PAST>
 __device__ __forceinline__ void to_lds(const char* from, uint32_t place) {
     uint32_t saved;
-    asm volatile(
-        "s_mov_b32 %0, m0\n\t"
-        "s_mov_b32 m0, %2\n\t"
-        "s_nop 0\n\t"
-        "global_load_lds_dwordx4 %1, off offset:%3\n\t"
-        "s_nop 0\n\t"
-        "s_mov_b32 m0, %0"
-        : "=&s"(saved)
-        : "v"(from), "s"(__builtin_amdgcn_readfirstlane(place - OFFSET)), "n"(OFFSET)
-        : "memory");
+    if constexpr (PAST)
+        QW_TO_LDS(" nt");
+    else
+        QW_TO_LDS("");
 }
-template <int N, int STEP, int J = 0>
+#undef QW_TO_LDS
+template <int N, int STEP, bool PAST, int J = 0>
 __device__ __forceinline__ void run_to_lds(const char* from, uint32_t place) {
     if constexpr (J < N) {
-        to_lds<J * STEP>(from, place + J * 1024);
-        run_to_lds<N, STEP, J + 1>(from, place);
+        to_lds<J * STEP, PAST>(from, place + J * 1024);
+        run_to_lds<N, STEP, PAST, J + 1>(from, place);
     }
 }
 template <int N>
@@ -222,28 +228,28 @@ __device__ __forceinline__ int64_t block_of(const PagedView& c, const Place& p, 
     return ((page * c.hkv + h) << (c.lg - 3)) + ((g & 2 ? p.slot1 : p.slot0) >> 3) + (g & 1);
 }
 
-template <int BITS, int D, bool INT8>
+template <int BITS, int D, bool INT8, bool PAST>
 __device__ __forceinline__ void params_to_lds(const PagedView& c, const f16* par, const Place& p, int h, int lane, uint32_t place) {
     constexpr int LPB = Shape<BITS, D, INT8>::PAR / 8;  // lanes of 8 keys' scales and biases
     if constexpr (LPB > 0) {
         if (lane < 4 * LPB)
-            to_lds<0>((const char*)(par + block_of(c, p, h, lane / LPB) * (8 * LPB)) + lane % LPB * 16, place);
+            to_lds<0, PAST>((const char*)(par + block_of(c, p, h, lane / LPB) * (8 * LPB)) + lane % LPB * 16, place);
     }
 }
-template <int BITS, int D, bool INT8>
+template <int BITS, int D, bool INT8, bool PAST>
 __device__ __forceinline__ void request_k(const PagedView& c, const Place& p, int h, int lane, uint32_t slot) {
     using S = Shape<BITS, D, INT8>;
     constexpr int ROW = D * BITS / 8;
     const char* row = k_row(c, p, h, lane, ROW);
-    run_to_lds<S::NK, 64>(row, slot);
-    run_to_lds<S::NK, 64>(row + 4 * ROW, slot + S::NK * 1024);
-    params_to_lds<BITS, D, INT8>(c, c.k_par, p, h, lane, slot + S::P0);
+    run_to_lds<S::NK, 64, PAST>(row, slot);
+    run_to_lds<S::NK, 64, PAST>(row + 4 * ROW, slot + S::NK * 1024);
+    params_to_lds<BITS, D, INT8, PAST>(c, c.k_par, p, h, lane, slot + S::P0);
 }
-template <int BITS, int D, bool INT8>
+template <int BITS, int D, bool INT8, bool PAST>
 __device__ __forceinline__ void request_v(const PagedView& c, const Place& p, int h, int lane, uint32_t slot) {
     using S = Shape<BITS, D, INT8>;
-    run_to_lds<S::NV, 256>(c.v + block_of(c, p, h, lane >> 4) * (D * BITS) + 16 * (lane & 15), slot + S::V0);
-    params_to_lds<BITS, D, INT8>(c, c.v_par, p, h, lane, slot + S::P0 + 512);
+    run_to_lds<S::NV, 256, PAST>(c.v + block_of(c, p, h, lane >> 4) * (D * BITS) + 16 * (lane & 15), slot + S::V0);
+    params_to_lds<BITS, D, INT8, PAST>(c, c.v_par, p, h, lane, slot + S::P0 + 512);
 }
 
 // fp16 keys stay in registers.
@@ -252,19 +258,23 @@ struct Chunk {
     u32x4 k[2][D / 32];
     u32x4 v[D / 16];
 };
-template <int D>
+template <bool PAST>
+__device__ __forceinline__ u32x4 load_piece(const char* at) {
+    return PAST ? __builtin_nontemporal_load((const u32x4*)at) : *(const u32x4*)at;
+}
+template <bool PAST, int D>
 __device__ __forceinline__ void load_k(Chunk<D>& x, const PagedView& c, const Place& p, int h, int lane) {
     const char* row = k_row(c, p, h, lane, 2 * D);
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int j = 0; j < D / 32; j++) x.k[t][j] = *(const u32x4*)(row + t * 8 * D + 64 * j);
+        for (int j = 0; j < D / 32; j++) x.k[t][j] = load_piece<PAST>(row + t * 8 * D + 64 * j);
 }
-template <int D>
+template <bool PAST, int D>
 __device__ __forceinline__ void load_v(Chunk<D>& x, const PagedView& c, const Place& p, int h, int lane) {
     const char* at = c.v + block_of(c, p, h, lane >> 4) * (D * 16) + 16 * (lane & 15);
 #pragma unroll
-    for (int j = 0; j < D / 16; j++) x.v[j] = *(const u32x4*)(at + 256 * j);
+    for (int j = 0; j < D / 16; j++) x.v[j] = load_piece<PAST>(at + 256 * j);
 }
 
 // 8 codes of a K piece, its step e, as halves code * 2^-24.
@@ -324,7 +334,7 @@ __host__ __device__ constexpr int key_floats(int rows) {
     return join > keys ? join : keys;
 }
 
-template <int BITS, int D, bool INT8, int TILES>
+template <int BITS, int D, bool INT8, int TILES, bool PAST>
 __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, TILES>::SIMD)) void paged_attend_kernel(AttendArgs a) {
     using C = Shape<BITS, D, INT8>;
     using F = Form<BITS, D, TILES>;
@@ -394,7 +404,7 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
         };
         auto place_of = [&](uint32_t r) {
             Place p{};
-            if (r >= r1) return p;  // (behind the piece: page 0, which every wave then requests and none uses)
+            if (r >= r1) return p;  // (behind the piece: not requested)
             const int i = (int)((r - r0) & 31) * 2;
             if (i == 0) look(r);
             p.page0 = __builtin_amdgcn_readlane(ahead.page, i);
@@ -428,11 +438,11 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
             if (c < q_rows) *(half8*)(sq + c * QS + d) = qr[i];
         }
         if constexpr (RING) {
-            request_k<BITS, D, INT8>(a.c, cur, h, afresh(lane), slot0);
-            request_v<BITS, D, INT8>(a.c, cur, h, afresh(lane), slot0);
+            request_k<BITS, D, INT8, PAST>(a.c, cur, h, afresh(lane), slot0);
+            request_v<BITS, D, INT8, PAST>(a.c, cur, h, afresh(lane), slot0);
         } else {
-            load_k(x, a.c, cur, h, afresh(lane));
-            load_v(x, a.c, cur, h, afresh(lane));
+            load_k<PAST>(x, a.c, cur, h, afresh(lane));
+            load_v<PAST>(x, a.c, cur, h, afresh(lane));
         }
         __syncthreads();
         float qsum[RT][NG];
@@ -531,9 +541,9 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (RING) {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read: its place takes the next
-                if (r + 1 < r1) request_k<BITS, D, INT8>(a.c, next, h, afresh(lane), slot0);
+                if (r + 1 < r1) request_k<BITS, D, INT8, PAST>(a.c, next, h, afresh(lane), slot0);
             } else {
-                load_k(x, a.c, next, h, afresh(lane));
+                if (r + 1 < r1) load_k<PAST>(x, a.c, next, h, afresh(lane));
             }
             __builtin_amdgcn_sched_barrier(0);
             const bool masked = top >= seen_all;
@@ -670,9 +680,9 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (RING) {
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (r + 1 < r1) request_v<BITS, D, INT8>(a.c, next, h, afresh(lane), slot0);
+                if (r + 1 < r1) request_v<BITS, D, INT8, PAST>(a.c, next, h, afresh(lane), slot0);
             } else {
-                load_v(x, a.c, next, h, afresh(lane));
+                if (r + 1 < r1) load_v<PAST>(x, a.c, next, h, afresh(lane));
             }
             __builtin_amdgcn_sched_barrier(0);
             cur = next;
@@ -850,14 +860,14 @@ size_t attend_lds(int R) {
     const int rows = std::min(R, 16), q_rows = TILES == 1 ? rows : 16 * TILES;
     return (size_t)key_floats<BITS, D, INT8, TILES>(rows) * 4 + TILES * Form<BITS, D, TILES>::WAVES * 16 * 8 + (size_t)q_rows * (D + 8) * 2;
 }
-template <int BITS, int D, bool INT8, int TILES>
+template <int BITS, int D, bool INT8, int TILES, bool PAST>
 int launch_attend(const AttendArgs& a, hipStream_t stream) {
     const size_t lds = attend_lds<BITS, D, INT8, TILES>(a.R);
     static_assert(BITS == 16 || 8 * Shape<BITS, D, INT8>::PAR <= 512, "K's and V's scales and biases of 32 keys have 512 bytes each");
-    const void* f = (const void*)paged_attend_kernel<BITS, D, INT8, TILES>;
+    const void* f = (const void*)paged_attend_kernel<BITS, D, INT8, TILES, PAST>;
     if (int rc = ensure_dynamic_lds(f, lds)) return rc;
     const dim3 grid(a.workers, a.c.hkv, (a.R + 16 * TILES - 1) / (16 * TILES));
-    hipLaunchKernelGGL((paged_attend_kernel<BITS, D, INT8, TILES>), grid, dim3(64 * Form<BITS, D, TILES>::WAVES), lds, stream, a);
+    hipLaunchKernelGGL((paged_attend_kernel<BITS, D, INT8, TILES, PAST>), grid, dim3(64 * Form<BITS, D, TILES>::WAVES), lds, stream, a);
     QW_HIP_CHECK(hipGetLastError());
     return QW_OK;
 }
@@ -949,6 +959,11 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     // 102, 1024 374 / 368; D = 256, 4 bits, 128 32.9 / 49.8, 1024 246 / 255.
     const int few = q.n_seq > 64 ? 8 : c.D == 256 ? 3 : c.bits == 16 ? 5 : 4;
     a.whole = rounds > 0 && most <= few * round;
+    // Keys that may be more than the 256 MB behind the L2 caches, each read once, go past the caches (us, without / with: 64
+    // sequences of up to 16k fp16 keys 491 / 438, 32 sparse ones of 32k fp16 keys, with the selection, 127 / 112, 4 of
+    // 32k Int8 keys with 5 rows 50.1 / 48.6). Fewer may be there from the last call (64 of up to 1024 fp16 keys, the same again and
+    // again, 44.5 / 52.1), and more row tiles than a workgroup's share them (128 rows of 4 sequences, 8k fp16 keys, 182 / 236).
+    const bool past = groups == 1 && most * q.n_seq * c.hkv * (c.D * c.bits / 4 + c.par_halves() / 2) > (256ll << 20);
     const int64_t parts = a.whole ? 0 : (int64_t)a.workers * 2 * c.hkv * a.R;
     void* ws = nullptr;
     const bool cuts = q.n_seq > 64 && rounds > 0 && !a.whole;
@@ -958,7 +973,8 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     a.cut = cuts ? (uint4*)(a.part_ml + parts) : nullptr;
     if (rounds > 0) {
         const int rc = by_shape(c.bits, c.int8(), c.D, tiles, [&](auto b, auto i8, auto d, auto t) {
-            return launch_attend<decltype(b)::value, decltype(d)::value, decltype(i8)::value, decltype(t)::value>(a, stream);
+            constexpr int B = decltype(b)::value, D = decltype(d)::value, T = decltype(t)::value;
+            return past ? launch_attend<B, D, decltype(i8)::value, T, true>(a, stream) : launch_attend<B, D, decltype(i8)::value, T, false>(a, stream);
         });
         if (rc) return rc;
     }

@@ -644,3 +644,14 @@ def test_many_rows(mode, D, L):
     s = Sequences(r, mode, 1, D, 32, lengths)
     q = queries(r, 3, 3, L, D)
     s.check(s.cache.attention(q, ints(s.table), ints(lengths), 0.07), q, 0.07)
+
+
+@pytest.mark.parametrize("mode,D", [("affine4", 256), ("int8", 128), ("fp16", 256), ("affine8", 128)])
+@pytest.mark.parametrize("L", [1, 5])
+def test_tables_of_more_than_the_caches_hold(mode, D, L):
+    """Tables whose width allows for more keys than the caches hold, of sequences that have few."""
+    r = rng(D + L)
+    lengths = [900, 0, 33, 260]
+    s = Sequences(r, mode, 8, D, 16, lengths, width=20000)
+    q = queries(r, 4, 32, L, D)
+    s.check(s.cache.attention(q, ints(s.table), ints(lengths), 0.07), q, 0.07)
