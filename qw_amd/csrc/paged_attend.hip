@@ -2,8 +2,7 @@
 //
 // out = softmax(scale q . k) v for each row over its sequence's keys, causal among the last n_rows of
 // them, in one pass with the running maximum and sum. Bound by reading the codes once from HBM: 64 sequences of
-// up to 16k fp16 keys (8 KV heads, D = 128) 489 us, 5.9 TB/s, what reading alone reaches; one of 128k keys 5.0 to 5.8 TB/s
-// in every mode. Short ones are bound by their start (lengths, table, queries and keys, one behind the other, 5 us), the
+// up to 16k fp16 keys (8 KV heads, D = 128) 435 us, 6.6 TB/s; one of 128k keys 5.0 to 5.8 TB/s in every mode. Short ones are bound by their start (lengths, table, queries and keys, one behind the other, 5 us), the
 // last joining and the second launch (4 us).
 //
 // Work is dealt in rounds of 128 or 256 keys to the workers of a head (a grid sized for the card, lengths read on the
@@ -21,7 +20,7 @@
 //   sum_k P (scale code + bias) = sum_k P' code - c0 sum_k P' + sum_k P (bias + c0 scale):
 // one more matrix product each for the last two. So P's and P's rounding meet what is left of a code beside the middle, not
 // the code and the bias that nearly cancel each other (17 sequences of 4 bits: an error of 0.00027 of the result for 0.00069,
-// of which 0.0002 is the result's own rounding, and 32.6 us for 31.7).
+// of which 0.0002 is the result's own rounding, for 0.9 us of 32).
 // The next round's K is requested behind this one's scores, its V behind this one's P V, into the place that they
 // leave: a wave always waits for loads that are half a round old, and never for another wave.
 #include <algorithm>
@@ -963,7 +962,7 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     // sequences of up to 16k fp16 keys 491 / 438, 32 sparse ones of 32k fp16 keys, with the selection, 127 / 112, 4 of
     // 32k Int8 keys with 5 rows 50.1 / 48.6). Fewer may be there from the last call (64 of up to 1024 fp16 keys, the same again and
     // again, 44.5 / 52.1), and more row tiles than a workgroup's share them (128 rows of 4 sequences, 8k fp16 keys, 182 / 236).
-    const bool past = groups == 1 && most * q.n_seq * c.hkv * (c.D * c.bits / 4 + c.par_halves() / 2) > (256ll << 20);
+    const bool past = groups == 1 && (double)most * q.n_seq * c.hkv * (c.D * c.bits / 4 + c.par_halves() / 2) > 256.0 * (1 << 20);
     const int64_t parts = a.whole ? 0 : (int64_t)a.workers * 2 * c.hkv * a.R;
     void* ws = nullptr;
     const bool cuts = q.n_seq > 64 && rounds > 0 && !a.whole;

@@ -7,7 +7,10 @@
 // step and base of one of the 16 rows (8 tokens' K and V), with its divisions, and hand them round; codes come
 // by a product and one correction of its remainder, and are packed as bytes as they are converted (two
 // keys' 4-bit codes as one number), so that V's words of 8 keys need no transposition. Where a call
-// covers part of such a word the rest is kept; tokens that a call does not have cost nothing.
+// covers part of such a word the rest is kept; tokens that a call does not have cost nothing. Bound by HBM where there are many
+// (65536 int8 tokens, 8 heads of D = 128, pages of 32: 83 us, 5.1 TB/s, and read back 71, 5.7), by the chain of loads and some
+// 1,100 instructions a wave where they fill the card once (6001 8-bit tokens, 4 heads of D = 256: 13.8 us, 2.8 TB/s). A token's
+// heads lie on one XCD, 8 pages side by side.
 #include <algorithm>
 
 #include "paged.hpp"
@@ -258,7 +261,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
     constexpr int LPR = D / 4, SUB = 64 / LPR, NG = INT8 ? 1 : D / kGroup;
     __shared__ half4v sm_lo[kStoreWaves][LPR], sm_hi[kStoreWaves][LPR];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    // (heads side by side: a token's row of all heads is read at about the same time)
+    // (heads side by side on an XCD: a token's row of all heads is read at about the same time)
     const int nw = blockDim.x >> 6, h = (int)((blockIdx.x >> 3) % c.hkv), ps = 1 << c.lg;
     const PagedUnit u = unit_of(a.s, (blockIdx.x >> 3) / c.hkv * 8 + (blockIdx.x & 7), ps, [&](int b) {
         const PagedSpan p = span_of(a.s, b, c.lg);
