@@ -417,7 +417,7 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
         };
 
         Chunk<D> x;  // (not RING)
-        const char* slot = (const char*)lds + wave * C::SLOT;
+        char* slot = (char*)lds + wave * C::SLOT;
         const uint32_t slot0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)slot;
         // the query rows: requested, with the first pages, before the keys, behind which they would wait
         constexpr int QN = TILES * 16 * (D / 8) / NT;
@@ -547,22 +547,33 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
             __builtin_amdgcn_sched_barrier(0);
             const bool masked = top >= seen_all;
             const int pos = (g & 2 ? cur.pos1 : cur.pos0) + 8 * (g & 1);
-            u32x4 km;  // the keys before the sequence's end: what stands behind it takes no part, whatever it is
-            if (masked) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) km[j] = (pos + 2 * j < len ? 0xFFFFu : 0u) | (pos + 2 * j + 1 < len ? 0xFFFF0000u : 0u);
-            }
             if constexpr (RING) {
                 if (r + 1 < r1)
                     wait_loads<C::K_LOADS>();
                 else
                     wait_loads<0>();
             }
+            if (masked) {  // what stands behind the sequence's end takes no part, whatever it is: zeros in place of V or its scales
+                constexpr int LPB = BITS == 16 ? 16 : C::PAR / 8;  // lanes of 8 keys
+                const int ln = afresh(lane), blk = ln / LPB, at = (blk & 2 ? cur.pos1 : cur.pos0) + 8 * (blk & 1);
+                u32x4 km;
+#pragma unroll
+                for (int j = 0; j < 4; j++) km[j] = (at + 2 * j < len ? 0xFFFFu : 0u) | (at + 2 * j + 1 < len ? 0xFFFF0000u : 0u);
+                if constexpr (BITS != 16) {
+                    u32x4* v = (u32x4*)(slot + C::P0 + 512) + ln;
+                    if (ln < 4 * LPB) *v &= km;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < C::NV; j++) {
+                        if constexpr (RING)
+                            *((u32x4*)(slot + C::V0 + j * 1024) + ln) &= km;
+                        else
+                            x.v[j] &= km;
+                    }
+                }
+            }
             const f16* vpar = kpar + 256;
-            auto v_scales = [&](const f16* par, int m) {  // of 8 keys in group m
-                const half8 x = *(const half8*)(par + 8 * m);
-                return masked ? as_h8(__builtin_bit_cast(u32x4, x) & km) : x;
-            };
+            auto v_scales = [&](const f16* par, int m) { return *(const half8*)(par + 8 * m); };  // of 8 keys in group m
             if constexpr (BITS != 16) {
                 uint32_t high = 0;
 #pragma unroll
@@ -636,7 +647,6 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
                         v = *(const u32x4*)(slot + C::V0 + j * 1024 + 16 * lane);
                     else
                         v = x.v[j];
-                    if (masked) v &= km;
 #pragma unroll
                     for (int t = 0; t < RT; t++) o[t][j] = mfma(as_h8(v), ph[t], o[t][j]);
                 }
