@@ -452,16 +452,14 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
             if constexpr (BITS != 16) {
 #pragma unroll
                 for (int m = 0; m < NG; m++) {
-                    float y = 0.0f;
+                    // ones times q: a row's sum in every lane that holds it
+                    float4v y = {0, 0, 0, 0};
 #pragma unroll
                     for (int j = 0; j < STEPS / NG; j++) {
                         const half8 q = *(const half8*)(sq + (16 * t + q_col) * QS + 32 * (m * (STEPS / NG) + j) + 8 * g);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) y += (float)q[e];
+                        y = mfma(half8{} + (f16)1.0f, q, y);
                     }
-                    y += lane_xor<16>(y, lane);
-                    y += lane_xor<32>(y, lane);
-                    qsum[t][m] = y * (INT8 ? -128.0f * 0x1p-24f : 0x1p-24f);  // in the codes' units
+                    qsum[t][m] = y[0] * (INT8 ? -128.0f * 0x1p-24f : 0x1p-24f);  // in the codes' units
                 }
             }
         }
@@ -973,13 +971,15 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     // 32k Int8 keys with 5 rows 50.1 / 48.6). Fewer may be there from the last call (64 of up to 1024 fp16 keys, the same again and
     // again, 44.5 / 52.1), and more row tiles than a workgroup's share them (128 rows of 4 sequences, 8k fp16 keys, 182 / 236).
     const bool past = groups == 1 && (double)most * q.n_seq * c.hkv * (c.D * c.bits / 4 + c.par_halves() / 2) > 256.0 * (1 << 20);
-    const int64_t parts = a.whole ? 0 : (int64_t)a.workers * 2 * c.hkv * a.R;
-    void* ws = nullptr;
+    const int64_t parts = (int64_t)a.workers * 2 * c.hkv * a.R;
     const bool cuts = q.n_seq > 64 && rounds > 0 && !a.whole;
-    if (int rc = workspace(kWsPaged, c.device, stream, (size_t)(parts * (c.D * 4 + 8) + (cuts ? a.workers * 16 : 0)), &ws)) return rc;
-    a.part_o = (float*)ws;
-    a.part_ml = (float2*)(a.part_o + parts * c.D);
-    a.cut = cuts ? (uint4*)(a.part_ml + parts) : nullptr;
+    if (!a.whole) {
+        void* ws = nullptr;
+        if (int rc = workspace(kWsPaged, c.device, stream, (size_t)(parts * (c.D * 4 + 8) + (cuts ? a.workers * 16 : 0)), &ws)) return rc;
+        a.part_o = (float*)ws;
+        a.part_ml = (float2*)(a.part_o + parts * c.D);
+        a.cut = cuts ? (uint4*)(a.part_ml + parts) : nullptr;
+    }
     if (rounds > 0) {
         const int rc = by_shape(c.bits, c.int8(), c.D, tiles, [&](auto b, auto i8, auto d, auto t) {
             constexpr int B = decltype(b)::value, D = decltype(d)::value, T = decltype(t)::value;

@@ -655,3 +655,22 @@ def test_tables_of_more_than_the_caches_hold(mode, D, L):
     s = Sequences(r, mode, 8, D, 16, lengths, width=20000)
     q = queries(r, 4, 32, L, D)
     s.check(s.cache.attention(q, ints(s.table), ints(lengths), 0.07), q, 0.07)
+
+
+def test_whole_calls_need_no_workspace():
+    """Short tables: a first call inside a capture, replayed as the sequences grow."""
+    r = rng(74)
+    s = Sequences(r, "affine8", 2, 128, 16, [100, 0, 77])
+    q, t, n = queries(r, 3, 8, 1, 128), ints(s.table), ints([100, 0, 77])
+    torch.cuda.synchronize()
+    stream = side_stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        out = s.cache.attention(q, t, n, 0.1)
+    for lengths in ([100, 0, 77], [3, 0, 0], [64, 0, 76]):
+        n.copy_(ints(lengths))
+        g.replay()
+        torch.cuda.synchronize()
+        s.check(out, q, 0.1, lengths=lengths)
+        assert torch.equal(out, s.cache.attention(q, t, n, 0.1))
