@@ -41,9 +41,12 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
         for (int t = threadIdx.x / 64; t < nt; t += 4) {
             double x = (double)pos[t] * f;
             x -= rint(x);
+            // what the angle's rounding to fp32 leaves turns them a little further: of 6.1M rotated values 915 differ from
+            // the 64-bit result's rounding (without 1848; cosines in 64 bits 693, but 4 % slower)
+            const float y = 2.0f * (float)x, rest = (float)(2.0 * x - (double)y) * 3.14159265f;
             float s, c;
-            sincospif(2.0f * (float)x, &s, &c);
-            sm[t * a.half + p] = float2{c, s};
+            sincospif(y, &s, &c);
+            sm[t * a.half + p] = float2{__builtin_fmaf(-s, rest, c), __builtin_fmaf(c, rest, s)};
         }
     }
     __syncthreads();
