@@ -15,6 +15,7 @@
 
 #include "paged.hpp"
 #include "quant.hpp"
+#include "rope.hpp"
 
 namespace qw {
 
@@ -256,8 +257,67 @@ struct StoreArgs {
     PagedSeqs s;
 };
 
-template <int BITS, bool INT8, int D>
-__global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedView c, StoreArgs a) {
+// Rotates 4 dims d .. of heads.
+struct Turner {
+    const RopeTurns& r;
+    double rate[4];
+    float2 cs[4];
+    int d, p, other;  // its first pair, the dims of the pairs' other halves (itself: adjacent ones)
+    bool turns, first;
+
+    __device__ __forceinline__ Turner(const RopeTurns& r_, int d_) : r(r_), d(d_), other(d_) {
+        turns = d < 2 * r.half, first = d < r.half;
+        if (!r.traditional && turns) other = first ? d + r.half : d - r.half;
+        p = r.traditional ? d >> 1 : min(d, other);
+        if (!turns) return;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < (r.traditional ? 2 : 4)) rate[e] = turn_rate(r, p + e);
+    }
+    __device__ __forceinline__ void at(int64_t token) {
+        if (!turns) return;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < (r.traditional ? 2 : 4)) cs[e] = turn_of(rate[e], r.positions[r.axes[p + e] * r.stride + token]);
+    }
+    __device__ __forceinline__ half4v of(half4v x, half4v z) const {  // z: the other halves (not of adjacent pairs)
+        if (!turns) return x;
+        if (r.traditional) z = half4v{x[1], x[0], x[3], x[2]};
+        half4v y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const bool one = r.traditional ? e % 2 == 0 : first;
+            const float2 t = r.traditional ? cs[e / 2] : cs[e];
+            float r1, r2;
+            rope_rot((float)(one ? x[e] : z[e]), (float)(one ? z[e] : x[e]), t.x, t.y, r1, r2);
+            y[e] = (f16)(one ? r1 : r2);
+        }
+        return y;
+    }
+};
+struct TurnArgs {
+    RopeTurns r;
+    f16* q_out;
+    int hq, groups;  // workgroups that store; those behind them rotate q, kTurnHeads heads of a token each
+};
+constexpr int kTurnHeads = 8;
+
+// TURN: k rotates on its way, q in workgroups of its own.
+template <int BITS, bool INT8, int D, bool TURN>
+__global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedView c, StoreArgs a, TurnArgs turn) {
+    if constexpr (TURN) {
+        if ((int)blockIdx.x >= turn.groups) {
+            const int per = (turn.hq + kTurnHeads - 1) / kTurnHeads, i = (int)blockIdx.x - turn.groups;
+            const int64_t token = i / per;
+            const int h0 = i % per * kTurnHeads;
+            Turner t(turn.r, threadIdx.x % (D / 4) * 4);
+            t.at(token);
+            const f16* q = a.k - (int64_t)turn.hq * D + token * a.k_token;
+            for (int h = h0 + threadIdx.x / (D / 4); h < min(h0 + kTurnHeads, turn.hq); h += blockDim.x / (D / 4))
+                *(half4v*)(turn.q_out + (token * turn.hq + h) * D + t.d) = t.of(*(const half4v*)(q + h * D + t.d), *(const half4v*)(q + h * D + t.other));
+            return;
+        }
+    }
     constexpr int LPR = D / 4, SUB = 64 / LPR, NG = INT8 ? 1 : D / kGroup;
     __shared__ half4v sm_lo[kStoreWaves][LPR], sm_hi[kStoreWaves][LPR];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -299,6 +359,21 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
                 xk[k] = half4v{}, xv[k] = half4v{};
                 if (in(k)) xk[k] = *(const half4v*)(kt + k * a.k_token), xv[k] = *(const half4v*)(vt + k * a.v_token);
             }
+        }
+        if constexpr (TURN) {
+            Turner t(turn.r, 4 * li);
+            half4v z[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                z[k] = half4v{};
+                if (in(k)) z[k] = *(const half4v*)(kt + k * a.k_token + (t.other - t.d));
+            }
+            each8([&](auto k) {
+                constexpr int K = decltype(k)::value;
+                if (!__any(in(K))) return;
+                t.at(in(K) ? t0 + K : p.first);
+                xk[K] = t.of(xk[K], z[K]);
+            });
         }
         if (page < 0 || page >= c.n_pages) return;  // (the whole workgroup's; the tokens were requested beside the table's entry)
         const bool live = blk <= last;
@@ -618,6 +693,14 @@ int64_t most_units(const PagedSeqs& s, int size) {
     return std::min<int64_t>(s.n_tokens, (int64_t)s.n_tokens / size + 2 * (int64_t)s.n_seq);
 }
 
+int store_waves(const PagedCache& c, const PagedSeqs& s) {
+    // waves for the blocks of 8 slots that an average sequence touches in a page, two a wave at D = 128. So many / 8 / 2 at
+    // most, us: a token each of 33 sequences, pages of 16, D = 128 4.7 / 7.7 / 4.7; 2048 each of 8, pages of 256, D = 128 19.7 /
+    // 19.5 / 32.0; 13107 each of 5, pages of 32, D = 128 65 / 163 / 66
+    const int blocks = std::min(c.page_size / 8, s.n_tokens / s.n_seq / 8 + 1);
+    return std::max(1, std::min(kStoreWaves, blocks * c.D / 256));
+}
+
 }  // namespace
 
 int paged_update(PagedCache& c, const void* k, const void* v, int64_t k_token, int64_t k_head, int64_t v_token,
@@ -631,17 +714,32 @@ int paged_update(PagedCache& c, const void* k, const void* v, int64_t k_token, i
     DeviceGuard dg(c.device);
     QW_REQUIRE(dg.ok, QW_ERR_HIP, "paged update: hipSetDevice failed");
     const StoreArgs a{(const f16*)k, (const f16*)v, k_token, k_head, v_token, v_head, s};
-    // waves for the blocks of 8 slots that an average sequence touches in a page, two a wave at D = 128. So many / 8 / 2 at
-    // most, us: a token each of 33 sequences, pages of 16, D = 128 4.7 / 7.7 / 4.7; 2048 each of 8, pages of 256, D = 128 19.7 /
-    // 19.5 / 32.0; 13107 each of 5, pages of 32, D = 128 65 / 163 / 66
-    const int blocks = std::min(c.page_size / 8, s.n_tokens / s.n_seq / 8 + 1);
-    const int waves = std::max(1, std::min(kStoreWaves, blocks * c.D / 256));
+    const int waves = store_waves(c, s);
     const int64_t groups = (most_units(s, c.page_size) + 7) / 8 * 8 * c.hkv;
     QW_REQUIRE(groups * 64 * waves <= UINT32_MAX, QW_ERR_UNSUPPORTED, "paged update: too many tokens for one call");
     const dim3 grid((unsigned)groups);
     by_mode(c, [&](auto bits, auto i8, auto d) {
-        hipLaunchKernelGGL((paged_update_kernel<decltype(bits)::value, decltype(i8)::value, decltype(d)::value>), grid,
-                           dim3(64 * waves), 0, stream, c.view, a);
+        hipLaunchKernelGGL((paged_update_kernel<decltype(bits)::value, decltype(i8)::value, decltype(d)::value, false>), grid,
+                           dim3(64 * waves), 0, stream, c.view, a, TurnArgs{});
+    });
+    QW_HIP_CHECK(hipGetLastError());
+    return QW_OK;
+}
+
+int paged_turn_update(PagedCache& c, const RopeTurns& r, const void* qkv, int hq, void* q_out, const PagedSeqs& s,
+                      hipStream_t stream) {
+    QW_REQUIRE(qkv && q_out && r.positions, QW_ERR_INVALID_ARGUMENT, "paged rope update: null qkv/positions/q_out");
+    const int64_t row = (int64_t)(hq + 2 * c.hkv) * c.D;
+    const f16* k = (const f16*)qkv + (int64_t)hq * c.D;
+    const StoreArgs a{k, k + (int64_t)c.hkv * c.D, row, c.D, row, c.D, s};
+    const int64_t groups = (most_units(s, c.page_size) + 7) / 8 * 8 * c.hkv;
+    const int64_t all = groups + (int64_t)s.n_tokens * ((hq + kTurnHeads - 1) / kTurnHeads);
+    const int waves = store_waves(c, s);
+    QW_REQUIRE(all * 64 * waves <= UINT32_MAX, QW_ERR_UNSUPPORTED, "paged rope update: too many tokens for one call");
+    const TurnArgs turn{r, (f16*)q_out, hq, (int)groups};
+    by_mode(c, [&](auto bits, auto i8, auto d) {
+        hipLaunchKernelGGL((paged_update_kernel<decltype(bits)::value, decltype(i8)::value, decltype(d)::value, true>),
+                           dim3((unsigned)all), dim3(64 * waves), 0, stream, c.view, a, turn);
     });
     QW_HIP_CHECK(hipGetLastError());
     return QW_OK;

@@ -16,18 +16,14 @@ namespace qw {
 
 namespace {
 
-constexpr int kMaxHalf = 256;   // pairs
 constexpr int kAngles = 2048;   // (cos, sin) of a workgroup
 
 struct RopeAxesArgs {
     const f16* qkv;
     f16* q_out;
     f16* k_out;
-    const int32_t* positions;
-    int64_t stride;  // of an axis
-    int n, hq, hkv, D, half, traditional, tokens;  // tokens of a workgroup
-    double log2_base, scale;  // scale over 2 pi
-    uint8_t axes[kMaxHalf];
+    RopeTurns r;
+    int n, hq, hkv, D, tokens;  // tokens of a workgroup
 };
 
 // VEC: 8 dims a thread (head_dim and half multiples of 8), else one.
@@ -35,23 +31,15 @@ template <bool VEC>
 __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
     __shared__ float2 sm[kAngles];
     const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.n - t0);
-    for (int p = threadIdx.x % 64; p < a.half; p += 64) {
-        const double f = exp2(-((double)p / a.half) * a.log2_base) * a.scale;
-        const int32_t* pos = a.positions + a.axes[p] * a.stride + t0;
-        for (int t = threadIdx.x / 64; t < nt; t += 4) {
-            double x = (double)pos[t] * f;
-            x -= rint(x);
-            // what the angle's rounding to fp32 leaves turns them a little further: of 6.1M rotated values 915 differ from
-            // the 64-bit result's rounding (without 1848; cosines in 64 bits 693, but 4 % slower)
-            const float y = 2.0f * (float)x, rest = (float)(2.0 * x - (double)y) * 3.14159265f;
-            float s, c;
-            sincospif(y, &s, &c);
-            sm[t * a.half + p] = float2{__builtin_fmaf(-s, rest, c), __builtin_fmaf(c, rest, s)};
-        }
+    const int half = a.r.half, traditional = a.r.traditional;
+    for (int p = threadIdx.x % 64; p < half; p += 64) {
+        const double f = turn_rate(a.r, p);
+        const int32_t* pos = a.r.positions + a.r.axes[p] * a.r.stride + t0;
+        for (int t = threadIdx.x / 64; t < nt; t += 4) sm[t * half + p] = turn_of(f, pos[t]);
     }
     __syncthreads();
     constexpr int N = VEC ? 8 : 1;
-    const int per = a.D / N, heads = a.hq + a.hkv, R = 2 * a.half;
+    const int per = a.D / N, heads = a.hq + a.hkv, R = 2 * half;
     const int total = nt * heads * per;
     for (int i = threadIdx.x; i < total; i += 256) {
         const int d = i % per * N, row = i / per, t = row / heads, h = row - t * heads;
@@ -67,21 +55,21 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
 #pragma unroll
             for (int e = 0; e < N; e++) y[e] = x[e];
         } else {
-            const bool first = a.traditional ? true : d < a.half;
+            const bool first = traditional ? true : d < half;
             alignas(16) f16 z[N];  // the other dims of its pairs
-            if (a.traditional) {
+            if (traditional) {
 #pragma unroll
                 for (int e = 0; e < N; e++) z[e] = VEC ? x[e ^ (N > 1)] : in[d ^ 1];
             } else if constexpr (VEC) {
-                *(half8*)z = *(const half8*)(in + (first ? d + a.half : d - a.half));
+                *(half8*)z = *(const half8*)(in + (first ? d + half : d - half));
             } else {
-                z[0] = in[first ? d + a.half : d - a.half];
+                z[0] = in[first ? d + half : d - half];
             }
 #pragma unroll
             for (int e = 0; e < N; e++) {
-                const bool one = a.traditional ? ((d + e) & 1) == 0 : first;
-                const int p = a.traditional ? (d + e) >> 1 : first ? d + e : d + e - a.half;
-                const float2 cs = sm[t * a.half + p];
+                const bool one = traditional ? ((d + e) & 1) == 0 : first;
+                const int p = traditional ? (d + e) >> 1 : first ? d + e : d + e - half;
+                const float2 cs = sm[t * half + p];
                 float r1, r2;
                 rope_rot((float)(one ? x[e] : z[e]), (float)(one ? z[e] : x[e]), cs.x, cs.y, r1, r2);
                 y[e] = (f16)(one ? r1 : r2);
@@ -97,8 +85,7 @@ __global__ __launch_bounds__(256) void rope_axes_kernel(RopeAxesArgs a) {
 
 }  // namespace
 
-int rope_axes(const RopeAxes& r, const void* qkv, int n_tokens, int hq, int hkv, int D, void* q_out, void* k_out,
-              hipStream_t stream) {
+int rope_turns(const RopeAxes& r, int n_tokens, int hq, int hkv, int D, RopeTurns& out) {
     QW_REQUIRE(n_tokens >= 0 && n_tokens <= (1 << 28) && hq > 0 && hkv > 0 && D > 0 && (int64_t)hq + 2 * (int64_t)hkv <= (1 << 24) / D,
                QW_ERR_INVALID_ARGUMENT, "rope axes: 0 .. 2^28 tokens, n_q_heads, n_kv_heads and head_dim > 0, a row of at most 2^24 values expected");
     QW_REQUIRE(r.rope_dims > 0 && r.rope_dims % 2 == 0 && r.rope_dims <= D && r.rope_dims <= 2 * kMaxHalf && D % 2 == 0,
@@ -107,30 +94,36 @@ int rope_axes(const RopeAxes& r, const void* qkv, int n_tokens, int hq, int hkv,
                "rope axes: a finite base > 0 and a finite scale expected");
     QW_REQUIRE(r.n_axes > 0 && r.axes && r.stride >= n_tokens, QW_ERR_INVALID_ARGUMENT,
                "rope axes: n_axes > 0, an axis for each pair, and a positions stride of n_tokens at least expected");
-    RopeAxesArgs a{};
     for (int p = 0; p < r.rope_dims / 2; p++) {
         QW_REQUIRE(r.axes[p] < r.n_axes, QW_ERR_INVALID_ARGUMENT, "rope axes: a pair's axis is not below n_axes");
-        a.axes[p] = r.axes[p];
+        out.axes[p] = r.axes[p];
     }
+    out.positions = r.positions;
+    out.stride = r.stride;
+    out.half = r.rope_dims / 2;
+    out.traditional = r.traditional;
+    out.log2_base = std::log2((double)r.base);
+    out.scale = (double)r.scale / 6.283185307179586476925;
+    return QW_OK;
+}
+
+int rope_axes(const RopeAxes& r, const void* qkv, int n_tokens, int hq, int hkv, int D, void* q_out, void* k_out,
+              hipStream_t stream) {
+    RopeAxesArgs a{};
+    if (int rc = rope_turns(r, n_tokens, hq, hkv, D, a.r)) return rc;
     if (n_tokens == 0) return QW_OK;
     QW_REQUIRE(qkv && q_out && k_out && r.positions, QW_ERR_INVALID_ARGUMENT, "rope axes: null qkv/positions/output");
     a.qkv = (const f16*)qkv;
     a.q_out = (f16*)q_out;
     a.k_out = (f16*)k_out;
-    a.positions = r.positions;
-    a.stride = r.stride;
     a.n = n_tokens, a.hq = hq, a.hkv = hkv, a.D = D;
-    a.half = r.rope_dims / 2;
-    a.traditional = r.traditional;
-    a.log2_base = std::log2((double)r.base);
-    a.scale = (double)r.scale / 6.283185307179586476925;
     // a token a workgroup while there are few, else as many as its angles' place holds, up to 8. One / 8, 32 + 8 heads of
     // D = 128, us: 64 tokens 5.3 / 19.5, 1500 10.5 / 22.2, 4099 19.2 / 26.9, 32768 154 / 145
-    a.tokens = std::max(1, std::min({8, n_tokens / 4096, kAngles / a.half}));
+    a.tokens = std::max(1, std::min({8, n_tokens / 4096, kAngles / a.r.half}));
     const int64_t groups = ((int64_t)n_tokens + a.tokens - 1) / a.tokens;
     QW_REQUIRE(groups * 256 <= UINT32_MAX, QW_ERR_UNSUPPORTED, "rope axes: too many tokens for one call");
     const dim3 grid((unsigned)groups);
-    const bool vec = D % 8 == 0 && a.half % 8 == 0 && ((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_out) % 16 == 0;
+    const bool vec = D % 8 == 0 && a.r.half % 8 == 0 && ((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_out) % 16 == 0;
     if (vec)
         hipLaunchKernelGGL(rope_axes_kernel<true>, grid, dim3(256), 0, stream, a);
     else
@@ -147,6 +140,14 @@ int paged_rope_update(PagedCache& c, const RopeAxes& r, const void* qkv, int hq,
     DeviceGuard dg(c.device);
     QW_REQUIRE(dg.ok, QW_ERR_HIP, "paged rope update: hipSetDevice failed");
     if (s.n_tokens == 0) return rope_axes(r, qkv, 0, hq, c.hkv, c.D, q_out, nullptr, stream);
+    // One launch for a step of few sequences: each workgroup forms its tokens' angles anew, one token behind the other. Two launches /
+    // one, 24 heads over 4, D = 256, replayed, us: 1 token 10.0 / 8.5, 64 of 64 sequences 10.5 / 10.8 (called one by one and
+    // read back 21.4 / 18.4), 256 of 256 11.6 / 20.5, 256 of 8 12.9 / 35.1.
+    if (s.n_tokens <= std::min(64, s.n_seq) && r.rope_dims % 8 == 0 && (uintptr_t)q_out % 8 == 0) {
+        RopeTurns t;
+        if (int rc = rope_turns(r, s.n_tokens, hq, c.hkv, c.D, t)) return rc;
+        return paged_turn_update(c, t, qkv, hq, q_out, s, stream);
+    }
     // the rotated keys pass through a workspace on their way into the pages
     void* k = nullptr;
     if (int rc = workspace(kWsPagedKeys, c.device, stream, (size_t)s.n_tokens * c.hkv * c.D * sizeof(f16), &k)) return rc;

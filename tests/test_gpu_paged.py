@@ -82,10 +82,10 @@ def rows(r, n, hkv, D, sigma=1.0):
     return (sigma * r.standard_normal((n, hkv, D))).astype(np.float16)
 
 
-def side_stream():
+def side_stream(i=0):
     """A stream of torch's, which hands its 32 out in turn. A workspace that a graph holds stays its stream's: a whole turn
-    leaves the tests behind this one the streams that they had."""
-    return [torch.cuda.Stream() for _ in range(32)][0]
+    leaves the tests behind this one the streams that they had. The same for the same i."""
+    return sorted((torch.cuda.Stream() for _ in range(32)), key=lambda s: s.cuda_stream)[i]
 
 
 class Sequences:
@@ -520,7 +520,7 @@ def test_first_use_inside_a_capture():
     s = Sequences(r, "affine4", 2, 128, 16, [3000])
     q, t, n = queries(r, 1, 8, 1, 128), ints(s.table), ints([3000])
     want = s.cache.attention(q, t, n, 0.1)
-    stream = side_stream()
+    stream = side_stream(1)
     stream.wait_stream(torch.cuda.current_stream())
     g = torch.cuda.CUDAGraph()
     refused = False

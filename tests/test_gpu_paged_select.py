@@ -283,7 +283,7 @@ def test_two_streams_and_threads():
         t, n = ints(s.table[b:b + 1]), ints([s.lengths[b]])
         args.append((q, t, n, s.cache.select_pages(q, t, n, 9, recent=1), s.cache.attention(q, t, n, 1 / 16)))
     torch.cuda.synchronize()
-    wrong, streams = [], [side_stream(), side_stream()]
+    wrong, streams = [], [side_stream(2), side_stream(3)]
 
     def work(b):
         q, t, n, picked, out = args[b]

@@ -134,3 +134,32 @@ def test_rope_axes_refusals():
         with pytest.raises(qw_amd.QwError):
             qw_amd.rope_axes(*args, **kw)
     assert qw_amd.rope_axes(x[:0], pos[:, :0], (8, 12, 12), **ok)[0].shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("mode,hq,hkv,D,sections,interleaved,traditional", [
+    ("fp16", 24, 4, 256, (16, 24, 24), False, False), ("affine8", 9, 3, 128, (8, 4, 4), True, True), ("int8", 2, 2, 256, (128,), False, False),
+    ("affine4", 20, 2, 128, (3, 2, 2), True, False), ("affine8", 8, 8, 256, (2, 2), False, True), ("int8", 3, 1, 128, (64,), False, True)])
+@pytest.mark.parametrize("counts", [[1] * 9, [3, 0, 0, 9] + [0] * 9, [1, 0, 5, 30], [3000, 1], [1] * 64, [1] * 65])
+def test_rotated_on_their_way(mode, hq, hkv, D, sections, interleaved, traditional, counts):
+    """Few tokens rotate in the launch that stores them, many before it: both as rope_axes and update give them, with tokens
+    that have no page among them."""
+    import qw_amd
+
+    r = rng(sum(counts) + D)
+    n, B, ps = sum(counts), len(counts), 16
+    starts = [int(x) for x in r.integers(0, 40, B)]
+    width = -(-(max(counts) + 40) // ps)
+    table = r.permutation(B * width).reshape(B, width)
+    table[B - 1, starts[B - 1] // ps] = -1
+    table = ints(table)
+    offsets = None if counts == [1] * B else ints(np.concatenate([[0], np.cumsum(counts)]))
+    qkv = dev(r.standard_normal((n, (hq + 2 * hkv) * D)).astype(np.float16))
+    pos = ints(r.integers(0, 100000, (len(sections), n)))
+    a, b = (qw_amd.PagedKVCache(mode, hkv, D, B * width, page_size=ps) for _ in range(2))
+    args = dict(interleaved=interleaved, traditional=traditional)
+    q = a.rope_update(qkv, pos, sections, hq, 1e6, table, ints(starts), offsets=offsets, **args)
+    q1, k1 = qw_amd.rope_axes(qkv, pos, sections, hq, hkv, D, 1e6, **args)
+    b.update(k1, qkv.view(n, -1, D)[:, hq + hkv:], table, ints(starts), offsets)
+    assert torch.equal(q, q1)
+    for x, y in zip(a.gather(table, ints(starts), n, offsets), b.gather(table, ints(starts), n, offsets)):
+        assert torch.equal(x, y)
