@@ -259,37 +259,39 @@ struct StoreArgs {
 
 // Rotates 4 dims d .. of heads.
 struct Turner {
-    const RopeTurns& r;
     double rate[4];
-    float2 cs[4];
+    float cos[4], sin[4];
     int d, p, other;  // its first pair, the dims of the pairs' other halves (itself: adjacent ones)
-    bool turns, first;
+    bool turns, first, adjacent;
 
-    __device__ __forceinline__ Turner(const RopeTurns& r_, int d_) : r(r_), d(d_), other(d_) {
-        turns = d < 2 * r.half, first = d < r.half;
-        if (!r.traditional && turns) other = first ? d + r.half : d - r.half;
-        p = r.traditional ? d >> 1 : min(d, other);
+    __device__ __forceinline__ Turner(const RopeTurns& r, int d_) : d(d_), other(d_) {
+        turns = d < 2 * r.half, first = d < r.half, adjacent = r.traditional != 0;
+        if (!adjacent && turns) other = first ? d + r.half : d - r.half;
+        p = adjacent ? d >> 1 : min(d, other);
         if (!turns) return;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            if (e < (r.traditional ? 2 : 4)) rate[e] = turn_rate(r, p + e);
+            if (e < (adjacent ? 2 : 4)) rate[e] = turn_rate(r, p + e);
     }
-    __device__ __forceinline__ void at(int64_t token) {
+    __device__ __forceinline__ void at(const RopeTurns& r, int64_t token) {
         if (!turns) return;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            if (e < (r.traditional ? 2 : 4)) cs[e] = turn_of(rate[e], r.positions[r.axes[p + e] * r.stride + token]);
+            if (e < (adjacent ? 2 : 4)) {
+                const float2 t = turn_of(rate[e], r.positions[r.axes[p + e] * r.stride + token]);
+                cos[e] = t.x, sin[e] = t.y;
+            }
     }
     __device__ __forceinline__ half4v of(half4v x, half4v z) const {  // z: the other halves (not of adjacent pairs)
         if (!turns) return x;
-        if (r.traditional) z = half4v{x[1], x[0], x[3], x[2]};
+        if (adjacent) z = half4v{x[1], x[0], x[3], x[2]};
         half4v y;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const bool one = r.traditional ? e % 2 == 0 : first;
-            const float2 t = r.traditional ? cs[e / 2] : cs[e];
+            const bool one = adjacent ? e % 2 == 0 : first;
+            const float c0 = cos[e / 2], c1 = cos[e], s0 = sin[e / 2], s1 = sin[e];
             float r1, r2;
-            rope_rot((float)(one ? x[e] : z[e]), (float)(one ? z[e] : x[e]), t.x, t.y, r1, r2);
+            rope_rot((float)(one ? x[e] : z[e]), (float)(one ? z[e] : x[e]), adjacent ? c0 : c1, adjacent ? s0 : s1, r1, r2);
             y[e] = (f16)(one ? r1 : r2);
         }
         return y;
@@ -311,7 +313,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
             const int64_t token = i / per;
             const int h0 = i % per * kTurnHeads;
             Turner t(turn.r, threadIdx.x % (D / 4) * 4);
-            t.at(token);
+            t.at(turn.r, token);
             const f16* q = a.k - (int64_t)turn.hq * D + token * a.k_token;
             for (int h = h0 + threadIdx.x / (D / 4); h < min(h0 + kTurnHeads, turn.hq); h += blockDim.x / (D / 4))
                 *(half4v*)(turn.q_out + (token * turn.hq + h) * D + t.d) = t.of(*(const half4v*)(q + h * D + t.d), *(const half4v*)(q + h * D + t.other));
@@ -371,7 +373,7 @@ __global__ __launch_bounds__(64 * kStoreWaves) void paged_update_kernel(PagedVie
             each8([&](auto k) {
                 constexpr int K = decltype(k)::value;
                 if (!__any(in(K))) return;
-                t.at(in(K) ? t0 + K : p.first);
+                t.at(turn.r, in(K) ? t0 + K : p.first);
                 xk[K] = t.of(xk[K], z[K]);
             });
         }

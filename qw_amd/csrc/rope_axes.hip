@@ -141,9 +141,9 @@ int paged_rope_update(PagedCache& c, const RopeAxes& r, const void* qkv, int hq,
     QW_REQUIRE(dg.ok, QW_ERR_HIP, "paged rope update: hipSetDevice failed");
     if (s.n_tokens == 0) return rope_axes(r, qkv, 0, hq, c.hkv, c.D, q_out, nullptr, stream);
     // One launch for a step of few sequences: each workgroup forms its tokens' angles anew, one token behind the other. Two launches /
-    // one, 24 heads over 4, D = 256, replayed, us: 1 token 10.0 / 8.5, 64 of 64 sequences 10.5 / 10.8 (called one by one and
-    // read back 21.4 / 18.4), 256 of 256 11.6 / 20.5, 256 of 8 12.9 / 35.1.
-    if (s.n_tokens <= std::min(64, s.n_seq) && r.rope_dims % 8 == 0 && (uintptr_t)q_out % 8 == 0) {
+    // one, replayed, us: 24 heads over 4, D = 256, 1 token 9.8 / 6.6, 64 of 64 sequences 10.3 / 7.2, 256 of 256 11.6 / 8.2, 256 of 8
+    // 12.7 / 13.7, 1024 of 1024 19.8 / 21.0; 32 over 8, D = 128, 256 of 256 11.3 / 9.7, 256 of 8 14.4 / 20.3.
+    if (s.n_tokens <= std::min(256, s.n_seq) && r.rope_dims % 8 == 0 && (uintptr_t)q_out % 8 == 0) {
         RopeTurns t;
         if (int rc = rope_turns(r, s.n_tokens, hq, c.hkv, c.D, t)) return rc;
         return paged_turn_update(c, t, qkv, hq, q_out, s, stream);

@@ -139,7 +139,7 @@ def test_rope_axes_refusals():
 @pytest.mark.parametrize("mode,hq,hkv,D,sections,interleaved,traditional", [
     ("fp16", 24, 4, 256, (16, 24, 24), False, False), ("affine8", 9, 3, 128, (8, 4, 4), True, True), ("int8", 2, 2, 256, (128,), False, False),
     ("affine4", 20, 2, 128, (3, 2, 2), True, False), ("affine8", 8, 8, 256, (2, 2), False, True), ("int8", 3, 1, 128, (64,), False, True)])
-@pytest.mark.parametrize("counts", [[1] * 9, [3, 0, 0, 9] + [0] * 9, [1, 0, 5, 30], [3000, 1], [1] * 64, [1] * 65])
+@pytest.mark.parametrize("counts", [[1] * 9, [3, 0, 0, 9] + [0] * 9, [1, 0, 5, 30], [3000, 1], [1] * 256, [1] * 257])
 def test_rotated_on_their_way(mode, hq, hkv, D, sections, interleaved, traditional, counts):
     """Few tokens rotate in the launch that stores them, many before it: both as rope_axes and update give them, with tokens
     that have no page among them."""
