@@ -468,7 +468,15 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
 
         float4v o[RT][D / 16], ob[RT];  // ob: the biases' part, group m's in row m
         float M[RT], l[RT];
-        int E = 0;
+        // V's steps so far are below 2^(E + 1) = step_end. P gives way by 2^E, so that P times the largest step takes a half's middle
+        // range and lesser products keep their bits; P that meets the middles (C0 the middle code) gives way where E > 0 alone,
+        // and the middles are lifted by as much instead: E is such that they then stay below 2^15. (10240 keys of 1e-3, each
+        // of 2^-19 of the first one's weight, 8 bits: with no E below 0 their values' differences were lost. 17 sequences of
+        // up to 8k 4-bit keys 32.4 us without, 33.3 so; Int8 the same.)
+        constexpr float C0 = BITS == 4 ? 8.0f : 128.0f;
+        int E = BITS == 16 ? 0 : -15;
+        float step_end = 0x1p-14f, drop = 0x1p-15f;
+        f16 lift = (f16)0x1p15f;
 #pragma unroll
         for (int t = 0; t < RT; t++) {
             M[t] = kNone, l[t] = 0.0f;
@@ -572,37 +580,15 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
             }
             const f16* vpar = kpar + 256;
             auto v_scales = [&](const f16* par, int m) { return *(const half8*)(par + 8 * m); };  // of 8 keys in group m
+            // two keys' steps and bases of a group: a lane group's 16 lanes have all that there are of its 8 keys
+            half2v step{}, base{};
             if constexpr (BITS != 16) {
-                uint32_t high = 0;
-#pragma unroll
-                for (int m = 0; m < NG; m++) {
-                    const u32x4 x = __builtin_bit_cast(u32x4, v_scales(vpar, m));
-                    high |= x[0] | x[1] | x[2] | x[3];
-                }
-                if (__any((high & 0x40004000u) != 0)) {  // V scales of 2 and more: P gives way, so that P times a scale fits a half
-                    float big = 0.0f;
-#pragma unroll 1
-                    for (int m = 0; m < NG; m++) {
-                        const half8 x = v_scales(vpar, m);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf((float)x[i]));
-                    }
-                    big = wave_reduce(big, OpMax());
-                    const int e = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(big) >> 23) - 127);
-                    if (e > E) {
-                        const float f = __builtin_amdgcn_exp2f((float)(E - e));
-                        E = e;
-#pragma unroll
-                        for (int t = 0; t < RT; t++) {
-                            l[t] *= f;
-                            ob[t] *= f;
-#pragma unroll
-                            for (int i = 0; i < D / 16; i++) o[t][i] *= f;
-                        }
-                    }
-                }
-                vpar += afresh(0);  // (read again below, not held)
+                const int c = afresh(col);
+                const f16* two = vpar + 8 * (c >> 2 & (NG - 1)) + 2 * (c & 3);
+                step = *(const half2v*)two;
+                if (!INT8) base = *(const half2v*)(two + 8 * NG);
             }
+            float mx[RT];
 #pragma unroll
             for (int t = 0; t < RT; t++) {
 #pragma unroll
@@ -611,12 +597,37 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
 #pragma unroll
                     for (int i = 0; i < 8; i++) s[t][i] = pos + i < seen[t] ? s[t][i] : -INFINITY;
                 }
-                float mx = fmaxf(fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])),
-                                 fmaxf(fmaxf(s[t][4], s[t][5]), fmaxf(s[t][6], s[t][7])));
-                if (__any(mx > M[t] + kLazy)) {
-                    mx = fmaxf(mx, lane_xor<16>(mx, lane));
-                    mx = fmaxf(mx, lane_xor<32>(mx, lane));
-                    const float m1 = fmaxf(M[t], mx), alpha = __builtin_amdgcn_exp2f(M[t] - m1);
+                mx[t] = fmaxf(fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])),
+                              fmaxf(fmaxf(s[t][4], s[t][5]), fmaxf(s[t][6], s[t][7])));
+            }
+            float down = 1.0f;
+            bool moved = false;
+            if constexpr (BITS != 16) {
+                half2v most = __builtin_elementwise_max(step, -step);
+                if constexpr (!INT8) {
+                    const half2v mid = __builtin_elementwise_fma(step, half2v{} + (f16)C0, base) * (half2v{} + (f16)0x1p-14f);
+                    most = __builtin_elementwise_max(most, __builtin_elementwise_max(mid, -mid));
+                }
+                const float big = (float)__builtin_elementwise_max(most[0], most[1]);
+                if (__any(!(big < step_end))) {
+                    const int e = min(__builtin_amdgcn_readfirstlane((int)(__float_as_uint(wave_reduce(big, OpMax())) >> 23)) - 127, 16);
+                    if (e > E) {
+                        down = __builtin_amdgcn_exp2f((float)(E - e));
+                        moved = true;
+                        E = e;
+                        step_end = __builtin_amdgcn_exp2f((float)(E + 1));
+                        drop = __builtin_amdgcn_exp2f((float)min(E, 0));
+                        lift = (f16)__builtin_amdgcn_exp2f((float)-min(E, 0));
+                    }
+                }
+                vpar += afresh(0);  // (read again below, not held)
+            }
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                if (__any(moved || mx[t] > M[t] + kLazy)) {
+                    mx[t] = fmaxf(mx[t], lane_xor<16>(mx[t], lane));
+                    mx[t] = fmaxf(mx[t], lane_xor<32>(mx[t], lane));
+                    const float m1 = fmaxf(M[t], mx[t]), alpha = __builtin_amdgcn_exp2f(M[t] - m1) * down;
                     M[t] = m1;
                     l[t] *= alpha;
                     ob[t] *= alpha;
@@ -635,7 +646,7 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
 #pragma unroll
                 for (int t = 0; t < RT; t++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) ph[t][i] = (f16)s[t][i];
+                    for (int i = 0; i < 8; i++) ph[t][i] = BITS == 16 ? (f16)s[t][i] : (f16)__builtin_fmaf(s[t][i], drop, 0.0f);
             }
             if constexpr (BITS == 16) {
 #pragma unroll
@@ -650,8 +661,7 @@ __global__ __launch_bounds__((64 * Form<BITS, D, TILES>::WAVES), (Form<BITS, D, 
                 }
             } else {
                 if constexpr (!INT8) {
-                    const f16 c0 = BITS == 4 ? 8.0f : 128.0f;
-                    half8 vb = __builtin_elementwise_fma(v_scales(vpar, min(col, NG - 1)), half8{} + c0, v_scales(vpar, NG + min(col, NG - 1)));
+                    half8 vb = __builtin_elementwise_fma(v_scales(vpar, min(col, NG - 1)), half8{} + (f16)C0, v_scales(vpar, NG + min(col, NG - 1))) * lift;
                     if (col >= NG) vb = half8{};
 #pragma unroll
                     for (int t = 0; t < RT; t++) ob[t] = mfma(vb, ph[t], ob[t]);
