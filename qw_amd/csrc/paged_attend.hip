@@ -975,7 +975,8 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     // more than 64, whose cuts take a search, up to 8: D = 128, 8 bits, 65 sequences 32.0 / 34.9, 128 41.0 / 50.8, 256 97.7 /
     // 102, 1024 374 / 368; D = 256, 4 bits, 128 32.9 / 49.8, 1024 246 / 255.
     const int few = q.n_seq > 64 ? 8 : c.D == 256 ? 3 : c.bits == 16 ? 5 : 4;
-    a.whole = rounds > 0 && most <= few * round;
+    // (one worker, where the query rows alone fill the card, reads all of every sequence)
+    a.whole = rounds > 0 && (a.workers == 1 || most <= few * round);
     // Keys that may be more than the 256 MB behind the L2 caches, each read once, go past the caches (us, without / with: 64
     // sequences of up to 16k fp16 keys 491 / 438, 32 sparse ones of 32k fp16 keys, with the selection, 127 / 112, 4 of
     // 32k Int8 keys with 5 rows 50.1 / 48.6). Fewer may be there from the last call (64 of up to 1024 fp16 keys, the same again and
