@@ -580,7 +580,10 @@ int qw_paged_gather(const qw_paged_cache* cache, void* k_out, void* v_out, int n
  *     counts twice, here as in the table; qw_paged_select writes such)
  *   out [n_seq][n_q_heads][n_rows][head_dim] fp16
  * Keys that a later row sees and this one does not must be finite. |scale| <= 2^40; at most 16384 rows
- * (n_rows * heads of a group) a KV head. n_seq = 0: nothing happens. */
+ * (n_rows * heads of a group) a KV head. n_seq = 0: nothing happens.
+ * The lengths stay on the device, so that how a call runs (not what it gives) goes by the room of its tables, or of its
+ * lists where they are shorter: one launch for room of some hundred keys a sequence, else two; keys past the caches where room and
+ * pool both hold more than 256 MB. A captured step over wide tables takes the forms of long sequences. */
 int qw_paged_attention(qw_paged_cache* cache, const void* q, int64_t q_seq_stride, int64_t q_head_stride,
                        int64_t q_row_stride, int n_seq, int n_q_heads, int n_rows, const int32_t* lengths,
                        const int32_t* table, int64_t table_stride, int table_width, const int32_t* picked,

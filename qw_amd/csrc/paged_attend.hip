@@ -981,7 +981,10 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     // sequences of up to 16k fp16 keys 491 / 438, 32 sparse ones of 32k fp16 keys, with the selection, 127 / 112, 4 of
     // 32k Int8 keys with 5 rows 50.1 / 48.6). Fewer may be there from the last call (64 of up to 1024 fp16 keys, the same again and
     // again, 44.5 / 52.1), and more row tiles than a workgroup's share them (128 rows of 4 sequences, 8k fp16 keys, 182 / 236).
-    const bool past = groups == 1 && (double)most * q.n_seq * c.hkv * (c.D * c.bits / 4 + c.par_halves() / 2) > 256.0 * (1 << 20);
+    // The host knows the lists' and tables' room and the pool's, not the lengths: sequences cannot have more keys of their own
+    // than the pool, however wide their tables (64 sequences of up to 1024 fp16 keys in tables of 8192 columns 40.3 / 34.1).
+    const double keys = std::min((double)most * q.n_seq, (double)c.n_pages * c.page_size);
+    const bool past = groups == 1 && keys * c.hkv * (c.D * c.bits / 4 + c.par_halves() / 2) > 256.0 * (1 << 20);
     const int64_t parts = (int64_t)a.workers * 2 * c.hkv * a.R;
     const bool cuts = q.n_seq > 64 && rounds > 0 && !a.whole;
     if (!a.whole) {

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from conftest import rng
-from test_gpu_paged import Sequences, dev, ints, queries, side_stream
+from test_gpu_paged import MODES, Sequences, dev, ints, queries, side_stream
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -34,3 +34,61 @@ def test_rows_that_fill_the_card_need_no_workspace(mode, lengths):
         torch.cuda.synchronize()
         s.check(out[:, 31:], q[:, 31:], 0.09, lengths=now)
         assert torch.equal(out, s.cache.attention(q, t, n, 0.09))
+
+
+def in_a_large_pool(r, mode, hkv, D, ps, lengths, width, nbytes):
+    """Sequences whose pages lie anywhere in a pool of more than nbytes bytes of codes."""
+    import qw_amd
+
+    s = Sequences(r, mode, hkv, D, ps, lengths)
+    s.cache.close()
+    s.n_pages = int(nbytes // (2 * ps * hkv * D * s.cache.bits // 8)) + 2
+    at = s.table >= 0
+    s.table = np.pad(s.table, ((0, 0), (0, width - s.width)), constant_values=-1)
+    s.width = width
+    named = int(at.sum())
+    s.table[:, :at.shape[1]][at] = np.concatenate([[s.n_pages - 1, 0], 1 + r.permutation(s.n_pages - 2)[:named - 2]])
+    s.cache = qw_amd.PagedKVCache(mode, hkv, D, s.n_pages, page_size=ps)
+    offsets = np.concatenate([[0], np.cumsum(lengths)])
+    s.cache.update(dev(np.concatenate(s.k)), dev(np.concatenate(s.v)), ints(s.table), ints([0] * len(lengths)), offsets=ints(offsets))
+    return s
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("n_seq,L,picks", [(3, 1, 0), (3, 3, 0), (70, 1, 0), (3, 1, 9), (70, 2, 9)])
+def test_keys_past_the_caches(mode, D, n_seq, L, picks):
+    """Tables and pools of more than the caches hold, on both sides of 64 sequences, of one and two row tiles, over all pages
+    and over picked ones."""
+    r = rng(D + n_seq + L + picks)
+    hkv, ps = 2, 16
+    lengths = [0, 33, 700] if n_seq == 3 else [int(x) for x in r.integers(0, 90, n_seq)]
+    lengths[1], lengths[n_seq - 1] = 150, 1700
+    s = in_a_large_pool(r, mode, hkv, D, ps, lengths, 40000, 300 * 2 ** 20)
+    hq = 8 * hkv if L > 2 else 4 * hkv
+    q, t, n = queries(r, n_seq, hq, L, D), ints(s.table), ints(lengths)
+    picked = None
+    if picks:
+        picked = np.full((n_seq, hkv, 20000), -1, dtype=np.int32)  # (as many as make a list's keys more than the caches hold)
+        for b, length in enumerate(lengths):
+            for h in range(hkv):
+                some = r.permutation(-(-length // ps))[:picks]
+                picked[b, h, :len(some)] = some
+    out = s.cache.attention(q, t, n, 0.08, picked=None if picked is None else ints(picked))
+    s.check(out, q, 0.08, picked=picked)
+
+
+@pytest.mark.parametrize("mode", MODES)
+def test_a_pool_named_over_and_over(mode):
+    """More keys than the pool holds, by a wide table that names its pages again and again, and sequences that share them."""
+    r = rng(81)
+    s = Sequences(r, mode, 8, 128, 16, [160])
+    table = np.full((5, 20000), -1)
+    table[:, :900] = s.table[0, np.arange(900) % 10]
+    lengths = [14400, 160, 1, 0, 333]
+    q = queries(r, 5, 16, 1, 128)
+    out = s.cache.attention(q, ints(table), ints(lengths), 0.1)
+    again = Sequences(r, mode, 8, 128, 16, [1])
+    again.lengths = lengths
+    again.k, again.v = ([np.tile(x[0], (90, 1, 1))[:m] for m in lengths] for x in (s.k, s.v))
+    again.check(out, q, 0.1)
