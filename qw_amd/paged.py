@@ -60,7 +60,10 @@ def _turned(qkv, positions, sections, width: int, what: str):
         raise QwError(1, f"{what}: positions must be [{len(sections)}, {n}] int32 on {qkv.device}")
     if n > 1 and positions.stride(1) != 1 or len(sections) > 1 and positions.stride(0) < n:
         positions = positions.contiguous()
-    return qkv.contiguous(), n, positions, positions.stride(0) if len(sections) > 1 else n
+    qkv = qkv.contiguous()
+    if qkv.data_ptr() % 16:
+        qkv = qkv.clone()
+    return qkv, n, positions, positions.stride(0) if len(sections) > 1 else n
 
 
 def rope_axes(qkv, positions, sections, n_q_heads: int, n_kv_heads: int, head_dim: int, rope_base: float,

@@ -92,3 +92,27 @@ def test_a_pool_named_over_and_over(mode):
     again.lengths = lengths
     again.k, again.v = ([np.tile(x[0], (90, 1, 1))[:m] for m in lengths] for x in (s.k, s.v))
     again.check(out, q, 0.1)
+
+
+@pytest.mark.parametrize("counts", [[1] * 5, [40, 0, 7]])
+@pytest.mark.parametrize("off", [1, 2, 4])
+def test_projections_at_any_offset(counts, off):
+    """A projection that begins inside a flat buffer, 2, 4 or 8 bytes off 16, one token a sequence and more."""
+    import qw_amd
+
+    r = rng(82 + off)
+    hq, hkv, D, n, B = 4, 2, 128, sum(counts), len(counts)
+    row = (hq + 2 * hkv) * D
+    flat = dev(r.standard_normal(n * row + off).astype(np.float16))
+    qkv = flat[off:].view(n, row)
+    pos, starts = ints(r.integers(0, 9000, (3, n))), ints([3] * B)
+    offsets = ints(np.concatenate([[0], np.cumsum(counts)]))
+    table = ints(r.permutation(4 * B).reshape(B, 4))
+    q0, k0 = qw_amd.rope_axes(qkv.clone(), pos, (8, 4, 4), hq, hkv, D, 1e4)
+    for x, y in zip(qw_amd.rope_axes(qkv, pos, (8, 4, 4), hq, hkv, D, 1e4), (q0, k0)):
+        assert torch.equal(x, y)
+    a, b = (qw_amd.PagedKVCache("affine8", hkv, D, 4 * B, page_size=16) for _ in range(2))
+    assert torch.equal(a.rope_update(qkv, pos, (8, 4, 4), hq, 1e4, table, starts, offsets=offsets), q0)
+    b.update(k0, qkv.view(n, -1, D)[:, hq + hkv:], table, starts, offsets)
+    for x, y in zip(a.gather(table, starts, n, offsets), b.gather(table, starts, n, offsets)):
+        assert torch.equal(x, y)
