@@ -136,7 +136,6 @@ int paged_rope_update(PagedCache& c, const RopeAxes& r, const void* qkv, int hq,
                       hipStream_t stream) {
     if (int rc = check_seqs(c, s, "paged rope update")) return rc;
     QW_REQUIRE((uintptr_t)qkv % 8 == 0, QW_ERR_INVALID_ARGUMENT, "paged rope update: qkv 8-byte aligned expected");
-    QW_REQUIRE(stream != hipStreamPerThread, QW_ERR_UNSUPPORTED, "paged rope update: hipStreamPerThread; name a stream");
     DeviceGuard dg(c.device);
     QW_REQUIRE(dg.ok, QW_ERR_HIP, "paged rope update: hipSetDevice failed");
     if (s.n_tokens == 0) return rope_axes(r, qkv, 0, hq, c.hkv, c.D, q_out, nullptr, stream);
@@ -148,7 +147,8 @@ int paged_rope_update(PagedCache& c, const RopeAxes& r, const void* qkv, int hq,
         if (int rc = rope_turns(r, s.n_tokens, hq, c.hkv, c.D, t)) return rc;
         return paged_turn_update(c, t, qkv, hq, q_out, s, stream);
     }
-    // the rotated keys pass through a workspace on their way into the pages
+    // the rotated keys pass through a workspace on their way into the pages (one handle, a stream a thread: they would share it)
+    QW_REQUIRE(stream != hipStreamPerThread, QW_ERR_UNSUPPORTED, "paged rope update: hipStreamPerThread; name a stream");
     void* k = nullptr;
     if (int rc = workspace(kWsPagedKeys, c.device, stream, (size_t)s.n_tokens * c.hkv * c.D * sizeof(f16), &k)) return rc;
     if (int rc = rope_axes(r, qkv, s.n_tokens, hq, c.hkv, c.D, q_out, k, stream)) return rc;

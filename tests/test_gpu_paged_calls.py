@@ -116,3 +116,29 @@ def test_projections_at_any_offset(counts, off):
     b.update(k0, qkv.view(n, -1, D)[:, hq + hkv:], table, starts, offsets)
     for x, y in zip(a.gather(table, starts, n, offsets), b.gather(table, starts, n, offsets)):
         assert torch.equal(x, y)
+
+
+def test_stream_per_thread_where_no_workspace_is_kept():
+    """A token a sequence rotates in the launch that stores it, on any stream; more pass through a workspace of their stream."""
+    import qw_amd
+
+    r = rng(83)
+    hq, hkv, D = 4, 2, 128
+    a, b = (qw_amd.PagedKVCache("fp16", hkv, D, 6, page_size=16) for _ in range(2))
+    qkv = dev(r.standard_normal((3, (hq + 2 * hkv) * D)).astype(np.float16))
+    pos, starts, table = ints(r.integers(0, 9000, (1, 3))), ints([0, 5, 17]), ints([[0, 1], [2, 3], [4, 5]])
+    want = a.rope_update(qkv, pos, (64,), hq, 1e4, table, starts)
+    q = torch.zeros_like(want)
+    torch.cuda.synchronize()
+
+    def call(n_seq):
+        return qw_amd.lib().qw_paged_rope_update(b._h, qkv.data_ptr(), hq, D, 0, 1e4, 1.0, pos.data_ptr(), 3, 1, bytes(64),
+                                                 q.data_ptr(), 3, n_seq, None, starts.data_ptr(), table.data_ptr(), 2, 2, 2)
+
+    assert call(1) == 2 and b"hipStreamPerThread" in qw_amd.lib().qw_last_error()
+    assert torch.all(q == 0)
+    assert call(3) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(q, want)
+    for x, y in zip(a.gather(table, starts, 3), b.gather(table, starts, 3)):
+        assert torch.equal(x, y)
