@@ -74,6 +74,7 @@ int PagedCache::init(int mode_, int group_size, int n_kv_heads, int head_dim, in
 }
 
 void PagedCache::release() {
+    if (!view.k) return;  // (a refused pool: no device call)
     DeviceGuard dg(device);
     (void)hipDeviceSynchronize();
     void* ptrs[7] = {view.k, view.v, view.k_par, view.v_par, view.lohi, view.codes, view.top};

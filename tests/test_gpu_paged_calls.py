@@ -142,3 +142,21 @@ def test_stream_per_thread_where_no_workspace_is_kept():
     assert torch.equal(q, want)
     for x, y in zip(a.gather(table, starts, 3), b.gather(table, starts, 3)):
         assert torch.equal(x, y)
+
+
+def test_a_refused_pool_leaves_a_capture_alone():
+    """A pool that is refused by its arguments is refused before any device call: one that waits for the device ends a capture."""
+    import qw_amd
+
+    x = torch.zeros(8, device="cuda")
+
+    def refused():
+        for args in (("fp16", 2, 64, 4), ("fp16", 2, 128, 0), ("turbo4", 2, 128, 4)):
+            with pytest.raises(qw_amd.QwError):
+                qw_amd.PagedKVCache(*args)
+        x.add_(1)
+
+    _, g = captured(refused, side_stream(6))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.all(x == 1)
