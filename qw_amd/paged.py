@@ -44,6 +44,7 @@ def _axes(sections: tuple, interleaved: bool) -> bytes:
     n = len(sections)
     if not 1 <= n <= 8 or any(int(s) != s or s < 0 for s in sections) or not 0 < sum(sections) <= 256:
         raise QwError(1, "rope_axes: 1 to 8 sections of pairs, none negative, 1 to 256 in all, expected")
+    sections = tuple(int(s) for s in sections)
     if not interleaved:
         return bytes(a for a, s in enumerate(sections) for _ in range(s))
     return bytes(p % n if p < n * sections[p % n] else 0 for p in range(sum(sections)))
