@@ -221,6 +221,7 @@ int KVCache::init(int mode_, int group_size, int n_kv_heads, int head_dim, int c
 }
 
 int KVCache::release() {
+    if (!fast_flag) return QW_OK;  // (a refused cache, or released: no device call)
     DeviceGuard dg(device);
     (void)hipDeviceSynchronize();
     void* ptrs[6] = {k_data, (void*)k_params, v_data, (void*)v_params, (void*)fast_flag,
