@@ -2,7 +2,7 @@
 //
 // out = softmax(scale q . k) v for each row over its sequence's keys, causal among the last n_rows of
 // them, in one pass with the running maximum and sum. Bound by reading the codes once from HBM: 64 sequences of
-// up to 16k fp16 keys (8 KV heads, D = 128) 435 us, 6.6 TB/s; one of 128k keys 5.0 to 5.8 TB/s in every mode. Short ones are bound by their start (lengths, table, queries and keys, one behind the other, 5 us), the
+// up to 16k fp16 keys (8 KV heads, D = 128) 435 us, 6.6 TB/s; one of 128k keys 5.0 to 5.8 TB/s in every mode. Short ones are bound by their start (lengths, table, queries and keys, one behind the other, 4 us), the
 // last joining and the second launch (4 us).
 //
 // Work is dealt in rounds of 128 or 256 keys to the workers of a head (a grid sized for the card, lengths read on the
@@ -19,8 +19,9 @@
 // is multiplied by a key's V scale in fp32 and rounded once to fp16, P'. With the codes' middle c0,
 //   sum_k P (scale code + bias) = sum_k P' code - c0 sum_k P' + sum_k P (bias + c0 scale):
 // one more matrix product each for the last two. So P's and P's rounding meet what is left of a code beside the middle, not
-// the code and the bias that nearly cancel each other (17 sequences of 4 bits: an error of 0.00027 of the result for 0.00069,
-// of which 0.0002 is the result's own rounding, for 0.9 us of 32).
+// the code and the bias that nearly cancel each other (17 sequences of 4 bits: an error of 0.00028 of the result for 0.00069,
+// for 0.9 us of 32). P is rounded because the matrix instructions take halves; a product of more bits costs two of them. Of
+// the 0.00028 the result's own rounding is 0.00021.
 // The next round's K is requested behind this one's scores, its V behind this one's P V, into the place that they
 // leave: a wave always waits for loads that are half a round old, and never for another wave.
 #include <algorithm>
@@ -973,14 +974,14 @@ int paged_attention(PagedCache& c, const PagedQuery& q, const int32_t* picked, i
     // 11.7 / 12.0, 5 rounds 15.6 / 12.1, fp16 12.8 / 12.8 and 17.2 / 13.1; D = 128, 8 bits, 3 rounds 9.0 / 11.2, 5
     // rounds 11.7 / 11.2, fp16 8.0 / 11.2 and 9.9 / 11.2. 16 sequences, D = 128, 5 rounds 12.4 / 13.9 and 11.0 / 16.3. With
     // more than 64, whose cuts take a search, up to 8: D = 128, 8 bits, 65 sequences 32.0 / 34.9, 128 41.0 / 50.8, 256 97.7 /
-    // 102, 1024 374 / 368; D = 256, 4 bits, 128 32.9 / 49.8, 1024 246 / 255.
+    // 102, 1024 374 / 368; D = 256, 4 bits, 128 32.9 / 49.8, 1024 246 / 255. (8 for all: that one of them loses 2 %.)
     const int few = q.n_seq > 64 ? 8 : c.D == 256 ? 3 : c.bits == 16 ? 5 : 4;
     // (one worker, where the query rows alone fill the card, reads all of every sequence)
     a.whole = rounds > 0 && (a.workers == 1 || most <= few * round);
     // Keys that may be more than the 256 MB behind the L2 caches, each read once, go past the caches (us, without / with: 64
-    // sequences of up to 16k fp16 keys 491 / 438, 32 sparse ones of 32k fp16 keys, with the selection, 127 / 112, 4 of
-    // 32k Int8 keys with 5 rows 50.1 / 48.6). Fewer may be there from the last call (64 of up to 1024 fp16 keys, the same again and
-    // again, 44.5 / 52.1), and more row tiles than a workgroup's share them (128 rows of 4 sequences, 8k fp16 keys, 182 / 236).
+    // sequences of up to 16k fp16 keys 491 / 438, 32 sparse ones of 32k fp16 keys, with the selection, 127 / 112). Fewer may be there
+    // from the last call (64 of up to 1024 fp16 keys, the same again and again, 44.5 / 52.1; where others came between, 200 MB
+    // of 4 sequences' Int8 keys with 5 rows, 50.1 / 48.6), and more row tiles than a workgroup's share them (128 rows of 4 sequences, 8k fp16 keys, 182 / 236).
     // The host knows the lists' and tables' room and the pool's, not the lengths: sequences cannot have more keys of their own
     // than the pool, however wide their tables (64 sequences of up to 1024 fp16 keys in tables of 8192 columns 40.3 / 34.1).
     const double keys = std::min((double)most * q.n_seq, (double)c.n_pages * c.page_size);

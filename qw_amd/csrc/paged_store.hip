@@ -698,8 +698,8 @@ int64_t most_units(const PagedSeqs& s, int size) {
 
 int store_waves(const PagedCache& c, const PagedSeqs& s) {
     // waves for the blocks of 8 slots that an average sequence touches in a page, two a wave at D = 128. So many / 8 / 2 at
-    // most, us: a token each of 33 sequences, pages of 16, D = 128 4.7 / 7.7 / 4.7; 2048 each of 8, pages of 256, D = 128 19.7 /
-    // 19.5 / 32.0; 13107 each of 5, pages of 32, D = 128 65 / 163 / 66
+    // most, the store alone, replayed over the same tokens, us: a token each of 33 sequences, pages of 16, D = 128 4.6 / 7.5 / 4.6; 2048
+    // each of 8, pages of 256 19.7 / 19.6 / 32.1; 13107 each of 5, pages of 32, Int8 63 / 163 / 64 (82 where they are in no cache)
     const int blocks = std::min(c.page_size / 8, s.n_tokens / s.n_seq / 8 + 1);
     return std::max(1, std::min(kStoreWaves, blocks * c.D / 256));
 }

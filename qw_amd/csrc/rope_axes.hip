@@ -118,7 +118,7 @@ int rope_axes(const RopeAxes& r, const void* qkv, int n_tokens, int hq, int hkv,
     a.k_out = (f16*)k_out;
     a.n = n_tokens, a.hq = hq, a.hkv = hkv, a.D = D;
     // a token a workgroup while there are few, else as many as its angles' place holds, up to 8. One / 8, 32 + 8 heads of
-    // D = 128, us: 64 tokens 5.3 / 19.5, 1500 10.5 / 22.2, 4099 19.2 / 26.9, 32768 154 / 145
+    // D = 128, replayed, us: 64 tokens 5.2 / 18.8, 1500 9.1 / 19.5, 4099 18.2 / 25.7, 32768 141 / 134
     a.tokens = std::max(1, std::min({8, n_tokens / 4096, kAngles / a.r.half}));
     const int64_t groups = ((int64_t)n_tokens + a.tokens - 1) / a.tokens;
     QW_REQUIRE(groups * 256 <= UINT32_MAX, QW_ERR_UNSUPPORTED, "rope axes: too many tokens for one call");
