@@ -563,7 +563,7 @@ int qw_paged_update(qw_paged_cache* cache, const void* k, const void* v, int64_t
                     const int32_t* starts, const int32_t* table, int64_t table_stride, int table_width, void* stream);
 
 /* Reads tokens back: positions starts[b] .. of each sequence, arguments as qw_paged_update, as the fp16
- * values that their codes stand for (qw_kv_dequantize's). k_out, v_out [n_tokens][n_kv_heads][head_dim];
+ * values that their codes stand for (qw_kv_dequantize's). k_out, v_out [n_tokens][n_kv_heads][head_dim], 8-byte aligned;
  * positions without a page are zeros, rows of no sequence stay as they were. */
 int qw_paged_gather(const qw_paged_cache* cache, void* k_out, void* v_out, int n_tokens, int n_seq,
                     const int32_t* offsets, const int32_t* starts, const int32_t* table, int64_t table_stride,
@@ -580,7 +580,7 @@ int qw_paged_gather(const qw_paged_cache* cache, void* k_out, void* v_out, int n
  *     reads, as columns of its sequence's table row (entries outside it are skipped; of
  *     each list the first min(n_picked, the sequence's pages) entries are read, and a page that is named twice
  *     counts twice, here as in the table; qw_paged_select writes such)
- *   out [n_seq][n_q_heads][n_rows][head_dim] fp16
+ *   out [n_seq][n_q_heads][n_rows][head_dim] fp16, 8-byte aligned
  * Keys that a later row sees and this one does not must be finite. |scale| <= 2^40; at most 16384 rows
  * (n_rows * heads of a group) a KV head. n_seq = 0: nothing happens.
  * The lengths stay on the device, so that how a call runs (not what it gives) goes by the room of its tables, or of its
@@ -619,7 +619,8 @@ int qw_rope_axes(const void* qkv, int n_tokens, int n_q_heads, int n_kv_heads, i
                  int traditional, float rope_base, float rope_scale, const int32_t* positions,
                  int64_t positions_stride, int n_axes, const uint8_t* axes, void* q_out, void* k_out, void* stream);
 
-/* qw_rope_axes, then qw_paged_update of the rotated keys and the projection's values; the rotated q to q_out. */
+/* qw_rope_axes, then qw_paged_update of the rotated keys and the projection's values; the rotated q to q_out. qkv 8-byte
+ * aligned. */
 int qw_paged_rope_update(qw_paged_cache* cache, const void* qkv, int n_q_heads, int rope_dims, int traditional,
                          float rope_base, float rope_scale, const int32_t* positions, int64_t positions_stride,
                          int n_axes, const uint8_t* axes, void* q_out, int n_tokens, int n_seq, const int32_t* offsets,
